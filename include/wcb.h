@@ -41,8 +41,9 @@ enum {
  * uploaded unchanged). wcb_gemv_dev takes the two quantised types only. */
 enum { WCB_DTYPE_F32 = 0, WCB_DTYPE_F16 = 1, WCB_DTYPE_Q4_K = 12, WCB_DTYPE_Q6_K = 14 };
 
-/* KV cache element type */
-enum { WCB_KV_F32 = 0, WCB_KV_F16 = 1 };
+/* KV cache element type. BF16: the paged operators below only (a model's own
+ * cache is F32 or F16); they use the same values for their activations' type. */
+enum { WCB_KV_F32 = 0, WCB_KV_F16 = 1, WCB_KV_BF16 = 2 };
 
 /* Load options (no counterpart in the reference, whose Model::new takes only a
  * TransformerConfig: model.rs:188). Fill them with wcb_load_opts_init, which
@@ -94,7 +95,8 @@ typedef struct wcb_load_opts {
 void wcb_load_opts_init(wcb_load_opts* opts);
 
 /* Size (field == NULL) or byte offset of a field of a struct of this header:
- * "wcb_load_opts", "wcb_gen_config" or "wcb_model_config". SIZE_MAX for an
+ * "wcb_load_opts", "wcb_gen_config", "wcb_model_config", "wcb_paged_kv",
+ * "wcb_paged_batch" or "wcb_rope". SIZE_MAX for an
  * unknown struct or field. A binding generated by hand (ctypes, Rust repr(C))
  * checks its own layout against these once at start-up. */
 size_t wcb_struct_layout(const char* struct_name, const char* field);
@@ -326,6 +328,149 @@ uint32_t wcb_attention_dev(const float* q, const float* k_cache, const float* v_
 uint32_t wcb_attention_dev_noalloc(const float* q, const float* k_cache, const float* v_cache, float* out,
                                    uint32_t n_tokens, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
                                    uint32_t max_seq, uint32_t kv_len, uint32_t position, void* stream);
+
+/* ---- Paged serving: append, attend, verify --------------------------------
+ * No counterpart in the reference, whose cache is one contiguous sequence
+ * (kv_cache.rs:6-73). Keys and values of many sequences live in one pool of
+ * pages; a page table says which pages hold which sequence. One step of a
+ * serving loop is: wcb_paged_append_dev (the new tokens' rotated keys and
+ * values go to their pages), wcb_paged_attention_dev (the new tokens attend to
+ * their pages), and, where the new tokens were drafted, wcb_spec_verify_dev.
+ * Device pointers of the current device, caller's stream; all return after
+ * enqueueing, allocate nothing and may be captured into a CUDA graph. What the
+ * kernels find wrong in device data (lengths, page ids, token ids) they skip,
+ * and report in the status word, where the caller gives one. Distinct calls
+ * may run at once as long as they share no output and no workspace.
+ */
+
+/* A pool of pages. Key (and value) of head h of the token in slot t of page p
+ * starts at element p * page_stride + t * token_stride + h * head_stride of k
+ * (and v); head_dim elements follow. A model's contiguous cache
+ * [slot][n_kv_heads][max_seq][head_dim] is the pool with page_size = max_seq.
+ * Strides in elements, multiples of 16 bytes; k and v 16-byte aligned. All
+ * strides 0: [page][slot][head][head_dim] without gaps. */
+typedef struct wcb_paged_kv {
+  uint32_t struct_size; /* sizeof(wcb_paged_kv) */
+  uint32_t dtype;       /* WCB_KV_F32, WCB_KV_F16 or WCB_KV_BF16 */
+  uint32_t n_kv_heads;
+  uint32_t head_dim;  /* 64 or 128 */
+  uint32_t page_size; /* tokens of a page, any number >= 1 */
+  uint32_t n_pages;
+  void* k;
+  void* v;
+  uint64_t page_stride, token_stride, head_stride;
+} wcb_paged_kv;
+
+/* The sequences of one step. The new tokens of sequence s are rows
+ * q_start[s] .. q_start[s+1] - 1 of the step's activations; kv_len[s] counts
+ * the sequence's tokens, new ones included, so that its i-th new token has
+ * position kv_len[s] - (q_start[s+1] - q_start[s]) + i and lies in slot
+ * position % page_size of page page_table[s * max_pages + position / page_size].
+ * Rows of no sequence (before q_start[0], from q_start[n_seqs] on) are neither
+ * read nor written. A sequence may have no new tokens. */
+typedef struct wcb_paged_batch {
+  uint32_t struct_size; /* sizeof(wcb_paged_batch) */
+  uint32_t n_seqs;      /* at most 65536 */
+  uint32_t n_tokens;    /* rows of the activations (a padded batch may have more than q_start[n_seqs]) */
+  uint32_t max_q_len;   /* most new tokens of a sequence: chooses kernels, longer sequences stay right */
+  uint32_t max_pages;   /* entries of a sequence's row in page_table */
+  uint32_t reserved;    /* 0 */
+  const int32_t* q_start;    /* device, [n_seqs + 1], not descending */
+  const int32_t* kv_len;     /* device, [n_seqs] */
+  const int32_t* page_table; /* device, [n_seqs][max_pages]; entries past a sequence's last token are not read */
+  uint32_t* status;          /* device, or NULL: WCB_PAGED_* bits are ORed into it */
+} wcb_paged_batch;
+
+/* Status bits. BAD_PAGE: a page id outside the pool, or a position outside the
+ * page table's row (the token is not stored, the key takes no part in the
+ * attention). BAD_ROWS: q_start outside 0 .. n_tokens or descending (the
+ * sequence is skipped). BAD_LEN: a new token's position is negative (not
+ * stored; its attention output is zero). BAD_TOKEN: a drafted token outside the
+ * vocabulary (turned down). BAD_PROBS: a row of target probabilities without
+ * a positive finite value (the sampled token is -1). */
+enum {
+  WCB_PAGED_BAD_PAGE = 1,
+  WCB_PAGED_BAD_ROWS = 2,
+  WCB_PAGED_BAD_LEN = 4,
+  WCB_PAGED_BAD_TOKEN = 8,
+  WCB_PAGED_BAD_PROBS = 16
+};
+
+/* Rotation of a head's first rot_dim dimensions (attention.rs:230-262 rotates
+ * pairs (2i, 2i+1) of all of them): pair i turns by position * inv_freq[i]. The
+ * pairs are (2i, 2i+1), or (i, i + rot_dim / 2) with halves = 1. rot_dim a
+ * multiple of 16, at most head_dim; 0 = no rotation. wcb_rope_init fills
+ * inv_freq[i] = theta^(-2i / rot_dim); scaled variants overwrite it. Angles are
+ * computed in 64 bits, so far positions lose nothing. */
+typedef struct wcb_rope {
+  uint32_t struct_size; /* sizeof(wcb_rope) */
+  uint32_t rot_dim;
+  uint32_t halves;
+  uint32_t reserved; /* 0 */
+  double inv_freq[64];
+} wcb_rope;
+
+uint32_t wcb_rope_init(wcb_rope* rope, uint32_t rot_dim, double theta, uint32_t halves);
+
+/* The new tokens' queries, keys and values: q [n_tokens][n_heads][head_dim],
+ * k and v [n_tokens][n_kv_heads][head_dim] with the given strides between
+ * tokens (elements, multiples of 16 bytes; a fused projection's output has one
+ * stride for all three). Queries and keys are divided by their head's root mean
+ * square and multiplied by q_norm / k_norm (device f32 [head_dim], NULL: no norm;
+ * x / sqrt(mean(x^2) + eps) * w), rotated, and rounded once: queries to q_out
+ * (type and layout of q, own stride, may be q itself), keys and values to their
+ * pages. rope NULL: no rotation. dtype: type of q, k, v and q_out: F32 with any cache type, F16 with an
+ * F16 cache, BF16 with a BF16 cache. q = NULL with n_heads = 0: keys and values
+ * only. Two rows that map to one slot leave one of the two there, or a mixture. */
+uint32_t wcb_paged_append_dev(const wcb_paged_kv* kv, const wcb_paged_batch* batch, const wcb_rope* rope,
+                              const void* q, const void* k, const void* v, void* q_out, uint32_t dtype,
+                              uint32_t n_heads, uint64_t q_stride, uint64_t k_stride, uint64_t v_stride,
+                              uint64_t q_out_stride, const float* q_norm, const float* k_norm, float eps, void* stream);
+
+/* Bytes of device workspace one wcb_paged_attention_dev call with these
+ * arguments may use (needs no GPU). The first 4096 bytes must be zero before
+ * the workspace's first use (every call leaves them zero); calls that use one
+ * workspace must not overlap on the GPU. */
+uint32_t wcb_paged_attention_workspace(const wcb_paged_kv* kv, const wcb_paged_batch* batch, uint32_t n_heads,
+                                       size_t* bytes);
+
+/* compute_attention (attention.rs:332-435) over pages: for each new token at
+ * position p of its sequence, softmax(scale * q . k_j) v_j over the keys j <= p,
+ * and j > p - window where window > 0; n_heads / n_kv_heads query heads share
+ * a key head (any whole ratio up to 64). q and out: [n_tokens][n_heads][head_dim]
+ * with their strides between tokens (elements, multiples of 16 bytes), types as
+ * for wcb_paged_append_dev. scale 0: 1 / sqrt(head_dim). lse (device f32
+ * [n_tokens][n_heads], or NULL): the natural logarithm of the softmax's sum,
+ * for joining with attention over other keys. A row with no key gives zeros and
+ * -infinity. Keys that a row does not see do not reach it, whatever they hold
+ * (infinities and NaN included). */
+uint32_t wcb_paged_attention_dev(const wcb_paged_kv* kv, const wcb_paged_batch* batch, const void* q, void* out,
+                                 uint32_t dtype, uint32_t n_heads, uint64_t q_stride, uint64_t out_stride,
+                                 void* workspace, size_t workspace_bytes, float scale, uint32_t window, float* lse,
+                                 void* stream);
+
+/* Verification of drafted tokens against the target's probabilities, with
+ * given random numbers. Sequence s has draft_len[s] (NULL: max_draft) drafted
+ * tokens draft[s * max_draft + i]; target [s][i][vocab] (i = 0 .. max_draft) are
+ * the target's probabilities at each drafted token's place and after the last
+ * one, draft_probs [s][i][vocab] the draft's (NULL: the draft was certain of its
+ * tokens). Strides between sequences and between rows in elements, 0 = no gaps.
+ * Token i is accepted as long as all before it were and
+ *   u_accept[s * max_draft + i] * draft_probs[x_i] < target[x_i].
+ * At the first token turned down the next token is drawn from
+ * max(target - draft_probs, 0) (from the target where that is zero throughout),
+ * after the last accepted one from the target: the lowest index whose sum up to
+ * and including itself exceeds u_sample[s] times the sum of all, sums in 64 bits.
+ * tokens [s][max_draft + 1]: the accepted tokens, the drawn one, then -1.
+ * accepted [s]: how many were accepted. Probabilities that are negative or not
+ * finite count as zero; u_sample is held to [0, 1). status as in wcb_paged_batch.
+ * The drawn tokens follow the target's distribution exactly where draft tokens
+ * were drawn from draft_probs. */
+uint32_t wcb_spec_verify_dev(const int32_t* draft, const int32_t* draft_len, const float* target,
+                             const float* draft_probs, const float* u_accept, const float* u_sample, uint32_t n_seqs,
+                             uint32_t max_draft, uint32_t vocab, int32_t* tokens, int32_t* accepted,
+                             uint64_t target_seq_stride, uint64_t target_row_stride, uint64_t draft_seq_stride,
+                             uint64_t draft_row_stride, uint32_t* status, void* stream);
 
 /* Device stream a model handle launches on (a cudaStream_t), for callers that
  * time or order work against it. */

@@ -219,6 +219,22 @@ size_t wcb_struct_layout(const char* s, const char* f) {
     WCB_FIELD(wcb_model_config, num_kv_heads) WCB_FIELD(wcb_model_config, intermediate_size)
     WCB_FIELD(wcb_model_config, max_seq_len) WCB_FIELD(wcb_model_config, head_dim)
     WCB_FIELD(wcb_model_config, rms_norm_eps) WCB_FIELD(wcb_model_config, rope_theta)
+  } else if (st == "wcb_paged_kv") {
+    if (!f) return sizeof(wcb_paged_kv);
+    WCB_FIELD(wcb_paged_kv, struct_size) WCB_FIELD(wcb_paged_kv, dtype) WCB_FIELD(wcb_paged_kv, n_kv_heads)
+    WCB_FIELD(wcb_paged_kv, head_dim) WCB_FIELD(wcb_paged_kv, page_size) WCB_FIELD(wcb_paged_kv, n_pages)
+    WCB_FIELD(wcb_paged_kv, k) WCB_FIELD(wcb_paged_kv, v) WCB_FIELD(wcb_paged_kv, page_stride)
+    WCB_FIELD(wcb_paged_kv, token_stride) WCB_FIELD(wcb_paged_kv, head_stride)
+  } else if (st == "wcb_paged_batch") {
+    if (!f) return sizeof(wcb_paged_batch);
+    WCB_FIELD(wcb_paged_batch, struct_size) WCB_FIELD(wcb_paged_batch, n_seqs) WCB_FIELD(wcb_paged_batch, n_tokens)
+    WCB_FIELD(wcb_paged_batch, max_q_len) WCB_FIELD(wcb_paged_batch, max_pages) WCB_FIELD(wcb_paged_batch, reserved)
+    WCB_FIELD(wcb_paged_batch, q_start) WCB_FIELD(wcb_paged_batch, kv_len) WCB_FIELD(wcb_paged_batch, page_table)
+    WCB_FIELD(wcb_paged_batch, status)
+  } else if (st == "wcb_rope") {
+    if (!f) return sizeof(wcb_rope);
+    WCB_FIELD(wcb_rope, struct_size) WCB_FIELD(wcb_rope, rot_dim) WCB_FIELD(wcb_rope, halves)
+    WCB_FIELD(wcb_rope, reserved) WCB_FIELD(wcb_rope, inv_freq)
   }
 #undef WCB_FIELD
   return SIZE_MAX;

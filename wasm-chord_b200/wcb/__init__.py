@@ -27,6 +27,14 @@ DTYPE_Q4_K = 12
 DTYPE_Q6_K = 14
 KV_F32 = 0
 KV_F16 = 1
+KV_BF16 = 2  # the paged operators only
+
+# status bits of the paged operators (WCB_PAGED_*)
+PAGED_BAD_PAGE = 1
+PAGED_BAD_ROWS = 2
+PAGED_BAD_LEN = 4
+PAGED_BAD_TOKEN = 8
+PAGED_BAD_PROBS = 16
 
 EXPORTED = [
     "wcb_gen_config_default", "wcb_model_load", "wcb_model_free", "wcb_model_config_get", "wcb_forward",
@@ -37,7 +45,8 @@ EXPORTED = [
     "wcb_tokenizer_info", "wcb_tokenizer_set_special", "wcb_tokenize", "wcb_detokenize", "wcb_generate_text",
     "wcb_attention_dev",
     "wcb_attention_dev_noalloc", "wcb_tp_id", "wcb_model_tp_handle", "wcb_model_tp_connect", "wcb_model_tp_abort",
-    "wcb_load_opts_init", "wcb_struct_layout",
+    "wcb_load_opts_init", "wcb_struct_layout", "wcb_rope_init", "wcb_paged_append_dev",
+    "wcb_paged_attention_workspace", "wcb_paged_attention_dev", "wcb_spec_verify_dev",
 ]
 
 # the ctypes mirrors of include/wcb.h's structs, checked against the library's
@@ -72,7 +81,26 @@ class _GenConfig(C.Structure):
                 ("eos_id", C.c_uint32)]
 
 
-STRUCTS.update({"wcb_load_opts": _LoadOpts, "wcb_model_config": _ModelConfig, "wcb_gen_config": _GenConfig})
+class _PagedKV(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("dtype", C.c_uint32), ("n_kv_heads", C.c_uint32),
+                ("head_dim", C.c_uint32), ("page_size", C.c_uint32), ("n_pages", C.c_uint32), ("k", C.c_void_p),
+                ("v", C.c_void_p), ("page_stride", C.c_uint64), ("token_stride", C.c_uint64),
+                ("head_stride", C.c_uint64)]
+
+
+class _PagedBatch(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("n_seqs", C.c_uint32), ("n_tokens", C.c_uint32),
+                ("max_q_len", C.c_uint32), ("max_pages", C.c_uint32), ("reserved", C.c_uint32),
+                ("q_start", C.c_void_p), ("kv_len", C.c_void_p), ("page_table", C.c_void_p), ("status", C.c_void_p)]
+
+
+class _Rope(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("rot_dim", C.c_uint32), ("halves", C.c_uint32),
+                ("reserved", C.c_uint32), ("inv_freq", C.c_double * 64)]
+
+
+STRUCTS.update({"wcb_load_opts": _LoadOpts, "wcb_model_config": _ModelConfig, "wcb_gen_config": _GenConfig,
+                "wcb_paged_kv": _PagedKV, "wcb_paged_batch": _PagedBatch, "wcb_rope": _Rope})
 
 _LIB = None
 
@@ -139,6 +167,13 @@ def lib() -> C.CDLL:
     L.wcb_generate_text.argtypes = [u32, u32, C.c_char_p, C.POINTER(_GenConfig), C.c_char_p, sz, C.POINTER(sz)]
     L.wcb_attention_dev.argtypes = [vp, vp, vp, vp, u32, u32, u32, u32, u32, u32, u32, vp]
     L.wcb_attention_dev_noalloc.argtypes = [vp, vp, vp, vp, u32, u32, u32, u32, u32, u32, u32, vp]
+    u64, f32 = C.c_uint64, C.c_float
+    L.wcb_rope_init.argtypes = [C.POINTER(_Rope), u32, C.c_double, u32]
+    # struct arguments as addresses: the descriptors below keep theirs
+    L.wcb_paged_append_dev.argtypes = [vp, vp, vp, vp, vp, vp, vp, u32, u32, u64, u64, u64, u64, vp, vp, f32, vp]
+    L.wcb_paged_attention_workspace.argtypes = [vp, vp, u32, C.POINTER(sz)]
+    L.wcb_paged_attention_dev.argtypes = [vp, vp, vp, vp, u32, u32, u64, u64, vp, sz, f32, u32, vp, vp]
+    L.wcb_spec_verify_dev.argtypes = [vp, vp, vp, vp, vp, vp, u32, u32, u32, vp, vp, u64, u64, u64, u64, vp, vp]
     L.wcb_tp_id.argtypes = [vp]
     L.wcb_model_tp_handle.argtypes = [u32, vp]
     L.wcb_model_tp_connect.argtypes = [u32, vp, u32]
@@ -529,6 +564,88 @@ def attention_dev_noalloc(q_ptr: int, k_ptr: int, v_ptr: int, out_ptr: int, n_to
     """wcb_attention_dev with the library's fixed scratch array (no GPU allocation)."""
     _check(lib().wcb_attention_dev_noalloc(q_ptr, k_ptr, v_ptr, out_ptr, n_tokens, n_heads, n_kv_heads, head_dim,
                                            max_seq, kv_len, position, stream or None))
+
+
+# ---- paged serving: append, attend, verify ----------------------------------
+class PagedKV:
+    """A pool of pages on the device (wcb_paged_kv). Strides in elements; all 0:
+    [page][slot][head][head_dim] without gaps. Keeps addresses, not the memory."""
+
+    def __init__(self, k_ptr: int, v_ptr: int, dtype: int, n_pages: int, page_size: int, n_kv_heads: int,
+                 head_dim: int, page_stride: int = 0, token_stride: int = 0, head_stride: int = 0):
+        self._c = _PagedKV(C.sizeof(_PagedKV), dtype, n_kv_heads, head_dim, page_size, n_pages, k_ptr, v_ptr,
+                           page_stride, token_stride, head_stride)
+        self._at = C.addressof(self._c)
+
+
+class PagedBatch:
+    """The sequences of one step (wcb_paged_batch): device arrays q_start [n_seqs + 1],
+    kv_len [n_seqs] (new tokens included) and page_table [n_seqs][max_pages], all int32.
+    status_ptr: a device uint32 that collects PAGED_* bits (0: none)."""
+
+    def __init__(self, q_start_ptr: int, kv_len_ptr: int, page_table_ptr: int, n_seqs: int, n_tokens: int,
+                 max_q_len: int, max_pages: int, status_ptr: int = 0):
+        self._c = _PagedBatch(C.sizeof(_PagedBatch), n_seqs, n_tokens, max_q_len, max_pages, 0, q_start_ptr,
+                              kv_len_ptr, page_table_ptr, status_ptr or None)
+        self._at = C.addressof(self._c)
+
+
+class Rope:
+    """A rotation by position (wcb_rope): pairs (2i, 2i + 1) of the first rot_dim
+    dimensions, or (i, i + rot_dim / 2) with halves. inv_freq (rot_dim / 2 values)
+    replaces theta^(-2i / rot_dim)."""
+
+    def __init__(self, rot_dim: int, theta: float = 10000.0, halves: bool = False,
+                 inv_freq: Optional[Sequence[float]] = None):
+        self._c = _Rope()
+        _check(lib().wcb_rope_init(C.byref(self._c), rot_dim, theta, int(halves)))
+        if inv_freq is not None:
+            if len(inv_freq) != rot_dim // 2:
+                raise ValueError("inv_freq has rot_dim / 2 values")
+            self._c.inv_freq[: rot_dim // 2] = [float(f) for f in inv_freq]
+        self._at = C.addressof(self._c)
+
+
+def paged_append_dev(kv: PagedKV, batch: PagedBatch, rope: Optional[Rope], q_ptr: int, k_ptr: int, v_ptr: int,
+                     q_out_ptr: int, dtype: int, n_heads: int, q_stride: int, k_stride: int, v_stride: int,
+                     q_out_stride: int, q_norm_ptr: int = 0, k_norm_ptr: int = 0, eps: float = 1e-5,
+                     stream: int = 0) -> None:
+    """wcb_paged_append_dev: normalises (optional) and rotates the new tokens' queries and
+    keys, writes the queries to q_out and keys and values to their pages. dtype: KV_* of
+    q, k, v and q_out; strides between tokens in elements."""
+    _check(lib().wcb_paged_append_dev(kv._at, batch._at, rope._at if rope else None, q_ptr, k_ptr, v_ptr, q_out_ptr,
+                                     dtype, n_heads, q_stride, k_stride, v_stride, q_out_stride, q_norm_ptr,
+                                     k_norm_ptr, eps, stream))
+
+
+def paged_attention_workspace(kv: PagedKV, batch: PagedBatch, n_heads: int) -> int:
+    """Bytes of device workspace of a paged_attention_dev call with these arguments. Zero
+    its first 4096 bytes once; calls that may overlap on the GPU need one each."""
+    n = C.c_size_t(0)
+    _check(lib().wcb_paged_attention_workspace(kv._at, batch._at, n_heads, C.byref(n)))
+    return n.value
+
+
+def paged_attention_dev(kv: PagedKV, batch: PagedBatch, q_ptr: int, out_ptr: int, dtype: int, n_heads: int,
+                        q_stride: int, out_stride: int, workspace_ptr: int, workspace_bytes: int, scale: float = 0.0,
+                        window: int = 0, lse_ptr: int = 0, stream: int = 0) -> None:
+    """wcb_paged_attention_dev: the new tokens attend causally to their sequences' pages.
+    scale 0: 1 / sqrt(head_dim); window > 0: the last `window` keys only; lse_ptr: the
+    logarithm of each row's sum (f32 [n_tokens][n_heads]), 0 = not wanted."""
+    _check(lib().wcb_paged_attention_dev(kv._at, batch._at, q_ptr, out_ptr, dtype, n_heads, q_stride, out_stride,
+                                        workspace_ptr, workspace_bytes, scale, window, lse_ptr, stream))
+
+
+def spec_verify_dev(draft_ptr: int, draft_len_ptr: int, target_ptr: int, draft_probs_ptr: int, u_accept_ptr: int,
+                    u_sample_ptr: int, n_seqs: int, max_draft: int, vocab: int, tokens_ptr: int, accepted_ptr: int,
+                    target_seq_stride: int = 0, target_row_stride: int = 0, draft_seq_stride: int = 0,
+                    draft_row_stride: int = 0, status_ptr: int = 0, stream: int = 0) -> None:
+    """wcb_spec_verify_dev: accepts or replaces drafted tokens by the target's
+    probabilities. draft_len_ptr 0: max_draft each; draft_probs_ptr 0: the draft was
+    certain of its tokens; strides in elements, 0 = no gaps."""
+    _check(lib().wcb_spec_verify_dev(draft_ptr, draft_len_ptr, target_ptr, draft_probs_ptr, u_accept_ptr, u_sample_ptr,
+                                     n_seqs, max_draft, vocab, tokens_ptr, accepted_ptr, target_seq_stride,
+                                     target_row_stride, draft_seq_stride, draft_row_stride, status_ptr, stream))
 
 
 def tp_unique_id() -> bytes:
