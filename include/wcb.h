@@ -387,13 +387,15 @@ typedef struct wcb_paged_batch {
  * sequence is skipped). BAD_LEN: a new token's position is negative (not
  * stored; its attention output is zero). BAD_TOKEN: a drafted token outside the
  * vocabulary (turned down). BAD_PROBS: a row of target probabilities without
- * a positive finite value (the sampled token is -1). */
+ * a positive finite value (the sampled token is -1). ABORTED: a wait inside a
+ * kernel ran out; the call's outputs are not valid. */
 enum {
   WCB_PAGED_BAD_PAGE = 1,
   WCB_PAGED_BAD_ROWS = 2,
   WCB_PAGED_BAD_LEN = 4,
   WCB_PAGED_BAD_TOKEN = 8,
-  WCB_PAGED_BAD_PROBS = 16
+  WCB_PAGED_BAD_PROBS = 16,
+  WCB_PAGED_ABORTED = 32
 };
 
 /* Rotation of a head's first rot_dim dimensions (attention.rs:230-262 rotates

@@ -301,6 +301,38 @@ def test_long_sequences_and_repeatability(gpu, act, cache, heads, kv_heads, dim)
     assert (room[:4096] == 0).all()
 
 
+@pytest.mark.parametrize("act", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,dim,page,by_head", [(8, 1, 128, 64, False), (4, 4, 128, 16, True), (8, 2, 64, 48, False), (15, 5, 64, 1, True)])
+@pytest.mark.parametrize("q_len,kv_len,window", [([257], [2600], 0), ([129, 1, 300, 0, 64], [129, 70, 1500, 5, 640], 0), ([200, 333], [900, 333], 130)])
+def test_attention_of_long_chunks(gpu, act, heads, kv_heads, dim, page, by_head, q_len, kv_len, window):
+    s = Step(q_len, kv_len, heads, kv_heads, dim, act, act, page, by_head, seed=16, gap=8)
+    room = s.attend(window=window)
+    s.check(window=window)
+    first, lse = s.out.clone(), s.lse.clone()
+    for _ in range(3):
+        s.out.fill_(7.0)
+        s.attend(window=window, room=room)
+        assert torch.equal(first, s.out) and torch.equal(lse, s.lse)
+    assert (room[:4096] == 0).all()
+
+
+@pytest.mark.parametrize("act", ["f16", "bf16"])
+def test_growing_scores_rescale(gpu, act):
+    """Scores that grow along the keys by far more than 2^8: the sums are rescaled again and again."""
+    s = Step([140, 1], [900, 700], 4, 2, 64, act, act, 16, seed=17)
+    s.q.abs_()
+    for i in range(2):
+        sl = s.slots(i)
+        ramp = torch.linspace(-4, 4, len(sl))[:, None, None]
+        k = s.by_token(s.k.float().cpu())
+        k[sl] = k[sl] * 0.1 + ramp
+        s.k.copy_(k.t.transpose(1, 2) if s.by_head else k.t)
+    s.attend()
+    s.check()
+    s.attend(scale=-0.3)
+    s.check(scale=-0.3)
+
+
 def test_scale_and_large_scores(gpu):
     s = Step([3, 1], [100, 50], 8, 2, 64, "f32", "f32", 16, seed=11)
     s.attend(scale=-3.0)

@@ -107,12 +107,30 @@ uint32_t check_rows(const void* p, uint64_t stride, uint64_t width, uint32_t dty
   return WCB_OK;
 }
 
-// Rows (new tokens * rep) of a CTA of the mma.sync kernel: the smallest block that holds the
-// longest sequence's, so that no multiplication is spent on rows that are not there.
-int block_rows(uint64_t max_rows) { return max_rows <= 16 ? 16 : max_rows <= 32 ? 32 : 64; }
+// Which kernels a call runs, from what the host knows: the types and the longest sequence's rows
+// (new tokens * rep). 16-bit types: sequences of more than TC_MIN rows go to the tensor-core kernel,
+// the others of the batch to the mma.sync kernel. Its row block is the smallest that holds
+// the longest sequence's rows, so that no product is spent on rows that are not there.
+constexpr uint64_t TC_MIN = 64;
+struct Plan {
+  int rows;     // row block of the mma.sync kernel, 0: not run
+  bool tc;
+  int split;    // sequences of more rows are the tensor-core kernel's
+};
+Plan plan(uint32_t dtype, uint64_t n_seqs, uint64_t max_rows) {
+  Plan p{};
+  p.tc = dtype != WCB_KV_F32 && max_rows > TC_MIN;
+  p.split = p.tc ? (n_seqs == 1 ? 0 : int(TC_MIN)) : INT_MAX;
+  const uint64_t r = p.tc ? (n_seqs == 1 ? 0 : TC_MIN) : max_rows;
+  p.rows = r == 0 ? 0 : r <= 16 ? 16 : r <= 32 ? 32 : 64;
+  return p;
+}
 
-size_t workspace_bytes(int rows, int head_dim) {
-  return TICKET_BYTES + sizeof(float) * size_t(ATTEND_CTAS) * 2 * size_t(rows) * size_t(head_dim + 2);
+// the kernels of a call run one after the other and share the pieces' memory
+size_t workspace_bytes(const Plan& p, int head_dim) {
+  const size_t row = sizeof(float) * 2 * size_t(head_dim + 2);
+  const size_t x = size_t(ATTEND_CTAS) * size_t(p.rows) * row, y = p.tc ? size_t(TC_CTAS) * TC_ROWS * row : 0;
+  return TICKET_BYTES + (x > y ? x : y);
 }
 
 }  // namespace
@@ -188,7 +206,11 @@ uint32_t wcb_paged_attention_workspace(const wcb_paged_kv* kv, const wcb_paged_b
   if (rc != WCB_OK) return rc;
   if (n_heads == 0 || n_heads > 4096 || n_heads % kv->n_kv_heads || n_heads / kv->n_kv_heads > 64)
     return bad("Invalid tensor shape: need n_heads % n_kv_heads == 0 (<= 64 per kv head)");
-  *bytes = workspace_bytes(block_rows(uint64_t(batch->max_q_len) * (n_heads / kv->n_kv_heads)), pool.head_dim);
+  const uint64_t rows = uint64_t(batch->max_q_len) * (n_heads / kv->n_kv_heads);
+  // the activations' type is not known here: the larger of the two
+  const size_t x = workspace_bytes(plan(WCB_KV_F32, batch->n_seqs, rows), pool.head_dim);
+  const size_t y = kv->dtype == WCB_KV_F32 ? 0 : workspace_bytes(plan(kv->dtype, batch->n_seqs, rows), pool.head_dim);
+  *bytes = x > y ? x : y;
   return WCB_OK;
 }
 
@@ -221,14 +243,21 @@ uint32_t wcb_paged_attention_dev(const wcb_paged_kv* kv, const wcb_paged_batch* 
   a.n_heads = int(n_heads);
   a.rep = int(n_heads / kv->n_kv_heads);
   a.window = int(window);
-  a.row_lo = 0;
-  a.row_hi = INT_MAX;
   a.tickets = static_cast<int*>(workspace);
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + TICKET_BYTES);
-  const int rows = block_rows(uint64_t(batch->max_q_len) * uint64_t(a.rep));
+  const Plan p = plan(dtype, batch->n_seqs, uint64_t(batch->max_q_len) * uint64_t(a.rep));
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = dtype == WCB_KV_F32 ? launch_attend_32(a, int(kv->dtype), rows, s)
-                                            : launch_attend_16(a, int(dtype), rows, s);
+  cudaError_t e = cudaSuccess;
+  if (p.tc) {
+    a.row_lo = p.split;
+    a.row_hi = INT_MAX;
+    e = launch_attend_tc(a, int(dtype), s);
+  }
+  if (p.rows && e == cudaSuccess) {
+    a.row_lo = 0;
+    a.row_hi = p.split;
+    e = dtype == WCB_KV_F32 ? launch_attend_32(a, int(kv->dtype), p.rows, s) : launch_attend_16(a, int(dtype), p.rows, s);
+  }
   return cuda_result(e, "paged attention");
 }
 

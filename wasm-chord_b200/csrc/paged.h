@@ -10,7 +10,7 @@ namespace wcb {
 namespace paged {
 
 enum { E_F32 = 0, E_F16 = 1, E_BF16 = 2 };  // element types (WCB_KV_*)
-enum { ST_BAD_PAGE = 1, ST_BAD_ROWS = 2, ST_BAD_LEN = 4, ST_BAD_TOKEN = 8, ST_BAD_PROBS = 16 };
+enum { ST_BAD_PAGE = 1, ST_BAD_ROWS = 2, ST_BAD_LEN = 4, ST_BAD_TOKEN = 8, ST_BAD_PROBS = 16, ST_ABORTED = 32 };
 
 // pool and batch as the kernels see them (wcb_paged_kv, wcb_paged_batch)
 struct Pool {
@@ -67,11 +67,15 @@ struct VerifyArgs {
 // Work of an attention call is cut into at most this many equal parts, one per
 // CTA (2 CTAs on each of 148 SMs); a part leaves at most two partial results.
 constexpr int ATTEND_CTAS = 296;
+constexpr int TC_CTAS = 148;      // parts of the tensor-core kernel: one CTA on each SM
+constexpr int TC_ROWS = 256;      // rows of its CTA
+constexpr int TC_TICKETS = 512;   // its first ticket, two a CTA
 constexpr size_t TICKET_BYTES = 4096;
 
 cudaError_t launch_append(const AppendArgs& a, int act, int cache, cudaStream_t s);
 cudaError_t launch_attend_16(const AttendArgs& a, int act, int rows, cudaStream_t s);
 cudaError_t launch_attend_32(const AttendArgs& a, int cache, int rows, cudaStream_t s);
+cudaError_t launch_attend_tc(const AttendArgs& a, int act, cudaStream_t s);
 cudaError_t launch_verify(const VerifyArgs& a, cudaStream_t s);
 
 }  // namespace paged

@@ -1,0 +1,683 @@
+// Attention of many new rows over a paged cache on the 5th-generation tensor
+// cores, 16-bit activations and cache (the formulas and the line of tiles:
+// paged_attn.cuh; here M = 256 rows and TK = 128 keys).
+//
+// One CTA per SM holds two tiles of 128 rows (row = token * rep + head), each with
+// a warpgroup for its softmax (one thread a row: no shuffles) and a thread that
+// issues its products; both share the K and V tiles that four loader warps bring
+// in by 16-byte cp.async through a ring of tiles in shared memory (a page may hold
+// any number of tokens and end anywhere inside a tile, which a box of a tensor
+// map could not follow). Per tile of keys:
+//   S = Q K^T      tcgen05.mma, both operands from shared memory, S in TMEM (f32)
+//   P = 2^(S - m)  read from TMEM, rounded to 16 bits, written back over S
+//   O += P V       tcgen05.mma, P from TMEM, V as it lies ([key][dim]: N-major)
+// The products of one tile of rows run while the other's softmax does: 128 x 128
+// exponentials at 16 a clock take as long as the tile's two products, so each of
+// the two units is the other's bound. The running maximum moves only when it grows
+// by more than 2^8 (O in TMEM is rescaled then; sums in f32 and P in 16 bits have
+// room for that factor), which is rare after the first tiles.
+// TMEM: S0 | S1 | O0 | O1, 512 columns at head_dim 128.
+#include "paged_attn.cuh"
+
+namespace wcb {
+namespace paged {
+namespace {
+
+constexpr int TC_THREADS = 448;  // 2 softmax warpgroups, 4 loader warps, 2 issuing warps
+constexpr int TC_TK = 128;
+constexpr int TC_M = 256;
+constexpr int TILE_PANEL = 128 * 128;  // bytes of 128 rows x 64 dims
+constexpr int HOLE_RING = 8;   // tiles: the loaders are at most 4 ahead of the softmax
+constexpr int ODD_RING = 16;   // units, likewise
+
+template <int HD>
+struct TcCfg {
+  static constexpr int PANELS = HD / 64;
+  static constexpr int TILE = PANELS * TILE_PANEL;  // bytes of 128 rows x HD
+  static constexpr int SLOTS = HD == 128 ? 4 : 6;   // K and V tiles in the ring
+  static constexpr int Q = 0;                       // two tiles of queries
+  static constexpr int RING = 2 * TILE;
+  static constexpr int OFFS = RING + SLOTS * TILE;  // [2][128] row offsets (64 bits)
+  static constexpr int BARS = OFFS + 2 * 128 * 8;
+  static constexpr int SMEM = BARS + 512 + 1024;    // + alignment to 1024
+};
+
+__device__ __forceinline__ uint64_t desc_kmajor(uint32_t addr) {
+  // 128-byte swizzle, rows of 128 bytes, 8-row groups 1024 bytes apart
+  return uint64_t((addr >> 4) & 0x3FFF) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
+         (uint64_t(2) << 61);
+}
+__device__ __forceinline__ uint64_t desc_nmajor(uint32_t addr) {
+  // the same tile read along its keys: 64-dim panels apart by TILE_PANEL, 8-key groups by 1024 bytes
+  return uint64_t((addr >> 4) & 0x3FFF) | (uint64_t(TILE_PANEL >> 4) << 16) | (uint64_t(1024 >> 4) << 32) |
+         (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+template <typename T>
+constexpr uint32_t idesc(int n, bool b_nmajor) {
+  const uint32_t f = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  return (1u << 4) | (f << 7) | (f << 10) | (b_nmajor ? 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(id), "r"(acc), "r"(0)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(id), "r"(acc), "r"(0)
+      : "memory");
+}
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+      "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+      "r"(r[31])
+      : "memory");
+}
+
+struct TcShared {
+  uint64_t full[8], empty[8];  // ring slots
+  uint64_t q_full[2], s_full[2], p_full[2], o_done[2];
+  uint64_t offs_full, piece_full[2], last_full[2];
+  uint32_t tmem;
+  int abort;                     // a wait ran out: everybody leaves
+  uint32_t holes[HOLE_RING][4];  // keys of a tile without a page
+  int odd[ODD_RING];             // by item: a ragged tile has infinities or NaN among its values
+  int last[2];
+  long long scan[16], place[2];
+};
+
+// Bounded wait: about 2^24 polls, or until another thread has given up.
+__device__ __forceinline__ bool tc_wait(TcShared* sh, uint64_t* bar, uint32_t parity) {
+  const uint32_t addr = smem_u32(bar);
+  for (uint32_t it = 0; it < (1u << 24); ++it) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((it & 63) == 63 && *reinterpret_cast<volatile int*>(&sh->abort)) return false;
+  }
+  *reinterpret_cast<volatile int*>(&sh->abort) = 1;
+  return false;
+}
+
+// the same for a whole warp, which goes on or leaves together
+__device__ __forceinline__ bool tc_wait_warp(TcShared* sh, uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, tc_wait(sh, bar, parity));
+}
+
+// The units of this CTA, walked by every role by itself.
+struct Walk {
+  Place pl;
+  long long at, unit0;
+  int s, kvh, rb, rows, table;
+  Seq sq;
+  Block blk;
+  int ta, tb;  // tiles of the current unit
+
+  __device__ __forceinline__ void start(const AttendArgs& a, const Place& p) {
+    pl = p;
+    table = table_tokens(a.pool, a.batch);
+    s = pl.seq;
+    sq = read_seq(a.batch, s);
+    rows = seq_rows(a, sq);
+    at = pl.begin;
+    const long long ht = head_tiles(a, sq, TC_M, TC_TK, table);
+    kvh = int((at - pl.seq_begin) / ht);
+    unit0 = pl.seq_begin + kvh * ht;
+    for (rb = 0;; ++rb) {
+      blk = row_block(a, sq, rows, rb, TC_M, TC_TK, table);
+      if (at < unit0 + blk.tiles) break;
+      unit0 += blk.tiles;
+    }
+    cut();
+  }
+  __device__ __forceinline__ void cut() {
+    ta = int(at - unit0);
+    tb = int(min(static_cast<long long>(blk.tiles), pl.end - unit0));
+  }
+  __device__ __forceinline__ bool next(const AttendArgs& a) {
+    at = unit0 + tb;
+    if (at >= pl.end) return false;
+    unit0 += blk.tiles;
+    ++rb;
+    if (rb * TC_M >= rows) {
+      rb = 0;
+      if (++kvh == a.pool.n_kv) {
+        kvh = 0;
+        do {
+          ++s;
+          sq = read_seq(a.batch, s);
+          rows = seq_rows(a, sq);
+        } while (rows == 0);
+      }
+    }
+    blk = row_block(a, sq, rows, rb, TC_M, TC_TK, table);
+    cut();
+    return true;
+  }
+  // tiles [ta, end) that rows 128 w .. of the block need (those after end see nothing); at least
+  // one, so that rows without a key are written too; 0: there are no such rows
+  __device__ __forceinline__ int end_of(const AttendArgs& a, int w) const {
+    const int r0 = rb * TC_M + 128 * w;
+    if (r0 >= rows) return ta;
+    const int r1 = min(rows, r0 + 128);
+    const int hi = min(sq.kv - sq.n + (r1 - 1) / a.rep + 1, table);
+    const int t = (max(hi, 0) + TC_TK - 1) / TC_TK - blk.tile0;
+    return max(min(t, tb), ta + 1);
+  }
+  // some key of the tile is seen by some rows of the block and not by others, or by none
+  __device__ __forceinline__ bool ragged(const AttendArgs& a, int i) const {
+    const int key0 = (blk.tile0 + i) * TC_TK;
+    return key0 + TC_TK > min(blk.hi, blk.pos0 + 1) || key0 < blk.lo || (a.window > 0 && key0 < blk.pos1 - a.window + 1);
+  }
+  __device__ __forceinline__ long long key_offset(const AttendArgs& a, int key, bool& hole) const {
+    hole = false;
+    if (key < blk.lo || key >= blk.hi) return -1;
+    const int page = __ldg(a.batch.page_table + int64_t(s) * a.batch.max_pages + key / a.pool.page_size);
+    if (page < 0 || page >= a.pool.n_pages) {
+      hole = true;
+      return -1;
+    }
+    return page * a.pool.page_stride + int64_t(key % a.pool.page_size) * a.pool.token_stride;
+  }
+};
+
+// byte offset of 16-byte chunk ch of row r in a swizzled tile
+__device__ __forceinline__ uint32_t tile_at(int r, int ch) {
+  return uint32_t((ch >> 3) * TILE_PANEL + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
+}
+
+template <typename T>
+__device__ __forceinline__ bool finite16(uint32_t w) {  // both halves
+  constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+  return (w & E) != E && ((w >> 16) & E) != E;
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(const __grid_constant__ AttendArgs a) {
+  using L = TcCfg<HD>;
+  constexpr int NS = L::SLOTS, CH = HD / 8;
+  extern __shared__ uint8_t raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  __shared__ TcShared sh;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t sbase = smem_u32(sm);
+
+  const Place pl = find_place<TC_THREADS>(a, TC_M, TC_TK, sh.scan, sh.place);
+  if (pl.begin >= pl.end) return;  // the whole CTA; nothing is held yet
+
+  if (tid == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&sh.full[i], 128);
+      mbar_init(&sh.empty[i], 2);
+    }
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(&sh.q_full[w], 128);
+      mbar_init(&sh.s_full[w], 1);
+      mbar_init(&sh.p_full[w], 128);
+      mbar_init(&sh.o_done[w], 1);
+      mbar_init(&sh.piece_full[w], 128);
+      mbar_init(&sh.last_full[w], 1);
+    }
+    mbar_init(&sh.offs_full, 128);
+    sh.abort = 0;
+    mbar_fence_init();
+  }
+  if (tid < ODD_RING) sh.odd[tid] = 0;
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  Walk wk;
+  wk.start(a, pl);
+
+  if (warp >= 12) {
+    // ---- issuing warps: products of row tile w --------------------------------
+    if (lane == 0) {
+      const int w = warp - 12;
+      const uint32_t ts = tmem + 128 * w, to = tmem + 256 + 128 * w;
+      const uint32_t qa = sbase + L::Q + w * L::TILE;
+      constexpr uint32_t ID_S = idesc<T>(128, false), ID_O = idesc<T>(HD, true);
+      uint32_t n = 0;                // ring tiles so far
+      uint32_t it = 0, steps = 0;    // items, and products P V so far
+      bool ok = true;
+      do {
+        const int end = wk.end_of(a, w);
+        if (end > wk.ta) ok = ok && tc_wait(&sh, &sh.q_full[w], it & 1);
+        for (int i = wk.ta; i < wk.tb && ok; ++i) {
+          const uint32_t sk = n % NS, fk = (n / NS) & 1, sv = (n + 1) % NS, fv = ((n + 1) / NS) & 1;
+          n += 2;
+          ok = tc_wait(&sh, &sh.full[sk], fk);
+          if (!ok) break;
+          if (i < end) {
+            // S lies over the last P: its product has to be done
+            if (i > wk.ta) ok = tc_wait(&sh, &sh.o_done[w], (steps - 1) & 1);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t kb = sbase + L::RING + sk * L::TILE;
+#pragma unroll
+            for (int k = 0; k < HD / 16; ++k) {
+              const uint32_t o = (k / 4) * TILE_PANEL + (k % 4) * 32;
+              mma_ss(ts, desc_kmajor(qa + o), desc_kmajor(kb + o), ID_S, k > 0);
+            }
+            tc_commit(&sh.s_full[w]);
+            tc_commit(&sh.empty[sk]);
+            ok = tc_wait(&sh, &sh.p_full[w], steps & 1) && tc_wait(&sh, &sh.full[sv], fv);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t vb = sbase + L::RING + sv * L::TILE;
+#pragma unroll
+            for (int k = 0; k < TC_TK / 16; ++k)
+              mma_ts(to, ts + 8 * k, desc_nmajor(vb + k * 2048), ID_O, i > wk.ta || k > 0);
+            tc_commit(&sh.o_done[w]);
+            tc_commit(&sh.empty[sv]);
+            ++steps;
+          } else {
+            bar_arrive(&sh.empty[sk]);
+            ok = tc_wait(&sh, &sh.full[sv], fv);
+            if (!ok) break;
+            bar_arrive(&sh.empty[sv]);
+          }
+        }
+        if (end > wk.ta) ++it;
+      } while (ok && wk.next(a));
+    }
+    __syncwarp();
+  } else if (warp >= 8) {
+    // ---- loaders --------------------------------------------------------------
+    const int lt = tid - 256;
+    long long* offs = reinterpret_cast<long long*>(sm + L::OFFS);
+    uint32_t n = 0, tiles = 0, item = 0;
+    constexpr int LAG = NS - 2;  // groups in flight
+    bool ok = true, holes_seen = false;
+    // what has to be looked at when tile n's copies have landed: values of a ragged tile
+    uint32_t odd_bits = 0;  // bit (n % 32): search ring tile n
+    uint32_t item_of[4] = {0, 0, 0, 0};
+    auto landed = [&](uint32_t m) {  // ring tile m is complete in this thread's view
+      const uint32_t sl = m % NS;
+      if ((odd_bits >> (m & 31)) & 1) {
+        uint8_t* t = sm + L::RING + sl * L::TILE;
+        bool odd = false;
+        for (int c = lt; c < 128 * CH; c += 128) {
+          uint4* x = reinterpret_cast<uint4*>(t + tile_at(c / CH, c % CH));
+          uint4 v = *x;
+          if (!(finite16<T>(v.x) && finite16<T>(v.y) && finite16<T>(v.z) && finite16<T>(v.w))) {
+            odd = true;
+            T e[8];
+            *reinterpret_cast<uint4*>(e) = v;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (!(fabsf(to_f32(e[j])) <= FLT_MAX)) e[j] = from_f32<T>(0.0f);
+            *x = *reinterpret_cast<const uint4*>(e);
+          }
+        }
+        if (odd) sh.odd[item_of[(m >> 1) & 3] % ODD_RING] = 1;
+      }
+      fence_proxy_async();
+      bar_arrive(&sh.full[sl]);
+    };
+    do {
+      if (lt == 0) sh.odd[(item + ODD_RING / 2) % ODD_RING] = 0;
+      const bool many = wk.blk.pos1 > wk.blk.pos0;
+      for (int i = wk.ta; i < wk.tb && ok; ++i, ++tiles) {
+        bool hole;
+        const long long off = wk.key_offset(a, (wk.blk.tile0 + i) * TC_TK + lt, hole);
+        const unsigned hb = __ballot_sync(0xffffffffu, hole);
+        offs[(tiles & 1) * 128 + lt] = off;
+        if (lane == 0) sh.holes[tiles % HOLE_RING][warp - 8] = hb;
+        holes_seen |= hole;
+        bar_arrive(&sh.offs_full);
+        ok = tc_wait_warp(&sh, &sh.offs_full, tiles & 1);
+        const long long* ro = offs + (tiles & 1) * 128;
+#pragma unroll 1
+        for (int kvi = 0; kvi < 2; ++kvi, ++n) {
+          const uint32_t sl = n % NS;
+          if (n >= NS && ok) ok = tc_wait_warp(&sh, &sh.empty[sl], ((n / NS) - 1) & 1);
+          if (!ok) break;
+          const T* base = static_cast<const T*>(kvi ? a.pool.v : a.pool.k) + wk.kvh * a.pool.head_stride;
+          const uint32_t dst = sbase + L::RING + sl * L::TILE;
+#pragma unroll 8
+          for (int c = lt; c < 128 * CH; c += 128) {
+            const int r = c / CH, ch = c % CH;
+            const long long o = ro[r];
+            cp16(dst + tile_at(r, ch), base + (o < 0 ? 0 : o) + ch * 8, o >= 0);
+          }
+          cp_commit();
+          odd_bits &= ~(1u << (n & 31));
+          if (kvi && many && wk.ragged(a, i)) odd_bits |= 1u << (n & 31);
+          item_of[(n >> 1) & 3] = item;
+          if (n >= LAG) {
+            cp_wait<LAG>();
+            landed(n - LAG);
+          }
+        }
+      }
+      ++item;
+    } while (ok && wk.next(a));
+    cp_wait<0>();
+    if (ok)
+      for (uint32_t m = n >= uint32_t(LAG) ? n - LAG : 0; m < n; ++m) landed(m);
+    if (holes_seen) report(a.batch, ST_BAD_PAGE);
+  } else {
+    // ---- softmax of row tile w: thread = row ----------------------------------
+    const int w = warp >> 2, row = tid & 127;
+    const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16;
+    const uint32_t ts = tmem + lanes + 128 * w, to = tmem + lanes + 256 + 128 * w;
+    uint32_t tiles = 0, steps = 0, item = 0, cuts = 0;
+    bool ok = true;
+    do {
+      const int r0 = wk.rb * TC_M + 128 * w, rn = min(128, wk.rows - r0);
+      const int end = wk.end_of(a, w);
+      if (end > wk.ta) {
+        // queries into shared memory; rows that are not there are zeros
+        uint8_t* qt = sm + L::Q + w * L::TILE;
+#pragma unroll 4
+        for (int c = row; c < 128 * CH; c += 128) {
+          const int r = c / CH, ch = c % CH;
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (r < rn) {
+            const int gr = r0 + r;
+            v = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (wk.sq.r0 + gr / a.rep) * a.q_stride +
+                                                     (wk.kvh * a.rep + gr % a.rep) * HD + ch * 8));
+          }
+          *reinterpret_cast<uint4*>(qt + tile_at(r, ch)) = v;
+        }
+        fence_proxy_async();
+        bar_arrive(&sh.q_full[w]);
+
+        const int gr = r0 + min(row, rn - 1);
+        const int pos = wk.sq.kv - wk.sq.n + gr / a.rep;
+        const int khi = min(pos + 1, wk.table), klo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+        float m = -INFINITY, l = 0.0f;  // m: the maximum that O and l are scaled by
+        for (int i = wk.ta; i < end && ok; ++i) {
+          const uint32_t* holes = sh.holes[(tiles + (i - wk.ta)) % HOLE_RING];
+          ok = tc_wait_warp(&sh, &sh.s_full[w], steps & 1);
+          if (!ok) break;
+          tc_fence_after();
+          const int key0 = (wk.blk.tile0 + i) * TC_TK;
+          const bool gaps = (holes[0] | holes[1] | holes[2] | holes[3]) != 0;
+          const bool mask = gaps || wk.ragged(a, i);
+          // bit c: key key0 + c is seen
+          const int lo = max(0, min(128, klo - key0)), hi = max(0, min(128, khi - key0));
+          uint32_t seen[4];
+          if (mask) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int b0 = max(0, min(32, lo - 32 * q)), b1 = max(0, min(32, hi - 32 * q));
+              const uint32_t below1 = b1 >= 32 ? 0xffffffffu : (1u << b1) - 1u, below0 = b0 >= 32 ? 0xffffffffu : (1u << b0) - 1u;
+              seen[q] = below1 & ~below0 & ~holes[q];
+            }
+          }
+          float top = -INFINITY;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t v[32];
+            tmem_ld32(ts + 32 * q, v);
+            tmem_wait_ld();
+            if (mask) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (!((seen[q] >> e) & 1)) v[e] = 0xff800000u;
+            }
+            float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              t0 = fmaxf(t0, __uint_as_float(v[e]));
+              t1 = fmaxf(t1, __uint_as_float(v[e + 1]));
+            }
+            top = fmaxf(top, fmaxf(t0, t1));
+          }
+          // a negative scale turns the order round: the largest product is then the smallest score
+          top = a.scale_log2 >= 0.0f ? top * a.scale_log2 : top;
+          if (a.scale_log2 < 0.0f) {
+            top = -INFINITY;
+#pragma unroll 1
+            for (int q = 0; q < 4; ++q) {
+              uint32_t v[32];
+              tmem_ld32(ts + 32 * q, v);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (!mask || ((seen[q] >> e) & 1)) top = fmaxf(top, __uint_as_float(v[e]) * a.scale_log2);
+            }
+          }
+          // rescale where some row's maximum grew by more than 2^8
+          const bool grow = top > m + 8.0f;  // also the first finite one
+          if (__any_sync(0xffffffffu, grow)) {
+            const float nm = fmaxf(m, top);
+            const float f = m == nm ? 1.0f : fast_exp2(m - (nm == -INFINITY ? 0.0f : nm));
+            if (i > wk.ta) {  // the last product is done: S was issued after it
+#pragma unroll 1
+              for (int q = 0; q < HD / 32; ++q) {
+                uint32_t v[32];
+                tmem_ld32(to + 32 * q, v);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+                tmem_st32(to + 32 * q, v);
+              }
+            }
+            l *= f;
+            m = nm;
+          }
+          const float use = m == -INFINITY ? 0.0f : m;
+          float l0 = 0.0f, l1 = 0.0f;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t v[32], p[16];
+            tmem_ld32(ts + 32 * q, v);
+            tmem_wait_ld();
+            if (mask) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                const float x = __uint_as_float(v[e]) * a.scale_log2;
+                v[e] = __float_as_uint(((seen[q] >> e) & 1) ? fast_exp2(x - use) : 0.0f);
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(fast_exp2(fmaf(__uint_as_float(v[e]), a.scale_log2, -use)));
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float x = __uint_as_float(v[2 * e]), y = __uint_as_float(v[2 * e + 1]);
+              l0 += x;
+              l1 += y;
+              p[e] = pack2<T>(x, y);
+            }
+            tmem_st16(ts + 16 * q, p);
+          }
+          l += l0 + l1;
+          tmem_wait_st();
+          tc_fence_before();
+          bar_arrive(&sh.p_full[w]);
+          ++steps;
+        }
+        if (ok) ok = tc_wait_warp(&sh, &sh.o_done[w], (steps - 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+
+        // results: normalised, or a piece [HD][256] + m [256] + l [256]
+        const bool whole = wk.ta == 0 && wk.tb == wk.blk.tiles;
+        constexpr size_t PIECE = size_t(TC_M) * (HD + 2);
+        float* piece = a.part + (size_t(blockIdx.x) * 2 + (wk.ta == 0 ? 1 : 0)) * PIECE + 128 * w + row;
+        const bool odd = *reinterpret_cast<volatile int*>(&sh.odd[item % ODD_RING]) != 0;
+        const int64_t tok = wk.sq.r0 + gr / a.rep;
+        const int hh = wk.kvh * a.rep + gr % a.rep;
+        const bool some = l > 0.0f || l != l;
+        const float inv = some ? 1.0f / l : 0.0f;
+        T* dst = static_cast<T*>(a.out) + tok * a.out_stride + hh * HD;
+#pragma unroll 1
+        for (int q = 0; q < HD / 32; ++q) {
+          uint32_t v[32];
+          tmem_ld32(to + 32 * q, v);
+          tmem_wait_ld();
+          if (odd) {
+            // infinities and NaN that were taken out of ragged tiles, for the rows that see them
+#pragma unroll 1
+            for (int i = wk.ta; i < end; ++i) {
+              if (!wk.ragged(a, i)) continue;
+              const int k0 = (wk.blk.tile0 + i) * TC_TK;
+#pragma unroll 1
+              for (int key = max(k0, klo); key < min(k0 + TC_TK, khi); ++key) {
+                bool hole;
+                const long long off = wk.key_offset(a, key, hole);
+                if (off < 0) continue;
+                const T* vp = static_cast<const T*>(a.pool.v) + wk.kvh * a.pool.head_stride + off + 32 * q;
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                  const float x = to_f32(vp[e]);
+                  if (!(fabsf(x) <= FLT_MAX)) v[e] = __float_as_uint(__uint_as_float(v[e]) + x);
+                }
+              }
+            }
+          }
+          if (row < rn) {
+            if (whole) {
+              float x[32];
+#pragma unroll
+              for (int e = 0; e < 32; ++e) x[e] = some ? __uint_as_float(v[e]) * inv : 0.0f;
+              store_vec<T, 32>(dst + 32 * q, x);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) piece[size_t(32 * q + e) * TC_M] = __uint_as_float(v[e]);
+            }
+          }
+        }
+        tc_fence_before();
+        if (row < rn) {
+          if (whole) {
+            if (a.lse) a.lse[tok * a.n_heads + hh] = some ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
+          } else {
+            piece[size_t(HD) * TC_M] = m;
+            piece[size_t(HD + 1) * TC_M] = l;
+          }
+        }
+        if (row == 0 && w == 0) {
+          uint32_t bits = 0;
+          if (wk.blk.pos1 >= wk.table) bits |= ST_BAD_PAGE;
+          if (wk.blk.pos0 < 0) bits |= ST_BAD_LEN;
+          report(a.batch, bits);
+        }
+      }
+      if (end > wk.ta && !(wk.ta == 0 && wk.tb == wk.blk.tiles)) {
+        // the last of the unit's CTAs joins this tile's pieces, in their order
+        const int c0 = int(wk.unit0 / wk.pl.per), c1 = int((wk.unit0 + wk.blk.tiles - 1) / wk.pl.per);
+        __threadfence();
+        bar_arrive(&sh.piece_full[w]);
+        ok = tc_wait_warp(&sh, &sh.piece_full[w], cuts & 1);
+        if (!ok) break;
+        if (row == 0) {
+          sh.last[w] = atomicInc(reinterpret_cast<unsigned*>(a.tickets) + TC_TICKETS + 2 * c0 + w, unsigned(c1 - c0)) == unsigned(c1 - c0);
+          bar_arrive(&sh.last_full[w]);
+        }
+        ok = tc_wait_warp(&sh, &sh.last_full[w], cuts & 1);
+        if (!ok) break;
+        ++cuts;
+        if (sh.last[w] && row < rn) {
+          __threadfence();
+          constexpr size_t PIECE = size_t(TC_M) * (HD + 2);
+          auto part = [&](int p) { return a.part + (size_t(p) * 2 + (p == c0 ? 1 : 0)) * PIECE + 128 * w + row; };
+          float m = -INFINITY;
+          for (int p = c0; p <= c1; ++p) m = fmaxf(m, __ldcg(part(p) + size_t(HD) * TC_M));
+          const float u = m == -INFINITY ? 0.0f : m;
+          float l = 0.0f;
+          for (int p = c0; p <= c1; ++p) l += fast_exp2(__ldcg(part(p) + size_t(HD) * TC_M) - u) * __ldcg(part(p) + size_t(HD + 1) * TC_M);
+          const bool some = l > 0.0f || l != l;
+          const float inv = some ? 1.0f / l : 0.0f;
+          const int gr = r0 + row;
+          const int64_t tok = wk.sq.r0 + gr / a.rep;
+          const int hh = wk.kvh * a.rep + gr % a.rep;
+          T* dst = static_cast<T*>(a.out) + tok * a.out_stride + hh * HD;
+#pragma unroll 1
+          for (int q = 0; q < HD / 32; ++q) {
+            float x[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] = 0.0f;
+            for (int p = c0; p <= c1; ++p) {
+              const float* pp = part(p);
+              const float f = fast_exp2(__ldcg(pp + size_t(HD) * TC_M) - u);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) x[e] += f * __ldcg(pp + size_t(32 * q + e) * TC_M);
+            }
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] = some ? x[e] * inv : 0.0f;
+            store_vec<T, 32>(dst + 32 * q, x);
+          }
+          if (a.lse) a.lse[tok * a.n_heads + hh] = some ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
+        }
+      }
+      tiles += uint32_t(wk.tb - wk.ta);
+      ++item;
+    } while (ok && wk.next(a));
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (tid == 0 && sh.abort) report(a.batch, ST_ABORTED);
+  if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+template <typename T, int HD>
+cudaError_t run_tc(const AttendArgs& a, cudaStream_t s) {
+  using L = TcCfg<HD>;
+  static_assert(L::SMEM + sizeof(TcShared) <= 227 * 1024, "shared memory");
+  cudaError_t e = cudaFuncSetAttribute(attend_tc_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+  if (e != cudaSuccess) return e;
+  attend_tc_kernel<T, HD><<<TC_CTAS, TC_THREADS, L::SMEM, s>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_attend_tc(const AttendArgs& a, int act, cudaStream_t s) {
+  if (act == E_F16) return a.pool.head_dim == 64 ? run_tc<__half, 64>(a, s) : run_tc<__half, 128>(a, s);
+  return a.pool.head_dim == 64 ? run_tc<__nv_bfloat16, 64>(a, s) : run_tc<__nv_bfloat16, 128>(a, s);
+}
+
+}  // namespace paged
+}  // namespace wcb

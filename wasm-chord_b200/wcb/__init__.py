@@ -35,6 +35,7 @@ PAGED_BAD_ROWS = 2
 PAGED_BAD_LEN = 4
 PAGED_BAD_TOKEN = 8
 PAGED_BAD_PROBS = 16
+PAGED_ABORTED = 32
 
 EXPORTED = [
     "wcb_gen_config_default", "wcb_model_load", "wcb_model_free", "wcb_model_config_get", "wcb_forward",
