@@ -138,12 +138,57 @@ __device__ __forceinline__ int seq_rows(const AttendArgs& a, const Seq& q) {
   const long long r = static_cast<long long>(q.n) * a.rep;
   return r > a.row_lo && r <= a.row_hi ? int(r) : 0;
 }
-// tiles of one key head of sequence s
-__device__ __forceinline__ long long head_tiles(const AttendArgs& a, const Seq& q, int M, int TK, int table) {
+// Tiles of one key head of a sequence; a whole warp, its lanes over the row blocks (a chunk
+// of a few thousand tokens has dozens, and every CTA of a call counts them).
+__device__ __forceinline__ long long head_tiles(const AttendArgs& a, const Seq& q, int rows, int M, int TK, int table) {
+  long long n = 0;
+  for (int rb = threadIdx.x & 31; rb * M < rows; rb += 32) n += row_block(a, q, rows, rb, M, TK, table).tiles;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  return n;
+}
+// The same for 32 sequences, one of each lane: those of one or two row blocks by their lane, the
+// others one after the other by the warp.
+__device__ __forceinline__ long long lane_tiles(const AttendArgs& a, const Seq& q, int M, int TK, int table) {
   const int rows = seq_rows(a, q);
   long long n = 0;
-  for (int rb = 0; rb * M < rows; ++rb) n += row_block(a, q, rows, rb, M, TK, table).tiles;
+  if (rows > 0 && rows <= 2 * M) {
+    n = row_block(a, q, rows, 0, M, TK, table).tiles;
+    if (rows > M) n += row_block(a, q, rows, 1, M, TK, table).tiles;
+  }
+  for (unsigned left = __ballot_sync(0xffffffffu, rows > 2 * M); left; left &= left - 1) {
+    const int src = __ffs(int(left)) - 1;
+    Seq w;
+    w.n = __shfl_sync(0xffffffffu, q.n, src);
+    w.kv = __shfl_sync(0xffffffffu, q.kv, src);
+    w.r0 = 0;
+    w.sound = true;
+    const long long sum = head_tiles(a, w, __shfl_sync(0xffffffffu, rows, src), M, TK, table);
+    if (int(threadIdx.x & 31) == src) n = sum;
+  }
   return n;
+}
+// Row block of line position `at` in a key head whose tiles begin at unit0 (moved to the block's
+// first tile); a whole warp.
+__device__ __forceinline__ int find_block(const AttendArgs& a, const Seq& q, int rows, int M, int TK, int table, long long at, long long& unit0) {
+  const int lane = threadIdx.x & 31;
+  for (int rb0 = 0;; rb0 += 32) {
+    const int rb = rb0 + lane;
+    const long long n = rb * M < rows ? row_block(a, q, rows, rb, M, TK, table).tiles : 0;
+    long long inc = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long t = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += t;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, n > 0 && at < unit0 + inc);
+    if (hit || (rb0 + 32) * M >= rows) {  // (the position is in the head, so there is a hit)
+      const int src = hit ? __ffs(int(hit)) - 1 : 0;
+      unit0 += __shfl_sync(0xffffffffu, inc - n, src);
+      return rb0 + src;
+    }
+    unit0 += __shfl_sync(0xffffffffu, inc, 31);
+  }
 }
 
 // Where on the line this CTA works.
@@ -153,7 +198,7 @@ struct Place {
   int seq;
 };
 
-// All THREADS threads. Blocks of THREADS sequences are summed; the one that holds the
+// All THREADS threads (whole warps). Blocks of THREADS sequences are summed; the one that holds the
 // CTA's first tile is found by a scan.
 template <int THREADS>
 __device__ __forceinline__ Place find_place(const AttendArgs& a, int M, int TK, long long* s_warp, long long* s_out) {
@@ -162,13 +207,13 @@ __device__ __forceinline__ Place find_place(const AttendArgs& a, int M, int TK, 
   const int table = table_tokens(a.pool, a.batch);
   const int n = a.batch.n_seqs;
   Place pl;
-  long long keep = 0, total = 0;
+  long long total = 0;
   bool unsound = false;
-  for (int s = tid; s < n; s += THREADS) {
-    const Seq q = read_seq(a.batch, s);
+  for (int s0 = 0; s0 < n; s0 += THREADS) {
+    Seq q{0, 0, 0, true};
+    if (s0 + tid < n) q = read_seq(a.batch, s0 + tid);
     unsound |= !q.sound;
-    keep = head_tiles(a, q, M, TK, table) * a.pool.n_kv;  // the last one is kept where one round is enough
-    total += keep;
+    total += lane_tiles(a, q, M, TK, table) * a.pool.n_kv;
   }
   if (unsound && blockIdx.x == 0) report(a.batch, ST_BAD_ROWS);
   long long inc = total;
@@ -207,7 +252,9 @@ __device__ __forceinline__ Place find_place(const AttendArgs& a, int M, int TK, 
     long long base = 0;
     for (int s0 = 0; s0 < n; s0 += THREADS) {
       const int s = s0 + tid;
-      long long v = s < n ? head_tiles(a, read_seq(a.batch, s), M, TK, table) * a.pool.n_kv : 0;
+      Seq q{0, 0, 0, true};
+      if (s < n) q = read_seq(a.batch, s);
+      const long long v = lane_tiles(a, q, M, TK, table) * a.pool.n_kv;
       inc = v;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -292,14 +339,11 @@ __global__ void __launch_bounds__(AT_THREADS) attend_kernel(const __grid_constan
   long long unit0;               // line position of the unit's first tile
   Block blk;
   {
-    const long long ht = head_tiles(a, sq, M, TK, table);
+    const long long ht = head_tiles(a, sq, rows, M, TK, table);
     kvh = int((at - pl.seq_begin) / ht);
     unit0 = pl.seq_begin + kvh * ht;
-    for (;; ++rb) {
-      blk = row_block(a, sq, rows, rb, M, TK, table);
-      if (at < unit0 + blk.tiles) break;
-      unit0 += blk.tiles;
-    }
+    rb = find_block(a, sq, rows, M, TK, table, at, unit0);
+    blk = row_block(a, sq, rows, rb, M, TK, table);
   }
 
   while (true) {

@@ -5,9 +5,11 @@
 // One CTA per SM holds two tiles of 128 rows (row = token * rep + head), each with
 // a warpgroup for its softmax (one thread a row: no shuffles) and a thread that
 // issues its products; both share the K and V tiles that four loader warps bring
-// in by 16-byte cp.async through a ring of tiles in shared memory (a page may hold
-// any number of tokens and end anywhere inside a tile, which a box of a tensor
-// map could not follow). Per tile of keys:
+// into a ring of tiles in shared memory. A tile that every row sees whole comes by
+// TMA, in boxes of gcd(page_size, 128) tokens, which never cross a page; other tiles
+// (the diagonal, the ends, pages whose gcd is below 8) come by 16-byte cp.async,
+// which can leave out single keys (measured: 2100 clocks for a 32 KB tile, against the
+// 2048 that a tile of keys takes the tensor cores). Per tile of keys:
 //   S = Q K^T      tcgen05.mma, both operands from shared memory, S in TMEM (f32)
 //   P = 2^(S - m)  read from TMEM, rounded to 16 bits, written back over S
 //   O += P V       tcgen05.mma, P from TMEM, V as it lies ([key][dim]: N-major)
@@ -17,6 +19,9 @@
 // by more than 2^8 (O in TMEM is rescaled then; sums in f32 and P in 16 bits have
 // room for that factor), which is rare after the first tiles.
 // TMEM: S0 | S1 | O0 | O1, 512 columns at head_dim 128.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include "paged_attn.cuh"
 
 namespace wcb {
@@ -27,6 +32,7 @@ constexpr int TC_THREADS = 448;  // 2 softmax warpgroups, 4 loader warps, 2 issu
 constexpr int TC_TK = 128;
 constexpr int TC_M = 256;
 constexpr int TILE_PANEL = 128 * 128;  // bytes of 128 rows x 64 dims
+constexpr int POLY_OF = 4;     // of so many pairs of exponentials one goes to the multiply-add units
 constexpr int HOLE_RING = 8;   // tiles: the loaders are at most 4 ahead of the softmax
 constexpr int ODD_RING = 16;   // units, likewise
 
@@ -60,15 +66,15 @@ constexpr uint32_t idesc(int n, bool b_nmajor) {
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(id), "r"(acc), "r"(0)
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(id), "r"(acc)
       : "memory");
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(id), "r"(acc), "r"(0)
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(id), "r"(acc)
       : "memory");
 }
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
@@ -101,20 +107,65 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
       "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
-      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
-      "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
-      "r"(r[31])
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr)
       : "memory");
+}
+
+// two f32 operations in one instruction
+__device__ __forceinline__ uint64_t pack_f32x2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpack_f32x2(uint64_t r, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(r)); }
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 2^x for two x <= 127 on the multiply-add units, for part of the exponentials: x = n + f with n the nearest
+// whole number (by adding 1.5 2^23), a polynomial of degree 5 in f on [-1/2, 1/2] fitted for the least largest
+// relative error (2^-22 as evaluated in 32 bits, as much as ex2.approx), n added to the exponent. Below -125 it
+// stays 2^-125. f keeps NaN (its result's bits do not): `nan` collects it.
+__device__ __forceinline__ float max_nan(float x, float y) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void poly_exp2(uint64_t v, float& x, float& y, uint64_t& nan) {
+  float a, b;
+  unpack_f32x2(v, a, b);
+  const uint64_t c = pack_f32x2(max_nan(a, -125.0f), max_nan(b, -125.0f));
+  const uint64_t t = add_f32x2(c, pack_f32x2(12582912.0f, 12582912.0f));
+  const uint64_t f = fma_f32x2(add_f32x2(t, pack_f32x2(-12582912.0f, -12582912.0f)), pack_f32x2(-1.0f, -1.0f), c);
+  nan = add_f32x2(nan, f);
+  uint64_t p = pack_f32x2(0.0013277939287945628f, 0.0013277939287945628f);
+  p = fma_f32x2(p, f, pack_f32x2(0.009675757959485054f, 0.009675757959485054f));
+  p = fma_f32x2(p, f, pack_f32x2(0.05550709739327431f, 0.05550709739327431f));
+  p = fma_f32x2(p, f, pack_f32x2(0.24022114276885986f, 0.24022114276885986f));
+  p = fma_f32x2(p, f, pack_f32x2(0.6931469440460205f, 0.6931469440460205f));
+  p = fma_f32x2(p, f, pack_f32x2(1.0000001192092896f, 1.0000001192092896f));
+  float ta, tb;
+  unpack_f32x2(p, a, b);
+  unpack_f32x2(t, ta, tb);
+  x = __uint_as_float(__float_as_uint(a) + (__float_as_uint(ta) << 23));
+  y = __uint_as_float(__float_as_uint(b) + (__float_as_uint(tb) << 23));
 }
 
 struct TcShared {
   uint64_t full[8], empty[8];  // ring slots
-  uint64_t q_full[2], s_full[2], p_full[2], o_done[2];
+  uint64_t q_full[2], s_full[2][2], p_full[2][2], o_done[2][2];  // [row tile][half of the keys]
   uint64_t offs_full, piece_full[2], last_full[2];
   uint32_t tmem;
   int abort;                     // a wait ran out: everybody leaves
@@ -141,6 +192,36 @@ __device__ __forceinline__ bool tc_wait(TcShared* sh, uint64_t* bar, uint32_t pa
   return false;
 }
 
+// The same by polling without suspension: a suspended thread wakes about 150 clocks late, which the chain
+// of a tile of keys (S, softmax, product, S, ..) pays several times.
+__device__ __forceinline__ bool tc_spin_warp(TcShared* sh, uint64_t* bar, uint32_t parity) {
+  const uint32_t addr = smem_u32(bar);
+  bool done = false;
+  for (uint32_t it = 0; it < (1u << 26); ++it) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    if (ok) {
+      done = true;
+      break;
+    }
+    if ((it & 255) == 255 && *reinterpret_cast<volatile int*>(&sh->abort)) break;
+  }
+  if (!done) *reinterpret_cast<volatile int*>(&sh->abort) = 1;
+  return __all_sync(0xffffffffu, done);
+}
+
+// box of tokens of one head: dims x .. x + 63 (x a multiple of 64), tokens from `slot` of `page`
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int head, int slot, int page, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(head), "r"(slot), "r"(page), "r"(smem_u32(bar))
+      : "memory");
+}
+
 // the same for a whole warp, which goes on or leaves together
 __device__ __forceinline__ bool tc_wait_warp(TcShared* sh, uint64_t* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, tc_wait(sh, bar, parity));
@@ -155,6 +236,7 @@ struct Walk {
   Block blk;
   int ta, tb;  // tiles of the current unit
 
+  // a whole warp
   __device__ __forceinline__ void start(const AttendArgs& a, const Place& p) {
     pl = p;
     table = table_tokens(a.pool, a.batch);
@@ -162,14 +244,11 @@ struct Walk {
     sq = read_seq(a.batch, s);
     rows = seq_rows(a, sq);
     at = pl.begin;
-    const long long ht = head_tiles(a, sq, TC_M, TC_TK, table);
+    const long long ht = head_tiles(a, sq, rows, TC_M, TC_TK, table);
     kvh = int((at - pl.seq_begin) / ht);
     unit0 = pl.seq_begin + kvh * ht;
-    for (rb = 0;; ++rb) {
-      blk = row_block(a, sq, rows, rb, TC_M, TC_TK, table);
-      if (at < unit0 + blk.tiles) break;
-      unit0 += blk.tiles;
-    }
+    rb = find_block(a, sq, rows, TC_M, TC_TK, table, at, unit0);
+    blk = row_block(a, sq, rows, rb, TC_M, TC_TK, table);
     cut();
   }
   __device__ __forceinline__ void cut() {
@@ -235,7 +314,9 @@ __device__ __forceinline__ bool finite16(uint32_t w) {  // both halves
 }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(const __grid_constant__ AttendArgs a) {
+__global__ void __launch_bounds__(TC_THREADS, 1)
+attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap kmap,
+                 const __grid_constant__ CUtensorMap vmap, int box) {
   using L = TcCfg<HD>;
   constexpr int NS = L::SLOTS, CH = HD / 8;
   extern __shared__ uint8_t raw[];
@@ -249,14 +330,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(const __grid_c
 
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
-      mbar_init(&sh.full[i], 128);
+      mbar_init(&sh.full[i], 4);
       mbar_init(&sh.empty[i], 2);
     }
     for (int w = 0; w < 2; ++w) {
       mbar_init(&sh.q_full[w], 128);
-      mbar_init(&sh.s_full[w], 1);
-      mbar_init(&sh.p_full[w], 128);
-      mbar_init(&sh.o_done[w], 1);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&sh.s_full[w][b], 1);
+        mbar_init(&sh.p_full[w][b], 4);
+        mbar_init(&sh.o_done[w][b], 1);
+      }
       mbar_init(&sh.piece_full[w], 128);
       mbar_init(&sh.last_full[w], 1);
     }
@@ -278,109 +361,154 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(const __grid_c
 
   if (warp >= 12) {
     // ---- issuing warps: products of row tile w --------------------------------
-    if (lane == 0) {
-      const int w = warp - 12;
-      const uint32_t ts = tmem + 128 * w, to = tmem + 256 + 128 * w;
-      const uint32_t qa = sbase + L::Q + w * L::TILE;
-      constexpr uint32_t ID_S = idesc<T>(128, false), ID_O = idesc<T>(HD, true);
-      uint32_t n = 0;                // ring tiles so far
-      uint32_t it = 0, steps = 0;    // items, and products P V so far
+    // The whole warp walks the loops, so that addresses and descriptors are uniform values; one
+    // lane, always the same, issues.
+    const int w = __shfl_sync(0xffffffffu, warp - 12, 0);
+    {
+      // elect.sync instead of lane == 0: the compiler then keeps descriptors in uniform registers
+      // (8 products issue in 600 clocks instead of 940)
+      uint32_t elected;
+      asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(elected));
+      const bool one = elected != 0;
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t ts = tm + 128 * w, to = tm + 256 + 128 * w;
+      const uint64_t qd = desc_kmajor(sbase + L::Q + w * L::TILE);
+      const uint64_t kd = desc_kmajor(sbase + L::RING), vd = desc_nmajor(sbase + L::RING);
+      constexpr uint32_t ID_S = idesc<T>(64, false), ID_O = idesc<T>(HD, true);
+      uint32_t slot = 0, phase = 0;  // of the next ring tile
+      uint32_t it = 0, t = 0;        // units, and tiles of keys so far
+      auto step = [&] {
+        if (++slot == NS) {
+          slot = 0;
+          phase ^= 1;
+        }
+      };
+      // S of half b of the K tile in ring slot ks
+      auto product_s = [&](uint32_t ks, int b) {
+        tc_fence_after();
+        const uint64_t kb = kd + uint64_t(ks * (L::TILE >> 4) + b * (64 * 128 >> 4));
+        if (one) {
+#pragma unroll
+          for (int k = 0; k < HD / 16; ++k) {
+            const uint32_t o = ((k / 4) * TILE_PANEL + (k % 4) * 32) >> 4;
+            mma_ss(ts + 64 * b, qd + o, kb + o, ID_S, k > 0);
+          }
+          tc_commit(&sh.s_full[w][b]);
+          if (b) tc_commit(&sh.empty[ks]);
+        }
+        __syncwarp();
+      };
       bool ok = true;
       do {
         const int end = wk.end_of(a, w);
-        if (end > wk.ta) ok = ok && tc_wait(&sh, &sh.q_full[w], it & 1);
-        for (int i = wk.ta; i < wk.tb && ok; ++i) {
-          const uint32_t sk = n % NS, fk = (n / NS) & 1, sv = (n + 1) % NS, fv = ((n + 1) / NS) & 1;
-          n += 2;
-          ok = tc_wait(&sh, &sh.full[sk], fk);
+        if (end > wk.ta) {
+          ok = tc_wait_warp(&sh, &sh.q_full[w], it & 1) && tc_wait_warp(&sh, &sh.full[slot], phase);
           if (!ok) break;
-          if (i < end) {
-            // S lies over the last P: its product has to be done
-            if (i > wk.ta) ok = tc_wait(&sh, &sh.o_done[w], (steps - 1) & 1);
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t kb = sbase + L::RING + sk * L::TILE;
+          product_s(slot, 0);
+          product_s(slot, 1);
+          ++it;
+        }
+        for (int i = wk.ta; i < wk.tb && ok; ++i) {
+          if (i < end) {  // K of this tile is used up
+            step();
+            const uint32_t vs = slot;
+            const uint64_t vb = vd + uint64_t(vs * (L::TILE >> 4));
+            ok = tc_wait_warp(&sh, &sh.full[slot], phase);
+            step();
+            const bool more = i + 1 < end;
+            if (more) ok = ok && tc_wait_warp(&sh, &sh.full[slot], phase);
 #pragma unroll
-            for (int k = 0; k < HD / 16; ++k) {
-              const uint32_t o = (k / 4) * TILE_PANEL + (k % 4) * 32;
-              mma_ss(ts, desc_kmajor(qa + o), desc_kmajor(kb + o), ID_S, k > 0);
+            for (int b = 0; b < 2; ++b) {
+              ok = ok && tc_spin_warp(&sh, &sh.p_full[w][b], t & 1);
+              if (!ok) break;
+              tc_fence_after();
+              if (one) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  mma_ts(to, ts + 64 * b + 8 * k, vb + (4 * b + k) * (2048 >> 4), ID_O, i > wk.ta || b > 0 || k > 0);
+                tc_commit(&sh.o_done[w][b]);
+                if (b) tc_commit(&sh.empty[vs]);
+              }
+              __syncwarp();
+              if (more) {  // the next S lies over this P: its product has to be done
+                ok = tc_spin_warp(&sh, &sh.o_done[w][b], t & 1);
+                if (!ok) break;
+                product_s(slot, b);
+              }
             }
-            tc_commit(&sh.s_full[w]);
-            tc_commit(&sh.empty[sk]);
-            ok = tc_wait(&sh, &sh.p_full[w], steps & 1) && tc_wait(&sh, &sh.full[sv], fv);
+            ++t;
+          } else {  // rows of this tile see none of these keys
+            ok = tc_wait_warp(&sh, &sh.full[slot], phase);
             if (!ok) break;
-            tc_fence_after();
-            const uint32_t vb = sbase + L::RING + sv * L::TILE;
-#pragma unroll
-            for (int k = 0; k < TC_TK / 16; ++k)
-              mma_ts(to, ts + 8 * k, desc_nmajor(vb + k * 2048), ID_O, i > wk.ta || k > 0);
-            tc_commit(&sh.o_done[w]);
-            tc_commit(&sh.empty[sv]);
-            ++steps;
-          } else {
-            bar_arrive(&sh.empty[sk]);
-            ok = tc_wait(&sh, &sh.full[sv], fv);
+            if (one) bar_arrive(&sh.empty[slot]);
+            step();
+            ok = tc_wait_warp(&sh, &sh.full[slot], phase);
             if (!ok) break;
-            bar_arrive(&sh.empty[sv]);
+            if (one) bar_arrive(&sh.empty[slot]);
+            step();
           }
         }
-        if (end > wk.ta) ++it;
       } while (ok && wk.next(a));
     }
-    __syncwarp();
   } else if (warp >= 8) {
     // ---- loaders --------------------------------------------------------------
     const int lt = tid - 256;
     long long* offs = reinterpret_cast<long long*>(sm + L::OFFS);
-    uint32_t n = 0, tiles = 0, item = 0;
-    constexpr int LAG = NS - 2;  // groups in flight
+    uint32_t n = 0, tiles = 0, item = 0, by_copy = 0;
     bool ok = true, holes_seen = false;
-    // what has to be looked at when tile n's copies have landed: values of a ragged tile
-    uint32_t odd_bits = 0;  // bit (n % 32): search ring tile n
-    uint32_t item_of[4] = {0, 0, 0, 0};
-    auto landed = [&](uint32_t m) {  // ring tile m is complete in this thread's view
-      const uint32_t sl = m % NS;
-      if ((odd_bits >> (m & 31)) & 1) {
-        uint8_t* t = sm + L::RING + sl * L::TILE;
-        bool odd = false;
-        for (int c = lt; c < 128 * CH; c += 128) {
-          uint4* x = reinterpret_cast<uint4*>(t + tile_at(c / CH, c % CH));
-          uint4 v = *x;
-          if (!(finite16<T>(v.x) && finite16<T>(v.y) && finite16<T>(v.z) && finite16<T>(v.w))) {
-            odd = true;
-            T e[8];
-            *reinterpret_cast<uint4*>(e) = v;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (!(fabsf(to_f32(e[j])) <= FLT_MAX)) e[j] = from_f32<T>(0.0f);
-            *x = *reinterpret_cast<const uint4*>(e);
-          }
-        }
-        if (odd) sh.odd[item_of[(m >> 1) & 3] % ODD_RING] = 1;
-      }
-      fence_proxy_async();
-      bar_arrive(&sh.full[sl]);
+    // the page of this thread's key of tile i; -1: none
+    auto page_of = [&](int i) {
+      const int key = (wk.blk.tile0 + i) * TC_TK + lt;
+      return key >= wk.blk.lo && key < wk.blk.hi
+                 ? __ldg(a.batch.page_table + int64_t(wk.s) * a.batch.max_pages + key / a.pool.page_size)
+                 : -1;
+    };
+    auto room = [&](uint32_t m) {
+      return m < NS || tc_wait_warp(&sh, &sh.empty[m % NS], ((m / NS) - 1) & 1);
     };
     do {
       if (lt == 0) sh.odd[(item + ODD_RING / 2) % ODD_RING] = 0;
       const bool many = wk.blk.pos1 > wk.blk.pos0;
-      for (int i = wk.ta; i < wk.tb && ok; ++i, ++tiles) {
-        bool hole;
-        const long long off = wk.key_offset(a, (wk.blk.tile0 + i) * TC_TK + lt, hole);
-        const unsigned hb = __ballot_sync(0xffffffffu, hole);
-        offs[(tiles & 1) * 128 + lt] = off;
+      int next = page_of(wk.ta);
+      for (int i = wk.ta; i < wk.tb && ok; ++i, ++tiles, n += 2) {
+        const int page = next;
+        if (i + 1 < wk.tb) next = page_of(i + 1);  // its latency passes while this tile waits for room
+        const int key = (wk.blk.tile0 + i) * TC_TK + lt, slot = key % a.pool.page_size;
+        const bool in = key >= wk.blk.lo && key < wk.blk.hi, there = in && page >= 0 && page < a.pool.n_pages;
+        const unsigned hb = __ballot_sync(0xffffffffu, in && !there);
         if (lane == 0) sh.holes[tiles % HOLE_RING][warp - 8] = hb;
-        holes_seen |= hole;
-        bar_arrive(&sh.offs_full);
-        ok = tc_wait_warp(&sh, &sh.offs_full, tiles & 1);
-        const long long* ro = offs + (tiles & 1) * 128;
+        holes_seen |= hb != 0;
+        const bool ragged = wk.ragged(a, i);
+        if (box > 0 && !ragged) {
 #pragma unroll 1
-        for (int kvi = 0; kvi < 2; ++kvi, ++n) {
-          const uint32_t sl = n % NS;
-          if (n >= NS && ok) ok = tc_wait_warp(&sh, &sh.empty[sl], ((n / NS) - 1) & 1);
+          for (int kvi = 0; kvi < 2 && ok; ++kvi) {
+            ok = room(n + kvi);
+            if (!ok) break;
+            uint64_t* bar = &sh.full[(n + kvi) % NS];
+            if (lane == 0) {  // warp 8's arrival brings the bytes to wait for
+              if (warp == 8) mbar_expect_tx(bar, L::TILE);
+              else bar_arrive(bar);
+            }
+            if (lt % box == 0) {
+              const uint32_t dst = sbase + L::RING + ((n + kvi) % NS) * L::TILE + lt * 128;
+#pragma unroll
+              for (int p = 0; p < L::PANELS; ++p)  // a page that is not there: past the last one, zeros
+                tma_load(dst + p * TILE_PANEL, kvi ? &vmap : &kmap, 64 * p, wk.kvh, slot, there ? page : a.pool.n_pages, bar);
+            }
+          }
+          continue;
+        }
+        offs[(by_copy & 1) * 128 + lt] = there ? page * a.pool.page_stride + int64_t(slot) * a.pool.token_stride : -1;
+        bar_arrive(&sh.offs_full);
+        ok = tc_wait_warp(&sh, &sh.offs_full, by_copy & 1);
+        const long long* ro = offs + (by_copy & 1) * 128;
+        ++by_copy;
+#pragma unroll 1
+        for (int kvi = 0; kvi < 2 && ok; ++kvi) {
+          ok = room(n + kvi);
           if (!ok) break;
           const T* base = static_cast<const T*>(kvi ? a.pool.v : a.pool.k) + wk.kvh * a.pool.head_stride;
-          const uint32_t dst = sbase + L::RING + sl * L::TILE;
+          const uint32_t dst = sbase + L::RING + ((n + kvi) % NS) * L::TILE;
 #pragma unroll 8
           for (int c = lt; c < 128 * CH; c += 128) {
             const int r = c / CH, ch = c % CH;
@@ -388,27 +516,46 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(const __grid_c
             cp16(dst + tile_at(r, ch), base + (o < 0 ? 0 : o) + ch * 8, o >= 0);
           }
           cp_commit();
-          odd_bits &= ~(1u << (n & 31));
-          if (kvi && many && wk.ragged(a, i)) odd_bits |= 1u << (n & 31);
-          item_of[(n >> 1) & 3] = item;
-          if (n >= LAG) {
-            cp_wait<LAG>();
-            landed(n - LAG);
+        }
+        if (!ok) break;
+#pragma unroll 1
+        for (int kvi = 0; kvi < 2; ++kvi) {
+          if (kvi == 0) cp_wait<1>();
+          else cp_wait<0>();
+          // keys that some rows see and others do not: infinities and NaN are taken out of their values
+          if (kvi && many && ragged) {
+            uint8_t* t = sm + L::RING + ((n + 1) % NS) * L::TILE;
+            bool odd = false;
+            for (int c = lt; c < 128 * CH; c += 128) {  // the chunks this thread copied
+              uint4* x = reinterpret_cast<uint4*>(t + tile_at(c / CH, c % CH));
+              const uint4 v = *x;
+              if (!(finite16<T>(v.x) && finite16<T>(v.y) && finite16<T>(v.z) && finite16<T>(v.w))) {
+                odd = true;
+                alignas(16) T e[8];
+                *reinterpret_cast<uint4*>(e) = v;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                  if (!(fabsf(to_f32(e[j])) <= FLT_MAX)) e[j] = from_f32<T>(0.0f);
+                *x = *reinterpret_cast<const uint4*>(e);
+              }
+            }
+            if (odd) sh.odd[item % ODD_RING] = 1;
           }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) bar_arrive(&sh.full[(n + kvi) % NS]);
         }
       }
       ++item;
     } while (ok && wk.next(a));
     cp_wait<0>();
-    if (ok)
-      for (uint32_t m = n >= uint32_t(LAG) ? n - LAG : 0; m < n; ++m) landed(m);
-    if (holes_seen) report(a.batch, ST_BAD_PAGE);
+    if (holes_seen && lane == 0) report(a.batch, ST_BAD_PAGE);
   } else {
     // ---- softmax of row tile w: thread = row ----------------------------------
     const int w = warp >> 2, row = tid & 127;
     const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16;
     const uint32_t ts = tmem + lanes + 128 * w, to = tmem + lanes + 256 + 128 * w;
-    uint32_t tiles = 0, steps = 0, item = 0, cuts = 0;
+    uint32_t tiles = 0, t = 0, item = 0, cuts = 0;  // tiles of the ring, tiles of keys with rows, units, units cut
     bool ok = true;
     do {
       const int r0 = wk.rb * TC_M + 128 * w, rn = min(128, wk.rows - r0);
@@ -416,128 +563,133 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(const __grid_c
       if (end > wk.ta) {
         // queries into shared memory; rows that are not there are zeros
         uint8_t* qt = sm + L::Q + w * L::TILE;
-#pragma unroll 4
-        for (int c = row; c < 128 * CH; c += 128) {
-          const int r = c / CH, ch = c % CH;
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (r < rn) {
-            const int gr = r0 + r;
-            v = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (wk.sq.r0 + gr / a.rep) * a.q_stride +
-                                                     (wk.kvh * a.rep + gr % a.rep) * HD + ch * 8));
-          }
-          *reinterpret_cast<uint4*>(qt + tile_at(r, ch)) = v;
+        // (a thread its own row: one division, all loads on their way at once)
+        const int gr = r0 + min(row, rn - 1);
+        {
+          const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (wk.sq.r0 + gr / a.rep) * a.q_stride +
+                                                            (wk.kvh * a.rep + gr % a.rep) * HD);
+          uint4 x[CH];
+#pragma unroll
+          for (int ch = 0; ch < CH; ++ch) x[ch] = row < rn ? __ldg(src + ch) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int ch = 0; ch < CH; ++ch) *reinterpret_cast<uint4*>(qt + tile_at(row, ch)) = x[ch];
         }
         fence_proxy_async();
         bar_arrive(&sh.q_full[w]);
 
-        const int gr = r0 + min(row, rn - 1);
         const int pos = wk.sq.kv - wk.sq.n + gr / a.rep;
         const int khi = min(pos + 1, wk.table), klo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
         float m = -INFINITY, l = 0.0f;  // m: the maximum that O and l are scaled by
         for (int i = wk.ta; i < end && ok; ++i) {
           const uint32_t* holes = sh.holes[(tiles + (i - wk.ta)) % HOLE_RING];
-          ok = tc_wait_warp(&sh, &sh.s_full[w], steps & 1);
-          if (!ok) break;
-          tc_fence_after();
-          const int key0 = (wk.blk.tile0 + i) * TC_TK;
-          const bool gaps = (holes[0] | holes[1] | holes[2] | holes[3]) != 0;
-          const bool mask = gaps || wk.ragged(a, i);
-          // bit c: key key0 + c is seen
-          const int lo = max(0, min(128, klo - key0)), hi = max(0, min(128, khi - key0));
-          uint32_t seen[4];
-          if (mask) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int b0 = max(0, min(32, lo - 32 * q)), b1 = max(0, min(32, hi - 32 * q));
-              const uint32_t below1 = b1 >= 32 ? 0xffffffffu : (1u << b1) - 1u, below0 = b0 >= 32 ? 0xffffffffu : (1u << b0) - 1u;
-              seen[q] = below1 & ~below0 & ~holes[q];
-            }
-          }
-          float top = -INFINITY;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t v[32];
-            tmem_ld32(ts + 32 * q, v);
-            tmem_wait_ld();
+          const bool cut = wk.ragged(a, i);
+#pragma unroll 1
+          for (int b = 0; b < 2; ++b) {
+            ok = tc_wait_warp(&sh, &sh.s_full[w][b], t & 1);
+            if (!ok) break;
+            tc_fence_after();
+            const int key0 = (wk.blk.tile0 + i) * TC_TK + 64 * b;
+            const bool mask = cut || (holes[2 * b] | holes[2 * b + 1]) != 0;
+            // bit c: key key0 + c is seen
+            uint32_t seen[2];
             if (mask) {
+              const int lo = max(0, min(64, klo - key0)), hi = max(0, min(64, khi - key0));
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (!((seen[q] >> e) & 1)) v[e] = 0xff800000u;
-            }
-            float t0 = -INFINITY, t1 = -INFINITY;
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              t0 = fmaxf(t0, __uint_as_float(v[e]));
-              t1 = fmaxf(t1, __uint_as_float(v[e + 1]));
-            }
-            top = fmaxf(top, fmaxf(t0, t1));
-          }
-          // a negative scale turns the order round: the largest product is then the smallest score
-          top = a.scale_log2 >= 0.0f ? top * a.scale_log2 : top;
-          if (a.scale_log2 < 0.0f) {
-            top = -INFINITY;
-#pragma unroll 1
-            for (int q = 0; q < 4; ++q) {
-              uint32_t v[32];
-              tmem_ld32(ts + 32 * q, v);
-              tmem_wait_ld();
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (!mask || ((seen[q] >> e) & 1)) top = fmaxf(top, __uint_as_float(v[e]) * a.scale_log2);
-            }
-          }
-          // rescale where some row's maximum grew by more than 2^8
-          const bool grow = top > m + 8.0f;  // also the first finite one
-          if (__any_sync(0xffffffffu, grow)) {
-            const float nm = fmaxf(m, top);
-            const float f = m == nm ? 1.0f : fast_exp2(m - (nm == -INFINITY ? 0.0f : nm));
-            if (i > wk.ta) {  // the last product is done: S was issued after it
-#pragma unroll 1
-              for (int q = 0; q < HD / 32; ++q) {
-                uint32_t v[32];
-                tmem_ld32(to + 32 * q, v);
-                tmem_wait_ld();
-#pragma unroll
-                for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-                tmem_st32(to + 32 * q, v);
+              for (int q = 0; q < 2; ++q) {
+                const int b0 = max(0, min(32, lo - 32 * q)), b1 = max(0, min(32, hi - 32 * q));
+                const uint32_t below1 = b1 >= 32 ? 0xffffffffu : (1u << b1) - 1u, below0 = b0 >= 32 ? 0xffffffffu : (1u << b0) - 1u;
+                seen[q] = below1 & ~below0 & ~holes[2 * b + q];
               }
             }
-            l *= f;
-            m = nm;
-          }
-          const float use = m == -INFINITY ? 0.0f : m;
-          float l0 = 0.0f, l1 = 0.0f;
+            // the row's 64 products in registers: TMEM is read once
+            uint32_t v[64];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t v[32], p[16];
-            tmem_ld32(ts + 32 * q, v);
+            for (int q = 0; q < 2; ++q) tmem_ld32(ts + 64 * b + 32 * q, *reinterpret_cast<uint32_t(*)[32]>(v + 32 * q));
             tmem_wait_ld();
             if (mask) {
+              const uint32_t none = a.scale_log2 < 0.0f ? 0x7f800000u : 0xff800000u;  // -infinity once scaled
 #pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                const float x = __uint_as_float(v[e]) * a.scale_log2;
-                v[e] = __float_as_uint(((seen[q] >> e) & 1) ? fast_exp2(x - use) : 0.0f);
+              for (int e = 0; e < 64; ++e)
+                if (!((seen[e / 32] >> (e % 32)) & 1)) v[e] = none;
+            }
+            float top;
+            if (a.scale_log2 >= 0.0f) {
+              float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+              for (int e = 0; e < 64; e += 8)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = fmaxf(x[j], fmaxf(__uint_as_float(v[e + 2 * j]), __uint_as_float(v[e + 2 * j + 1])));
+              top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * a.scale_log2;
+            } else {  // a negative scale turns the order round
+              float x = INFINITY;
+#pragma unroll
+              for (int e = 0; e < 64; ++e) x = fminf(x, __uint_as_float(v[e]));
+              top = x * a.scale_log2;
+            }
+            // rescale where some row's maximum grew by more than 2^8
+            const bool grow = top > m + 8.0f;  // also the first finite one
+            if (__any_sync(0xffffffffu, grow)) {
+              const float nm = fmaxf(m, top);
+              const float f = m == nm ? 1.0f : fast_exp2(m - (nm == -INFINITY ? 0.0f : nm));
+              if (i > wk.ta || b) {  // after the last product
+                ok = tc_wait_warp(&sh, &sh.o_done[w][1 - b], (b ? t : t - 1) & 1);
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll 1
+                for (int q = 0; q < HD / 16; ++q) {
+                  uint32_t o[16];
+                  tmem_ld16(to + 16 * q, o);
+                  tmem_wait_ld();
+#pragma unroll
+                  for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                  tmem_st16(to + 16 * q, o);
+                }
               }
-            } else {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(fast_exp2(fmaf(__uint_as_float(v[e]), a.scale_log2, -use)));
+              l *= f;
+              m = nm;
             }
+            const uint64_t scale2 = pack_f32x2(a.scale_log2, a.scale_log2);
+            const float use = m == -INFINITY ? 0.0f : m;
+            const uint64_t use2 = pack_f32x2(-use, -use);
+            uint64_t sum[2] = {0, 0}, nan = 0;
+            // masked products need their zeros exactly: all of them by ex2.approx
+            auto exponentials = [&](auto poly) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float x = __uint_as_float(v[2 * e]), y = __uint_as_float(v[2 * e + 1]);
-              l0 += x;
-              l1 += y;
-              p[e] = pack2<T>(x, y);
-            }
-            tmem_st16(ts + 16 * q, p);
+              for (int q = 0; q < 2; ++q) {
+                uint32_t p[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                  float x, y;
+                  const uint64_t z = fma_f32x2(pack_f32x2(__uint_as_float(v[32 * q + 2 * e]), __uint_as_float(v[32 * q + 2 * e + 1])), scale2, use2);
+                  if (decltype(poly)::value && e % POLY_OF == POLY_OF - 1) {
+                    poly_exp2(z, x, y, nan);
+                  } else {
+                    unpack_f32x2(z, x, y);
+                    x = fast_exp2(x);
+                    y = fast_exp2(y);
+                  }
+                  sum[e & 1] = add_f32x2(sum[e & 1], pack_f32x2(x, y));
+                  p[e] = pack2<T>(x, y);
+                }
+                tmem_st16(ts + 64 * b + 16 * q, p);
+              }
+            };
+            if (mask) exponentials(std::false_type());
+            else exponentials(std::true_type());
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&sh.p_full[w][b]);
+            float x0, y0, x1, y1;
+            unpack_f32x2(sum[0], x0, y0);
+            unpack_f32x2(sum[1], x1, y1);
+            l += (x0 + y0) + (x1 + y1);
+            unpack_f32x2(nan, x0, y0);
+            if (x0 != x0 || y0 != y0) l = x0 + y0;
           }
-          l += l0 + l1;
-          tmem_wait_st();
-          tc_fence_before();
-          bar_arrive(&sh.p_full[w]);
-          ++steps;
+          ++t;
         }
-        if (ok) ok = tc_wait_warp(&sh, &sh.o_done[w], (steps - 1) & 1);
+        if (ok) ok = tc_wait_warp(&sh, &sh.o_done[w][1], (t - 1) & 1);
         if (!ok) break;
         tc_fence_after();
 
@@ -548,7 +700,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(const __grid_c
         const bool odd = *reinterpret_cast<volatile int*>(&sh.odd[item % ODD_RING]) != 0;
         const int64_t tok = wk.sq.r0 + gr / a.rep;
         const int hh = wk.kvh * a.rep + gr % a.rep;
-        const bool some = l > 0.0f || l != l;
+        const bool some = (l > 0.0f && m > -INFINITY) || l != l;
         const float inv = some ? 1.0f / l : 0.0f;
         T* dst = static_cast<T*>(a.out) + tok * a.out_stride + hh * HD;
 #pragma unroll 1
@@ -634,19 +786,20 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(const __grid_c
           const int hh = wk.kvh * a.rep + gr % a.rep;
           T* dst = static_cast<T*>(a.out) + tok * a.out_stride + hh * HD;
 #pragma unroll 1
-          for (int q = 0; q < HD / 32; ++q) {
-            float x[32];
+          for (int q = 0; q < HD / 64; ++q) {
+            float x[64];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) x[e] = 0.0f;
+            for (int e = 0; e < 64; ++e) x[e] = 0.0f;
+#pragma unroll 1
             for (int p = c0; p <= c1; ++p) {
               const float* pp = part(p);
               const float f = fast_exp2(__ldcg(pp + size_t(HD) * TC_M) - u);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) x[e] += f * __ldcg(pp + size_t(32 * q + e) * TC_M);
+              for (int e = 0; e < 64; ++e) x[e] += f * __ldcg(pp + size_t(64 * q + e) * TC_M);
             }
 #pragma unroll
-            for (int e = 0; e < 32; ++e) x[e] = some ? x[e] * inv : 0.0f;
-            store_vec<T, 32>(dst + 32 * q, x);
+            for (int e = 0; e < 64; ++e) x[e] = some ? x[e] * inv : 0.0f;
+            store_vec<T, 64>(dst + 64 * q, x);
           }
           if (a.lse) a.lse[tok * a.n_heads + hh] = some ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
         }
@@ -662,13 +815,41 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(const __grid_c
   if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
+// Tensor map of the pool's keys or values: (dim, head, token, page), boxes of 64 dims x `box` tokens.
+// False where the pool cannot be described: strides of 2^40 bytes and more.
+bool make_map(CUtensorMap* map, const Pool& p, const void* base, bool bf16, int box) {
+  static const PFN_cuTensorMapEncodeTiled encode = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) f = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled>(f);
+  }();
+  if (!encode) return false;
+  const cuuint64_t dims[4] = {cuuint64_t(p.head_dim), cuuint64_t(p.n_kv), cuuint64_t(p.page_size), cuuint64_t(p.n_pages)};
+  // a dimension of one may have any stride: one that the encoder takes
+  const cuuint64_t least = cuuint64_t(p.head_dim) * 2;
+  const cuuint64_t strides[3] = {p.n_kv > 1 ? cuuint64_t(p.head_stride) * 2 : least, p.page_size > 1 ? cuuint64_t(p.token_stride) * 2 : least,
+                                 p.n_pages > 1 ? cuuint64_t(p.page_stride) * 2 : least};
+  for (cuuint64_t s : strides)
+    if (s >= (cuuint64_t(1) << 40)) return false;
+  const cuuint32_t boxes[4] = {64, 1, cuuint32_t(box), 1}, steps[4] = {1, 1, 1, 1};
+  return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, boxes,
+                steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int HD>
 cudaError_t run_tc(const AttendArgs& a, cudaStream_t s) {
   using L = TcCfg<HD>;
   static_assert(L::SMEM + sizeof(TcShared) <= 227 * 1024, "shared memory");
   cudaError_t e = cudaFuncSetAttribute(attend_tc_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
   if (e != cudaSuccess) return e;
-  attend_tc_kernel<T, HD><<<TC_CTAS, TC_THREADS, L::SMEM, s>>>(a);
+  int box = TC_TK;
+  while (a.pool.page_size % box) box /= 2;
+  CUtensorMap km{}, vm{};
+  constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+  if (box < 8 || !make_map(&km, a.pool, a.pool.k, BF, box) || !make_map(&vm, a.pool, a.pool.v, BF, box)) box = 0;
+  attend_tc_kernel<T, HD><<<TC_CTAS, TC_THREADS, L::SMEM, s>>>(a, km, vm, box);
   return cudaGetLastError();
 }
 
