@@ -111,7 +111,7 @@ uint32_t check_rows(const void* p, uint64_t stride, uint64_t width, uint32_t dty
 // (new tokens * rep). 16-bit types: sequences of more than TC_MIN rows go to the tensor-core kernel,
 // the others of the batch to the mma.sync kernel. Its row block is the smallest that holds
 // the longest sequence's rows, so that no product is spent on rows that are not there.
-constexpr uint64_t TC_MIN = 64;
+constexpr uint64_t TC_MIN = 32;
 struct Plan {
   int rows;     // row block of the mma.sync kernel, 0: not run
   bool tc;
@@ -122,7 +122,7 @@ Plan plan(uint32_t dtype, uint64_t n_seqs, uint64_t max_rows) {
   p.tc = dtype != WCB_KV_F32 && max_rows > TC_MIN;
   p.split = p.tc ? (n_seqs == 1 ? 0 : int(TC_MIN)) : INT_MAX;
   const uint64_t r = p.tc ? (n_seqs == 1 ? 0 : TC_MIN) : max_rows;
-  p.rows = r == 0 ? 0 : r <= 16 ? 16 : r <= 32 ? 32 : 64;
+  p.rows = r == 0 ? 0 : r <= 8 ? 8 : r <= 16 ? 16 : 32;
   return p;
 }
 

@@ -6,7 +6,7 @@
 // pass over K and V with a running maximum m and sum l (both f32):
 //   m' = max(m, s_j), l' = l 2^(m - m') + 2^(s_j - m'), o' = o 2^(m - m') + 2^(s_j - m') v_j,
 // s in units of log2. Rows of a key head: the rep query heads that share it, of
-// every new token (row = token * rep + head), in blocks of 16 WM rows.
+// every new token (row = token * rep + head), in blocks of 8 NB rows.
 //
 // Split: a unit is (sequence, key head, row block); its keys are TK-key tiles.
 // All tiles of all units lie on one line, cut into one equal part per CTA, so
@@ -16,19 +16,32 @@
 // cut leaves (o, m, l) pieces in the workspace, at most two a CTA; the CTA that
 // finishes last joins them in their order, so results do not depend on timing.
 //
-// Tile: 4 warps, WM along rows and WN = 4 / WM along the tile's keys; K and V
-// arrive by 16-byte cp.async through STAGES buffers; the page of every key is
-// looked up one tile earlier into shared memory. Keys that do not exist (past
-// the end, a page outside the pool) are filled with zeros, never read. Where
-// some rows of a block see a key and others do not, V is first searched
+// Products: transposed, S^T = K Q^T and O^T = V^T P^T, so that keys and dims fill the 16 rows of an
+// mma and the few rows of a decode step its 8 columns (8 rows a key head at most need
+// half the products, registers and exponentials of the other way round). The 4 warps share
+// a tile's keys, each with its own m, l and O, joined at a unit's end. m moves only where some
+// score passes it by 2^8 (sums in f32 and P have room for that), by one vote a tile.
+//
+// Tile: K and V
+// arrive in rows of 128-byte panels, swizzled, through STAGES buffers: whole tiles by
+// TMA in boxes of gcd(page_size, TK) tokens, which never cross a page; tiles that
+// begin or end inside, and pools whose gcd is below 8, by 16-byte cp.async, which
+// leaves out single keys. The page of every key is looked up one tile
+// earlier. Keys that do not exist (past the end, a page outside the pool) are
+// zeros, never read. Where some rows of a block see a key and others do not, V is first searched
 // for infinities and NaN: 0 * inf must not reach the rows that do not see it.
 //
-// 16-bit types: m16n8k16. P is kept as a sum of two 16-bit numbers for WM = 1
-// (the tensor cores idle there anyway), rounded once for larger WM. f32
+// 16-bit types: m16n8k16. P is kept as a sum of two 16-bit numbers for NB = 1
+// (the tensor cores idle there anyway), rounded once for larger NB. f32
 // activations: m16n8k8 in tf32 with q and p (and an f32 cache's k and v) split
 // into two tf32 numbers each, which keeps 21 bits; an f16 or bf16 cache is exact
-// in tf32.
+// in tf32. The tensor cores cut their sums off instead of rounding them, so long sums are
+// kept short: small products have accumulators of their own, and a tile's P V is summed
+// by itself and added to O by an ordinary multiply-add.
 #pragma once
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include <type_traits>
 
 #include "device_common.cuh"
@@ -91,6 +104,13 @@ __device__ __forceinline__ float fast_exp2(float x) {
   return y;
 }
 
+// an 8 x 8 block of 16-bit values, a row (2t, 2t + 1) in lane 4 g + t, transposed
+__device__ __forceinline__ uint32_t transposed8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
 // two consecutive elements of a 32-bit word as f32
 template <typename CT>
 __device__ __forceinline__ float2 pair_f32(uint32_t w);
@@ -113,6 +133,51 @@ template <>
 __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// ---- tiles by TMA ------------------------------------------------------------
+
+// box of tokens of one head: a 128-byte panel of dims from x on, tokens from `slot` of `page`
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int head, int slot, int page, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(head), "r"(slot), "r"(page), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// Tensor map of the pool's keys or values: (dim, head, token, page), boxes of 128 bytes of dims x
+// `box` tokens, 128-byte swizzle. False where the pool cannot be described (strides of 2^40 bytes and more).
+template <typename CT>
+bool make_map(CUtensorMap* map, const Pool& p, const void* base, int box) {
+  static const PFN_cuTensorMapEncodeTiled encode = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) f = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled>(f);
+  }();
+  if (!encode) return false;
+  constexpr CUtensorMapDataType kind = sizeof(CT) == 4                          ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                       : std::is_same<CT, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                                                : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const cuuint64_t dims[4] = {cuuint64_t(p.head_dim), cuuint64_t(p.n_kv), cuuint64_t(p.page_size), cuuint64_t(p.n_pages)};
+  // a dimension of one may have any stride: one that the encoder takes
+  const cuuint64_t least = cuuint64_t(p.head_dim) * sizeof(CT);
+  const cuuint64_t strides[3] = {p.n_kv > 1 ? cuuint64_t(p.head_stride) * sizeof(CT) : least,
+                                 p.page_size > 1 ? cuuint64_t(p.token_stride) * sizeof(CT) : least,
+                                 p.n_pages > 1 ? cuuint64_t(p.page_stride) * sizeof(CT) : least};
+  for (cuuint64_t s : strides)
+    if (s >= (cuuint64_t(1) << 40)) return false;
+  const cuuint32_t boxes[4] = {128 / sizeof(CT), 1, cuuint32_t(box), 1}, steps[4] = {1, 1, 1, 1};
+  return encode(map, kind, 4, const_cast<void*>(base), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// Both maps; the box's tokens, or 0 where tiles of TK keys cannot come by TMA: a box starts on a
+// group of 8 rows (1024 bytes, the swizzle's period) and stays in one page.
+template <typename CT>
+int make_maps(CUtensorMap* k, CUtensorMap* v, const Pool& p, int TK) {
+  int box = TK;
+  while (p.page_size % box) box /= 2;
+  return box >= 8 && make_map<CT>(k, p, p.k, box) && make_map<CT>(v, p, p.v, box) ? box : 0;
 }
 
 // ---- the line of tiles ------------------------------------------------------
@@ -288,48 +353,71 @@ __device__ __forceinline__ Place find_place(const AttendArgs& a, int M, int TK, 
 
 // ---- the kernel -------------------------------------------------------------
 
-template <typename AT, typename CT, int HD, int WM>
+constexpr float SLACK = 8.0f;  // how far (in powers of two) a score may pass the maximum before it moves
+
+template <typename AT, typename CT, int HD, int NB>
 struct AttnCfg {
   static constexpr bool F32A = std::is_same<AT, float>::value;
   static constexpr bool F32C = std::is_same<CT, float>::value;
-  static constexpr int WN = 4 / WM;
-  static constexpr int TK = F32C ? 32 : 64;  // keys of a tile
-  static constexpr int KW = TK / WN;         // keys of a warp
-  static constexpr int M = 16 * WM;
-  static constexpr int ROW = HD * int(sizeof(CT)) + 16;  // bytes of a staged row: 16 more than a multiple of 128
-  static constexpr int STAGE = 2 * TK * ROW;
-  static constexpr int STAGES = 3;
-  static constexpr int QBYTES = F32A ? M * HD * 8 : 0;  // q as tf32 pairs in fragment order
-  static constexpr int OPITCH = HD + 4;                 // floats; joining the warps' results
-  static constexpr int JOIN = WN > 1 ? 4 * 16 * OPITCH * 4 + 4 * 16 * 8 : 0;
+  static constexpr int TK = 64;       // keys of a tile
+  static constexpr int KW = TK / 4;   // keys of a warp: the rows of one mma
+  static constexpr int M = 8 * NB;    // rows of a block
+  static constexpr int PANELS = HD * int(sizeof(CT)) / 128;
+  static constexpr int PANEL = TK * 128;            // bytes: TK rows of 128
+  static constexpr int STAGE = 2 * PANELS * PANEL;  // K, then V
+  static constexpr int STAGES = STAGE > 32768 ? 2 : 3;
+  static constexpr int QBYTES = F32A ? NB * (HD / 8) * 512 : 0;  // q as tf32 pairs in fragment order
+  static constexpr int OPITCH = HD + 4;                          // floats; joining the warps' results
+  static constexpr int JOIN = 4 * M * OPITCH * 4 + 4 * M * 8;
   static constexpr int RING = STAGES * STAGE > JOIN ? STAGES * STAGE : JOIN;
   static constexpr int OFFS = (STAGES + 1) * TK * 8 + (STAGES + 1) * 2 * 4;
-  static constexpr int SMEM = RING + QBYTES + OFFS;
-  static constexpr bool TWO_P = !F32A && WM == 1;
+  static constexpr int SMEM = RING + QBYTES + OFFS + 1024;  // + alignment to the swizzle's period
+  static constexpr bool TWO_P = !F32A && NB == 1;
 };
 
-template <typename AT, typename CT, int HD, int WM>
-__global__ void __launch_bounds__(AT_THREADS) attend_kernel(const __grid_constant__ AttendArgs a) {
-  using L = AttnCfg<AT, CT, HD, WM>;
-  constexpr int TK = L::TK, KW = L::KW, M = L::M, WN = L::WN, ROW = L::ROW, S = L::STAGES;
+template <typename AT, typename CT, int HD, int NB>
+__global__ void __launch_bounds__(AT_THREADS)
+attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap kmap,
+              const __grid_constant__ CUtensorMap vmap, int box) {
+  using L = AttnCfg<AT, CT, HD, NB>;
+  constexpr int TK = L::TK, KW = L::KW, M = L::M, S = L::STAGES;
   constexpr bool F32A = L::F32A, F32C = L::F32C;
-  constexpr int NT = KW / 8;   // 8-key column blocks of a warp
-  constexpr int ND = HD / 8;   // 8-dim column blocks of the output
+  constexpr int MB = HD / 16;                    // 16-dim blocks of the output
   constexpr int CH = HD * int(sizeof(CT)) / 16;  // 16-byte chunks of a row
-  extern __shared__ __align__(128) uint8_t sm[];
+  constexpr int VT = L::PANELS * L::PANEL;       // bytes from a stage's K to its V
+  extern __shared__ uint8_t raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint4* qfrag = reinterpret_cast<uint4*>(sm + L::RING);
-  long long* offs = reinterpret_cast<long long*>(sm + L::RING + L::QBYTES);  // [S + 1][TK]: element offset of a key's row, -1 = none
-  unsigned* holes = reinterpret_cast<unsigned*>(offs + (S + 1) * TK);        // [S + 1][TK / 32]: keys below the end without a page
-  __shared__ long long s_scan[8], s_place[2];
+  long long* offs = reinterpret_cast<long long*>(sm + L::RING + L::QBYTES);  // [S + 1][TK]: a key's page or row offset, -1 = none
+  unsigned* holes = reinterpret_cast<unsigned*>(offs + (S + 1) * TK);        // [S + 1][2]: keys below the end without a page
+  __shared__ long long s_scan[4], s_place[2];
   __shared__ int s_last;
+  __shared__ uint64_t s_full[S];  // a stage's bytes are there (tiles by TMA)
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int wm = warp % WM, wn = warp / WM;
   const int g = lane >> 2, t = lane & 3;
   const uint32_t sbase = smem_u32(sm);
   const int table = table_tokens(a.pool, a.batch);
   const Place pl = find_place<AT_THREADS>(a, M, TK, s_scan, s_place);
   if (pl.begin >= pl.end) return;
+  if (tid == 0) {
+    for (int i = 0; i < S; ++i) mbar_init(&s_full[i], 1);
+    mbar_fence_init();
+  }
+  uint32_t phase = 0;  // bit i: of s_full[i]
+  bool landed = true;
+
+  // byte offset of 16-byte chunk c of row r in a stage's K or V; elements by row and dim
+  auto chunk_at = [](int r, int c) { return uint32_t((c >> 3) * L::PANEL + r * 128 + (((c & 7) ^ (r & 7)) << 4)); };
+  auto elem_at = [&](int r, int d) {
+    constexpr int V = 16 / int(sizeof(CT));
+    return chunk_at(r, d / V) + uint32_t(d % V) * uint32_t(sizeof(CT));
+  };
+  // ldmatrix of this warp's 16 keys, two chunks: what a lane adds for its row and chunk (the swizzle's
+  // xor leaves bits 1 and 2 of the chunk apart). K: the matrices go keys first, V (transposed): chunks first
+  const int kw0 = warp * KW;
+  const uint32_t lane_k = uint32_t(kw0 + (lane & 15)) * 128 + (uint32_t((lane >> 4) ^ (lane & 7)) << 4);
+  const uint32_t lane_v = uint32_t(kw0 + (lane & 7) + 8 * (lane >> 4)) * 128 + (uint32_t(((lane >> 3) & 1) ^ (lane & 7)) << 4);
 
   // walk to the unit of the first tile
   int s = pl.seq, kvh = 0, rb = 0;
@@ -352,7 +440,9 @@ __global__ void __launch_bounds__(AT_THREADS) attend_kernel(const __grid_constan
     const CT* kbase = static_cast<const CT*>(a.pool.k) + kvh * a.pool.head_stride;
     const CT* vbase = static_cast<const CT*>(a.pool.v) + kvh * a.pool.head_stride;
 
-    // the page of every key of tile i, into ring slot i % (S + 1)
+    // every key of tile i exists (its page may still be missing): it comes by TMA
+    auto whole_tile = [&](int i) { return box > 0 && (blk.tile0 + i) * TK >= blk.lo && (blk.tile0 + i + 1) * TK <= blk.hi; };
+    // the page of every key of tile i (an element offset where the tile comes by cp.async), into ring slot i % (S + 1)
     auto look_up = [&](int i) {
       if (tid < TK) {
         const int key = (blk.tile0 + i) * TK + tid;
@@ -361,24 +451,39 @@ __global__ void __launch_bounds__(AT_THREADS) attend_kernel(const __grid_constan
         if (key >= blk.lo && key < blk.hi) {
           const int page = __ldg(a.batch.page_table + int64_t(s) * a.batch.max_pages + key / a.pool.page_size);
           if (page >= 0 && page < a.pool.n_pages)
-            off = page * a.pool.page_stride + int64_t(key % a.pool.page_size) * a.pool.token_stride;
+            off = whole_tile(i) ? page : page * a.pool.page_stride + int64_t(key % a.pool.page_size) * a.pool.token_stride;
           else hole = true;
         }
         offs[(i % (S + 1)) * TK + tid] = off;
         const unsigned any = __ballot_sync(0xffffffffu, hole);
-        if (lane == 0) holes[(i % (S + 1)) * (TK / 32) + warp] = any;
+        if (lane == 0) holes[(i % (S + 1)) * 2 + warp] = any;
       }
     };
     auto request = [&](int i) {
       const uint32_t dst = sbase + uint32_t((i % S) * L::STAGE);
+      const long long* ro = offs + (i % (S + 1)) * TK;
+      if (whole_tile(i)) {
+        if (tid == 0) mbar_expect_tx(&s_full[i % S], L::STAGE);
+        if (tid < TK && tid % box == 0) {
+          const long long page = ro[tid];
+          const int at_page = page < 0 ? a.pool.n_pages : int(page);  // a page that is not there: past the last one, zeros
+          const int slot = ((blk.tile0 + i) * TK + tid) % a.pool.page_size;
 #pragma unroll
+          for (int p = 0; p < L::PANELS; ++p) {
+            tma_load(dst + p * L::PANEL + tid * 128, &kmap, p * (128 / int(sizeof(CT))), kvh, slot, at_page, &s_full[i % S]);
+            tma_load(dst + VT + p * L::PANEL + tid * 128, &vmap, p * (128 / int(sizeof(CT))), kvh, slot, at_page, &s_full[i % S]);
+          }
+        }
+        return;
+      }
+#pragma unroll 8
       for (int c = tid; c < TK * CH; c += AT_THREADS) {
         const int key = c / CH, ch = c % CH;
-        const long long off = offs[(i % (S + 1)) * TK + key];
+        const long long off = ro[key];
         const int64_t e = (off < 0 ? 0 : off) + ch * (16 / int(sizeof(CT)));
-        const uint32_t d = dst + uint32_t(key * ROW + ch * 16);
+        const uint32_t d = dst + chunk_at(key, ch);
         cp16(d, kbase + e, off >= 0);
-        cp16(d + TK * ROW, vbase + e, off >= 0);
+        cp16(d + VT, vbase + e, off >= 0);
       }
     };
 
@@ -392,34 +497,28 @@ __global__ void __launch_bounds__(AT_THREADS) attend_kernel(const __grid_constan
       const int gr = r0 + r;
       return static_cast<const AT*>(a.q) + (sq.r0 + gr / a.rep) * a.q_stride + (kvh * a.rep + gr % a.rep) * HD;
     };
-    uint32_t qf[F32A ? 1 : HD / 16][4];
+    uint32_t qf[F32A ? 1 : NB][F32A ? 1 : HD / 16][2];
     if constexpr (!F32A) {
-      const int ra = 16 * wm + g, rc = ra + 8;
-      const AT* pa = q_row(min(ra, rn - 1));
-      const AT* pc = q_row(min(rc, rn - 1));
 #pragma unroll
-      for (int k = 0; k < HD / 16; ++k) {
-        qf[k][0] = __ldg(reinterpret_cast<const uint32_t*>(pa + 16 * k + 2 * t));
-        qf[k][1] = __ldg(reinterpret_cast<const uint32_t*>(pc + 16 * k + 2 * t));
-        qf[k][2] = __ldg(reinterpret_cast<const uint32_t*>(pa + 16 * k + 8 + 2 * t));
-        qf[k][3] = __ldg(reinterpret_cast<const uint32_t*>(pc + 16 * k + 8 + 2 * t));
+      for (int nb = 0; nb < NB; ++nb) {
+        const AT* p = q_row(min(8 * nb + g, rn - 1));
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) {
+          qf[nb][k][0] = __ldg(reinterpret_cast<const uint32_t*>(p + 16 * k + 2 * t));
+          qf[nb][k][1] = __ldg(reinterpret_cast<const uint32_t*>(p + 16 * k + 8 + 2 * t));
+        }
       }
     } else {
-      // fragment order [m-tile][k-step][hi | lo][lane]: k index t is dim 2t (16-bit cache) or t,
-      // k index t + 4 is dim 2t + 1 or t + 4, as the K fragments hold them
-      for (int i = tid; i < WM * (HD / 8) * 32; i += AT_THREADS) {
-        const int ln = i & 31, k = (i >> 5) % (HD / 8), m = (i >> 5) / (HD / 8);
-        const int gg = ln >> 2, tt = ln & 3;
-        const float* pa = reinterpret_cast<const float*>(q_row(min(16 * m + gg, rn - 1))) + 8 * k;
-        const float* pc = reinterpret_cast<const float*>(q_row(min(16 * m + gg + 8, rn - 1))) + 8 * k;
-        const int d0 = F32C ? tt : 2 * tt, d1 = F32C ? tt + 4 : 2 * tt + 1;
-        uint4 hi, lo;
-        split_tf32(__ldg(pa + d0), hi.x, lo.x);
-        split_tf32(__ldg(pc + d0), hi.y, lo.y);
-        split_tf32(__ldg(pa + d1), hi.z, lo.z);
-        split_tf32(__ldg(pc + d1), hi.w, lo.w);
-        qfrag[((m * (HD / 8) + k) * 2) * 32 + ln] = hi;
-        qfrag[((m * (HD / 8) + k) * 2 + 1) * 32 + ln] = lo;
+      // fragment order [nb][k-step][lane]: (hi, hi, lo, lo) of k indices t and t + 4, which are dims 2t and
+      // 2t + 1 (16-bit cache) or t and t + 4, as the K fragments hold them
+      for (int i = tid; i < NB * (HD / 8) * 32; i += AT_THREADS) {
+        const int ln = i & 31, k = (i >> 5) % (HD / 8), nb = (i >> 5) / (HD / 8);
+        const int tt = ln & 3;
+        const float* p = reinterpret_cast<const float*>(q_row(min(8 * nb + (ln >> 2), rn - 1))) + 8 * k;
+        uint4 f;
+        split_tf32(__ldg(p + (F32C ? tt : 2 * tt)), f.x, f.z);
+        split_tf32(__ldg(p + (F32C ? tt + 4 : 2 * tt + 1)), f.y, f.w);
+        qfrag[i] = f;
       }
     }
     __syncthreads();
@@ -429,309 +528,339 @@ __global__ void __launch_bounds__(AT_THREADS) attend_kernel(const __grid_constan
       cp_commit();
     }
 
-    float o[ND][4];
+    float o[MB][NB][4];  // (dim g, row 2t), (dim g, row 2t + 1), (dim g + 8, ..)
 #pragma unroll
-    for (int n = 0; n < ND; ++n)
+    for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[n][e] = 0.0f;
-    float mx[2] = {-INFINITY, -INFINITY}, ls[2] = {0.0f, 0.0f};
-    // positions of this thread's two rows (rows past the block see what its last row sees; nothing of theirs is kept)
-    int pos[2];
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) pos[h] = sq.kv - sq.n + (r0 + min(16 * wm + g + 8 * h, rn - 1)) / a.rep;
+        for (int e = 0; e < 4; ++e) o[mb][nb][e] = 0.0f;
+    // this lane's rows 2t and 2t + 1 of each 8: the maximum (the same in every lane of a row), the lane's part of the sum, the
+    // position (rows past the block see what its last row sees; nothing of theirs is kept)
+    float mx[NB][2], ls[NB][2];
+    int pos[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        mx[nb][h] = -INFINITY;
+        ls[nb][h] = 0.0f;
+        pos[nb][h] = sq.kv - sq.n + (r0 + min(8 * nb + 2 * t + h, rn - 1)) / a.rep;
+      }
 
     bool hole_seen = false;
     for (int i = ta; i < tb; ++i) {
-      cp_wait<S - 2>();
+      if (whole_tile(i)) {
+        landed &= mbar_wait(&s_full[i % S], (phase >> (i % S)) & 1);
+        phase ^= 1u << (i % S);
+      } else {
+        cp_wait<S - 2>();
+        fence_proxy_async();  // the stage may be TMA's next
+      }
       __syncthreads();
       // offs of tile i + S - 1 were written before this barrier; its stage was read before it
       if (i + S - 1 < tb) request(i + S - 1);
       cp_commit();
       if (i + S < tb) look_up(i + S);  // into the place of tile i - 1, which every warp has left
       const int key0 = (blk.tile0 + i) * TK;
-      const uint32_t ks = sbase + uint32_t((i % S) * L::STAGE), vs = ks + TK * ROW;
-      const int kw0 = wn * KW;  // this warp's keys in the tile
-      unsigned gaps = 0;
-#pragma unroll
-      for (int w = 0; w < TK / 32; ++w) gaps |= holes[(i % (S + 1)) * (TK / 32) + w];
-      const bool hole = gaps != 0;
+      const uint32_t ks = sbase + uint32_t((i % S) * L::STAGE), vs = ks + VT;
+      const bool hole = (holes[(i % (S + 1)) * 2] | holes[(i % (S + 1)) * 2 + 1]) != 0;
       hole_seen |= hole;
       // some key of the tile is not seen by every row
       const bool ragged = key0 + TK > min(blk.hi, blk.pos0 + 1) || key0 < blk.lo ||
                           (a.window > 0 && key0 < blk.pos1 - a.window + 1) || hole;
 
-      // S = Q K^T
-      float sc[NT][4];
+      // S^T = K Q^T: (key g, row 2t), (key g, row 2t + 1), (key g + 8, ..)
+      float sc[NB][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[n][e] = 0.0f;
+        for (int e = 0; e < 4; ++e) sc[nb][e] = 0.0f;
       if constexpr (!F32A) {
-        // one ldmatrix.x4: keys 8n .. +8 of two k-steps' halves: (dims 0-7, 8-15, 16-23, 24-31)
 #pragma unroll
-        for (int k = 0; k < HD / 32; ++k) {
+        for (int k = 0; k < HD / 16; ++k) {
+          uint32_t x[4];
+          ldsm4(x, ks + uint32_t((k >> 2) * L::PANEL) + (lane_k ^ uint32_t((k & 3) * 32)));
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            uint32_t b[4];
-            ldsm4(b, ks + uint32_t((kw0 + 8 * n + (lane & 7)) * ROW + (32 * k + 8 * (lane >> 3)) * 2));
-            mma16(sc[n], qf[2 * k], b[0], b[1], AT());
-            mma16(sc[n], qf[2 * k + 1], b[2], b[3], AT());
-          }
-        }
-      } else if constexpr (!F32C) {
-#pragma unroll 2
-        for (int k = 0; k < HD / 32; ++k) {
-          uint32_t qh[4][4], ql[4][4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint4 h = qfrag[((wm * (HD / 8) + 4 * k + j) * 2) * 32 + lane];
-            const uint4 l = qfrag[((wm * (HD / 8) + 4 * k + j) * 2 + 1) * 32 + lane];
-            qh[j][0] = h.x; qh[j][1] = h.y; qh[j][2] = h.z; qh[j][3] = h.w;
-            ql[j][0] = l.x; ql[j][1] = l.y; ql[j][2] = l.z; ql[j][3] = l.w;
-          }
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            uint32_t b[4];
-            ldsm4(b, ks + uint32_t((kw0 + 8 * n + (lane & 7)) * ROW + (32 * k + 8 * (lane >> 3)) * 2));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float2 f = pair_f32<CT>(b[j]);
-              mma8(sc[n], qh[j], __float_as_uint(f.x), __float_as_uint(f.y));
-              mma8(sc[n], ql[j], __float_as_uint(f.x), __float_as_uint(f.y));
-            }
-          }
+          for (int nb = 0; nb < NB; ++nb) mma16(sc[nb], x, qf[nb][k][0], qf[nb][k][1], AT());
         }
       } else {
-#pragma unroll 2
-        for (int k = 0; k < HD / 16; ++k) {
-          uint32_t qh[2][4], ql[2][4];
+        float sl[NB][4];  // the small products
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const uint4 h = qfrag[((wm * (HD / 8) + 2 * k + j) * 2) * 32 + lane];
-            const uint4 l = qfrag[((wm * (HD / 8) + 2 * k + j) * 2 + 1) * 32 + lane];
-            qh[j][0] = h.x; qh[j][1] = h.y; qh[j][2] = h.z; qh[j][3] = h.w;
-            ql[j][0] = l.x; ql[j][1] = l.y; ql[j][2] = l.z; ql[j][3] = l.w;
-          }
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            uint32_t b[4];
-            ldsm4(b, ks + uint32_t((kw0 + 8 * n + (lane & 7)) * ROW + (16 * k + 4 * (lane >> 3)) * 4));
+          for (int e = 0; e < 4; ++e) sl[nb][e] = 0.0f;
+        if constexpr (!F32C) {
+#pragma unroll 4
+          for (int k = 0; k < HD / 16; ++k) {  // two k-steps of 8 dims
+            uint32_t x[4];
+            ldsm4(x, ks + uint32_t((k >> 2) * L::PANEL) + (lane_k ^ uint32_t((k & 3) * 32)));
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              uint32_t h0, l0, h1, l1;
-              split_tf32(__uint_as_float(b[2 * j]), h0, l0);
-              split_tf32(__uint_as_float(b[2 * j + 1]), h1, l1);
-              mma8(sc[n], qh[j], h0, h1);
-              mma8(sc[n], qh[j], l0, l1);
-              mma8(sc[n], ql[j], h0, h1);
+              const float2 u = pair_f32<CT>(x[2 * j]), v = pair_f32<CT>(x[2 * j + 1]);
+              const uint32_t f[4] = {__float_as_uint(u.x), __float_as_uint(v.x), __float_as_uint(u.y), __float_as_uint(v.y)};
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) {
+                const uint4 q = qfrag[(nb * (HD / 8) + 2 * k + j) * 32 + lane];
+                mma8(sc[nb], f, q.x, q.y);
+                mma8(sl[nb], f, q.z, q.w);
+              }
+            }
+          }
+        } else {
+#pragma unroll 4
+          for (int k = 0; k < HD / 8; ++k) {
+            uint32_t x[4], h[4], l[4];
+            ldsm4(x, ks + uint32_t((k >> 2) * L::PANEL) + (lane_k ^ uint32_t((k & 3) * 32)));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) split_tf32(__uint_as_float(x[j]), h[j], l[j]);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+              const uint4 q = qfrag[(nb * (HD / 8) + k) * 32 + lane];
+              mma8(sc[nb], h, q.x, q.y);
+              mma8(sl[nb], l, q.x, q.y);
+              mma8(sl[nb], h, q.z, q.w);
             }
           }
         }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[nb][e] += sl[nb][e];
       }
 
-      // scale, masks, running maximum
-      float top[2] = {mx[0], mx[1]};
+      // scale, masks, maximum
+      bool grow = false;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
+      for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float v = sc[n][e] * a.scale_log2;
+          float v = sc[nb][e] * a.scale_log2;
           if (ragged) {
-            const int kk = kw0 + 8 * n + 2 * t + (e & 1), key = key0 + kk, p = pos[e >> 1];
+            const int kk = kw0 + g + 8 * (e >> 1), key = key0 + kk, p = pos[nb][e & 1];
             const bool seen = key <= p && key < blk.hi && key >= blk.lo && (a.window <= 0 || key > p - a.window) &&
                               (!hole || offs[(i % (S + 1)) * TK + kk] >= 0);
             if (!seen) v = -INFINITY;
           }
-          sc[n][e] = v;
-          top[e >> 1] = fmaxf(top[e >> 1], v);
+          sc[nb][e] = v;
+          grow |= v > mx[nb][e & 1] + SLACK;
         }
       }
-      float fac[2], use[2];
+      const bool moved = __any_sync(0xffffffffu, grow);
+      float fac[NB][2];
+      if (moved) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-        use[h] = top[h] == -INFINITY ? 0.0f : top[h];
-        fac[h] = fast_exp2(mx[h] - use[h]);
-        mx[h] = top[h];
-        ls[h] *= fac[h];
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float top = fmaxf(mx[nb][h], fmaxf(sc[nb][h], sc[nb][h + 2]));
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            fac[nb][h] = mx[nb][h] == top ? 1.0f : fast_exp2(mx[nb][h] - top);
+            mx[nb][h] = top;
+            ls[nb][h] *= fac[nb][h];
+          }
+        // O takes its factor here: a maximum moves in the first tile and rarely after it
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[mb][nb][e] *= fac[nb][e & 1];
       }
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          sc[n][e] = fast_exp2(sc[n][e] - use[e >> 1]);
-          ls[e >> 1] += sc[n][e];
+          const float m = mx[nb][e & 1];
+          sc[nb][e] = fast_exp2(sc[nb][e] - (m == -INFINITY ? 0.0f : m));
+          ls[nb][e & 1] += sc[nb][e];
         }
-#pragma unroll
-      for (int n = 0; n < ND; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[n][e] *= fac[e >> 1];
 
       // keys that some rows see and others do not: an infinity or NaN among their values is added
       // to the rows that see it, and taken out of the tile
-      if (ragged && (blk.pos1 > blk.pos0)) {
+      if (ragged && blk.pos1 > blk.pos0) {
         bool odd = false;
-        CT* vt = reinterpret_cast<CT*>(sm + (i % S) * L::STAGE + TK * ROW);
-        for (int c = tid; c < TK * HD; c += AT_THREADS) {
-          const float v = to_f32(vt[(c / HD) * (ROW / int(sizeof(CT))) + c % HD]);
-          odd |= !(fabsf(v) <= FLT_MAX);
-        }
+        uint8_t* vt = sm + (i % S) * L::STAGE + VT;
+        auto val = [&](int r, int d) -> CT& { return *reinterpret_cast<CT*>(vt + elem_at(r, d)); };
+        for (int c = tid; c < TK * HD; c += AT_THREADS) odd |= !(fabsf(to_f32(val(c / HD, c % HD))) <= FLT_MAX);
         if (__syncthreads_or(odd)) {
           for (int kk = kw0; kk < kw0 + KW; ++kk) {
             const int key = key0 + kk;
 #pragma unroll
-            for (int n = 0; n < ND; ++n)
+            for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float v = to_f32(vt[kk * (ROW / int(sizeof(CT))) + 8 * n + 2 * t + (e & 1)]);
-                const int p = pos[e >> 1];
-                if (!(fabsf(v) <= FLT_MAX) && key <= p && (a.window <= 0 || key > p - a.window)) o[n][e] += v;
-              }
+              for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float v = to_f32(val(kk, 16 * mb + g + 8 * (e >> 1)));
+                  const int p = pos[nb][e & 1];
+                  if (!(fabsf(v) <= FLT_MAX) && key <= p && (a.window <= 0 || key > p - a.window)) o[mb][nb][e] += v;
+                }
           }
           __syncthreads();
           for (int c = tid; c < TK * HD; c += AT_THREADS) {
-            CT* x = vt + (c / HD) * (ROW / int(sizeof(CT))) + c % HD;
-            if (!(fabsf(to_f32(*x)) <= FLT_MAX)) *x = from_f32<CT>(0.0f);
+            CT& x = val(c / HD, c % HD);
+            if (!(fabsf(to_f32(x)) <= FLT_MAX)) x = from_f32<CT>(0.0f);
           }
+          fence_proxy_async();
           __syncthreads();
         }
       }
 
-      // O += P V
+      // O^T += V^T P^T
       if constexpr (!F32A) {
+        uint32_t ph[NB][2], pw[NB][2];  // keys 2t, 2t + 1 (and + 8) of row g: S^T's blocks transposed
 #pragma unroll
-        for (int k = 0; k < KW / 16; ++k) {
-          uint32_t ph[4], pl2[4];
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float x = sc[2 * k + (j >> 1)][(j & 1) * 2], y = sc[2 * k + (j >> 1)][(j & 1) * 2 + 1];
-            ph[j] = pack2<AT>(x, y);
+          for (int h = 0; h < 2; ++h) {
+            const float x = sc[nb][2 * h], y = sc[nb][2 * h + 1];
+            const uint32_t w = pack2<AT>(x, y);
+            ph[nb][h] = transposed8(w);
             if constexpr (L::TWO_P) {
-              const float2 f = pair_f32<AT>(ph[j]);
-              pl2[j] = pack2<AT>(x - f.x, y - f.y);
+              const float2 f = pair_f32<AT>(w);
+              pw[nb][h] = transposed8(pack2<AT>(x - f.x, y - f.y));
             }
           }
-          // one ldmatrix.x4.trans: 16 keys x 16 dims
 #pragma unroll
-          for (int n = 0; n < ND / 2; ++n) {
-            uint32_t b[4];
-            ldsm4t(b, vs + uint32_t((kw0 + 16 * k + (lane & 15)) * ROW + (16 * n + 8 * (lane >> 4)) * 2));
-            mma16(o[2 * n], ph, b[0], b[1], AT());
-            mma16(o[2 * n + 1], ph, b[2], b[3], AT());
-            if constexpr (L::TWO_P) {
-              mma16(o[2 * n], pl2, b[0], b[1], AT());
-              mma16(o[2 * n + 1], pl2, b[2], b[3], AT());
-            }
+        for (int mb = 0; mb < MB; ++mb) {
+          uint32_t x[4];
+          ldsm4t(x, vs + uint32_t((mb >> 2) * L::PANEL) + (lane_v ^ uint32_t((mb & 3) * 32)));
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            mma16(o[mb][nb], x, ph[nb][0], ph[nb][1], AT());
+            if constexpr (L::TWO_P) mma16(o[mb][nb], x, pw[nb][0], pw[nb][1], AT());
           }
         }
       } else {
+        // two k-steps of 8 keys. k index t and t + 4: keys 2t and 2t + 1 (16-bit cache) or t and t + 4. P's values
+        // for them lie in other lanes: of key k and row g in lane 4 k + g / 2
+        uint32_t ph[2][NB][2], pw[2][NB][2];
 #pragma unroll
-        for (int k = 0; k < NT; ++k) {  // 8 keys: key 2t is k index t, key 2t + 1 is t + 4
-          uint32_t ph[4], pw[4];
-          split_tf32(sc[k][0], ph[0], pw[0]);
-          split_tf32(sc[k][2], ph[1], pw[1]);
-          split_tf32(sc[k][1], ph[2], pw[2]);
-          split_tf32(sc[k][3], ph[3], pw[3]);
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int key = F32C ? t + 4 * h : 2 * t + h;
+              const float x = __shfl_sync(0xffffffffu, sc[nb][2 * j], 4 * key + (g >> 1));
+              const float y = __shfl_sync(0xffffffffu, sc[nb][2 * j + 1], 4 * key + (g >> 1));
+              split_tf32((g & 1) ? y : x, ph[j][nb][h], pw[j][nb][h]);
+            }
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+          float x[NB][4];
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[nb][e] = 0.0f;
           if constexpr (!F32C) {
+            uint32_t w[4];
+            ldsm4t(w, vs + uint32_t((mb >> 2) * L::PANEL) + (lane_v ^ uint32_t((mb & 3) * 32)));
 #pragma unroll
-            for (int n = 0; n < ND / 4; ++n) {  // 8 keys x 32 dims
-              uint32_t b[4];
-              ldsm4t(b, vs + uint32_t((kw0 + 8 * k + (lane & 7)) * ROW + (32 * n + 8 * (lane >> 3)) * 2));
+            for (int j = 0; j < 2; ++j) {
+              const float2 u = pair_f32<CT>(w[2 * j]), v = pair_f32<CT>(w[2 * j + 1]);
+              const uint32_t f[4] = {__float_as_uint(u.x), __float_as_uint(v.x), __float_as_uint(u.y), __float_as_uint(v.y)};
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const float2 f = pair_f32<CT>(b[j]);
-                mma8(o[4 * n + j], ph, __float_as_uint(f.x), __float_as_uint(f.y));
-                mma8(o[4 * n + j], pw, __float_as_uint(f.x), __float_as_uint(f.y));
+              for (int nb = 0; nb < NB; ++nb) {
+                mma8(x[nb], f, pw[j][nb][0], pw[j][nb][1]);
+                mma8(x[nb], f, ph[j][nb][0], ph[j][nb][1]);
               }
             }
           } else {
 #pragma unroll
-            for (int n = 0; n < ND; ++n) {
-              const float f0 = ldsf(vs + uint32_t((kw0 + 8 * k + 2 * t) * ROW + (8 * n + g) * 4));
-              const float f1 = ldsf(vs + uint32_t((kw0 + 8 * k + 2 * t + 1) * ROW + (8 * n + g) * 4));
-              uint32_t h0, l0, h1, l1;
-              split_tf32(f0, h0, l0);
-              split_tf32(f1, h1, l1);
-              mma8(o[n], ph, h0, h1);
-              mma8(o[n], ph, l0, l1);
-              mma8(o[n], pw, h0, h1);
+            for (int j = 0; j < 2; ++j) {
+              uint32_t h[4], l[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)  // (dim g, key t), (dim g + 8, key t), (.., key t + 4)
+                split_tf32(ldsf(vs + elem_at(kw0 + 8 * j + t + 4 * (e >> 1), 16 * mb + g + 8 * (e & 1))), h[e], l[e]);
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) {
+                mma8(x[nb], l, ph[j][nb][0], ph[j][nb][1]);
+                mma8(x[nb], h, pw[j][nb][0], pw[j][nb][1]);
+                mma8(x[nb], h, ph[j][nb][0], ph[j][nb][1]);
+              }
             }
           }
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[mb][nb][e] += x[nb][e];
         }
       }
     }
     cp_wait<0>();
+    if (!landed) report(a.batch, ST_ABORTED);
     if (hole_seen && tid == 0) report(a.batch, ST_BAD_PAGE);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {  // the four lanes of a row
-      ls[h] += __shfl_xor_sync(0xffffffffu, ls[h], 1);
-      ls[h] += __shfl_xor_sync(0xffffffffu, ls[h], 2);
-    }
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) ls[nb][h] += __shfl_xor_sync(0xffffffffu, ls[nb][h], d);
     if (tid == 0 && blk.pos1 >= table) report(a.batch, ST_BAD_PAGE);
     if (tid == 0 && blk.pos0 < 0) report(a.batch, ST_BAD_LEN);
 
+    // four results of row r from dim d on, l and m of the row
+    auto finish = [&](int r, int d, float4 x, float m, float l) {
+      const int gr = r0 + r;
+      const bool some = l > 0.0f || l != l;
+      const float inv = some ? 1.0f / l : 0.0f;
+      const int64_t tok = sq.r0 + gr / a.rep;
+      const int hh = kvh * a.rep + gr % a.rep;
+      AT* dst = static_cast<AT*>(a.out) + tok * a.out_stride + hh * HD + d;
+      const float v0 = some ? x.x * inv : 0.0f, v1 = some ? x.y * inv : 0.0f;
+      const float v2 = some ? x.z * inv : 0.0f, v3 = some ? x.w * inv : 0.0f;
+      if constexpr (F32A) *reinterpret_cast<float4*>(dst) = make_float4(v0, v1, v2, v3);
+      else *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<AT>(v0, v1), pack2<AT>(v2, v3));
+      if (d == 0 && a.lse) a.lse[tok * a.n_heads + hh] = some ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
+    };
+
+    // the four warps' results, joined through shared memory (the ring is empty)
     const bool whole = ta == 0 && tb == blk.tiles;
     float* piece = a.part + (size_t(blockIdx.x) * 2 + (ta == 0 ? 1 : 0)) * size_t(M) * (HD + 2);  // [M][HD], then [M][2]
-    auto put = [&](int r, int d, float x, float y, float m, float l) {  // two results of row r
-      if (whole) {
-        const int gr = r0 + r;
-        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-        AT* dst = static_cast<AT*>(a.out) + (sq.r0 + gr / a.rep) * a.out_stride + (kvh * a.rep + gr % a.rep) * HD + d;
-        const bool some = inv != 0.0f || l != l;
-        x = some ? x * inv : 0.0f;
-        y = some ? y * inv : 0.0f;
-        if constexpr (F32A) *reinterpret_cast<float2*>(dst) = make_float2(x, y);
-        else *reinterpret_cast<uint32_t*>(dst) = pack2<AT>(x, y);
-        if (d == 0 && a.lse)
-          a.lse[int64_t(sq.r0 + gr / a.rep) * a.n_heads + kvh * a.rep + gr % a.rep] =
-              some ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
-      } else {
-        *reinterpret_cast<float2*>(piece + size_t(r) * HD + d) = make_float2(x, y);
-        if (d == 0) *reinterpret_cast<float2*>(piece + size_t(M) * HD + 2 * r) = make_float2(m, l);
-      }
-    };
-    if constexpr (WN == 1) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = 16 * wm + g + 8 * h;
-        if (r < rn)
-#pragma unroll
-          for (int n = 0; n < ND; ++n) put(r, 8 * n + 2 * t, o[n][2 * h], o[n][2 * h + 1], mx[h], ls[h]);
-      }
-    } else {
-      // the WN warps of a row tile, joined through shared memory (the ring is empty)
+    {
       float* os = reinterpret_cast<float*>(sm);
-      float2* ml = reinterpret_cast<float2*>(sm + 4 * 16 * L::OPITCH * 4);
+      float2* ml = reinterpret_cast<float2*>(sm + 4 * M * L::OPITCH * 4);
       __syncthreads();
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = warp * 16 + g + 8 * h;
+      for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-        for (int n = 0; n < ND; ++n)
-          *reinterpret_cast<float2*>(os + r * L::OPITCH + 8 * n + 2 * t) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
-        if (t == 0) ml[r] = make_float2(mx[h], ls[h]);
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int mb = 0; mb < MB; ++mb)
+            os[(warp * M + 8 * nb + 2 * t + (e & 1)) * L::OPITCH + 16 * mb + g + 8 * (e >> 1)] = o[mb][nb][e];
+        if (g == 0) {
+          ml[warp * M + 8 * nb + 2 * t] = make_float2(mx[nb][0], ls[nb][0]);
+          ml[warp * M + 8 * nb + 2 * t + 1] = make_float2(mx[nb][1], ls[nb][1]);
+        }
       }
       __syncthreads();
-      for (int c = tid; c < rn * (HD / 2); c += AT_THREADS) {
-        const int r = c / (HD / 2), d = 2 * (c % (HD / 2));
-        const int w0 = r / 16, rr = r % 16;  // warps w0, w0 + WM, ..
+      for (int c = tid; c < rn * (HD / 4); c += AT_THREADS) {
+        const int r = c / (HD / 4), d = 4 * (c % (HD / 4));
         float m = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < WN; ++j) m = fmaxf(m, ml[(w0 + j * WM) * 16 + rr].x);
+        for (int w = 0; w < 4; ++w) m = fmaxf(m, ml[w * M + r].x);
         const float u = m == -INFINITY ? 0.0f : m;
-        float l = 0.0f, x = 0.0f, y = 0.0f;
+        float l = 0.0f;
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int j = 0; j < WN; ++j) {
-          const int w = (w0 + j * WM) * 16 + rr;
-          const float2 q = ml[w];
+        for (int w = 0; w < 4; ++w) {
+          const float2 q = ml[w * M + r];
           const float f = fast_exp2(q.x - u);
-          const float2 v = *reinterpret_cast<const float2*>(os + w * L::OPITCH + d);
+          const float4 v = *reinterpret_cast<const float4*>(os + (w * M + r) * L::OPITCH + d);
           l += f * q.y;
-          x += f * v.x;
-          y += f * v.y;
+          x.x += f * v.x;
+          x.y += f * v.y;
+          x.z += f * v.z;
+          x.w += f * v.w;
         }
-        put(r, d, x, y, m, l);
+        if (whole) finish(r, d, x, m, l);
+        else {
+          *reinterpret_cast<float4*>(piece + size_t(r) * HD + d) = x;
+          if (d == 0) *reinterpret_cast<float2*>(piece + size_t(M) * HD + 2 * r) = make_float2(m, l);
+        }
       }
     }
 
@@ -747,16 +876,15 @@ __global__ void __launch_bounds__(AT_THREADS) attend_kernel(const __grid_constan
         __threadfence();
         for (int c = tid; c < rn * (HD / 4); c += AT_THREADS) {
           const int r = c / (HD / 4), d = 4 * (c % (HD / 4));
+          auto part = [&](int p) { return a.part + (size_t(p) * 2 + (p == c0 ? 1 : 0)) * size_t(M) * (HD + 2); };
           float m = -INFINITY;
-          for (int p = c0; p <= c1; ++p) {
-            const float* pc = a.part + (size_t(p) * 2 + (p == c0 ? 1 : 0)) * size_t(M) * (HD + 2);
-            m = fmaxf(m, __ldcg(reinterpret_cast<const float2*>(pc + size_t(M) * HD + 2 * r)).x);
-          }
+          for (int p = c0; p <= c1; ++p) m = fmaxf(m, __ldcg(reinterpret_cast<const float2*>(part(p) + size_t(M) * HD + 2 * r)).x);
           const float u = m == -INFINITY ? 0.0f : m;
           float l = 0.0f;
           float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
           for (int p = c0; p <= c1; ++p) {
-            const float* pc = a.part + (size_t(p) * 2 + (p == c0 ? 1 : 0)) * size_t(M) * (HD + 2);
+            const float* pc = part(p);
             const float2 q = __ldcg(reinterpret_cast<const float2*>(pc + size_t(M) * HD + 2 * r));
             const float4 v = __ldcg(reinterpret_cast<const float4*>(pc + size_t(r) * HD + d));
             const float f = fast_exp2(q.x - u);
@@ -766,17 +894,7 @@ __global__ void __launch_bounds__(AT_THREADS) attend_kernel(const __grid_constan
             x.z += f * v.z;
             x.w += f * v.w;
           }
-          const int gr = r0 + r;
-          const bool some = l > 0.0f || l != l;
-          const float inv = some ? 1.0f / l : 0.0f;
-          const int64_t tok = sq.r0 + gr / a.rep;
-          const int hh = kvh * a.rep + gr % a.rep;
-          AT* dst = static_cast<AT*>(a.out) + tok * a.out_stride + hh * HD + d;
-          const float v0 = some ? x.x * inv : 0.0f, v1 = some ? x.y * inv : 0.0f;
-          const float v2 = some ? x.z * inv : 0.0f, v3 = some ? x.w * inv : 0.0f;
-          if constexpr (F32A) *reinterpret_cast<float4*>(dst) = make_float4(v0, v1, v2, v3);
-          else *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<AT>(v0, v1), pack2<AT>(v2, v3));
-          if (d == 0 && a.lse) a.lse[tok * a.n_heads + hh] = some ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
+          finish(r, d, x, m, l);
         }
       }
     }
@@ -801,23 +919,25 @@ __global__ void __launch_bounds__(AT_THREADS) attend_kernel(const __grid_constan
   }
 }
 
-template <typename AT, typename CT, int HD, int WM>
+template <typename AT, typename CT, int HD, int NB>
 cudaError_t run_attend(const AttendArgs& a, cudaStream_t st) {
-  using L = AttnCfg<AT, CT, HD, WM>;
+  using L = AttnCfg<AT, CT, HD, NB>;
   static_assert(L::SMEM <= 227 * 1024, "shared memory");
   // the limit is a property of the kernel on the current device: set on every call (no
   // state that a second device or thread could find half made)
-  cudaError_t e = cudaFuncSetAttribute(attend_kernel<AT, CT, HD, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+  cudaError_t e = cudaFuncSetAttribute(attend_kernel<AT, CT, HD, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
   if (e != cudaSuccess) return e;
-  attend_kernel<AT, CT, HD, WM><<<ATTEND_CTAS, AT_THREADS, L::SMEM, st>>>(a);
+  CUtensorMap km{}, vm{};
+  const int box = make_maps<CT>(&km, &vm, a.pool, L::TK);
+  attend_kernel<AT, CT, HD, NB><<<ATTEND_CTAS, AT_THREADS, L::SMEM, st>>>(a, km, vm, box);
   return cudaGetLastError();
 }
 
 template <typename AT, typename CT>
 cudaError_t run_attend_rows(const AttendArgs& a, int rows, cudaStream_t st) {
   if (a.pool.head_dim == 64)
-    return rows == 16 ? run_attend<AT, CT, 64, 1>(a, st) : rows == 32 ? run_attend<AT, CT, 64, 2>(a, st) : run_attend<AT, CT, 64, 4>(a, st);
-  return rows == 16 ? run_attend<AT, CT, 128, 1>(a, st) : rows == 32 ? run_attend<AT, CT, 128, 2>(a, st) : run_attend<AT, CT, 128, 4>(a, st);
+    return rows == 8 ? run_attend<AT, CT, 64, 1>(a, st) : rows == 16 ? run_attend<AT, CT, 64, 2>(a, st) : run_attend<AT, CT, 64, 4>(a, st);
+  return rows == 8 ? run_attend<AT, CT, 128, 1>(a, st) : rows == 16 ? run_attend<AT, CT, 128, 2>(a, st) : run_attend<AT, CT, 128, 4>(a, st);
 }
 
 }  // namespace

@@ -13,15 +13,22 @@
 //   S = Q K^T      tcgen05.mma, both operands from shared memory, S in TMEM (f32)
 //   P = 2^(S - m)  read from TMEM, rounded to 16 bits, written back over S
 //   O += P V       tcgen05.mma, P from TMEM, V as it lies ([key][dim]: N-major)
-// The products of one tile of rows run while the other's softmax does: 128 x 128
-// exponentials at 16 a clock take as long as the tile's two products, so each of
-// the two units is the other's bound. The running maximum moves only when it grows
-// by more than 2^8 (O in TMEM is rescaled then; sums in f32 and P in 16 bits have
-// room for that factor), which is rare after the first tiles.
+// S is made in two halves of 64 keys, each with its own barriers, so that one half's
+// products run while the other's exponentials do (S in one piece: every tile
+// waited for its own two products, 2.64 ms against 2.42 at the size below; a half
+// costs more shared-memory reads of Q, so that the products of a tile of 128 keys
+// take 2560 clocks of the SM instead of 2048).
+// The running maximum is taken anew only where a half's sum of exponentials shows
+// that it has to be (O in TMEM is rescaled then; sums in f32 and P in 16 bits have
+// room for the factor): one vote on the sum instead of 64 comparisons a row.
 // TMEM: S0 | S1 | O0 | O1, 512 columns at head_dim 128.
-#include <cuda.h>
-#include <cudaTypedefs.h>
-
+//
+// 2047 new tokens over 32767 keys, 64/8 heads of 128, bf16: 2.36 ms, 903 TFLOP/s (54 %
+// of the measured cuBLAS rate). What bounds it: the exponentials of the two softmax warps of
+// a scheduler and what surrounds them (1250 clocks a half with both row tiles; 600 without
+// the exponentials themselves, when the products' 2560 clocks become the bound, 2.0 ms).
+// Part of the exponentials by a polynomial on the multiply-add units (a quarter, an eighth) gained
+// nothing: those pay as many clocks for it.
 #include "paged_attn.cuh"
 
 namespace wcb {
@@ -32,7 +39,7 @@ constexpr int TC_THREADS = 448;  // 2 softmax warpgroups, 4 loader warps, 2 issu
 constexpr int TC_TK = 128;
 constexpr int TC_M = 256;
 constexpr int TILE_PANEL = 128 * 128;  // bytes of 128 rows x 64 dims
-constexpr int POLY_OF = 4;     // of so many pairs of exponentials one goes to the multiply-add units
+constexpr float GROWTH = 8192.0f;  // a half's sum of exponentials may grow to this before the maximum is taken anew
 constexpr int HOLE_RING = 8;   // tiles: the loaders are at most 4 ahead of the softmax
 constexpr int ODD_RING = 16;   // units, likewise
 
@@ -134,35 +141,6 @@ __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
   return r;
 }
 
-// 2^x for two x <= 127 on the multiply-add units, for part of the exponentials: x = n + f with n the nearest
-// whole number (by adding 1.5 2^23), a polynomial of degree 5 in f on [-1/2, 1/2] fitted for the least largest
-// relative error (2^-22 as evaluated in 32 bits, as much as ex2.approx), n added to the exponent. Below -125 it
-// stays 2^-125. f keeps NaN (its result's bits do not): `nan` collects it.
-__device__ __forceinline__ float max_nan(float x, float y) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ void poly_exp2(uint64_t v, float& x, float& y, uint64_t& nan) {
-  float a, b;
-  unpack_f32x2(v, a, b);
-  const uint64_t c = pack_f32x2(max_nan(a, -125.0f), max_nan(b, -125.0f));
-  const uint64_t t = add_f32x2(c, pack_f32x2(12582912.0f, 12582912.0f));
-  const uint64_t f = fma_f32x2(add_f32x2(t, pack_f32x2(-12582912.0f, -12582912.0f)), pack_f32x2(-1.0f, -1.0f), c);
-  nan = add_f32x2(nan, f);
-  uint64_t p = pack_f32x2(0.0013277939287945628f, 0.0013277939287945628f);
-  p = fma_f32x2(p, f, pack_f32x2(0.009675757959485054f, 0.009675757959485054f));
-  p = fma_f32x2(p, f, pack_f32x2(0.05550709739327431f, 0.05550709739327431f));
-  p = fma_f32x2(p, f, pack_f32x2(0.24022114276885986f, 0.24022114276885986f));
-  p = fma_f32x2(p, f, pack_f32x2(0.6931469440460205f, 0.6931469440460205f));
-  p = fma_f32x2(p, f, pack_f32x2(1.0000001192092896f, 1.0000001192092896f));
-  float ta, tb;
-  unpack_f32x2(p, a, b);
-  unpack_f32x2(t, ta, tb);
-  x = __uint_as_float(__float_as_uint(a) + (__float_as_uint(ta) << 23));
-  y = __uint_as_float(__float_as_uint(b) + (__float_as_uint(tb) << 23));
-}
-
 struct TcShared {
   uint64_t full[8], empty[8];  // ring slots
   uint64_t q_full[2], s_full[2][2], p_full[2][2], o_done[2][2];  // [row tile][half of the keys]
@@ -190,36 +168,6 @@ __device__ __forceinline__ bool tc_wait(TcShared* sh, uint64_t* bar, uint32_t pa
   }
   *reinterpret_cast<volatile int*>(&sh->abort) = 1;
   return false;
-}
-
-// The same by polling without suspension: a suspended thread wakes about 150 clocks late, which the chain
-// of a tile of keys (S, softmax, product, S, ..) pays several times.
-__device__ __forceinline__ bool tc_spin_warp(TcShared* sh, uint64_t* bar, uint32_t parity) {
-  const uint32_t addr = smem_u32(bar);
-  bool done = false;
-  for (uint32_t it = 0; it < (1u << 26); ++it) {
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(ok)
-        : "r"(addr), "r"(parity)
-        : "memory");
-    if (ok) {
-      done = true;
-      break;
-    }
-    if ((it & 255) == 255 && *reinterpret_cast<volatile int*>(&sh->abort)) break;
-  }
-  if (!done) *reinterpret_cast<volatile int*>(&sh->abort) = 1;
-  return __all_sync(0xffffffffu, done);
-}
-
-// box of tokens of one head: dims x .. x + 63 (x a multiple of 64), tokens from `slot` of `page`
-__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int head, int slot, int page, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-      "l"(map), "r"(x), "r"(head), "r"(slot), "r"(page), "r"(smem_u32(bar))
-      : "memory");
 }
 
 // the same for a whole warp, which goes on or leaves together
@@ -419,7 +367,7 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
             if (more) ok = ok && tc_wait_warp(&sh, &sh.full[slot], phase);
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-              ok = ok && tc_spin_warp(&sh, &sh.p_full[w][b], t & 1);
+              ok = ok && tc_wait_warp(&sh, &sh.p_full[w][b], t & 1);
               if (!ok) break;
               tc_fence_after();
               if (one) {
@@ -431,7 +379,7 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
               }
               __syncwarp();
               if (more) {  // the next S lies over this P: its product has to be done
-                ok = tc_spin_warp(&sh, &sh.o_done[w][b], t & 1);
+                ok = tc_wait_warp(&sh, &sh.o_done[w][b], t & 1);
                 if (!ok) break;
                 product_s(slot, b);
               }
@@ -612,48 +560,12 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
               for (int e = 0; e < 64; ++e)
                 if (!((seen[e / 32] >> (e % 32)) & 1)) v[e] = none;
             }
-            float top;
-            if (a.scale_log2 >= 0.0f) {
-              float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-              for (int e = 0; e < 64; e += 8)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[j] = fmaxf(x[j], fmaxf(__uint_as_float(v[e + 2 * j]), __uint_as_float(v[e + 2 * j + 1])));
-              top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * a.scale_log2;
-            } else {  // a negative scale turns the order round
-              float x = INFINITY;
-#pragma unroll
-              for (int e = 0; e < 64; ++e) x = fminf(x, __uint_as_float(v[e]));
-              top = x * a.scale_log2;
-            }
-            // rescale where some row's maximum grew by more than 2^8
-            const bool grow = top > m + 8.0f;  // also the first finite one
-            if (__any_sync(0xffffffffu, grow)) {
-              const float nm = fmaxf(m, top);
-              const float f = m == nm ? 1.0f : fast_exp2(m - (nm == -INFINITY ? 0.0f : nm));
-              if (i > wk.ta || b) {  // after the last product
-                ok = tc_wait_warp(&sh, &sh.o_done[w][1 - b], (b ? t : t - 1) & 1);
-                if (!ok) break;
-                tc_fence_after();
-#pragma unroll 1
-                for (int q = 0; q < HD / 16; ++q) {
-                  uint32_t o[16];
-                  tmem_ld16(to + 16 * q, o);
-                  tmem_wait_ld();
-#pragma unroll
-                  for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                  tmem_st16(to + 16 * q, o);
-                }
-              }
-              l *= f;
-              m = nm;
-            }
             const uint64_t scale2 = pack_f32x2(a.scale_log2, a.scale_log2);
-            const float use = m == -INFINITY ? 0.0f : m;
-            const uint64_t use2 = pack_f32x2(-use, -use);
-            uint64_t sum[2] = {0, 0}, nan = 0;
-            // masked products need their zeros exactly: all of them by ex2.approx
-            auto exponentials = [&](auto poly) {
+            uint64_t sum[2];
+            auto exponentials = [&] {  // P, into S's place, and its sum
+              const float use = m == -INFINITY ? 0.0f : m;
+              const uint64_t use2 = pack_f32x2(-use, -use);
+              sum[0] = sum[1] = 0;
 #pragma unroll
               for (int q = 0; q < 2; ++q) {
                 uint32_t p[16];
@@ -661,31 +573,73 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
                 for (int e = 0; e < 16; ++e) {
                   float x, y;
                   const uint64_t z = fma_f32x2(pack_f32x2(__uint_as_float(v[32 * q + 2 * e]), __uint_as_float(v[32 * q + 2 * e + 1])), scale2, use2);
-                  if (decltype(poly)::value && e % POLY_OF == POLY_OF - 1) {
-                    poly_exp2(z, x, y, nan);
-                  } else {
-                    unpack_f32x2(z, x, y);
-                    x = fast_exp2(x);
-                    y = fast_exp2(y);
-                  }
+                  unpack_f32x2(z, x, y);
+                  x = fast_exp2(x);
+                  y = fast_exp2(y);
                   sum[e & 1] = add_f32x2(sum[e & 1], pack_f32x2(x, y));
                   p[e] = pack2<T>(x, y);
                 }
                 tmem_st16(ts + 64 * b + 16 * q, p);
               }
             };
-            if (mask) exponentials(std::false_type());
-            else exponentials(std::true_type());
+            auto total = [&] {
+              float x0, y0, x1, y1;
+              unpack_f32x2(sum[0], x0, y0);
+              unpack_f32x2(sum[1], x1, y1);
+              return (x0 + y0) + (x1 + y1);
+            };
+            // Most halves need no maximum: the last one still serves as long as the sum shows that no
+            // exponential left the range of f16 and of a sound sum (GROWTH); a row's sum is wanted anyway.
+            float part;
+            bool again = __any_sync(0xffffffffu, mask || m == -INFINITY);
+            if (!again) {
+              exponentials();
+              part = total();
+              again = __any_sync(0xffffffffu, !(part <= GROWTH));
+            }
+            if (again) {
+              float top;
+              if (a.scale_log2 >= 0.0f) {
+                float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int e = 0; e < 64; e += 8)
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) x[j] = fmaxf(x[j], fmaxf(__uint_as_float(v[e + 2 * j]), __uint_as_float(v[e + 2 * j + 1])));
+                top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * a.scale_log2;
+              } else {  // a negative scale turns the order round
+                float x = INFINITY;
+#pragma unroll
+                for (int e = 0; e < 64; ++e) x = fminf(x, __uint_as_float(v[e]));
+                top = x * a.scale_log2;
+              }
+              if (__any_sync(0xffffffffu, top > m)) {
+                const float nm = fmaxf(m, top);
+                const float f = m == nm ? 1.0f : fast_exp2(m - (nm == -INFINITY ? 0.0f : nm));
+                if (i > wk.ta || b) {  // after the last product
+                  ok = tc_wait_warp(&sh, &sh.o_done[w][1 - b], (b ? t : t - 1) & 1);
+                  if (!ok) break;
+                  tc_fence_after();
+#pragma unroll 1
+                  for (int q = 0; q < HD / 16; ++q) {
+                    uint32_t o[16];
+                    tmem_ld16(to + 16 * q, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                    tmem_st16(to + 16 * q, o);
+                  }
+                }
+                l *= f;
+                m = nm;
+              }
+              exponentials();
+              part = total();
+            }
+            l += part;
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive(&sh.p_full[w][b]);
-            float x0, y0, x1, y1;
-            unpack_f32x2(sum[0], x0, y0);
-            unpack_f32x2(sum[1], x1, y1);
-            l += (x0 + y0) + (x1 + y1);
-            unpack_f32x2(nan, x0, y0);
-            if (x0 != x0 || y0 != y0) l = x0 + y0;
           }
           ++t;
         }
@@ -815,40 +769,14 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
   if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
-// Tensor map of the pool's keys or values: (dim, head, token, page), boxes of 64 dims x `box` tokens.
-// False where the pool cannot be described: strides of 2^40 bytes and more.
-bool make_map(CUtensorMap* map, const Pool& p, const void* base, bool bf16, int box) {
-  static const PFN_cuTensorMapEncodeTiled encode = [] {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) f = nullptr;
-    return reinterpret_cast<PFN_cuTensorMapEncodeTiled>(f);
-  }();
-  if (!encode) return false;
-  const cuuint64_t dims[4] = {cuuint64_t(p.head_dim), cuuint64_t(p.n_kv), cuuint64_t(p.page_size), cuuint64_t(p.n_pages)};
-  // a dimension of one may have any stride: one that the encoder takes
-  const cuuint64_t least = cuuint64_t(p.head_dim) * 2;
-  const cuuint64_t strides[3] = {p.n_kv > 1 ? cuuint64_t(p.head_stride) * 2 : least, p.page_size > 1 ? cuuint64_t(p.token_stride) * 2 : least,
-                                 p.n_pages > 1 ? cuuint64_t(p.page_stride) * 2 : least};
-  for (cuuint64_t s : strides)
-    if (s >= (cuuint64_t(1) << 40)) return false;
-  const cuuint32_t boxes[4] = {64, 1, cuuint32_t(box), 1}, steps[4] = {1, 1, 1, 1};
-  return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, boxes,
-                steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <typename T, int HD>
 cudaError_t run_tc(const AttendArgs& a, cudaStream_t s) {
   using L = TcCfg<HD>;
   static_assert(L::SMEM + sizeof(TcShared) <= 227 * 1024, "shared memory");
   cudaError_t e = cudaFuncSetAttribute(attend_tc_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
   if (e != cudaSuccess) return e;
-  int box = TC_TK;
-  while (a.pool.page_size % box) box /= 2;
   CUtensorMap km{}, vm{};
-  constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
-  if (box < 8 || !make_map(&km, a.pool, a.pool.k, BF, box) || !make_map(&vm, a.pool, a.pool.v, BF, box)) box = 0;
+  const int box = make_maps<T>(&km, &vm, a.pool, TC_TK);
   attend_tc_kernel<T, HD><<<TC_CTAS, TC_THREADS, L::SMEM, s>>>(a, km, vm, box);
   return cudaGetLastError();
 }
