@@ -64,12 +64,13 @@ struct VerifyArgs {
   uint32_t* status;
 };
 
-// Work of an attention call is cut into at most this many equal parts, one per
-// CTA (2 CTAs on each of 148 SMs); a part leaves at most two partial results.
-constexpr int ATTEND_CTAS = 296;
-constexpr int TC_CTAS = 148;      // parts of the tensor-core kernel: one CTA on each SM
+// Work of an attention call is cut into equal parts, one per CTA; a part leaves at most two
+// partial results.
+constexpr int SMS = 148;
+constexpr int ATTEND_CTAS = 4 * SMS;  // most CTAs of the mma.sync kernel
+constexpr int TC_CTAS = SMS;      // parts of the tensor-core kernel: one CTA on each SM
 constexpr int TC_ROWS = 256;      // rows of its CTA
-constexpr int TC_TICKETS = 512;   // its first ticket, two a CTA
+constexpr int TC_TICKETS = 640;   // its first ticket, two a CTA
 constexpr size_t TICKET_BYTES = 4096;
 
 cudaError_t launch_append(const AppendArgs& a, int act, int cache, cudaStream_t s);

@@ -365,7 +365,7 @@ struct AttnCfg {
   static constexpr int PANELS = HD * int(sizeof(CT)) / 128;
   static constexpr int PANEL = TK * 128;            // bytes: TK rows of 128
   static constexpr int STAGE = 2 * PANELS * PANEL;  // K, then V
-  static constexpr int STAGES = STAGE > 32768 ? 2 : 3;
+  static constexpr int STAGES = STAGE > 16384 ? 2 : 3;
   static constexpr int QBYTES = F32A ? NB * (HD / 8) * 512 : 0;  // q as tf32 pairs in fragment order
   static constexpr int OPITCH = HD + 4;                          // floats; joining the warps' results
   static constexpr int JOIN = 4 * M * OPITCH * 4 + 4 * M * 8;
@@ -373,10 +373,14 @@ struct AttnCfg {
   static constexpr int OFFS = (STAGES + 1) * TK * 8 + (STAGES + 1) * 2 * 4;
   static constexpr int SMEM = RING + QBYTES + OFFS + 1024;  // + alignment to the swizzle's period
   static constexpr bool TWO_P = !F32A && NB == 1;
+  // CTAs of an SM: what shared memory holds, as far as the registers of the rows go
+  static constexpr int FIT = 227 * 1024 / (SMEM + 2048);
+  static constexpr int WANT = NB == 1 ? (HD == 64 ? 4 : 3) : 2;
+  static constexpr int PER_SM = FIT < 1 ? 1 : FIT < WANT ? FIT : WANT;
 };
 
 template <typename AT, typename CT, int HD, int NB>
-__global__ void __launch_bounds__(AT_THREADS)
+__global__ void __launch_bounds__(AT_THREADS, (AttnCfg<AT, CT, HD, NB>::PER_SM))
 attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap kmap,
               const __grid_constant__ CUtensorMap vmap, int box) {
   using L = AttnCfg<AT, CT, HD, NB>;
@@ -929,7 +933,7 @@ cudaError_t run_attend(const AttendArgs& a, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   CUtensorMap km{}, vm{};
   const int box = make_maps<CT>(&km, &vm, a.pool, L::TK);
-  attend_kernel<AT, CT, HD, NB><<<ATTEND_CTAS, AT_THREADS, L::SMEM, st>>>(a, km, vm, box);
+  attend_kernel<AT, CT, HD, NB><<<SMS * L::PER_SM, AT_THREADS, L::SMEM, st>>>(a, km, vm, box);
   return cudaGetLastError();
 }
 

@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(VF_THREADS) verify_kernel(const __grid_constan
 cudaError_t launch_verify(const VerifyArgs& a, cudaStream_t s) {
   // CTAs of a sequence: enough for two on each SM, slices of at least 2048 probabilities
   int c = 1;
-  while (c < MAX_CLUSTER && a.n_seqs * c < ATTEND_CTAS && a.vocab / (2 * c) >= 2048) c *= 2;
+  while (c < MAX_CLUSTER && a.n_seqs * c < 2 * SMS && a.vocab / (2 * c) >= 2048) c *= 2;
   const int n_chunks = (a.vocab + CHUNK - 1) / CHUNK;
   const int per = (n_chunks + c - 1) / c;
   cudaLaunchConfig_t cfg{};
