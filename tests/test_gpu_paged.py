@@ -301,11 +301,11 @@ def test_long_sequences_and_repeatability(gpu, act, cache, heads, kv_heads, dim)
     assert (room[:4096] == 0).all()
 
 
-@pytest.mark.parametrize("act", ["f16", "bf16"])
+@pytest.mark.parametrize("act,cache", PAIRS)
 @pytest.mark.parametrize("heads,kv_heads,dim,page,by_head", [(8, 1, 128, 64, False), (4, 4, 128, 16, True), (8, 2, 64, 48, False), (15, 5, 64, 1, True)])
 @pytest.mark.parametrize("q_len,kv_len,window", [([257], [2600], 0), ([129, 1, 300, 0, 64], [129, 70, 1500, 5, 640], 0), ([200, 333], [900, 333], 130)])
-def test_attention_of_long_chunks(gpu, act, heads, kv_heads, dim, page, by_head, q_len, kv_len, window):
-    s = Step(q_len, kv_len, heads, kv_heads, dim, act, act, page, by_head, seed=16, gap=8)
+def test_attention_of_long_chunks(gpu, act, cache, heads, kv_heads, dim, page, by_head, q_len, kv_len, window):
+    s = Step(q_len, kv_len, heads, kv_heads, dim, act, cache, page, by_head, seed=16, gap=8)
     room = s.attend(window=window)
     s.check(window=window)
     first, lse = s.out.clone(), s.lse.clone()
@@ -316,10 +316,11 @@ def test_attention_of_long_chunks(gpu, act, heads, kv_heads, dim, page, by_head,
     assert (room[:4096] == 0).all()
 
 
-@pytest.mark.parametrize("act", ["f16", "bf16"])
-def test_growing_scores_rescale(gpu, act):
+@pytest.mark.parametrize("act,cache", PAIRS)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_growing_scores_rescale(gpu, act, cache, dim):
     """Scores that grow along the keys by far more than 2^8: the sums are rescaled again and again."""
-    s = Step([140, 1], [900, 700], 4, 2, 64, act, act, 16, seed=17)
+    s = Step([140, 1], [900, 700], 4, 2, dim, act, cache, 16, seed=17)
     s.q.abs_()
     for i in range(2):
         sl = s.slots(i)
@@ -331,6 +332,21 @@ def test_growing_scores_rescale(gpu, act):
     s.check()
     s.attend(scale=-0.3)
     s.check(scale=-0.3)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("q_len", [1, 90])
+@pytest.mark.parametrize("qs,ks,vs", [(1e-20, 1e18, 1e-25), (1e20, 1e-21, 1e30), (1.0, 1.0, 1.0)])
+def test_f32_of_any_range(gpu, dim, q_len, qs, ks, vs):
+    """f32 queries, keys and values far from 1, and sizes that differ from key to key."""
+    s = Step([q_len], [400], 4, 2, dim, "f32", "f32", 16, seed=18)
+    g = torch.Generator().manual_seed(5)
+    j = torch.exp2(torch.randint(-6, 1, (s.pages, 16, 1, 1), generator=g).float()).cuda()
+    s.q *= qs
+    s.k *= ks * j
+    s.v *= vs * j.flip(0)
+    s.attend()
+    s.check()
 
 
 def test_scale_and_large_scores(gpu):

@@ -77,6 +77,7 @@ cudaError_t launch_append(const AppendArgs& a, int act, int cache, cudaStream_t 
 cudaError_t launch_attend_16(const AttendArgs& a, int act, int rows, cudaStream_t s);
 cudaError_t launch_attend_32(const AttendArgs& a, int cache, int rows, cudaStream_t s);
 cudaError_t launch_attend_tc(const AttendArgs& a, int act, cudaStream_t s);
+cudaError_t launch_attend_tc32(const AttendArgs& a, int cache, cudaStream_t s);
 cudaError_t launch_verify(const VerifyArgs& a, cudaStream_t s);
 
 }  // namespace paged

@@ -1,0 +1,698 @@
+// Attention of many new rows over a paged cache on the 5th-generation tensor
+// cores, f32 activations over an f32 or f16 cache (the formulas and the line of tiles:
+// paged_attn.cuh; the 16-bit kernel this one is built like: paged_attn_tc.cu).
+//
+// f32 numbers go to the tensor cores as sums of two f16 numbers, x = 2^e (hi + lo), 22 bits: the
+// exponents are a row's (q) or 16 keys' (k and v), so that the largest of them lies below 2^14 and
+// what is lost of the others is below 2^-38 of it. An f16 cache needs no splitting.
+//   S  = Qlo Khi + Qhi Klo + Qhi Khi             (two products over an f16 cache)
+//   O' = Plo Vhi + Phi Vlo + Phi Vhi             (one half of 64 keys)
+//   O  = O 2^(m - m') + O' 2^e                   in registers, by ordinary f32 arithmetic
+// The last line is why this is not the 16-bit kernel with more products: sums in TMEM over a long
+// sequence are cut off at every step, which f32 outputs would show; over 64 keys they are not. TMEM: S of each
+// row tile in two halves of 64 keys, over which Phi and Plo are written, and two O' of each
+// row tile, one of them being added to O while the products of the next are made.
+//
+// Keys and values of an f32 cache are loaded, scaled and split by the four loader warps (each 16 keys
+// of a half, so a group's exponent is one warp's affair); those of an f16 cache come by TMA where
+// the tile is whole. head_dim 64: two row tiles of 128 rows; 128: one (Q in two parts and a
+// ring of K and V in two parts fill the shared memory).
+#include "paged_tc.cuh"
+
+namespace wcb {
+namespace paged {
+namespace {
+
+template <typename CT, int HD>
+struct Tc32Cfg {
+  static constexpr bool F32C = std::is_same<CT, float>::value;
+  static constexpr int RT = HD == 64 ? 2 : 1;       // row tiles
+  static constexpr int M = 128 * RT;
+  static constexpr int THREADS = 128 * (RT + 2);    // softmax warpgroups, loaders, issuing warps
+  static constexpr int PART = HD / 64 * TILE_PANEL;  // bytes of 128 rows x HD in f16
+  static constexpr int SLOT = (F32C ? 2 : 1) * PART;
+  static constexpr int SLOTS = F32C ? (HD == 64 ? 4 : 2) : (HD == 64 ? 6 : 4);
+  static constexpr int Q = 0;                        // [row tile][hi, lo]
+  static constexpr int RING = RT * 2 * PART;
+  static constexpr int OFFS = RING + SLOTS * SLOT;   // [2][128] row offsets (f16 cache)
+  static constexpr int SMEM = OFFS + 2 * 128 * 8 + 1024;
+  // registers of a thread by role; together no more than the launch's (65536 / THREADS a thread)
+  static constexpr int R_SOFT = RT == 2 ? 184 : 240, R_LOAD = RT == 2 ? 96 : 152, R_MMA = RT == 2 ? 48 : 56;
+  static constexpr int LAUNCH = RT == 2 ? 128 : 168;
+  static_assert(RT * R_SOFT + R_LOAD + R_MMA <= (RT + 2) * LAUNCH, "register split");
+};
+
+constexpr int EXP_RING = 8;  // tiles
+
+struct Tc32Shared : TcShared {
+  // (read four at a time)
+  alignas(16) int kexp[EXP_RING][8];
+  alignas(16) int vexp[EXP_RING][8];  // of 16 keys: their numbers are 2^exp times what the tile holds
+};
+
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((max(-126, min(127, e)) + 127) << 23); }
+// the exponent that brings numbers up to `top` below 2^14; `none` where there are only zeros
+__device__ __forceinline__ int group_exp(float top, int none) {
+  const int e = int(__float_as_uint(top) >> 23) - 127;  // top in [2^e, 2^(e + 1)); below 2^-126: -127
+  return top > 0.0f ? max(-100, min(120, e - 13)) : none;
+}
+// two numbers as two f16 each
+__device__ __forceinline__ void split_f16(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  // an infinity or NaN stays in hi alone
+  lo = pack2<__half>(fabsf(f.x) <= FLT_MAX ? x - f.x : 0.0f, fabsf(f.y) <= FLT_MAX ? y - f.y : 0.0f);
+}
+
+template <typename CT, int HD>
+__global__ void __launch_bounds__((Tc32Cfg<CT, HD>::THREADS), 1)
+attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap kmap,
+                   const __grid_constant__ CUtensorMap vmap, int box) {
+  using L = Tc32Cfg<CT, HD>;
+  constexpr bool F32C = L::F32C;
+  constexpr int NS = L::SLOTS, RT = L::RT, M = L::M;
+  extern __shared__ uint8_t raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  __shared__ Tc32Shared sh;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t sbase = smem_u32(sm);
+
+  const Place pl = find_place<L::THREADS>(a, M, TC_TK, sh.scan, sh.place);
+  if (pl.begin >= pl.end) return;  // the whole CTA; nothing is held yet
+
+  if (tid == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&sh.full[i], 4);
+      mbar_init(&sh.empty[i], RT);
+    }
+    for (int w = 0; w < RT; ++w) {
+      mbar_init(&sh.q_full[w], 128);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&sh.s_full[w][b], 1);
+        mbar_init(&sh.p_full[w][b], 4);
+        mbar_init(&sh.o_done[w][b], 1);
+      }
+      mbar_init(&sh.piece_full[w], 128);
+      mbar_init(&sh.last_full[w], 1);
+    }
+    mbar_init(&sh.offs_full, 128);
+    sh.abort = 0;
+    mbar_fence_init();
+  }
+  if (tid < ODD_RING) sh.odd[tid] = 0;
+  if (warp == 4 * (RT + 1)) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  Walk<M> wk;
+  wk.start(a, pl);
+
+  if (warp >= 4 * (RT + 1)) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::R_MMA));
+    // ---- issuing warps (paged_attn_tc.cu says how) ------------------------------
+    const int w = __shfl_sync(0xffffffffu, warp - 4 * (RT + 1), 0);
+    if (w < RT) {
+      uint32_t elected;
+      asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(elected));
+      const bool one = elected != 0;
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t ts = tm + 128 * w, to = tm + 256 + 128 * w;  // (one row tile: O' of 128 columns at 256 and 384)
+      const uint64_t qd = desc_kmajor(sbase + L::Q + w * 2 * L::PART);
+      const uint64_t kd = desc_kmajor(sbase + L::RING), vd = desc_nmajor(sbase + L::RING);
+      constexpr uint32_t ID_S = idesc<__half>(64, false), ID_O = idesc<__half>(HD, true);
+      constexpr uint32_t LO = L::PART >> 4;  // from a tile's hi to its lo, in descriptors
+      uint32_t slot = 0, phase = 0;          // of the next ring tile
+      uint32_t it = 0, t = 0;                // units, and tiles of keys so far
+      auto step = [&] {
+        if (++slot == NS) {
+          slot = 0;
+          phase ^= 1;
+        }
+      };
+      auto product_s = [&](uint32_t ks, int b) {
+        tc_fence_after();
+        const uint64_t kb = kd + uint64_t(ks * (L::SLOT >> 4) + b * (64 * 128 >> 4));
+        if (one) {
+#pragma unroll
+          for (int k = 0; k < HD / 16; ++k) {
+            const uint32_t o = ((k / 4) * TILE_PANEL + (k % 4) * 32) >> 4;
+            mma_ss(ts + 64 * b, qd + LO + o, kb + o, ID_S, k > 0);
+            if (F32C) mma_ss(ts + 64 * b, qd + o, kb + LO + o, ID_S, 1);
+          }
+#pragma unroll
+          for (int k = 0; k < HD / 16; ++k) {
+            const uint32_t o = ((k / 4) * TILE_PANEL + (k % 4) * 32) >> 4;
+            mma_ss(ts + 64 * b, qd + o, kb + o, ID_S, 1);
+          }
+          tc_commit(&sh.s_full[w][b]);
+          if (b) tc_commit(&sh.empty[ks]);
+        }
+        __syncwarp();
+      };
+      bool ok = true;
+      do {
+        const int end = wk.end_of(a, w);
+        if (end > wk.ta) {
+          ok = tc_wait_warp(&sh, &sh.q_full[w], it & 1) && tc_wait_warp(&sh, &sh.full[slot], phase);
+          if (!ok) break;
+          product_s(slot, 0);
+          product_s(slot, 1);
+          ++it;
+        }
+        for (int i = wk.ta; i < wk.tb && ok; ++i) {
+          if (i < end) {  // K of this tile is used up
+            step();
+            const uint32_t vs = slot;
+            const uint64_t vb = vd + uint64_t(vs * (L::SLOT >> 4));
+            ok = tc_wait_warp(&sh, &sh.full[slot], phase);
+            step();
+            const bool more = i + 1 < end;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              ok = ok && tc_wait_warp(&sh, &sh.p_full[w][b], t & 1);
+              if (!ok) break;
+              tc_fence_after();
+              if (one) {
+                const uint32_t od = to + HD * b;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  const uint64_t v = vb + (4 * b + k) * (2048 >> 4);
+                  mma_ts(od, ts + 64 * b + 32 + 8 * k, v, ID_O, k > 0);
+                  if (F32C) mma_ts(od, ts + 64 * b + 8 * k, v + LO, ID_O, 1);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) mma_ts(od, ts + 64 * b + 8 * k, vb + (4 * b + k) * (2048 >> 4), ID_O, 1);
+                tc_commit(&sh.o_done[w][b]);
+                if (b) tc_commit(&sh.empty[vs]);
+              }
+              __syncwarp();
+              if (more) {  // the next S lies over this P: its product has to be done
+                if (b == 0) ok = tc_wait_warp(&sh, &sh.full[slot], phase);
+                ok = ok && tc_wait_warp(&sh, &sh.o_done[w][b], t & 1);
+                if (!ok) break;
+                product_s(slot, b);
+              }
+            }
+            ++t;
+          } else {  // rows of this tile see none of these keys
+            ok = tc_wait_warp(&sh, &sh.full[slot], phase);
+            if (!ok) break;
+            if (one) bar_arrive(&sh.empty[slot]);
+            step();
+            ok = tc_wait_warp(&sh, &sh.full[slot], phase);
+            if (!ok) break;
+            if (one) bar_arrive(&sh.empty[slot]);
+            step();
+          }
+        }
+      } while (ok && wk.next(a));
+    }
+  } else if (warp >= 4 * RT) {
+    if constexpr (RT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::R_LOAD));
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::R_LOAD));
+    // ---- loaders --------------------------------------------------------------
+    const int lt = tid - 128 * RT, lw = warp - 4 * RT;
+    long long* offs = reinterpret_cast<long long*>(sm + L::OFFS);
+    uint32_t n = 0, tiles = 0, item = 0, by_copy = 0;
+    bool ok = true, holes_seen = false;
+    // this thread's key of a tile. f32: 16 keys of each half are one warp's (lanes 0 .. 15, 16 .. 31)
+    const int my_key = F32C ? 64 * (lane >> 4) + 16 * lw + (lane & 15) : lt;
+    auto page_of = [&](int i) {
+      const int key = (wk.blk.tile0 + i) * TC_TK + my_key;
+      return key >= wk.blk.lo && key < wk.blk.hi
+                 ? __ldg(a.batch.page_table + int64_t(wk.s) * a.batch.max_pages + key / a.pool.page_size)
+                 : -1;
+    };
+    auto room = [&](uint32_t m) {
+      return m < NS || tc_wait_warp(&sh, &sh.empty[m % NS], ((m / NS) - 1) & 1);
+    };
+    do {
+      if (lt == 0) sh.odd[(item + ODD_RING / 2) % ODD_RING] = 0;
+      const bool many = wk.blk.pos1 > wk.blk.pos0;
+      int next = page_of(wk.ta);
+      for (int i = wk.ta; i < wk.tb && ok; ++i, ++tiles, n += 2) {
+        const int page = next;
+        if (i + 1 < wk.tb) next = page_of(i + 1);
+        const int key = (wk.blk.tile0 + i) * TC_TK + my_key, at_slot = key % a.pool.page_size;
+        const bool in = key >= wk.blk.lo && key < wk.blk.hi, there = in && page >= 0 && page < a.pool.n_pages;
+        const unsigned hb = __ballot_sync(0xffffffffu, in && !there);
+        if (lane == 0) {
+          if (F32C) {
+            uint16_t* h = reinterpret_cast<uint16_t*>(sh.holes[tiles % HOLE_RING]);  // by 16 keys
+            h[lw] = uint16_t(hb);
+            h[4 + lw] = uint16_t(hb >> 16);
+          } else {
+            sh.holes[tiles % HOLE_RING][lw] = hb;
+          }
+        }
+        holes_seen |= hb != 0;
+        const long long off = there ? page * a.pool.page_stride + int64_t(at_slot) * a.pool.token_stride : -1;
+        if constexpr (F32C) {
+          constexpr int LPR = HD / 4;        // lanes of a row (16 bytes each): 16 or 32
+          constexpr int RPI = 32 / LPR;      // rows of an iteration
+          constexpr int IT = 16 / RPI;       // iterations of 16 rows
+          const int sub = lane % LPR, rr = lane / LPR;
+          const float* base[2] = {static_cast<const float*>(a.pool.k) + wk.kvh * a.pool.head_stride + 4 * sub,
+                                  static_cast<const float*>(a.pool.v) + wk.kvh * a.pool.head_stride + 4 * sub};
+#pragma unroll 1
+          for (int u = 0; u < 4; ++u) {  // K's halves, V's halves
+            const int kvi = u >> 1, b = u & 1;
+            float4 x[IT];
+#pragma unroll
+            for (int j = 0; j < IT; ++j) {
+              const long long o = __shfl_sync(0xffffffffu, off, 16 * b + RPI * j + rr);
+              x[j] = o >= 0 ? __ldg(reinterpret_cast<const float4*>(base[kvi] + o)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+            if (b == 0) {
+              ok = room(n + kvi);
+              if (!ok) break;
+            }
+            float top = 0.0f;
+            bool odd = false;
+#pragma unroll
+            for (int j = 0; j < IT; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                float& y = (&x[j].x)[e];
+                const float z = fabsf(y);
+                if (!(z <= FLT_MAX)) {
+                  // infinities and NaN: a value's is added to O at the end, to the rows that see it
+                  if (kvi) {
+                    odd = true;
+                    y = 0.0f;
+                  }
+                } else {
+                  top = fmaxf(top, z);
+                }
+              }
+            if (odd) sh.odd[item % ODD_RING] = 1;
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            const int ge = group_exp(top, kvi ? -126 : 0);  // zeros among values never make the largest exponent
+            if (lane == 0) (kvi ? sh.vexp : sh.kexp)[tiles % EXP_RING][4 * b + lw] = ge;
+            const float f = pow2(-ge);
+            uint8_t* dst = sm + L::RING + ((n + kvi) % NS) * L::SLOT;
+#pragma unroll
+            for (int j = 0; j < IT; ++j) {
+              uint2 h, l;
+              split_f16(x[j].x * f, x[j].y * f, h.x, l.x);
+              split_f16(x[j].z * f, x[j].w * f, h.y, l.y);
+              const uint32_t o = tile_at(64 * b + 16 * lw + RPI * j + rr, sub >> 1) + 8 * (sub & 1);
+              *reinterpret_cast<uint2*>(dst + o) = h;
+              *reinterpret_cast<uint2*>(dst + L::PART + o) = l;
+            }
+            if (b == 1) {
+              fence_proxy_async();
+              __syncwarp();
+              if (lane == 0) bar_arrive(&sh.full[(n + kvi) % NS]);
+            }
+          }
+        } else {
+          constexpr int CH = HD / 8;
+          const bool ragged = wk.ragged(a, i);
+          if (box > 0 && !ragged) {
+#pragma unroll 1
+            for (int kvi = 0; kvi < 2 && ok; ++kvi) {
+              ok = room(n + kvi);
+              if (!ok) break;
+              uint64_t* bar = &sh.full[(n + kvi) % NS];
+              if (lane == 0) {  // the first warp's arrival brings the bytes to wait for
+                if (lw == 0) mbar_expect_tx(bar, L::SLOT);
+                else bar_arrive(bar);
+              }
+              if (lt % box == 0) {
+                const uint32_t dst = sbase + L::RING + ((n + kvi) % NS) * L::SLOT + lt * 128;
+#pragma unroll
+                for (int p = 0; p < HD / 64; ++p)  // a page that is not there: past the last one, zeros
+                  tma_load(dst + p * TILE_PANEL, kvi ? &vmap : &kmap, 64 * p, wk.kvh, at_slot, there ? page : a.pool.n_pages, bar);
+              }
+            }
+            continue;
+          }
+          offs[(by_copy & 1) * 128 + lt] = off;
+          bar_arrive(&sh.offs_full);
+          ok = tc_wait_warp(&sh, &sh.offs_full, by_copy & 1);
+          const long long* ro = offs + (by_copy & 1) * 128;
+          ++by_copy;
+#pragma unroll 1
+          for (int kvi = 0; kvi < 2 && ok; ++kvi) {
+            ok = room(n + kvi);
+            if (!ok) break;
+            const __half* base = static_cast<const __half*>(kvi ? a.pool.v : a.pool.k) + wk.kvh * a.pool.head_stride;
+            const uint32_t dst = sbase + L::RING + ((n + kvi) % NS) * L::SLOT;
+#pragma unroll 8
+            for (int c = lt; c < 128 * CH; c += 128) {
+              const int r = c / CH, ch = c % CH;
+              const long long o = ro[r];
+              cp16(dst + tile_at(r, ch), base + (o < 0 ? 0 : o) + ch * 8, o >= 0);
+            }
+            cp_commit();
+          }
+          if (!ok) break;
+#pragma unroll 1
+          for (int kvi = 0; kvi < 2; ++kvi) {
+            if (kvi == 0) cp_wait<1>();
+            else cp_wait<0>();
+            // keys that some rows see and others do not: infinities and NaN are taken out of their values
+            if (kvi && many && ragged) {
+              uint8_t* t = sm + L::RING + ((n + 1) % NS) * L::SLOT;
+              bool odd = false;
+              for (int c = lt; c < 128 * CH; c += 128) {  // the chunks this thread copied
+                uint4* x = reinterpret_cast<uint4*>(t + tile_at(c / CH, c % CH));
+                const uint4 v = *x;
+                if (!(finite16<__half>(v.x) && finite16<__half>(v.y) && finite16<__half>(v.z) && finite16<__half>(v.w))) {
+                  odd = true;
+                  alignas(16) __half e[8];
+                  *reinterpret_cast<uint4*>(e) = v;
+#pragma unroll
+                  for (int j = 0; j < 8; ++j)
+                    if (!(fabsf(to_f32(e[j])) <= FLT_MAX)) e[j] = from_f32<__half>(0.0f);
+                  *x = *reinterpret_cast<const uint4*>(e);
+                }
+              }
+              if (odd) sh.odd[item % ODD_RING] = 1;
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&sh.full[(n + kvi) % NS]);
+          }
+        }
+      }
+      ++item;
+    } while (ok && wk.next(a));
+    cp_wait<0>();
+    if (holes_seen && lane == 0) report(a.batch, ST_BAD_PAGE);
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::R_SOFT));
+    // ---- softmax of row tile w: thread = row ----------------------------------
+    const int w = warp >> 2, row = tid & 127;
+    const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16;
+    const uint32_t ts = tmem + lanes + 128 * w, to = tmem + lanes + 256 + 128 * w;
+    uint32_t tiles = 0, t = 0, item = 0, cuts = 0;  // tiles of the ring, tiles of keys with rows, units, units cut
+    bool ok = true;
+    do {
+      const int r0 = wk.rb * M + 128 * w, rn = min(128, wk.rows - r0);
+      const int end = wk.end_of(a, w);
+      if (end > wk.ta) {
+        // the row's query, scaled and split; rows that are not there are zeros
+        const int gr = r0 + min(row, rn - 1);
+        float qinv;
+        {
+          const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + (wk.sq.r0 + gr / a.rep) * a.q_stride +
+                                                              (wk.kvh * a.rep + gr % a.rep) * HD);
+          float top = 0.0f;
+#pragma unroll
+          for (int j = 0; j < HD / 4; ++j) {
+            const float4 x = __ldg(src + j);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float z = fabsf((&x.x)[e]);
+              if (z <= FLT_MAX) top = fmaxf(top, z);
+            }
+          }
+          const int ge = group_exp(top, 0);
+          qinv = pow2(ge);
+          const float f = row < rn ? pow2(-ge) : 0.0f;
+          uint8_t* qt = sm + L::Q + w * 2 * L::PART;
+#pragma unroll
+          for (int ch = 0; ch < HD / 8; ++ch) {
+            const float4 x = __ldg(src + 2 * ch), y = __ldg(src + 2 * ch + 1);
+            uint4 h, l;
+            split_f16(x.x * f, x.y * f, h.x, l.x);
+            split_f16(x.z * f, x.w * f, h.y, l.y);
+            split_f16(y.x * f, y.y * f, h.z, l.z);
+            split_f16(y.z * f, y.w * f, h.w, l.w);
+            *reinterpret_cast<uint4*>(qt + tile_at(row, ch)) = h;
+            *reinterpret_cast<uint4*>(qt + L::PART + tile_at(row, ch)) = l;
+          }
+        }
+        fence_proxy_async();
+        bar_arrive(&sh.q_full[w]);
+
+        const int pos = wk.sq.kv - wk.sq.n + gr / a.rep;
+        const int khi = min(pos + 1, wk.table), klo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+        float m = -INFINITY, l = 0.0f;  // m: the maximum that O and l are scaled by
+        float o[HD];
+#pragma unroll
+        for (int d = 0; d < HD; ++d) o[d] = 0.0f;
+        float due = 0.0f;  // factor of the half whose O' is not added yet
+        auto add_half = [&](int b) {
+#pragma unroll
+          for (int q = 0; q < HD / 16; ++q) {
+            uint32_t x[16];
+            tmem_ld16(to + HD * b + 16 * q, x);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[16 * q + e] = fmaf(__uint_as_float(x[e]), due, o[16 * q + e]);
+          }
+        };
+        for (int i = wk.ta; i < end && ok; ++i) {
+          const uint32_t rt = tiles + (i - wk.ta);  // ring tile pair
+          const uint32_t* holes = sh.holes[rt % HOLE_RING];
+          const bool cut = wk.ragged(a, i);
+#pragma unroll 1
+          for (int b = 0; b < 2; ++b) {
+            ok = tc_wait_warp(&sh, &sh.s_full[w][b], t & 1);
+            if (F32C && b == 0) ok = ok && tc_wait_warp(&sh, &sh.full[(2 * rt + 1) % NS], ((2 * rt + 1) / NS) & 1);  // the values' exponents
+            if (!ok) break;
+            tc_fence_after();
+            const int key0 = (wk.blk.tile0 + i) * TC_TK + 64 * b;
+            const bool mask = cut || (holes[2 * b] | holes[2 * b + 1]) != 0;
+            uint32_t v[64];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) tmem_ld32(ts + 64 * b + 32 * q, *reinterpret_cast<uint32_t(*)[32]>(v + 32 * q));
+            // factors of 16 keys each: of the products, and of P (relative to the half's largest exponent `ref`)
+            float kf[4], vf[4];
+            // never zero, or a masked product's infinity would become NaN
+            auto factor = [&](float f) { return copysignf(fmaxf(fabsf(a.scale_log2) * f, 1e-37f), a.scale_log2); };
+            int ref = 0;
+            if constexpr (F32C) {
+              const int4 ke = *reinterpret_cast<const int4*>(&sh.kexp[rt % EXP_RING][4 * b]);
+              const int4 ve = *reinterpret_cast<const int4*>(&sh.vexp[rt % EXP_RING][4 * b]);
+              ref = max(max(ve.x, ve.y), max(ve.z, ve.w));
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                kf[q] = factor(qinv * pow2((&ke.x)[q]));
+                const int d = (&ve.x)[q] - ref;
+                vf[q] = d < -126 ? 0.0f : pow2(d);
+              }
+            } else {
+              kf[0] = factor(qinv);
+            }
+            tmem_wait_ld();
+            if (mask) {
+              const uint32_t none = a.scale_log2 < 0.0f ? 0x7f800000u : 0xff800000u;  // -infinity once scaled
+              const int lo = max(0, min(64, klo - key0)), hi = max(0, min(64, khi - key0));
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                const int b0 = max(0, min(32, lo - 32 * q)), b1 = max(0, min(32, hi - 32 * q));
+                const uint32_t below1 = b1 >= 32 ? 0xffffffffu : (1u << b1) - 1u, below0 = b0 >= 32 ? 0xffffffffu : (1u << b0) - 1u;
+                const uint32_t seen = below1 & ~below0 & ~holes[2 * b + q];
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  if (!((seen >> e) & 1)) v[32 * q + e] = none;
+              }
+            }
+            float sum;
+            auto exponentials = [&] {
+              const float use = m == -INFINITY ? 0.0f : m;
+              float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                uint32_t p[16], r[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                  const int c = 32 * q + 2 * e, gq = F32C ? c / 16 : 0;
+                  float x = fast_exp2(fmaf(__uint_as_float(v[c]), kf[gq], -use)), y = fast_exp2(fmaf(__uint_as_float(v[c + 1]), kf[gq], -use));
+                  s0 += x;
+                  s1 += y;
+                  if (F32C) {
+                    x *= vf[gq];
+                    y *= vf[gq];
+                  }
+                  const __half2 h = __floats2half2_rn(x, y);
+                  const float2 f = __half22float2(h);
+                  p[e] = *reinterpret_cast<const uint32_t*>(&h);
+                  r[e] = pack2<__half>(x - f.x, y - f.y);
+                }
+                tmem_st16(ts + 64 * b + 16 * q, p);
+                tmem_st16(ts + 64 * b + 32 + 16 * q, r);
+              }
+              sum = s0 + s1;
+            };
+            // (paged_attn_tc.cu: the maximum only where the sum asks for it)
+            bool again = __any_sync(0xffffffffu, mask || m == -INFINITY);
+            if (!again) {
+              exponentials();
+              again = __any_sync(0xffffffffu, !(sum <= GROWTH));
+            }
+            if (again) {
+              float top = -INFINITY;
+#pragma unroll
+              for (int e = 0; e < 64; ++e) top = fmaxf(top, __uint_as_float(v[e]) * kf[F32C ? e / 16 : 0]);
+              if (__any_sync(0xffffffffu, top > m)) {
+                const float nm = fmaxf(m, top);
+                const float f = m == nm ? 1.0f : fast_exp2(m - (nm == -INFINITY ? 0.0f : nm));
+#pragma unroll
+                for (int d = 0; d < HD; ++d) o[d] *= f;
+                due *= f;
+                l *= f;
+                m = nm;
+              }
+              exponentials();
+            }
+            l += sum;
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&sh.p_full[w][b]);
+            // the half before this one
+            if (i > wk.ta || b) {
+              ok = tc_wait_warp(&sh, &sh.o_done[w][1 - b], (b ? t : t - 1) & 1);
+              if (!ok) break;
+              tc_fence_after();
+              add_half(1 - b);
+              tc_fence_before();
+            }
+            due = pow2(ref);
+          }
+          ++t;
+        }
+        if (ok) ok = tc_wait_warp(&sh, &sh.o_done[w][1], (t - 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        add_half(1);
+        tc_fence_before();
+
+        // infinities and NaN that were taken out of the values, for the rows that see them
+        if (*reinterpret_cast<volatile int*>(&sh.odd[item % ODD_RING]) != 0) {
+#pragma unroll 1
+          for (int i = wk.ta; i < end; ++i) {
+            if (!F32C && !wk.ragged(a, i)) continue;
+            const int k0 = (wk.blk.tile0 + i) * TC_TK;
+#pragma unroll 1
+            for (int key = max(k0, klo); key < min(k0 + TC_TK, khi); ++key) {
+              bool hole;
+              const long long off = wk.key_offset(a, key, hole);
+              if (off < 0) continue;
+              const CT* vp = static_cast<const CT*>(a.pool.v) + wk.kvh * a.pool.head_stride + off;
+#pragma unroll
+              for (int d = 0; d < HD; ++d) {
+                const float x = to_f32(vp[d]);
+                if (!(fabsf(x) <= FLT_MAX)) o[d] += x;
+              }
+            }
+          }
+        }
+        // results: normalised, or a piece [HD][M] + m [M] + l [M]
+        const bool whole = wk.ta == 0 && wk.tb == wk.blk.tiles;
+        const int64_t tok = wk.sq.r0 + gr / a.rep;
+        const int hh = wk.kvh * a.rep + gr % a.rep;
+        constexpr size_t PIECE = size_t(M) * (HD + 2);
+        if (row < rn) {
+          if (whole) {
+            const bool some = (l > 0.0f && m > -INFINITY) || l != l;
+            const float inv = some ? 1.0f / l : 0.0f;
+#pragma unroll
+            for (int d = 0; d < HD; ++d) o[d] = some ? o[d] * inv : 0.0f;
+            store_vec<float, HD>(static_cast<float*>(a.out) + tok * a.out_stride + hh * HD, o);
+            if (a.lse) a.lse[tok * a.n_heads + hh] = some ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
+          } else {
+            float* piece = a.part + (size_t(blockIdx.x) * 2 + (wk.ta == 0 ? 1 : 0)) * PIECE + 128 * w + row;
+#pragma unroll
+            for (int d = 0; d < HD; ++d) piece[size_t(d) * M] = o[d];
+            piece[size_t(HD) * M] = m;
+            piece[size_t(HD + 1) * M] = l;
+          }
+        }
+        if (row == 0 && w == 0) {
+          uint32_t bits = 0;
+          if (wk.blk.pos1 >= wk.table) bits |= ST_BAD_PAGE;
+          if (wk.blk.pos0 < 0) bits |= ST_BAD_LEN;
+          report(a.batch, bits);
+        }
+        if (!whole) {
+          // the last of the unit's CTAs joins this tile's pieces, in their order
+          const int c0 = int(wk.unit0 / wk.pl.per), c1 = int((wk.unit0 + wk.blk.tiles - 1) / wk.pl.per);
+          __threadfence();
+          bar_arrive(&sh.piece_full[w]);
+          ok = tc_wait_warp(&sh, &sh.piece_full[w], cuts & 1);
+          if (!ok) break;
+          if (row == 0) {
+            sh.last[w] = atomicInc(reinterpret_cast<unsigned*>(a.tickets) + TC_TICKETS + 2 * c0 + w, unsigned(c1 - c0)) == unsigned(c1 - c0);
+            bar_arrive(&sh.last_full[w]);
+          }
+          ok = tc_wait_warp(&sh, &sh.last_full[w], cuts & 1);
+          if (!ok) break;
+          ++cuts;
+          if (sh.last[w] && row < rn) {
+            __threadfence();
+            auto part = [&](int p) { return a.part + (size_t(p) * 2 + (p == c0 ? 1 : 0)) * PIECE + 128 * w + row; };
+            m = -INFINITY;
+            for (int p = c0; p <= c1; ++p) m = fmaxf(m, __ldcg(part(p) + size_t(HD) * M));
+            const float u = m == -INFINITY ? 0.0f : m;
+            l = 0.0f;
+#pragma unroll
+            for (int d = 0; d < HD; ++d) o[d] = 0.0f;
+#pragma unroll 1
+            for (int p = c0; p <= c1; ++p) {
+              const float* pp = part(p);
+              const float f = fast_exp2(__ldcg(pp + size_t(HD) * M) - u);
+              l += f * __ldcg(pp + size_t(HD + 1) * M);
+#pragma unroll
+              for (int d = 0; d < HD; ++d) o[d] = fmaf(f, __ldcg(pp + size_t(d) * M), o[d]);
+            }
+            const bool some = l > 0.0f || l != l;
+            const float inv = some ? 1.0f / l : 0.0f;
+#pragma unroll
+            for (int d = 0; d < HD; ++d) o[d] = some ? o[d] * inv : 0.0f;
+            store_vec<float, HD>(static_cast<float*>(a.out) + tok * a.out_stride + hh * HD, o);
+            if (a.lse) a.lse[tok * a.n_heads + hh] = some ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
+          }
+        }
+      }
+      tiles += uint32_t(wk.tb - wk.ta);
+      ++item;
+    } while (ok && wk.next(a));
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (tid == 0 && sh.abort) report(a.batch, ST_ABORTED);
+  if (warp == 4 * (RT + 1)) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+template <typename CT, int HD>
+cudaError_t run_tc32(const AttendArgs& a, cudaStream_t s) {
+  using L = Tc32Cfg<CT, HD>;
+  static_assert(L::SMEM + sizeof(Tc32Shared) <= 227 * 1024, "shared memory");
+  // the register split draws on what the kernel is launched with
+  static const bool fits = [] {
+    cudaFuncAttributes at;
+    return cudaFuncGetAttributes(&at, attend_tc32_kernel<CT, HD>) == cudaSuccess &&
+           (L::RT + 2) * at.numRegs >= L::RT * L::R_SOFT + L::R_LOAD + L::R_MMA;
+  }();
+  if (!fits) return cudaErrorInvalidKernelImage;
+  cudaError_t e = cudaFuncSetAttribute(attend_tc32_kernel<CT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+  if (e != cudaSuccess) return e;
+  CUtensorMap km{}, vm{};
+  int box = 0;
+  if constexpr (!L::F32C) box = make_maps<CT>(&km, &vm, a.pool, TC_TK);
+  attend_tc32_kernel<CT, HD><<<TC_CTAS, L::THREADS, L::SMEM, s>>>(a, km, vm, box);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_attend_tc32(const AttendArgs& a, int cache, cudaStream_t s) {
+  if (cache == E_F16) return a.pool.head_dim == 64 ? run_tc32<__half, 64>(a, s) : run_tc32<__half, 128>(a, s);
+  return a.pool.head_dim == 64 ? run_tc32<float, 64>(a, s) : run_tc32<float, 128>(a, s);
+}
+
+}  // namespace paged
+}  // namespace wcb

@@ -25,7 +25,7 @@ LIB = os.path.join(PKG, "libwcb.so")
 SYNTH_LIB = os.path.join(PKG, "libwcb_synth.so")
 
 CUDA_SOURCES = ["kernels.cu", "gemm_tc.cu", "decode_step.cu", "noalloc.cu", "batch_decode.cu", "attn_prefill.cu", "sample_dev.cu",
-                "paged_append.cu", "paged_attn_16.cu", "paged_attn_32.cu", "paged_attn_tc.cu", "spec_verify.cu"]
+                "paged_append.cu", "paged_attn_16.cu", "paged_attn_32.cu", "paged_attn_tc.cu", "paged_attn_tc32.cu", "spec_verify.cu"]
 HOST_SOURCES = ["gguf.cpp", "sampler.cpp", "model.cpp", "api.cpp", "nccl_rt.cpp", "tokenizer.cpp", "paged.cpp"]
 GENCODE = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
