@@ -242,6 +242,7 @@ uint32_t wcb_paged_attention_dev(const wcb_paged_kv* kv, const wcb_paged_batch* 
   a.scale_log2 = float((scale != 0.0f ? double(scale) : 1.0 / std::sqrt(double(kv->head_dim))) * 1.4426950408889634074);
   a.n_heads = int(n_heads);
   a.rep = int(n_heads / kv->n_kv_heads);
+  a.rep_inv = (uint64_t(1) << 40) / uint64_t(a.rep) + 1;
   a.window = int(window);
   a.tickets = static_cast<int*>(workspace);
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + TICKET_BYTES);

@@ -49,6 +49,7 @@ struct AttendArgs {
   int64_t q_stride, out_stride;
   float scale_log2;  // scale * log2(e)
   int n_heads, rep;  // rep: query heads of a key head
+  uint64_t rep_inv;  // 2^40 / rep, rounded up: rows are divided by rep in many places
   int window;        // 0: none
   int row_lo, row_hi;  // sequences with row_lo < rows (new tokens * rep) <= row_hi are this launch's
   int* tickets;      // one per CTA, zero between calls

@@ -182,6 +182,10 @@ int make_maps(CUtensorMap* k, CUtensorMap* v, const Pool& p, int TK) {
 
 // ---- the line of tiles ------------------------------------------------------
 
+// row / rep and row % rep, exact for rows below 2^33 (2^40 / rep + 1 is too large by at most rep <= 64 parts in 2^40)
+__device__ __forceinline__ int token_of(const AttendArgs& a, int row) { return int((uint64_t(uint32_t(row)) * a.rep_inv) >> 40); }
+__device__ __forceinline__ int head_of(const AttendArgs& a, int row) { return row - token_of(a, row) * a.rep; }
+
 // Keys of rows [r0, r1) of a sequence's key head: lo <= key < hi (in the cache's
 // table), first and last token's positions.
 struct Block {
@@ -190,8 +194,8 @@ struct Block {
 __device__ __forceinline__ Block row_block(const AttendArgs& a, const Seq& q, int rows, int rb, int M, int TK, int table) {
   Block b;
   const int r0 = rb * M, r1 = min(rows, r0 + M);
-  b.pos0 = q.kv - q.n + r0 / a.rep;
-  b.pos1 = q.kv - q.n + (r1 - 1) / a.rep;
+  b.pos0 = q.kv - q.n + token_of(a, r0);
+  b.pos1 = q.kv - q.n + token_of(a, r1 - 1);
   b.hi = min(b.pos1 + 1, table);
   b.lo = a.window > 0 ? max(0, b.pos0 - a.window + 1) : 0;
   b.tile0 = b.lo / TK;
@@ -263,40 +267,58 @@ struct Place {
   int seq;
 };
 
-// All THREADS threads (whole warps). Blocks of THREADS sequences are summed; the one that holds the
-// CTA's first tile is found by a scan.
+// All THREADS threads (whole warps). THREADS sequences at a time are counted, neighbours by different
+// warps (a long chunk keeps a warp busy), and their tiles summed up; the sequence that holds the CTA's
+// first tile is found by a scan.
 template <int THREADS>
-__device__ __forceinline__ Place find_place(const AttendArgs& a, int M, int TK, long long* s_warp, long long* s_out) {
+struct PlaceShared {
+  long long count[THREADS];
+  long long warp[THREADS / 32];
+  long long found[2];
+};
+template <int THREADS>
+__device__ __forceinline__ Place find_place(const AttendArgs& a, int M, int TK, PlaceShared<THREADS>& sh) {
   constexpr int NW = THREADS / 32;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int table = table_tokens(a.pool, a.batch);
   const int n = a.batch.n_seqs;
   Place pl;
-  long long total = 0;
   bool unsound = false;
-  for (int s0 = 0; s0 < n; s0 += THREADS) {
+  // sh.count of sequences s0 .. s0 + THREADS - 1, this thread's sum up to its own, the sum of all
+  auto count = [&](int s0, long long& mine, long long& upto, long long& all) {
+    const int slot = lane * NW + warp, s = s0 + slot;
     Seq q{0, 0, 0, true};
-    if (s0 + tid < n) q = read_seq(a.batch, s0 + tid);
+    if (s < n) q = read_seq(a.batch, s);
     unsound |= !q.sound;
-    total += lane_tiles(a, q, M, TK, table) * a.pool.n_kv;
+    sh.count[slot] = lane_tiles(a, q, M, TK, table) * a.pool.n_kv;
+    __syncthreads();
+    mine = sh.count[tid];
+    long long inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long t = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += t;
+    }
+    if (lane == 31) sh.warp[warp] = inc;
+    __syncthreads();
+    long long before = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      if (w < warp) before += sh.warp[w];
+      all += sh.warp[w];
+    }
+    upto = before + inc;
+  };
+  if (tid == 0) sh.found[0] = -1;
+  long long mine, upto, sum, all = 0;
+  for (int s0 = 0; s0 < n; s0 += THREADS) {
+    if (s0) __syncthreads();
+    count(s0, mine, upto, sum);
+    all += sum;
   }
   if (unsound && blockIdx.x == 0) report(a.batch, ST_BAD_ROWS);
-  long long inc = total;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long t = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += t;
-  }
-  if (lane == 31) s_warp[warp] = inc;
-  if (tid == 0) s_out[0] = -1;
-  __syncthreads();
-  long long all = 0, before = 0;
-#pragma unroll
-  for (int w = 0; w < NW; ++w) {
-    if (w < warp) before += s_warp[w];
-    all += s_warp[w];
-  }
-  pl.per = (all + gridDim.x - 1) / gridDim.x;
+  pl.per = all < 0x7fffffff ? (int(all) + int(gridDim.x) - 1) / int(gridDim.x) : (all + gridDim.x - 1) / gridDim.x;
   if (pl.per < 1) pl.per = 1;
   pl.begin = pl.per * blockIdx.x;
   pl.end = min(all, pl.begin + pl.per);
@@ -306,49 +328,28 @@ __device__ __forceinline__ Place find_place(const AttendArgs& a, int M, int TK, 
     pl.begin = pl.end = 0;
     return pl;  // no work; uniform over the CTA
   }
-  if (n <= THREADS) {
-    const long long first = before + inc - total;
-    if (total > 0 && first <= pl.begin && pl.begin < first + total) {
-      s_out[0] = tid;
-      s_out[1] = first;
+  long long base = 0;
+  for (int s0 = 0;; s0 += THREADS) {
+    if (n > THREADS) {  // (else the one count still stands)
+      __syncthreads();
+      count(s0, mine, upto, sum);
+    }
+    const long long first = base + upto - mine;
+    if (mine > 0 && first <= pl.begin && pl.begin < first + mine) {
+      sh.found[0] = s0 + tid;
+      sh.found[1] = first;
     }
     __syncthreads();
-  } else {
-    long long base = 0;
-    for (int s0 = 0; s0 < n; s0 += THREADS) {
-      const int s = s0 + tid;
-      Seq q{0, 0, 0, true};
-      if (s < n) q = read_seq(a.batch, s);
-      const long long v = lane_tiles(a, q, M, TK, table) * a.pool.n_kv;
-      inc = v;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long t = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += t;
-      }
-      __syncthreads();  // the last round's sums are read
-      if (lane == 31) s_warp[warp] = inc;
-      __syncthreads();
-      before = 0;
-      long long sum = 0;
-#pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        if (w < warp) before += s_warp[w];
-        sum += s_warp[w];
-      }
-      const long long first = base + before + inc - v;
-      if (v > 0 && first <= pl.begin && pl.begin < first + v) {
-        s_out[0] = s;
-        s_out[1] = first;
-      }
-      __syncthreads();
-      base += sum;
-      if (s_out[0] >= 0) break;
-    }
+    base += sum;
+    if (sh.found[0] >= 0 || s0 + THREADS >= n) break;
   }
-  pl.seq = int(s_out[0]);
-  pl.seq_begin = s_out[1];
+  pl.seq = int(sh.found[0]);
+  pl.seq_begin = sh.found[1];
   return pl;
+}
+// (64-bit division is long; nearly every call's counts fit in 32)
+__device__ __forceinline__ int quotient(long long x, long long y) {
+  return x < 0x7fffffff && y < 0x7fffffff ? int(x) / int(y) : int(x / y);
 }
 
 // ---- the kernel -------------------------------------------------------------
@@ -394,7 +395,7 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
   uint4* qfrag = reinterpret_cast<uint4*>(sm + L::RING);
   long long* offs = reinterpret_cast<long long*>(sm + L::RING + L::QBYTES);  // [S + 1][TK]: a key's page or row offset, -1 = none
   unsigned* holes = reinterpret_cast<unsigned*>(offs + (S + 1) * TK);        // [S + 1][2]: keys below the end without a page
-  __shared__ long long s_scan[4], s_place[2];
+  __shared__ PlaceShared<AT_THREADS> s_place;
   __shared__ int s_last;
   __shared__ uint64_t s_full[S];  // a stage's bytes are there (tiles by TMA)
 
@@ -402,7 +403,7 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
   const int g = lane >> 2, t = lane & 3;
   const uint32_t sbase = smem_u32(sm);
   const int table = table_tokens(a.pool, a.batch);
-  const Place pl = find_place<AT_THREADS>(a, M, TK, s_scan, s_place);
+  const Place pl = find_place<AT_THREADS>(a, M, TK, s_place);
   if (pl.begin >= pl.end) return;
   if (tid == 0) {
     for (int i = 0; i < S; ++i) mbar_init(&s_full[i], 1);
@@ -432,7 +433,7 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
   Block blk;
   {
     const long long ht = head_tiles(a, sq, rows, M, TK, table);
-    kvh = int((at - pl.seq_begin) / ht);
+    kvh = quotient(at - pl.seq_begin, ht);
     unit0 = pl.seq_begin + kvh * ht;
     rb = find_block(a, sq, rows, M, TK, table, at, unit0);
     blk = row_block(a, sq, rows, rb, M, TK, table);
@@ -499,7 +500,7 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
     // queries of the block. Row r of the block: token (r0 + r) / rep, head (r0 + r) % rep
     auto q_row = [&](int r) -> const AT* {
       const int gr = r0 + r;
-      return static_cast<const AT*>(a.q) + (sq.r0 + gr / a.rep) * a.q_stride + (kvh * a.rep + gr % a.rep) * HD;
+      return static_cast<const AT*>(a.q) + (sq.r0 + token_of(a, gr)) * a.q_stride + (kvh * a.rep + head_of(a, gr)) * HD;
     };
     uint32_t qf[F32A ? 1 : NB][F32A ? 1 : HD / 16][2];
     if constexpr (!F32A) {
@@ -549,7 +550,7 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
       for (int h = 0; h < 2; ++h) {
         mx[nb][h] = -INFINITY;
         ls[nb][h] = 0.0f;
-        pos[nb][h] = sq.kv - sq.n + (r0 + min(8 * nb + 2 * t + h, rn - 1)) / a.rep;
+        pos[nb][h] = sq.kv - sq.n + token_of(a, r0 + min(8 * nb + 2 * t + h, rn - 1));
       }
 
     bool hole_seen = false;
@@ -811,8 +812,8 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
       const int gr = r0 + r;
       const bool some = l > 0.0f || l != l;
       const float inv = some ? 1.0f / l : 0.0f;
-      const int64_t tok = sq.r0 + gr / a.rep;
-      const int hh = kvh * a.rep + gr % a.rep;
+      const int64_t tok = sq.r0 + token_of(a, gr);
+      const int hh = kvh * a.rep + head_of(a, gr);
       AT* dst = static_cast<AT*>(a.out) + tok * a.out_stride + hh * HD + d;
       const float v0 = some ? x.x * inv : 0.0f, v1 = some ? x.y * inv : 0.0f;
       const float v2 = some ? x.z * inv : 0.0f, v3 = some ? x.w * inv : 0.0f;
@@ -871,7 +872,7 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
     if (!whole) {
       // the last of the unit's CTAs joins its pieces, in their order
       const long long u1 = unit0 + blk.tiles - 1;
-      const int c0 = int(unit0 / pl.per), c1 = int(u1 / pl.per);
+      const int c0 = quotient(unit0, pl.per), c1 = quotient(u1, pl.per);
       __threadfence();
       __syncthreads();
       if (tid == 0) s_last = atomicInc(reinterpret_cast<unsigned*>(a.tickets) + c0, unsigned(c1 - c0)) == unsigned(c1 - c0);
@@ -881,22 +882,36 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
         for (int c = tid; c < rn * (HD / 4); c += AT_THREADS) {
           const int r = c / (HD / 4), d = 4 * (c % (HD / 4));
           auto part = [&](int p) { return a.part + (size_t(p) * 2 + (p == c0 ? 1 : 0)) * size_t(M) * (HD + 2); };
-          float m = -INFINITY;
-          for (int p = c0; p <= c1; ++p) m = fmaxf(m, __ldcg(reinterpret_cast<const float2*>(part(p) + size_t(M) * HD + 2 * r)).x);
-          const float u = m == -INFINITY ? 0.0f : m;
-          float l = 0.0f;
+          // eight pieces at a time: their loads are on the way together
+          float m = -INFINITY, l = 0.0f;
           float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-          for (int p = c0; p <= c1; ++p) {
-            const float* pc = part(p);
-            const float2 q = __ldcg(reinterpret_cast<const float2*>(pc + size_t(M) * HD + 2 * r));
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(pc + size_t(r) * HD + d));
-            const float f = fast_exp2(q.x - u);
-            l += f * q.y;
-            x.x += f * v.x;
-            x.y += f * v.y;
-            x.z += f * v.z;
-            x.w += f * v.w;
+          for (int p0 = c0; p0 <= c1; p0 += 8) {
+            float2 q[8];
+            float4 v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float* pc = part(min(p0 + j, c1));
+              q[j] = __ldcg(reinterpret_cast<const float2*>(pc + size_t(M) * HD + 2 * r));
+              v[j] = __ldcg(reinterpret_cast<const float4*>(pc + size_t(r) * HD + d));
+            }
+            float nm = m;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) nm = fmaxf(nm, q[j].x);
+            const float u = nm == -INFINITY ? 0.0f : nm, f0 = fast_exp2(m - u);
+            m = nm;
+            l *= f0;
+            x = make_float4(x.x * f0, x.y * f0, x.z * f0, x.w * f0);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float f = p0 + j <= c1 ? fast_exp2(q[j].x - u) : 0.0f;
+              if (p0 + j <= c1) {
+                l += f * q[j].y;
+                x.x += f * v[j].x;
+                x.y += f * v[j].y;
+                x.z += f * v[j].z;
+                x.w += f * v[j].w;
+              }
+            }
           }
           finish(r, d, x, m, l);
         }

@@ -59,10 +59,11 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
   extern __shared__ uint8_t raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   __shared__ TcShared sh;
+  __shared__ PlaceShared<TC_THREADS> s_place;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t sbase = smem_u32(sm);
 
-  const Place pl = find_place<TC_THREADS>(a, TC_M, TC_TK, sh.scan, sh.place);
+  const Place pl = find_place<TC_THREADS>(a, TC_M, TC_TK, s_place);
   if (pl.begin >= pl.end) return;  // the whole CTA; nothing is held yet
 
   if (tid == 0) {
@@ -294,27 +295,32 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
     const uint32_t ts = tmem + lanes + 128 * w, to = tmem + lanes + 256 + 128 * w;
     uint32_t tiles = 0, t = 0, item = 0, cuts = 0;  // tiles of the ring, tiles of keys with rows, units, units cut
     bool ok = true;
+    // the row tile's queries, and at a unit's end its results on their way out
+    uint8_t* qt = sm + L::Q + w * L::TILE;
+    constexpr int RPI = 32 / CH;             // rows that a warp moves at once
+    const int r32 = 32 * (warp & 3);         // its first row
     do {
       const int r0 = wk.rb * TC_M + 128 * w, rn = min(128, wk.rows - r0);
       const int end = wk.end_of(a, w);
       if (end > wk.ta) {
-        // queries into shared memory; rows that are not there are zeros
-        uint8_t* qt = sm + L::Q + w * L::TILE;
-        // (a thread its own row: one division, all loads on their way at once)
+        // queries into shared memory: a warp its own 32 rows, whole rows at a time; rows that are not there are zeros
         const int gr = r0 + min(row, rn - 1);
         {
-          const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (wk.sq.r0 + gr / a.rep) * a.q_stride +
-                                                            (wk.kvh * a.rep + gr % a.rep) * HD);
-          uint4 x[CH];
+          uint4 x[32 / RPI];
 #pragma unroll
-          for (int ch = 0; ch < CH; ++ch) x[ch] = row < rn ? __ldg(src + ch) : make_uint4(0, 0, 0, 0);
+          for (int j = 0; j < 32 / RPI; ++j) {
+            const int r = r32 + RPI * j + lane / CH, g = r0 + r;
+            x[j] = r < rn ? __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (wk.sq.r0 + token_of(a, g)) * a.q_stride +
+                                                                 (wk.kvh * a.rep + head_of(a, g)) * HD) + lane % CH)
+                          : make_uint4(0, 0, 0, 0);
+          }
 #pragma unroll
-          for (int ch = 0; ch < CH; ++ch) *reinterpret_cast<uint4*>(qt + tile_at(row, ch)) = x[ch];
+          for (int j = 0; j < 32 / RPI; ++j) *reinterpret_cast<uint4*>(qt + tile_at(r32 + RPI * j + lane / CH, lane % CH)) = x[j];
         }
         fence_proxy_async();
         bar_arrive(&sh.q_full[w]);
 
-        const int pos = wk.sq.kv - wk.sq.n + gr / a.rep;
+        const int pos = wk.sq.kv - wk.sq.n + token_of(a, gr);
         const int khi = min(pos + 1, wk.table), klo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
         float m = -INFINITY, l = 0.0f;  // m: the maximum that O and l are scaled by
         for (int i = wk.ta; i < end && ok; ++i) {
@@ -441,11 +447,33 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
         constexpr size_t PIECE = size_t(TC_M) * (HD + 2);
         float* piece = a.part + (size_t(blockIdx.x) * 2 + (wk.ta == 0 ? 1 : 0)) * PIECE + 128 * w + row;
         const bool odd = *reinterpret_cast<volatile int*>(&sh.odd[item % ODD_RING]) != 0;
-        const int64_t tok = wk.sq.r0 + gr / a.rep;
-        const int hh = wk.kvh * a.rep + gr % a.rep;
+        const int64_t tok = wk.sq.r0 + token_of(a, gr);
+        const int hh = wk.kvh * a.rep + head_of(a, gr);
         const bool some = (l > 0.0f && m > -INFINITY) || l != l;
         const float inv = some ? 1.0f / l : 0.0f;
-        T* dst = static_cast<T*>(a.out) + tok * a.out_stride + hh * HD;
+        // rows leave through shared memory, each warp its own: a thread's row by itself would be 32 lines a store
+        auto stage = [&](const float (&x)[32], int q) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint4 y;
+            y.x = pack2<T>(x[8 * c], x[8 * c + 1]);
+            y.y = pack2<T>(x[8 * c + 2], x[8 * c + 3]);
+            y.z = pack2<T>(x[8 * c + 4], x[8 * c + 5]);
+            y.w = pack2<T>(x[8 * c + 6], x[8 * c + 7]);
+            *reinterpret_cast<uint4*>(qt + tile_at(row, 4 * q + c)) = y;
+          }
+        };
+        auto send = [&] {
+          __syncwarp();
+#pragma unroll 4
+          for (int j = 0; j < 32 / RPI; ++j) {
+            const int r = r32 + RPI * j + lane / CH, g = r0 + r;
+            if (r < rn)
+              *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (wk.sq.r0 + token_of(a, g)) * a.out_stride + (wk.kvh * a.rep + head_of(a, g)) * HD +
+                                        8 * (lane % CH)) = *reinterpret_cast<const uint4*>(qt + tile_at(r, lane % CH));
+          }
+          __syncwarp();
+        };
 #pragma unroll 1
         for (int q = 0; q < HD / 32; ++q) {
           uint32_t v[32];
@@ -471,19 +499,18 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
               }
             }
           }
-          if (row < rn) {
-            if (whole) {
-              float x[32];
+          if (whole) {
+            float x[32];
 #pragma unroll
-              for (int e = 0; e < 32; ++e) x[e] = some ? __uint_as_float(v[e]) * inv : 0.0f;
-              store_vec<T, 32>(dst + 32 * q, x);
-            } else {
+            for (int e = 0; e < 32; ++e) x[e] = some ? __uint_as_float(v[e]) * inv : 0.0f;
+            stage(x, q);
+          } else if (row < rn) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) piece[size_t(32 * q + e) * TC_M] = __uint_as_float(v[e]);
-            }
+            for (int e = 0; e < 32; ++e) piece[size_t(32 * q + e) * TC_M] = __uint_as_float(v[e]);
           }
         }
         tc_fence_before();
+        if (whole) send();
         if (row < rn) {
           if (whole) {
             if (a.lse) a.lse[tok * a.n_heads + hh] = some ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
@@ -498,53 +525,52 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
           if (wk.blk.pos0 < 0) bits |= ST_BAD_LEN;
           report(a.batch, bits);
         }
-      }
-      if (end > wk.ta && !(wk.ta == 0 && wk.tb == wk.blk.tiles)) {
-        // the last of the unit's CTAs joins this tile's pieces, in their order
-        const int c0 = int(wk.unit0 / wk.pl.per), c1 = int((wk.unit0 + wk.blk.tiles - 1) / wk.pl.per);
-        __threadfence();
-        bar_arrive(&sh.piece_full[w]);
-        ok = tc_wait_warp(&sh, &sh.piece_full[w], cuts & 1);
-        if (!ok) break;
-        if (row == 0) {
-          sh.last[w] = atomicInc(reinterpret_cast<unsigned*>(a.tickets) + TC_TICKETS + 2 * c0 + w, unsigned(c1 - c0)) == unsigned(c1 - c0);
-          bar_arrive(&sh.last_full[w]);
-        }
-        ok = tc_wait_warp(&sh, &sh.last_full[w], cuts & 1);
-        if (!ok) break;
-        ++cuts;
-        if (sh.last[w] && row < rn) {
+        if (!whole) {
+          // the last of the unit's CTAs joins this tile's pieces, in their order
+          const int c0 = quotient(wk.unit0, wk.pl.per), c1 = quotient(wk.unit0 + wk.blk.tiles - 1, wk.pl.per);
           __threadfence();
-          constexpr size_t PIECE = size_t(TC_M) * (HD + 2);
-          auto part = [&](int p) { return a.part + (size_t(p) * 2 + (p == c0 ? 1 : 0)) * PIECE + 128 * w + row; };
-          float m = -INFINITY;
-          for (int p = c0; p <= c1; ++p) m = fmaxf(m, __ldcg(part(p) + size_t(HD) * TC_M));
-          const float u = m == -INFINITY ? 0.0f : m;
-          float l = 0.0f;
-          for (int p = c0; p <= c1; ++p) l += fast_exp2(__ldcg(part(p) + size_t(HD) * TC_M) - u) * __ldcg(part(p) + size_t(HD + 1) * TC_M);
-          const bool some = l > 0.0f || l != l;
-          const float inv = some ? 1.0f / l : 0.0f;
-          const int gr = r0 + row;
-          const int64_t tok = wk.sq.r0 + gr / a.rep;
-          const int hh = wk.kvh * a.rep + gr % a.rep;
-          T* dst = static_cast<T*>(a.out) + tok * a.out_stride + hh * HD;
-#pragma unroll 1
-          for (int q = 0; q < HD / 64; ++q) {
-            float x[64];
-#pragma unroll
-            for (int e = 0; e < 64; ++e) x[e] = 0.0f;
-#pragma unroll 1
-            for (int p = c0; p <= c1; ++p) {
-              const float* pp = part(p);
-              const float f = fast_exp2(__ldcg(pp + size_t(HD) * TC_M) - u);
-#pragma unroll
-              for (int e = 0; e < 64; ++e) x[e] += f * __ldcg(pp + size_t(64 * q + e) * TC_M);
-            }
-#pragma unroll
-            for (int e = 0; e < 64; ++e) x[e] = some ? x[e] * inv : 0.0f;
-            store_vec<T, 64>(dst + 64 * q, x);
+          bar_arrive(&sh.piece_full[w]);
+          ok = tc_wait_warp(&sh, &sh.piece_full[w], cuts & 1);
+          if (!ok) break;
+          if (row == 0) {
+            sh.last[w] = atomicInc(reinterpret_cast<unsigned*>(a.tickets) + TC_TICKETS + 2 * c0 + w, unsigned(c1 - c0)) == unsigned(c1 - c0);
+            bar_arrive(&sh.last_full[w]);
           }
-          if (a.lse) a.lse[tok * a.n_heads + hh] = some ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
+          ok = tc_wait_warp(&sh, &sh.last_full[w], cuts & 1);
+          if (!ok) break;
+          ++cuts;
+          if (sh.last[w]) {
+            __threadfence();
+            auto part = [&](int p) { return a.part + (size_t(p) * 2 + (p == c0 ? 1 : 0)) * PIECE + 128 * w + row; };
+            float jm = -INFINITY, jl = 0.0f;
+            if (row < rn)
+              for (int p = c0; p <= c1; ++p) jm = fmaxf(jm, __ldcg(part(p) + size_t(HD) * TC_M));
+            const float u = jm == -INFINITY ? 0.0f : jm;
+            if (row < rn)
+              for (int p = c0; p <= c1; ++p) jl += fast_exp2(__ldcg(part(p) + size_t(HD) * TC_M) - u) * __ldcg(part(p) + size_t(HD + 1) * TC_M);
+            const bool any = jl > 0.0f || jl != jl;
+            const float jinv = any ? 1.0f / jl : 0.0f;
+#pragma unroll 1
+            for (int q = 0; q < HD / 32; ++q) {
+              float x[32];
+#pragma unroll
+              for (int e = 0; e < 32; ++e) x[e] = 0.0f;
+              if (row < rn) {
+#pragma unroll 2
+                for (int p = c0; p <= c1; ++p) {
+                  const float* pp = part(p);
+                  const float f = fast_exp2(__ldcg(pp + size_t(HD) * TC_M) - u);
+#pragma unroll
+                  for (int e = 0; e < 32; ++e) x[e] = fmaf(f, __ldcg(pp + size_t(32 * q + e) * TC_M), x[e]);
+                }
+              }
+#pragma unroll
+              for (int e = 0; e < 32; ++e) x[e] = any ? x[e] * jinv : 0.0f;
+              stage(x, q);
+            }
+            send();
+            if (a.lse && row < rn) a.lse[tok * a.n_heads + hh] = any ? (jm + log2f(jl)) * 0.69314718055994531f : -INFINITY;
+          }
         }
       }
       tiles += uint32_t(wk.tb - wk.ta);

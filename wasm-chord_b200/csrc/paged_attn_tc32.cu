@@ -75,10 +75,11 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
   extern __shared__ uint8_t raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   __shared__ Tc32Shared sh;
+  __shared__ PlaceShared<L::THREADS> s_place;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t sbase = smem_u32(sm);
 
-  const Place pl = find_place<L::THREADS>(a, M, TC_TK, sh.scan, sh.place);
+  const Place pl = find_place<L::THREADS>(a, M, TC_TK, s_place);
   if (pl.begin >= pl.end) return;  // the whole CTA; nothing is held yet
 
   if (tid == 0) {
@@ -395,46 +396,56 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
     const uint32_t ts = tmem + lanes + 128 * w, to = tmem + lanes + 256 + 128 * w;
     uint32_t tiles = 0, t = 0, item = 0, cuts = 0;  // tiles of the ring, tiles of keys with rows, units, units cut
     bool ok = true;
+    // the row tile's queries (two f16 parts), and at a unit's end its results on their way out
+    uint8_t* qt = sm + L::Q + w * 2 * L::PART;
+    constexpr int LPR = HD / 4, RPI = 32 / LPR;  // lanes of a row, rows that a warp moves at once
+    const int r32 = 32 * (warp & 3);             // its first row
     do {
       const int r0 = wk.rb * M + 128 * w, rn = min(128, wk.rows - r0);
       const int end = wk.end_of(a, w);
       if (end > wk.ta) {
-        // the row's query, scaled and split; rows that are not there are zeros
+        // the queries, scaled and split: a warp its own 32 rows, whole rows at a time; rows that are not there are zeros
         const int gr = r0 + min(row, rn - 1);
-        float qinv;
-        {
-          const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + (wk.sq.r0 + gr / a.rep) * a.q_stride +
-                                                              (wk.kvh * a.rep + gr % a.rep) * HD);
-          float top = 0.0f;
+        float qinv = 1.0f;
 #pragma unroll
-          for (int j = 0; j < HD / 4; ++j) {
-            const float4 x = __ldg(src + j);
+        for (int j0 = 0; j0 < 32 / RPI; j0 += 8) {
+          float4 x[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int r = r32 + RPI * (j0 + j) + lane / LPR, g = r0 + r;
+            x[j] = r < rn ? __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + (wk.sq.r0 + token_of(a, g)) * a.q_stride +
+                                                                  (wk.kvh * a.rep + head_of(a, g)) * HD) + lane % LPR)
+                          : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float top = 0.0f;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float z = fabsf((&x.x)[e]);
+              const float z = fabsf((&x[j].x)[e]);
               if (z <= FLT_MAX) top = fmaxf(top, z);
             }
-          }
-          const int ge = group_exp(top, 0);
-          qinv = pow2(ge);
-          const float f = row < rn ? pow2(-ge) : 0.0f;
-          uint8_t* qt = sm + L::Q + w * 2 * L::PART;
 #pragma unroll
-          for (int ch = 0; ch < HD / 8; ++ch) {
-            const float4 x = __ldg(src + 2 * ch), y = __ldg(src + 2 * ch + 1);
-            uint4 h, l;
-            split_f16(x.x * f, x.y * f, h.x, l.x);
-            split_f16(x.z * f, x.w * f, h.y, l.y);
-            split_f16(y.x * f, y.y * f, h.z, l.z);
-            split_f16(y.z * f, y.w * f, h.w, l.w);
-            *reinterpret_cast<uint4*>(qt + tile_at(row, ch)) = h;
-            *reinterpret_cast<uint4*>(qt + L::PART + tile_at(row, ch)) = l;
+            for (int d = LPR / 2; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            const int ge = group_exp(top, 0);
+            const float f = pow2(-ge), back = pow2(ge);
+#pragma unroll
+            for (int i = 0; i < RPI; ++i) {
+              const float v = __shfl_sync(0xffffffffu, back, i * LPR);
+              if (lane == RPI * (j0 + j) + i) qinv = v;
+            }
+            uint2 h, l;
+            split_f16(x[j].x * f, x[j].y * f, h.x, l.x);
+            split_f16(x[j].z * f, x[j].w * f, h.y, l.y);
+            const uint32_t o = tile_at(r32 + RPI * (j0 + j) + lane / LPR, (lane % LPR) >> 1) + 8 * (lane & 1);
+            *reinterpret_cast<uint2*>(qt + o) = h;
+            *reinterpret_cast<uint2*>(qt + L::PART + o) = l;
           }
         }
         fence_proxy_async();
         bar_arrive(&sh.q_full[w]);
 
-        const int pos = wk.sq.kv - wk.sq.n + gr / a.rep;
+        const int pos = wk.sq.kv - wk.sq.n + token_of(a, gr);
         const int khi = min(pos + 1, wk.table), klo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
         float m = -INFINITY, l = 0.0f;  // m: the maximum that O and l are scaled by
         float o[HD];
@@ -591,24 +602,40 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
         }
         // results: normalised, or a piece [HD][M] + m [M] + l [M]
         const bool whole = wk.ta == 0 && wk.tb == wk.blk.tiles;
-        const int64_t tok = wk.sq.r0 + gr / a.rep;
-        const int hh = wk.kvh * a.rep + gr % a.rep;
+        const int64_t tok = wk.sq.r0 + token_of(a, gr);
+        const int hh = wk.kvh * a.rep + head_of(a, gr);
         constexpr size_t PIECE = size_t(M) * (HD + 2);
-        if (row < rn) {
-          if (whole) {
-            const bool some = (l > 0.0f && m > -INFINITY) || l != l;
-            const float inv = some ? 1.0f / l : 0.0f;
+        // rows leave through shared memory, each warp its own: a thread's row by itself would be 32 lines a store
+        auto send = [&] {
+          const bool some = (l > 0.0f && m > -INFINITY) || l != l;
+          const float inv = some ? 1.0f / l : 0.0f;
 #pragma unroll
-            for (int d = 0; d < HD; ++d) o[d] = some ? o[d] * inv : 0.0f;
-            store_vec<float, HD>(static_cast<float*>(a.out) + tok * a.out_stride + hh * HD, o);
-            if (a.lse) a.lse[tok * a.n_heads + hh] = some ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
-          } else {
-            float* piece = a.part + (size_t(blockIdx.x) * 2 + (wk.ta == 0 ? 1 : 0)) * PIECE + 128 * w + row;
+          for (int c = 0; c < HD / 4; ++c) {
+            float4 y;
 #pragma unroll
-            for (int d = 0; d < HD; ++d) piece[size_t(d) * M] = o[d];
-            piece[size_t(HD) * M] = m;
-            piece[size_t(HD + 1) * M] = l;
+            for (int e = 0; e < 4; ++e) (&y.x)[e] = some ? o[4 * c + e] * inv : 0.0f;
+            *reinterpret_cast<float4*>(qt + (c / (HD / 8)) * L::PART + tile_at(row, c % (HD / 8))) = y;
           }
+          __syncwarp();
+#pragma unroll 4
+          for (int j = 0; j < 32 / RPI; ++j) {
+            const int r = r32 + RPI * j + lane / LPR, g = r0 + r, c = lane % LPR;
+            if (r < rn)
+              *reinterpret_cast<float4*>(static_cast<float*>(a.out) + (wk.sq.r0 + token_of(a, g)) * a.out_stride +
+                                         (wk.kvh * a.rep + head_of(a, g)) * HD + 4 * c) =
+                  *reinterpret_cast<const float4*>(qt + (c / (HD / 8)) * L::PART + tile_at(r, c % (HD / 8)));
+          }
+          __syncwarp();
+          if (a.lse && row < rn) a.lse[tok * a.n_heads + hh] = some ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
+        };
+        if (whole) {
+          send();
+        } else if (row < rn) {
+          float* piece = a.part + (size_t(blockIdx.x) * 2 + (wk.ta == 0 ? 1 : 0)) * PIECE + 128 * w + row;
+#pragma unroll
+          for (int d = 0; d < HD; ++d) piece[size_t(d) * M] = o[d];
+          piece[size_t(HD) * M] = m;
+          piece[size_t(HD + 1) * M] = l;
         }
         if (row == 0 && w == 0) {
           uint32_t bits = 0;
@@ -618,7 +645,7 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
         }
         if (!whole) {
           // the last of the unit's CTAs joins this tile's pieces, in their order
-          const int c0 = int(wk.unit0 / wk.pl.per), c1 = int((wk.unit0 + wk.blk.tiles - 1) / wk.pl.per);
+          const int c0 = quotient(wk.unit0, wk.pl.per), c1 = quotient(wk.unit0 + wk.blk.tiles - 1, wk.pl.per);
           __threadfence();
           bar_arrive(&sh.piece_full[w]);
           ok = tc_wait_warp(&sh, &sh.piece_full[w], cuts & 1);
@@ -630,29 +657,26 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
           ok = tc_wait_warp(&sh, &sh.last_full[w], cuts & 1);
           if (!ok) break;
           ++cuts;
-          if (sh.last[w] && row < rn) {
+          if (sh.last[w]) {
             __threadfence();
-            auto part = [&](int p) { return a.part + (size_t(p) * 2 + (p == c0 ? 1 : 0)) * PIECE + 128 * w + row; };
             m = -INFINITY;
-            for (int p = c0; p <= c1; ++p) m = fmaxf(m, __ldcg(part(p) + size_t(HD) * M));
-            const float u = m == -INFINITY ? 0.0f : m;
             l = 0.0f;
 #pragma unroll
             for (int d = 0; d < HD; ++d) o[d] = 0.0f;
+            if (row < rn) {
+              auto part = [&](int p) { return a.part + (size_t(p) * 2 + (p == c0 ? 1 : 0)) * PIECE + 128 * w + row; };
+              for (int p = c0; p <= c1; ++p) m = fmaxf(m, __ldcg(part(p) + size_t(HD) * M));
+              const float u = m == -INFINITY ? 0.0f : m;
 #pragma unroll 1
-            for (int p = c0; p <= c1; ++p) {
-              const float* pp = part(p);
-              const float f = fast_exp2(__ldcg(pp + size_t(HD) * M) - u);
-              l += f * __ldcg(pp + size_t(HD + 1) * M);
+              for (int p = c0; p <= c1; ++p) {
+                const float* pp = part(p);
+                const float f = fast_exp2(__ldcg(pp + size_t(HD) * M) - u);
+                l += f * __ldcg(pp + size_t(HD + 1) * M);
 #pragma unroll
-              for (int d = 0; d < HD; ++d) o[d] = fmaf(f, __ldcg(pp + size_t(d) * M), o[d]);
+                for (int d = 0; d < HD; ++d) o[d] = fmaf(f, __ldcg(pp + size_t(d) * M), o[d]);
+              }
             }
-            const bool some = l > 0.0f || l != l;
-            const float inv = some ? 1.0f / l : 0.0f;
-#pragma unroll
-            for (int d = 0; d < HD; ++d) o[d] = some ? o[d] * inv : 0.0f;
-            store_vec<float, HD>(static_cast<float*>(a.out) + tok * a.out_stride + hh * HD, o);
-            if (a.lse) a.lse[tok * a.n_heads + hh] = some ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
+            send();
           }
         }
       }

@@ -109,7 +109,6 @@ struct TcShared {
   uint32_t holes[HOLE_RING][4];  // keys of a tile without a page
   int odd[ODD_RING];             // by item: a ragged tile has infinities or NaN among its values
   int last[2];
-  long long scan[16], place[2];
 };
 
 // Bounded wait: about 2^24 polls, or until another thread has given up.
@@ -153,7 +152,7 @@ struct Walk {
     rows = seq_rows(a, sq);
     at = pl.begin;
     const long long ht = head_tiles(a, sq, rows, M, TC_TK, table);
-    kvh = int((at - pl.seq_begin) / ht);
+    kvh = quotient(at - pl.seq_begin, ht);
     unit0 = pl.seq_begin + kvh * ht;
     rb = find_block(a, sq, rows, M, TC_TK, table, at, unit0);
     blk = row_block(a, sq, rows, rb, M, TC_TK, table);
@@ -189,7 +188,7 @@ struct Walk {
     const int r0 = rb * M + 128 * w;
     if (r0 >= rows) return ta;
     const int r1 = min(rows, r0 + 128);
-    const int hi = min(sq.kv - sq.n + (r1 - 1) / a.rep + 1, table);
+    const int hi = min(sq.kv - sq.n + token_of(a, r1 - 1) + 1, table);
     const int t = (max(hi, 0) + TC_TK - 1) / TC_TK - blk.tile0;
     return max(min(t, tb), ta + 1);
   }
