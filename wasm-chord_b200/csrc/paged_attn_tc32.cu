@@ -56,13 +56,21 @@ __device__ __forceinline__ int group_exp(float top, int none) {
   const int e = int(__float_as_uint(top) >> 23) - 127;  // top in [2^e, 2^(e + 1)); below 2^-126: -127
   return top > 0.0f ? max(-100, min(120, e - 13)) : none;
 }
-// two numbers as two f16 each
-__device__ __forceinline__ void split_f16(float x, float y, uint32_t& hi, uint32_t& lo) {
+// (two f32 operations in one instruction)
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// two finite numbers as two f16 each
+__device__ __forceinline__ void split_f16(uint64_t z, uint32_t& hi, uint32_t& lo) {
+  float x, y;
+  unpack_f32x2(z, x, y);
   const __half2 h = __floats2half2_rn(x, y);
   const float2 f = __half22float2(h);
   hi = *reinterpret_cast<const uint32_t*>(&h);
-  // an infinity or NaN stays in hi alone
-  lo = pack2<__half>(fabsf(f.x) <= FLT_MAX ? x - f.x : 0.0f, fabsf(f.y) <= FLT_MAX ? y - f.y : 0.0f);
+  unpack_f32x2(add_f32x2(z, pack_f32x2(-f.x, -f.y)), x, y);
+  lo = pack2<__half>(x, y);
 }
 
 template <typename CT, int HD>
@@ -260,49 +268,74 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
           const int sub = lane % LPR, rr = lane / LPR;
           const float* base[2] = {static_cast<const float*>(a.pool.k) + wk.kvh * a.pool.head_stride + 4 * sub,
                                   static_cast<const float*>(a.pool.v) + wk.kvh * a.pool.head_stride + 4 * sub};
-#pragma unroll 1
-          for (int u = 0; u < 4; ++u) {  // K's halves, V's halves
-            const int kvi = u >> 1, b = u & 1;
-            float4 x[IT];
+          // K's halves, V's halves: the next one is on its way while one is split. (A rolled loop, like all that is long here:
+          // the roles' code together has to stay in the instruction cache. Unrolled, the kernel took 1.81 ms where
+          // it takes 1.50 ms at 46 sequences of 919 new tokens, 32/4 heads of 64.)
+          float4 y[IT], ahead[IT];
+          auto load = [&](int u) {
+            const float* from = u < 2 ? base[0] : base[1];
 #pragma unroll
             for (int j = 0; j < IT; ++j) {
-              const long long o = __shfl_sync(0xffffffffu, off, 16 * b + RPI * j + rr);
-              x[j] = o >= 0 ? __ldg(reinterpret_cast<const float4*>(base[kvi] + o)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              const long long o = __shfl_sync(0xffffffffu, off, 16 * (u & 1) + RPI * j + rr);
+              ahead[j] = o >= 0 ? __ldg(reinterpret_cast<const float4*>(from + o)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             }
+          };
+#pragma unroll 1
+          for (int u = -1; u < 4; ++u) {
+            const int kvi = u >> 1, b = u & 1;
+#pragma unroll
+            for (int j = 0; j < IT; ++j) y[j] = ahead[j];
+            if (u < 3) load(u + 1);
+            if (u < 0) continue;
             if (b == 0) {
-              ok = room(n + kvi);
+              ok = ok && room(n + kvi);
               if (!ok) break;
             }
             float top = 0.0f;
-            bool odd = false;
+            uint64_t zero = 0;  // NaN where a number is not finite
 #pragma unroll
-            for (int j = 0; j < IT; ++j)
+            for (int j = 0; j < IT; ++j) {
+              top = fmaxf(fmaxf(top, fmaxf(fabsf(y[j].x), fabsf(y[j].y))), fmaxf(fabsf(y[j].z), fabsf(y[j].w)));
+              zero = fma_f32x2(pack_f32x2(y[j].x, y[j].y), 0, zero);
+              zero = fma_f32x2(pack_f32x2(y[j].z, y[j].w), 0, zero);
+            }
+            float z0, z1;
+            unpack_f32x2(zero, z0, z1);
+            const bool bad = __any_sync(0xffffffffu, z0 != z0 || z1 != z1);
+            if (bad) {
+              // infinities and NaN take no part in the exponent; a value's is added to O at the end, to the
+              // rows that see it
+              top = 0.0f;
+              bool odd = false;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                float& y = (&x[j].x)[e];
-                const float z = fabsf(y);
-                if (!(z <= FLT_MAX)) {
-                  // infinities and NaN: a value's is added to O at the end, to the rows that see it
-                  if (kvi) {
+              for (int j = 0; j < IT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  float& v = (&y[j].x)[e];
+                  if (fabsf(v) <= FLT_MAX) {
+                    top = fmaxf(top, fabsf(v));
+                  } else if (kvi) {
                     odd = true;
-                    y = 0.0f;
+                    v = 0.0f;
                   }
-                } else {
-                  top = fmaxf(top, z);
                 }
-              }
-            if (odd) sh.odd[item % ODD_RING] = 1;
+              if (odd) sh.odd[item % ODD_RING] = 1;
+            }
 #pragma unroll
             for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
             const int ge = group_exp(top, kvi ? -126 : 0);  // zeros among values never make the largest exponent
             if (lane == 0) (kvi ? sh.vexp : sh.kexp)[tiles % EXP_RING][4 * b + lw] = ge;
-            const float f = pow2(-ge);
+            const uint64_t f = pack_f32x2(pow2(-ge), pow2(-ge));
             uint8_t* dst = sm + L::RING + ((n + kvi) % NS) * L::SLOT;
 #pragma unroll
             for (int j = 0; j < IT; ++j) {
               uint2 h, l;
-              split_f16(x[j].x * f, x[j].y * f, h.x, l.x);
-              split_f16(x[j].z * f, x[j].w * f, h.y, l.y);
+              const uint64_t z0 = mul_f32x2(pack_f32x2(y[j].x, y[j].y), f), z1 = mul_f32x2(pack_f32x2(y[j].z, y[j].w), f);
+              split_f16(z0, h.x, l.x);
+              split_f16(z1, h.y, l.y);
+              if (bad) {  // an infinity or NaN stays in hi alone
+                if (!finite16<__half>(h.x) || !finite16<__half>(h.y)) l = make_uint2(0, 0);
+              }
               const uint32_t o = tile_at(64 * b + 16 * lw + RPI * j + rr, sub >> 1) + 8 * (sub & 1);
               *reinterpret_cast<uint2*>(dst + o) = h;
               *reinterpret_cast<uint2*>(dst + L::PART + o) = l;
@@ -407,7 +440,7 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
         // the queries, scaled and split: a warp its own 32 rows, whole rows at a time; rows that are not there are zeros
         const int gr = r0 + min(row, rn - 1);
         float qinv = 1.0f;
-#pragma unroll
+#pragma unroll 1
         for (int j0 = 0; j0 < 32 / RPI; j0 += 8) {
           float4 x[8];
 #pragma unroll
@@ -419,12 +452,8 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
           }
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            float top = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float z = fabsf((&x[j].x)[e]);
-              if (z <= FLT_MAX) top = fmaxf(top, z);
-            }
+            // (a row with an infinity or NaN gives NaN)
+            float top = fmaxf(fmaxf(fabsf(x[j].x), fabsf(x[j].y)), fmaxf(fabsf(x[j].z), fabsf(x[j].w)));
 #pragma unroll
             for (int d = LPR / 2; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
             const int ge = group_exp(top, 0);
@@ -435,8 +464,8 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
               if (lane == RPI * (j0 + j) + i) qinv = v;
             }
             uint2 h, l;
-            split_f16(x[j].x * f, x[j].y * f, h.x, l.x);
-            split_f16(x[j].z * f, x[j].w * f, h.y, l.y);
+            split_f16(mul_f32x2(pack_f32x2(x[j].x, x[j].y), pack_f32x2(f, f)), h.x, l.x);
+            split_f16(mul_f32x2(pack_f32x2(x[j].z, x[j].w), pack_f32x2(f, f)), h.y, l.y);
             const uint32_t o = tile_at(r32 + RPI * (j0 + j) + lane / LPR, (lane % LPR) >> 1) + 8 * (lane & 1);
             *reinterpret_cast<uint2*>(qt + o) = h;
             *reinterpret_cast<uint2*>(qt + L::PART + o) = l;
@@ -512,50 +541,48 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
             float sum;
             auto exponentials = [&] {
               const float use = m == -INFINITY ? 0.0f : m;
-              float s0 = 0.0f, s1 = 0.0f;
+              uint64_t s2[2] = {0, 0};
 #pragma unroll
-              for (int q = 0; q < 2; ++q) {
-                uint32_t p[16], r[16];
+              for (int q = 0; q < 4; ++q) {
+                uint32_t p[8], r[8];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                  const int c = 32 * q + 2 * e, gq = F32C ? c / 16 : 0;
-                  float x = fast_exp2(fmaf(__uint_as_float(v[c]), kf[gq], -use)), y = fast_exp2(fmaf(__uint_as_float(v[c + 1]), kf[gq], -use));
-                  s0 += x;
-                  s1 += y;
-                  if (F32C) {
-                    x *= vf[gq];
-                    y *= vf[gq];
-                  }
-                  const __half2 h = __floats2half2_rn(x, y);
-                  const float2 f = __half22float2(h);
-                  p[e] = *reinterpret_cast<const uint32_t*>(&h);
-                  r[e] = pack2<__half>(x - f.x, y - f.y);
+                for (int e = 0; e < 8; ++e) {
+                  const int c = 16 * q + 2 * e, gq = F32C ? q : 0;
+                  float x, y;
+                  unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), pack_f32x2(kf[gq], kf[gq]), pack_f32x2(-use, -use)), x, y);
+                  uint64_t z = pack_f32x2(fast_exp2(x), fast_exp2(y));
+                  s2[e & 1] = add_f32x2(s2[e & 1], z);
+                  if (F32C) z = mul_f32x2(z, pack_f32x2(vf[gq], vf[gq]));
+                  split_f16(z, p[e], r[e]);
                 }
-                tmem_st16(ts + 64 * b + 16 * q, p);
-                tmem_st16(ts + 64 * b + 32 + 16 * q, r);
+                tmem_st8(ts + 64 * b + 8 * q, p);
+                tmem_st8(ts + 64 * b + 32 + 8 * q, r);
               }
-              sum = s0 + s1;
+              float x0, y0, x1, y1;
+              unpack_f32x2(s2[0], x0, y0);
+              unpack_f32x2(s2[1], x1, y1);
+              sum = (x0 + y0) + (x1 + y1);
             };
             // (paged_attn_tc.cu: the maximum only where the sum asks for it)
-            bool again = __any_sync(0xffffffffu, mask || m == -INFINITY);
-            if (!again) {
-              exponentials();
-              again = __any_sync(0xffffffffu, !(sum <= GROWTH));
-            }
-            if (again) {
-              float top = -INFINITY;
+            for (bool again = __any_sync(0xffffffffu, mask || m == -INFINITY);;) {
+              if (again) {
+                float top = -INFINITY;
 #pragma unroll
-              for (int e = 0; e < 64; ++e) top = fmaxf(top, __uint_as_float(v[e]) * kf[F32C ? e / 16 : 0]);
-              if (__any_sync(0xffffffffu, top > m)) {
-                const float nm = fmaxf(m, top);
-                const float f = m == nm ? 1.0f : fast_exp2(m - (nm == -INFINITY ? 0.0f : nm));
+                for (int e = 0; e < 64; ++e) top = fmaxf(top, __uint_as_float(v[e]) * kf[F32C ? e / 16 : 0]);
+                if (__any_sync(0xffffffffu, top > m)) {
+                  const float nm = fmaxf(m, top);
+                  const float f = m == nm ? 1.0f : fast_exp2(m - (nm == -INFINITY ? 0.0f : nm));
 #pragma unroll
-                for (int d = 0; d < HD; ++d) o[d] *= f;
-                due *= f;
-                l *= f;
-                m = nm;
+                  for (int d = 0; d < HD; ++d) o[d] *= f;
+                  due *= f;
+                  l *= f;
+                  m = nm;
+                }
               }
               exponentials();
+              if (again) break;
+              again = __any_sync(0xffffffffu, !(sum <= GROWTH));
+              if (!again) break;
             }
             l += sum;
             tmem_wait_st();
