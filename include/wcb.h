@@ -366,8 +366,9 @@ typedef struct wcb_paged_kv {
  * the sequence's tokens, new ones included, so that its i-th new token has
  * position kv_len[s] - (q_start[s+1] - q_start[s]) + i and lies in slot
  * position % page_size of page page_table[s * max_pages + position / page_size].
- * Rows of no sequence (before q_start[0], from q_start[n_seqs] on) are neither
- * read nor written. A sequence may have no new tokens. */
+ * Rows of no sequence (before q_start[0], from q_start[n_seqs] to n_tokens) are
+ * not written, and what they hold does not matter. A sequence may have no new
+ * tokens. */
 typedef struct wcb_paged_batch {
   uint32_t struct_size; /* sizeof(wcb_paged_batch) */
   uint32_t n_seqs;      /* at most 65536 */

@@ -42,6 +42,7 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "device_common.cuh"
@@ -938,13 +939,26 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
   }
 }
 
+// The shared-memory limit is a property of a kernel on a device: set the first time a device runs it. Two threads may
+// both find it unset and both set it; neither launches before it is.
+template <typename K>
+cudaError_t allow_shared(K kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
+}
+
 template <typename AT, typename CT, int HD, int NB>
 cudaError_t run_attend(const AttendArgs& a, cudaStream_t st) {
   using L = AttnCfg<AT, CT, HD, NB>;
   static_assert(L::SMEM <= 227 * 1024, "shared memory");
-  // the limit is a property of the kernel on the current device: set on every call (no
-  // state that a second device or thread could find half made)
-  cudaError_t e = cudaFuncSetAttribute(attend_kernel<AT, CT, HD, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_shared(attend_kernel<AT, CT, HD, NB>, L::SMEM, done);
   if (e != cudaSuccess) return e;
   CUtensorMap km{}, vm{};
   const int box = make_maps<CT>(&km, &vm, a.pool, L::TK);

@@ -588,7 +588,8 @@ template <typename T, int HD>
 cudaError_t run_tc(const AttendArgs& a, cudaStream_t s) {
   using L = TcCfg<HD>;
   static_assert(L::SMEM + sizeof(TcShared) <= 227 * 1024, "shared memory");
-  cudaError_t e = cudaFuncSetAttribute(attend_tc_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_shared(attend_tc_kernel<T, HD>, L::SMEM, done);
   if (e != cudaSuccess) return e;
   CUtensorMap km{}, vm{};
   const int box = make_maps<T>(&km, &vm, a.pool, TC_TK);

@@ -729,7 +729,8 @@ cudaError_t run_tc32(const AttendArgs& a, cudaStream_t s) {
            (L::RT + 2) * at.numRegs >= L::RT * L::R_SOFT + L::R_LOAD + L::R_MMA;
   }();
   if (!fits) return cudaErrorInvalidKernelImage;
-  cudaError_t e = cudaFuncSetAttribute(attend_tc32_kernel<CT, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_shared(attend_tc32_kernel<CT, HD>, L::SMEM, done);
   if (e != cudaSuccess) return e;
   CUtensorMap km{}, vm{};
   int box = 0;

@@ -31,7 +31,7 @@ __device__ __forceinline__ double rest(const float* p, const float* q, int certa
   return pj > qj ? double(pj) - double(qj) : 0.0;
 }
 
-__global__ void __launch_bounds__(VF_THREADS) verify_kernel(const __grid_constant__ VerifyArgs a, int chunks_per_cta) {
+__global__ void __launch_bounds__(VF_THREADS, 3) verify_kernel(const __grid_constant__ VerifyArgs a, int chunks_per_cta) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = int(cluster.num_blocks()), rank = int(cluster.block_rank());
@@ -213,7 +213,8 @@ __global__ void __launch_bounds__(VF_THREADS) verify_kernel(const __grid_constan
 }  // namespace
 
 cudaError_t launch_verify(const VerifyArgs& a, cudaStream_t s) {
-  // CTAs of a sequence: enough for two on each SM, slices of at least 2048 probabilities
+  // CTAs of a sequence: until there are two for each SM, with slices of at least 2048 probabilities.
+  // (192 sequences of 100003: 2 CTAs 36.3 us, 1: 46, 3: 40, 4: 39)
   int c = 1;
   while (c < MAX_CLUSTER && a.n_seqs * c < 2 * SMS && a.vocab / (2 * c) >= 2048) c *= 2;
   const int n_chunks = (a.vocab + CHUNK - 1) / CHUNK;
