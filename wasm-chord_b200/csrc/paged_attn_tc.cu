@@ -587,7 +587,7 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
 template <typename T, int HD>
 cudaError_t run_tc(const AttendArgs& a, cudaStream_t s) {
   using L = TcCfg<HD>;
-  static_assert(L::SMEM + sizeof(TcShared) <= 227 * 1024, "shared memory");
+  static_assert(L::SMEM + sizeof(TcShared) + sizeof(PlaceShared<TC_THREADS>) <= 227 * 1024, "shared memory");
   static std::atomic<uint64_t> done{0};
   const cudaError_t e = allow_shared(attend_tc_kernel<T, HD>, L::SMEM, done);
   if (e != cudaSuccess) return e;

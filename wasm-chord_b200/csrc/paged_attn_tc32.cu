@@ -3,17 +3,17 @@
 // paged_attn.cuh; the 16-bit kernel this one is built like: paged_attn_tc.cu).
 //
 // f32 numbers go to the tensor cores as sums of two f16 numbers, x = 2^e (hi + lo), 22 bits: the
-// exponents are a row's (q) or 16 keys' (k and v), so that the largest of them lies below 2^14 and
+// exponents are a row's (q) or 8 keys' (k and v), so that the largest of them lies below 2^14 and
 // what is lost of the others is below 2^-38 of it. An f16 cache needs no splitting.
 //   S  = Qlo Khi + Qhi Klo + Qhi Khi             (two products over an f16 cache)
 //   O' = Plo Vhi + Phi Vlo + Phi Vhi             (one half of 64 keys)
 //   O  = O 2^(m - m') + O' 2^e                   in registers, by ordinary f32 arithmetic
 // The last line is why this is not the 16-bit kernel with more products: sums in TMEM over a long
 // sequence are cut off at every step, which f32 outputs would show; over 64 keys they are not. TMEM: S of each
-// row tile in two halves of 64 keys, over which Phi and Plo are written, and two O' of each
+// row tile in two halves of 64 keys, over which Phi and Plo are written (16 columns in place of 16), and two O' of each
 // row tile, one of them being added to O while the products of the next are made.
 //
-// Keys and values of an f32 cache are loaded, scaled and split by the four loader warps (each 16 keys
+// Keys and values of an f32 cache are loaded, scaled and split by eight loader warps (each 8 keys
 // of a half, so a group's exponent is one warp's affair); those of an f16 cache come by TMA where
 // the tile is whole. head_dim 64: two row tiles of 128 rows; 128: one (Q in two parts and a
 // ring of K and V in two parts fill the shared memory).
@@ -28,7 +28,9 @@ struct Tc32Cfg {
   static constexpr bool F32C = std::is_same<CT, float>::value;
   static constexpr int RT = HD == 64 ? 2 : 1;       // row tiles
   static constexpr int M = 128 * RT;
-  static constexpr int THREADS = 128 * (RT + 2);    // softmax warpgroups, loaders, issuing warps
+  static constexpr int LW = F32C ? 8 : 4;           // loader warps: those of an f32 cache have the splitting to do
+  static constexpr int WGS = RT + LW / 4 + 1;       // softmax warpgroups, loaders, issuing warps
+  static constexpr int THREADS = 128 * WGS;
   static constexpr int PART = HD / 64 * TILE_PANEL;  // bytes of 128 rows x HD in f16
   static constexpr int SLOT = (F32C ? 2 : 1) * PART;
   static constexpr int SLOTS = F32C ? (HD == 64 ? 4 : 2) : (HD == 64 ? 6 : 4);
@@ -36,18 +38,19 @@ struct Tc32Cfg {
   static constexpr int RING = RT * 2 * PART;
   static constexpr int OFFS = RING + SLOTS * SLOT;   // [2][128] row offsets (f16 cache)
   static constexpr int SMEM = OFFS + 2 * 128 * 8 + 1024;
-  // registers of a thread by role; together no more than the launch's (65536 / THREADS a thread)
-  static constexpr int R_SOFT = RT == 2 ? 184 : 240, R_LOAD = RT == 2 ? 96 : 152, R_MMA = RT == 2 ? 48 : 56;
-  static constexpr int LAUNCH = RT == 2 ? 128 : 168;
-  static_assert(RT * R_SOFT + R_LOAD + R_MMA <= (RT + 2) * LAUNCH, "register split");
+  // registers of a thread by role; together no more than the launch's
+  static constexpr int LAUNCH = 65536 / THREADS / 8 * 8;
+  static constexpr int R_MMA = 40, R_LOAD = F32C ? (RT == 2 ? 48 : 96) : 80;
+  static constexpr int R_SOFT = RT == 2 ? (F32C ? 168 : 192) : 240;
+  static_assert(RT * R_SOFT + LW / 4 * R_LOAD + R_MMA <= WGS * LAUNCH, "register split");
 };
 
 constexpr int EXP_RING = 8;  // tiles
 
 struct Tc32Shared : TcShared {
   // (read four at a time)
-  alignas(16) int kexp[EXP_RING][8];
-  alignas(16) int vexp[EXP_RING][8];  // of 16 keys: their numbers are 2^exp times what the tile holds
+  alignas(16) int kexp[EXP_RING][16];
+  alignas(16) int vexp[EXP_RING][16];  // of 8 keys: their numbers are 2^exp times what the tile holds
 };
 
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((max(-126, min(127, e)) + 127) << 23); }
@@ -79,7 +82,7 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
                    const __grid_constant__ CUtensorMap vmap, int box) {
   using L = Tc32Cfg<CT, HD>;
   constexpr bool F32C = L::F32C;
-  constexpr int NS = L::SLOTS, RT = L::RT, M = L::M;
+  constexpr int NS = L::SLOTS, RT = L::RT, M = L::M, MMA_WARP = 4 * RT + L::LW;
   extern __shared__ uint8_t raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   __shared__ Tc32Shared sh;
@@ -92,7 +95,7 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
 
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
-      mbar_init(&sh.full[i], 4);
+      mbar_init(&sh.full[i], L::LW);
       mbar_init(&sh.empty[i], RT);
     }
     for (int w = 0; w < RT; ++w) {
@@ -110,7 +113,7 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
     mbar_fence_init();
   }
   if (tid < ODD_RING) sh.odd[tid] = 0;
-  if (warp == 4 * (RT + 1)) {
+  if (warp == MMA_WARP) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -121,10 +124,10 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
   Walk<M> wk;
   wk.start(a, pl);
 
-  if (warp >= 4 * (RT + 1)) {
+  if (warp >= MMA_WARP) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::R_MMA));
     // ---- issuing warps (paged_attn_tc.cu says how) ------------------------------
-    const int w = __shfl_sync(0xffffffffu, warp - 4 * (RT + 1), 0);
+    const int w = __shfl_sync(0xffffffffu, warp - MMA_WARP, 0);
     if (w < RT) {
       uint32_t elected;
       asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(elected));
@@ -191,11 +194,11 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                   const uint64_t v = vb + (4 * b + k) * (2048 >> 4);
-                  mma_ts(od, ts + 64 * b + 32 + 8 * k, v, ID_O, k > 0);
-                  if (F32C) mma_ts(od, ts + 64 * b + 8 * k, v + LO, ID_O, 1);
+                  mma_ts(od, ts + 64 * b + 16 * k + 8, v, ID_O, k > 0);
+                  if (F32C) mma_ts(od, ts + 64 * b + 16 * k, v + LO, ID_O, 1);
                 }
 #pragma unroll
-                for (int k = 0; k < 4; ++k) mma_ts(od, ts + 64 * b + 8 * k, vb + (4 * b + k) * (2048 >> 4), ID_O, 1);
+                for (int k = 0; k < 4; ++k) mma_ts(od, ts + 64 * b + 16 * k, vb + (4 * b + k) * (2048 >> 4), ID_O, 1);
                 tc_commit(&sh.o_done[w][b]);
                 if (b) tc_commit(&sh.empty[vs]);
               }
@@ -222,15 +225,14 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
       } while (ok && wk.next(a));
     }
   } else if (warp >= 4 * RT) {
-    if constexpr (RT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::R_LOAD));
-    else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::R_LOAD));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::R_LOAD));
     // ---- loaders --------------------------------------------------------------
     const int lt = tid - 128 * RT, lw = warp - 4 * RT;
     long long* offs = reinterpret_cast<long long*>(sm + L::OFFS);
     uint32_t n = 0, tiles = 0, item = 0, by_copy = 0;
     bool ok = true, holes_seen = false;
-    // this thread's key of a tile. f32: 16 keys of each half are one warp's (lanes 0 .. 15, 16 .. 31)
-    const int my_key = F32C ? 64 * (lane >> 4) + 16 * lw + (lane & 15) : lt;
+    // this thread's key of a tile. f32: 8 keys of each half are one warp's (lanes 0 .. 7, 8 .. 15; the others have none)
+    const int my_key = F32C ? 64 * ((lane >> 3) & 1) + 8 * lw + (lane & 7) : lt;
     auto page_of = [&](int i) {
       const int key = (wk.blk.tile0 + i) * TC_TK + my_key;
       return key >= wk.blk.lo && key < wk.blk.hi
@@ -249,12 +251,12 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
         if (i + 1 < wk.tb) next = page_of(i + 1);
         const int key = (wk.blk.tile0 + i) * TC_TK + my_key, at_slot = key % a.pool.page_size;
         const bool in = key >= wk.blk.lo && key < wk.blk.hi, there = in && page >= 0 && page < a.pool.n_pages;
-        const unsigned hb = __ballot_sync(0xffffffffu, in && !there);
+        const unsigned hb = __ballot_sync(0xffffffffu, in && !there) & (F32C ? 0xffffu : 0xffffffffu);
         if (lane == 0) {
           if (F32C) {
-            uint16_t* h = reinterpret_cast<uint16_t*>(sh.holes[tiles % HOLE_RING]);  // by 16 keys
-            h[lw] = uint16_t(hb);
-            h[4 + lw] = uint16_t(hb >> 16);
+            uint8_t* h = reinterpret_cast<uint8_t*>(sh.holes[tiles % HOLE_RING]);  // by 8 keys
+            h[lw] = uint8_t(hb);
+            h[8 + lw] = uint8_t(hb >> 8);
           } else {
             sh.holes[tiles % HOLE_RING][lw] = hb;
           }
@@ -262,12 +264,12 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
         holes_seen |= hb != 0;
         const long long off = there ? page * a.pool.page_stride + int64_t(at_slot) * a.pool.token_stride : -1;
         if constexpr (F32C) {
-          constexpr int LPR = HD / 4;        // lanes of a row (16 bytes each): 16 or 32
+          constexpr int LPR = HD / 8;        // lanes of a row (8 numbers each): 8 or 16
           constexpr int RPI = 32 / LPR;      // rows of an iteration
-          constexpr int IT = 16 / RPI;       // iterations of 16 rows
+          constexpr int IT = 2 * 8 / RPI;    // 16-byte words of a lane: two of each of its rows
           const int sub = lane % LPR, rr = lane / LPR;
-          const float* base[2] = {static_cast<const float*>(a.pool.k) + wk.kvh * a.pool.head_stride + 4 * sub,
-                                  static_cast<const float*>(a.pool.v) + wk.kvh * a.pool.head_stride + 4 * sub};
+          const float* base[2] = {static_cast<const float*>(a.pool.k) + wk.kvh * a.pool.head_stride + 8 * sub,
+                                  static_cast<const float*>(a.pool.v) + wk.kvh * a.pool.head_stride + 8 * sub};
           // K's halves, V's halves: the next one is on its way while one is split. (A rolled loop, like all that is long here:
           // the roles' code together has to stay in the instruction cache. Unrolled, the kernel took 1.81 ms where
           // it takes 1.50 ms at 46 sequences of 919 new tokens, 32/4 heads of 64.)
@@ -275,9 +277,10 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
           auto load = [&](int u) {
             const float* from = u < 2 ? base[0] : base[1];
 #pragma unroll
-            for (int j = 0; j < IT; ++j) {
-              const long long o = __shfl_sync(0xffffffffu, off, 16 * (u & 1) + RPI * j + rr);
+            for (int j = 0; j < IT; j += 2) {
+              const long long o = __shfl_sync(0xffffffffu, off, 8 * (u & 1) + RPI * (j / 2) + rr);
               ahead[j] = o >= 0 ? __ldg(reinterpret_cast<const float4*>(from + o)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              ahead[j + 1] = o >= 0 ? __ldg(reinterpret_cast<const float4*>(from + o) + 1) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             }
           };
 #pragma unroll 1
@@ -324,21 +327,22 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
 #pragma unroll
             for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
             const int ge = group_exp(top, kvi ? -126 : 0);  // zeros among values never make the largest exponent
-            if (lane == 0) (kvi ? sh.vexp : sh.kexp)[tiles % EXP_RING][4 * b + lw] = ge;
+            if (lane == 0) (kvi ? sh.vexp : sh.kexp)[tiles % EXP_RING][8 * b + lw] = ge;
             const uint64_t f = pack_f32x2(pow2(-ge), pow2(-ge));
             uint8_t* dst = sm + L::RING + ((n + kvi) % NS) * L::SLOT;
 #pragma unroll
-            for (int j = 0; j < IT; ++j) {
-              uint2 h, l;
-              const uint64_t z0 = mul_f32x2(pack_f32x2(y[j].x, y[j].y), f), z1 = mul_f32x2(pack_f32x2(y[j].z, y[j].w), f);
-              split_f16(z0, h.x, l.x);
-              split_f16(z1, h.y, l.y);
+            for (int j = 0; j < IT; j += 2) {
+              uint4 h, l;
+              split_f16(mul_f32x2(pack_f32x2(y[j].x, y[j].y), f), h.x, l.x);
+              split_f16(mul_f32x2(pack_f32x2(y[j].z, y[j].w), f), h.y, l.y);
+              split_f16(mul_f32x2(pack_f32x2(y[j + 1].x, y[j + 1].y), f), h.z, l.z);
+              split_f16(mul_f32x2(pack_f32x2(y[j + 1].z, y[j + 1].w), f), h.w, l.w);
               if (bad) {  // an infinity or NaN stays in hi alone
-                if (!finite16<__half>(h.x) || !finite16<__half>(h.y)) l = make_uint2(0, 0);
+                if (!finite16<__half>(h.x) || !finite16<__half>(h.y) || !finite16<__half>(h.z) || !finite16<__half>(h.w)) l = make_uint4(0, 0, 0, 0);
               }
-              const uint32_t o = tile_at(64 * b + 16 * lw + RPI * j + rr, sub >> 1) + 8 * (sub & 1);
-              *reinterpret_cast<uint2*>(dst + o) = h;
-              *reinterpret_cast<uint2*>(dst + L::PART + o) = l;
+              const uint32_t o = tile_at(64 * b + 8 * lw + RPI * (j / 2) + rr, sub);
+              *reinterpret_cast<uint4*>(dst + o) = h;
+              *reinterpret_cast<uint4*>(dst + L::PART + o) = l;
             }
             if (b == 1) {
               fence_proxy_async();
@@ -440,15 +444,18 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
         // the queries, scaled and split: a warp its own 32 rows, whole rows at a time; rows that are not there are zeros
         const int gr = r0 + min(row, rn - 1);
         float qinv = 1.0f;
+        // a row's places in q and out, in its thread; other lanes ask for them
+        const long long q_at = (wk.sq.r0 + token_of(a, gr)) * a.q_stride + (wk.kvh * a.rep + head_of(a, gr)) * HD;
+        const long long o_at = (wk.sq.r0 + token_of(a, gr)) * a.out_stride + (wk.kvh * a.rep + head_of(a, gr)) * HD;
 #pragma unroll 1
         for (int j0 = 0; j0 < 32 / RPI; j0 += 8) {
           float4 x[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const int r = r32 + RPI * (j0 + j) + lane / LPR, g = r0 + r;
-            x[j] = r < rn ? __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + (wk.sq.r0 + token_of(a, g)) * a.q_stride +
-                                                                  (wk.kvh * a.rep + head_of(a, g)) * HD) + lane % LPR)
-                          : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const int r = RPI * (j0 + j) + lane / LPR;
+            const long long from = __shfl_sync(0xffffffffu, q_at, r);
+            x[j] = r32 + r < rn ? __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + from) + lane % LPR)
+                                : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
           }
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
@@ -503,88 +510,109 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
             tc_fence_after();
             const int key0 = (wk.blk.tile0 + i) * TC_TK + 64 * b;
             const bool mask = cut || (holes[2 * b] | holes[2 * b + 1]) != 0;
-            uint32_t v[64];
-#pragma unroll
-            for (int q = 0; q < 2; ++q) tmem_ld32(ts + 64 * b + 32 * q, *reinterpret_cast<uint32_t(*)[32]>(v + 32 * q));
-            // factors of 16 keys each: of the products, and of P (relative to the half's largest exponent `ref`)
-            float kf[4], vf[4];
+            const uint32_t sa = ts + 64 * b;
+            uint32_t v[2][16];
+            tmem_ld16(sa, v[0]);
+            // factors of 8 keys each: of the products, and of P (relative to the half's largest exponent `ref`)
+            float kf[8], vf[8];
             // never zero, or a masked product's infinity would become NaN
             auto factor = [&](float f) { return copysignf(fmaxf(fabsf(a.scale_log2) * f, 1e-37f), a.scale_log2); };
             int ref = 0;
             if constexpr (F32C) {
-              const int4 ke = *reinterpret_cast<const int4*>(&sh.kexp[rt % EXP_RING][4 * b]);
-              const int4 ve = *reinterpret_cast<const int4*>(&sh.vexp[rt % EXP_RING][4 * b]);
-              ref = max(max(ve.x, ve.y), max(ve.z, ve.w));
+              ref = -126;
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                kf[q] = factor(qinv * pow2((&ke.x)[q]));
-                const int d = (&ve.x)[q] - ref;
+              for (int q = 0; q < 2; ++q) {
+                const int4 ke = *reinterpret_cast<const int4*>(&sh.kexp[rt % EXP_RING][8 * b + 4 * q]);
+                const int4 ve = *reinterpret_cast<const int4*>(&sh.vexp[rt % EXP_RING][8 * b + 4 * q]);
+                ref = max(ref, max(max(ve.x, ve.y), max(ve.z, ve.w)));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  kf[4 * q + j] = factor(qinv * pow2((&ke.x)[j]));
+                  vf[4 * q + j] = float((&ve.x)[j]);
+                }
+              }
+#pragma unroll
+              for (int q = 0; q < 8; ++q) {
+                const int d = int(vf[q]) - ref;
                 vf[q] = d < -126 ? 0.0f : pow2(d);
               }
             } else {
               kf[0] = factor(qinv);
             }
-            tmem_wait_ld();
+            uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
             if (mask) {
-              const uint32_t none = a.scale_log2 < 0.0f ? 0x7f800000u : 0xff800000u;  // -infinity once scaled
               const int lo = max(0, min(64, klo - key0)), hi = max(0, min(64, khi - key0));
 #pragma unroll
               for (int q = 0; q < 2; ++q) {
                 const int b0 = max(0, min(32, lo - 32 * q)), b1 = max(0, min(32, hi - 32 * q));
                 const uint32_t below1 = b1 >= 32 ? 0xffffffffu : (1u << b1) - 1u, below0 = b0 >= 32 ? 0xffffffffu : (1u << b0) - 1u;
-                const uint32_t seen = below1 & ~below0 & ~holes[2 * b + q];
-#pragma unroll
-                for (int e = 0; e < 32; ++e)
-                  if (!((seen >> e) & 1)) v[32 * q + e] = none;
+                seen[q] = below1 & ~below0 & ~holes[2 * b + q];
               }
             }
-            float sum;
-            auto exponentials = [&] {
-              const float use = m == -INFINITY ? 0.0f : m;
-              uint64_t s2[2] = {0, 0};
+            // S is read twice, 16 keys at a time: for the maximum, then for P, whose two parts take the 16 columns' place
+            const uint32_t none = a.scale_log2 < 0.0f ? 0x7f800000u : 0xff800000u;  // -infinity once scaled
+            auto keys = [&](int c, uint32_t (&x)[16]) {  // columns 16 c .. of S, the next ones on their way
+              tmem_wait_ld();
+              if (mask) {
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                uint32_t p[8], r[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                  const int c = 16 * q + 2 * e, gq = F32C ? q : 0;
-                  float x, y;
-                  unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), pack_f32x2(kf[gq], kf[gq]), pack_f32x2(-use, -use)), x, y);
-                  uint64_t z = pack_f32x2(fast_exp2(x), fast_exp2(y));
-                  s2[e & 1] = add_f32x2(s2[e & 1], z);
-                  if (F32C) z = mul_f32x2(z, pack_f32x2(vf[gq], vf[gq]));
-                  split_f16(z, p[e], r[e]);
-                }
-                tmem_st8(ts + 64 * b + 8 * q, p);
-                tmem_st8(ts + 64 * b + 32 + 8 * q, r);
+                for (int e = 0; e < 16; ++e)
+                  if (!((seen[c >> 1] >> (16 * (c & 1) + e)) & 1)) x[e] = none;
               }
+            };
+            float top = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t (&x)[16] = v[c & 1];
+              keys(c, x);
+              tmem_ld16(sa + (c < 3 ? 16 * (c + 1) : 0), v[(c + 1) & 1]);  // (after the last: the first again)
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                const float f = kf[F32C ? 2 * c + q : 0];
+                float hi = __uint_as_float(x[8 * q]), lo = hi;
+#pragma unroll
+                for (int e = 1; e < 8; ++e) {
+                  if (a.scale_log2 >= 0.0f) hi = fmaxf(hi, __uint_as_float(x[8 * q + e]));
+                  else lo = fminf(lo, __uint_as_float(x[8 * q + e]));
+                }
+                top = fmaxf(top, (a.scale_log2 >= 0.0f ? hi : lo) * f);
+              }
+            }
+            if (__any_sync(0xffffffffu, top > m + SLACK)) {
+              const float nm = fmaxf(m, top);
+              const float f = m == nm ? 1.0f : fast_exp2(m - (nm == -INFINITY ? 0.0f : nm));
+#pragma unroll
+              for (int d = 0; d < HD; ++d) o[d] *= f;
+              due *= f;
+              l *= f;
+              m = nm;
+            }
+            const float use = m == -INFINITY ? 0.0f : m;
+            uint64_t s2[2] = {0, 0};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t (&x)[16] = v[c & 1];
+              keys(c, x);
+              if (c < 3) tmem_ld16(sa + 16 * (c + 1), v[(c + 1) & 1]);
+              uint32_t p[8], r[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const int gq = F32C ? 2 * c + e / 4 : 0;
+                float y0, y1;
+                unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), pack_f32x2(kf[gq], kf[gq]), pack_f32x2(-use, -use)), y0, y1);
+                uint64_t z = pack_f32x2(fast_exp2(y0), fast_exp2(y1));
+                s2[e & 1] = add_f32x2(s2[e & 1], z);
+                if (F32C) z = mul_f32x2(z, pack_f32x2(vf[gq], vf[gq]));
+                split_f16(z, p[e], r[e]);
+              }
+              tmem_st8(sa + 16 * c, p);
+              tmem_st8(sa + 16 * c + 8, r);
+            }
+            {
               float x0, y0, x1, y1;
               unpack_f32x2(s2[0], x0, y0);
               unpack_f32x2(s2[1], x1, y1);
-              sum = (x0 + y0) + (x1 + y1);
-            };
-            // (paged_attn_tc.cu: the maximum only where the sum asks for it)
-            for (bool again = __any_sync(0xffffffffu, mask || m == -INFINITY);;) {
-              if (again) {
-                float top = -INFINITY;
-#pragma unroll
-                for (int e = 0; e < 64; ++e) top = fmaxf(top, __uint_as_float(v[e]) * kf[F32C ? e / 16 : 0]);
-                if (__any_sync(0xffffffffu, top > m)) {
-                  const float nm = fmaxf(m, top);
-                  const float f = m == nm ? 1.0f : fast_exp2(m - (nm == -INFINITY ? 0.0f : nm));
-#pragma unroll
-                  for (int d = 0; d < HD; ++d) o[d] *= f;
-                  due *= f;
-                  l *= f;
-                  m = nm;
-                }
-              }
-              exponentials();
-              if (again) break;
-              again = __any_sync(0xffffffffu, !(sum <= GROWTH));
-              if (!again) break;
+              l += (x0 + y0) + (x1 + y1);
             }
-            l += sum;
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -646,11 +674,11 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
           __syncwarp();
 #pragma unroll 4
           for (int j = 0; j < 32 / RPI; ++j) {
-            const int r = r32 + RPI * j + lane / LPR, g = r0 + r, c = lane % LPR;
-            if (r < rn)
-              *reinterpret_cast<float4*>(static_cast<float*>(a.out) + (wk.sq.r0 + token_of(a, g)) * a.out_stride +
-                                         (wk.kvh * a.rep + head_of(a, g)) * HD + 4 * c) =
-                  *reinterpret_cast<const float4*>(qt + (c / (HD / 8)) * L::PART + tile_at(r, c % (HD / 8)));
+            const int r = RPI * j + lane / LPR, c = lane % LPR;
+            const long long to_at = __shfl_sync(0xffffffffu, o_at, r);
+            if (r32 + r < rn)
+              *reinterpret_cast<float4*>(static_cast<float*>(a.out) + to_at + 4 * c) =
+                  *reinterpret_cast<const float4*>(qt + (c / (HD / 8)) * L::PART + tile_at(r32 + r, c % (HD / 8)));
           }
           __syncwarp();
           if (a.lse && row < rn) a.lse[tok * a.n_heads + hh] = some ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
@@ -715,18 +743,18 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
   __syncthreads();
   tc_fence_after();
   if (tid == 0 && sh.abort) report(a.batch, ST_ABORTED);
-  if (warp == 4 * (RT + 1)) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  if (warp == MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
 template <typename CT, int HD>
 cudaError_t run_tc32(const AttendArgs& a, cudaStream_t s) {
   using L = Tc32Cfg<CT, HD>;
-  static_assert(L::SMEM + sizeof(Tc32Shared) <= 227 * 1024, "shared memory");
+  static_assert(L::SMEM + sizeof(Tc32Shared) + sizeof(PlaceShared<L::THREADS>) <= 227 * 1024, "shared memory");
   // the register split draws on what the kernel is launched with
   static const bool fits = [] {
     cudaFuncAttributes at;
     return cudaFuncGetAttributes(&at, attend_tc32_kernel<CT, HD>) == cudaSuccess &&
-           (L::RT + 2) * at.numRegs >= L::RT * L::R_SOFT + L::R_LOAD + L::R_MMA;
+           L::WGS * at.numRegs >= L::RT * L::R_SOFT + L::LW / 4 * L::R_LOAD + L::R_MMA;
   }();
   if (!fits) return cudaErrorInvalidKernelImage;
   static std::atomic<uint64_t> done{0};
