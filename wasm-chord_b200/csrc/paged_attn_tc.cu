@@ -197,7 +197,7 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
     // the page of this thread's key of tile i; -1: none
     auto page_of = [&](int i) {
       const int key = (wk.blk.tile0 + i) * TC_TK + lt;
-      return key >= wk.blk.lo && key < wk.blk.hi
+      return key + max(box - 1, 0) >= wk.blk.lo && key < wk.blk.hi  // (a box that begins before the first key)
                  ? __ldg(a.batch.page_table + int64_t(wk.s) * a.batch.max_pages + key / a.pool.page_size)
                  : -1;
     };
@@ -217,9 +217,11 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
         if (lane == 0) sh.holes[tiles % HOLE_RING][warp - 8] = hb;
         holes_seen |= hb != 0;
         const bool ragged = wk.ragged(a, i);
-        if (box > 0 && !ragged) {
+        // a ragged tile's keys may be there whole, they are masked; its values have to be looked at
+        const int by_tma = box == 0 ? 0 : ragged ? 1 : 2;
+        if (by_tma > 0) {
 #pragma unroll 1
-          for (int kvi = 0; kvi < 2 && ok; ++kvi) {
+          for (int kvi = 0; kvi < by_tma && ok; ++kvi) {
             ok = room(n + kvi);
             if (!ok) break;
             uint64_t* bar = &sh.full[(n + kvi) % NS];
@@ -231,10 +233,11 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
               const uint32_t dst = sbase + L::RING + ((n + kvi) % NS) * L::TILE + lt * 128;
 #pragma unroll
               for (int p = 0; p < L::PANELS; ++p)  // a page that is not there: past the last one, zeros
-                tma_load(dst + p * TILE_PANEL, kvi ? &vmap : &kmap, 64 * p, wk.kvh, slot, there ? page : a.pool.n_pages, bar);
+                tma_load(dst + p * TILE_PANEL, kvi ? &vmap : &kmap, 64 * p, wk.kvh, slot, page >= 0 && page < a.pool.n_pages ? page : a.pool.n_pages, bar);
             }
           }
-          continue;
+          if (by_tma == 2) continue;
+          if (!ok) break;
         }
         offs[(by_copy & 1) * 128 + lt] = there ? page * a.pool.page_stride + int64_t(slot) * a.pool.token_stride : -1;
         bar_arrive(&sh.offs_full);
@@ -242,7 +245,7 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
         const long long* ro = offs + (by_copy & 1) * 128;
         ++by_copy;
 #pragma unroll 1
-        for (int kvi = 0; kvi < 2 && ok; ++kvi) {
+        for (int kvi = by_tma; kvi < 2 && ok; ++kvi) {
           ok = room(n + kvi);
           if (!ok) break;
           const T* base = static_cast<const T*>(kvi ? a.pool.v : a.pool.k) + wk.kvh * a.pool.head_stride;
@@ -257,7 +260,7 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
         }
         if (!ok) break;
 #pragma unroll 1
-        for (int kvi = 0; kvi < 2; ++kvi) {
+        for (int kvi = by_tma; kvi < 2; ++kvi) {
           if (kvi == 0) cp_wait<1>();
           else cp_wait<0>();
           // keys that some rows see and others do not: infinities and NaN are taken out of their values
@@ -305,14 +308,16 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
       if (end > wk.ta) {
         // queries into shared memory: a warp its own 32 rows, whole rows at a time; rows that are not there are zeros
         const int gr = r0 + min(row, rn - 1);
+        // a row's places in q and out, in its thread; other lanes ask for them
+        const long long q_at = (wk.sq.r0 + token_of(a, gr)) * a.q_stride + (wk.kvh * a.rep + head_of(a, gr)) * HD;
+        const long long o_at = (wk.sq.r0 + token_of(a, gr)) * a.out_stride + (wk.kvh * a.rep + head_of(a, gr)) * HD;
         {
           uint4 x[32 / RPI];
 #pragma unroll
           for (int j = 0; j < 32 / RPI; ++j) {
-            const int r = r32 + RPI * j + lane / CH, g = r0 + r;
-            x[j] = r < rn ? __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (wk.sq.r0 + token_of(a, g)) * a.q_stride +
-                                                                 (wk.kvh * a.rep + head_of(a, g)) * HD) + lane % CH)
-                          : make_uint4(0, 0, 0, 0);
+            const int r = RPI * j + lane / CH;
+            const long long from = __shfl_sync(0xffffffffu, q_at, r);
+            x[j] = r32 + r < rn ? __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + from) + lane % CH) : make_uint4(0, 0, 0, 0);
           }
 #pragma unroll
           for (int j = 0; j < 32 / RPI; ++j) *reinterpret_cast<uint4*>(qt + tile_at(r32 + RPI * j + lane / CH, lane % CH)) = x[j];
@@ -467,10 +472,10 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
           __syncwarp();
 #pragma unroll 4
           for (int j = 0; j < 32 / RPI; ++j) {
-            const int r = r32 + RPI * j + lane / CH, g = r0 + r;
-            if (r < rn)
-              *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (wk.sq.r0 + token_of(a, g)) * a.out_stride + (wk.kvh * a.rep + head_of(a, g)) * HD +
-                                        8 * (lane % CH)) = *reinterpret_cast<const uint4*>(qt + tile_at(r, lane % CH));
+            const int r = RPI * j + lane / CH;
+            const long long to_at = __shfl_sync(0xffffffffu, o_at, r);
+            if (r32 + r < rn)
+              *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + to_at + 8 * (lane % CH)) = *reinterpret_cast<const uint4*>(qt + tile_at(r32 + r, lane % CH));
           }
           __syncwarp();
         };

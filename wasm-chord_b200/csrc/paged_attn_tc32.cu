@@ -235,7 +235,7 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
     const int my_key = F32C ? 64 * ((lane >> 3) & 1) + 8 * lw + (lane & 7) : lt;
     auto page_of = [&](int i) {
       const int key = (wk.blk.tile0 + i) * TC_TK + my_key;
-      return key >= wk.blk.lo && key < wk.blk.hi
+      return key + max(box - 1, 0) >= wk.blk.lo && key < wk.blk.hi  // (a box that begins before the first key)
                  ? __ldg(a.batch.page_table + int64_t(wk.s) * a.batch.max_pages + key / a.pool.page_size)
                  : -1;
     };
@@ -353,9 +353,11 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
         } else {
           constexpr int CH = HD / 8;
           const bool ragged = wk.ragged(a, i);
-          if (box > 0 && !ragged) {
+          // a ragged tile's keys may be there whole, they are masked; its values have to be looked at
+          const int by_tma = box == 0 ? 0 : ragged ? 1 : 2;
+          if (by_tma > 0) {
 #pragma unroll 1
-            for (int kvi = 0; kvi < 2 && ok; ++kvi) {
+            for (int kvi = 0; kvi < by_tma && ok; ++kvi) {
               ok = room(n + kvi);
               if (!ok) break;
               uint64_t* bar = &sh.full[(n + kvi) % NS];
@@ -367,10 +369,11 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
                 const uint32_t dst = sbase + L::RING + ((n + kvi) % NS) * L::SLOT + lt * 128;
 #pragma unroll
                 for (int p = 0; p < HD / 64; ++p)  // a page that is not there: past the last one, zeros
-                  tma_load(dst + p * TILE_PANEL, kvi ? &vmap : &kmap, 64 * p, wk.kvh, at_slot, there ? page : a.pool.n_pages, bar);
+                  tma_load(dst + p * TILE_PANEL, kvi ? &vmap : &kmap, 64 * p, wk.kvh, at_slot, page >= 0 && page < a.pool.n_pages ? page : a.pool.n_pages, bar);
               }
             }
-            continue;
+            if (by_tma == 2) continue;
+            if (!ok) break;
           }
           offs[(by_copy & 1) * 128 + lt] = off;
           bar_arrive(&sh.offs_full);
@@ -378,7 +381,7 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
           const long long* ro = offs + (by_copy & 1) * 128;
           ++by_copy;
 #pragma unroll 1
-          for (int kvi = 0; kvi < 2 && ok; ++kvi) {
+          for (int kvi = by_tma; kvi < 2 && ok; ++kvi) {
             ok = room(n + kvi);
             if (!ok) break;
             const __half* base = static_cast<const __half*>(kvi ? a.pool.v : a.pool.k) + wk.kvh * a.pool.head_stride;
@@ -393,7 +396,7 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
           }
           if (!ok) break;
 #pragma unroll 1
-          for (int kvi = 0; kvi < 2; ++kvi) {
+          for (int kvi = by_tma; kvi < 2; ++kvi) {
             if (kvi == 0) cp_wait<1>();
             else cp_wait<0>();
             // keys that some rows see and others do not: infinities and NaN are taken out of their values
