@@ -439,7 +439,7 @@ uint32_t wcb_paged_attention_workspace(const wcb_paged_kv* kv, const wcb_paged_b
 
 /* compute_attention (attention.rs:332-435) over pages: for each new token at
  * position p of its sequence, softmax(scale * q . k_j) v_j over the keys j <= p,
- * and j > p - window where window > 0; n_heads / n_kv_heads query heads share
+ * and j > p - window where window > 0 (at most 2^30); n_heads / n_kv_heads query heads share
  * a key head (any whole ratio up to 64). q and out: [n_tokens][n_heads][head_dim]
  * with their strides between tokens (elements, multiples of 16 bytes), types as
  * for wcb_paged_append_dev. scale 0: 1 / sqrt(head_dim). lse (device f32

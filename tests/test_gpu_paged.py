@@ -393,6 +393,68 @@ def test_attention_in_a_graph_follows_the_lengths(gpu):
         s.check()
 
 
+FIRST_CALL = """
+import sys
+sys.path.insert(0, {pkg!r}); sys.path.insert(0, {tests!r})
+import torch, wcb
+import test_gpu_paged as t
+for act, cache in t.PAIRS:
+    for q_len in ([1, 2], [90, 3]):
+        s = t.Step(q_len, [300, 40], 8, 2, 64, act, cache, 16, seed=40)
+        room, side, graph = s.workspace(), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            s.attend(room=room, stream=torch.cuda.current_stream().cuda_stream)
+        graph.replay()
+        graph.replay()
+        s.check()
+print("captured first")
+"""
+
+
+def test_the_first_call_may_be_a_captured_one(gpu):
+    """Every kernel's set-up on its first call is allowed while a stream is captured: in a process of its own."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = FIRST_CALL.format(pkg=os.path.join(os.path.dirname(here), "wasm-chord_b200"), tests=here)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured first" in r.stdout, r.stderr[-2000:]
+
+
+def test_two_graphs_share_a_workspace(gpu):
+    """Replayed one after the other, in either order: a call leaves its workspace as it found it."""
+    a = Step([1, 30], [3000, 500], 8, 2, 128, "f16", "f16", 16, seed=41)
+    b = Step([4, 1, 200], [900, 2500, 800], 8, 2, 128, "f16", "f16", 16, seed=42)
+    room = max((a.workspace(), b.workspace()), key=lambda w: w.numel())
+    graphs = []
+    for s in (a, b):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            s.attend(room=room, stream=torch.cuda.current_stream().cuda_stream)
+        graphs.append(g)
+    for order in ((0, 1), (1, 0), (0, 0, 1, 1)):
+        for s in (a, b):
+            s.out.fill_(7.0)
+            s.lse.fill_(7.0)
+        for i in order:
+            graphs[i].replay()
+        a.check()
+        b.check()
+
+
+@pytest.mark.parametrize("act", ["f32", "f16"])
+def test_largest_and_smallest_batches(gpu, act):
+    """Sequences without new tokens only; a padded batch; the longest row counts wrong on the host's side."""
+    s = Step([0, 0, 0], [5, 0, 100], 8, 2, 64, act, "f16", 16, seed=43)
+    s.attend()
+    assert (s.out == 7.0).all() and (s.lse == 7.0).all()
+    s = Step([3, 70, 1], [40, 90, 7], 8, 2, 64, act, "f16", 16, seed=44, extra=50)
+    s.batch._c.max_q_len = 1  # the largest is 70
+    s.attend()
+    s.check()
+
+
 def test_two_streams_with_a_workspace_each(gpu):
     a = Step([1, 30], [3000, 500], 8, 2, 128, "f16", "f16", 16, seed=14)
     b = Step([4, 1], [900, 2500], 8, 2, 128, "f16", "f16", 16, seed=15)

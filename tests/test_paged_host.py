@@ -146,7 +146,7 @@ def test_rope_refuses():
     (dict(n_heads=0), "n_heads"), (dict(n_heads=6), "n_heads"), (dict(n_heads=4 * 65), "n_heads"), (dict(q_ptr=0), "null"), (dict(out_ptr=0), "null"),
     (dict(out_ptr=A), "out must not be q"), (dict(q_stride=500), "shorter"), (dict(out_stride=514), "16 bytes"), (dict(workspace_ptr=0), "workspace"),
     (dict(workspace_ptr=A + 8), "workspace"), (dict(workspace_bytes=4096), "workspace"), (dict(scale=float("nan")), "scale"),
-    (dict(scale=float("inf")), "scale"), (dict(window=1 << 31), "window"), (dict(lse_ptr=A + 2), "lse"),
+    (dict(scale=float("inf")), "scale"), (dict(window=(1 << 30) + 1), "window"), (dict(lse_ptr=A + 2), "lse"),
 ])
 def test_attention_refuses(change, words):
     refused(words, attend, **change)

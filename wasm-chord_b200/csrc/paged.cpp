@@ -232,7 +232,7 @@ uint32_t wcb_paged_attention_dev(const wcb_paged_kv* kv, const wcb_paged_batch* 
                "wcb_paged_attention_workspace says");
   if (reinterpret_cast<uintptr_t>(lse) & 3) return bad("Invalid argument: lse must be 4-byte aligned");
   if (!std::isfinite(scale)) return bad("Invalid argument: scale must be finite");
-  if (window > unsigned(INT_MAX)) return bad("Invalid argument: window < 2^31");
+  if (window > (1u << 30)) return bad("Invalid argument: window <= 2^30");
   if (q == out) return bad("Invalid argument: out must not be q");
   a.q = q;
   a.out = out;

@@ -69,10 +69,10 @@ __device__ __forceinline__ Seq read_seq(const Batch& b, int s) {
   q.n = q.sound ? hi - lo : 0;
   return q;
 }
-// tokens that the page table's row can name
+// tokens that the page table's row can name (and 32 bits count, with room for the tile after the last)
 __device__ __forceinline__ int table_tokens(const Pool& p, const Batch& b) {
   const long long n = static_cast<long long>(b.max_pages) * p.page_size;
-  return n > 0x7fffffff ? 0x7fffffff : int(n);
+  return n > 0x7ffff000 ? 0x7ffff000 : int(n);
 }
 __device__ __forceinline__ void report(const Batch& b, uint32_t bits) {
   if (b.status && bits) atomicOr(b.status, bits);
