@@ -335,7 +335,7 @@ def test_growing_scores_rescale(gpu, act, cache, dim):
 
 
 @pytest.mark.parametrize("dim", [64, 128])
-@pytest.mark.parametrize("q_len", [1, 90])
+@pytest.mark.parametrize("q_len", [1, 90, 300])
 @pytest.mark.parametrize("qs,ks,vs", [(1e-20, 1e18, 1e-25), (1e20, 1e-21, 1e30), (1.0, 1.0, 1.0)])
 def test_f32_of_any_range(gpu, dim, q_len, qs, ks, vs):
     """f32 queries, keys and values far from 1, and sizes that differ from key to key."""

@@ -432,7 +432,11 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
   long long at = pl.begin;       // line position
   long long unit0;               // line position of the unit's first tile
   Block blk;
-  {
+  if (rows <= M) {  // one block a head
+    blk = row_block(a, sq, rows, 0, M, TK, table);
+    kvh = quotient(at - pl.seq_begin, blk.tiles);
+    unit0 = pl.seq_begin + static_cast<long long>(kvh) * blk.tiles;
+  } else {
     const long long ht = head_tiles(a, sq, rows, M, TK, table);
     kvh = quotient(at - pl.seq_begin, ht);
     unit0 = pl.seq_begin + kvh * ht;
