@@ -11,7 +11,7 @@
 // Split: a unit is (sequence, key head, row block); its keys are TK-key tiles.
 // All tiles of all units lie on one line, cut into one equal part per CTA, so
 // that ragged lengths leave no CTA idle and one long sequence fills the GPU. A CTA
-// finds its place from the lengths on the device (nothing is planned on the
+// (a unit counts V tiles more than it has, for its queries, its start and its end) finds its place from the lengths on the device (nothing is planned on the
 // host, so a captured call follows the lengths of its replay). A unit that is
 // cut leaves (o, m, l) pieces in the workspace, at most two a CTA; the CTA that
 // finishes last joins them in their order, so results do not depend on timing.
@@ -208,23 +208,23 @@ __device__ __forceinline__ int seq_rows(const AttendArgs& a, const Seq& q) {
   const long long r = static_cast<long long>(q.n) * a.rep;
   return r > a.row_lo && r <= a.row_hi ? int(r) : 0;
 }
-// Tiles of one key head of a sequence; a whole warp, its lanes over the row blocks (a chunk
+// Places on the line of one key head of a sequence, its tiles and V for each unit; a whole warp, its lanes over the row blocks (a chunk
 // of a few thousand tokens has dozens, and every CTA of a call counts them).
-__device__ __forceinline__ long long head_tiles(const AttendArgs& a, const Seq& q, int rows, int M, int TK, int table) {
+__device__ __forceinline__ long long head_tiles(const AttendArgs& a, const Seq& q, int rows, int M, int TK, int V, int table) {
   long long n = 0;
-  for (int rb = threadIdx.x & 31; rb * M < rows; rb += 32) n += row_block(a, q, rows, rb, M, TK, table).tiles;
+  for (int rb = threadIdx.x & 31; rb * M < rows; rb += 32) n += row_block(a, q, rows, rb, M, TK, table).tiles + V;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
   return n;
 }
 // The same for 32 sequences, one of each lane: those of one or two row blocks by their lane, the
 // others one after the other by the warp.
-__device__ __forceinline__ long long lane_tiles(const AttendArgs& a, const Seq& q, int M, int TK, int table) {
+__device__ __forceinline__ long long lane_tiles(const AttendArgs& a, const Seq& q, int M, int TK, int V, int table) {
   const int rows = seq_rows(a, q);
   long long n = 0;
   if (rows > 0 && rows <= 2 * M) {
-    n = row_block(a, q, rows, 0, M, TK, table).tiles;
-    if (rows > M) n += row_block(a, q, rows, 1, M, TK, table).tiles;
+    n = row_block(a, q, rows, 0, M, TK, table).tiles + V;
+    if (rows > M) n += row_block(a, q, rows, 1, M, TK, table).tiles + V;
   }
   for (unsigned left = __ballot_sync(0xffffffffu, rows > 2 * M); left; left &= left - 1) {
     const int src = __ffs(int(left)) - 1;
@@ -233,18 +233,18 @@ __device__ __forceinline__ long long lane_tiles(const AttendArgs& a, const Seq& 
     w.kv = __shfl_sync(0xffffffffu, q.kv, src);
     w.r0 = 0;
     w.sound = true;
-    const long long sum = head_tiles(a, w, __shfl_sync(0xffffffffu, rows, src), M, TK, table);
+    const long long sum = head_tiles(a, w, __shfl_sync(0xffffffffu, rows, src), M, TK, V, table);
     if (int(threadIdx.x & 31) == src) n = sum;
   }
   return n;
 }
 // Row block of line position `at` in a key head whose tiles begin at unit0 (moved to the block's
 // first tile); a whole warp.
-__device__ __forceinline__ int find_block(const AttendArgs& a, const Seq& q, int rows, int M, int TK, int table, long long at, long long& unit0) {
+__device__ __forceinline__ int find_block(const AttendArgs& a, const Seq& q, int rows, int M, int TK, int V, int table, long long at, long long& unit0) {
   const int lane = threadIdx.x & 31;
   for (int rb0 = 0;; rb0 += 32) {
     const int rb = rb0 + lane;
-    const long long n = rb * M < rows ? row_block(a, q, rows, rb, M, TK, table).tiles : 0;
+    const long long n = rb * M < rows ? row_block(a, q, rows, rb, M, TK, table).tiles + V : 0;
     long long inc = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -278,7 +278,7 @@ struct PlaceShared {
   long long found[2];
 };
 template <int THREADS>
-__device__ __forceinline__ Place find_place(const AttendArgs& a, int M, int TK, PlaceShared<THREADS>& sh) {
+__device__ __forceinline__ Place find_place(const AttendArgs& a, int M, int TK, int V, PlaceShared<THREADS>& sh) {
   constexpr int NW = THREADS / 32;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int table = table_tokens(a.pool, a.batch);
@@ -291,7 +291,7 @@ __device__ __forceinline__ Place find_place(const AttendArgs& a, int M, int TK, 
     Seq q{0, 0, 0, true};
     if (s < n) q = read_seq(a.batch, s);
     unsound |= !q.sound;
-    sh.count[slot] = lane_tiles(a, q, M, TK, table) * a.pool.n_kv;
+    sh.count[slot] = lane_tiles(a, q, M, TK, V, table) * a.pool.n_kv;
     __syncthreads();
     mine = sh.count[tid];
     long long inc = mine;
@@ -362,6 +362,7 @@ struct AttnCfg {
   static constexpr bool F32A = std::is_same<AT, float>::value;
   static constexpr bool F32C = std::is_same<CT, float>::value;
   static constexpr int TK = 64;       // keys of a tile
+  static constexpr int V = 1;         // what a unit costs beside its tiles, in tiles
   static constexpr int KW = TK / 4;   // keys of a warp: the rows of one mma
   static constexpr int M = 8 * NB;    // rows of a block
   static constexpr int PANELS = HD * int(sizeof(CT)) / 128;
@@ -386,7 +387,7 @@ __global__ void __launch_bounds__(AT_THREADS, (AttnCfg<AT, CT, HD, NB>::PER_SM))
 attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap kmap,
               const __grid_constant__ CUtensorMap vmap, int box) {
   using L = AttnCfg<AT, CT, HD, NB>;
-  constexpr int TK = L::TK, KW = L::KW, M = L::M, S = L::STAGES;
+  constexpr int TK = L::TK, KW = L::KW, M = L::M, S = L::STAGES, V = L::V;
   constexpr bool F32A = L::F32A, F32C = L::F32C;
   constexpr int MB = HD / 16;                    // 16-dim blocks of the output
   constexpr int CH = HD * int(sizeof(CT)) / 16;  // 16-byte chunks of a row
@@ -404,7 +405,7 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
   const int g = lane >> 2, t = lane & 3;
   const uint32_t sbase = smem_u32(sm);
   const int table = table_tokens(a.pool, a.batch);
-  const Place pl = find_place<AT_THREADS>(a, M, TK, s_place);
+  const Place pl = find_place<AT_THREADS>(a, M, TK, V, s_place);
   if (pl.begin >= pl.end) return;
   if (tid == 0) {
     for (int i = 0; i < S; ++i) mbar_init(&s_full[i], 1);
@@ -429,23 +430,23 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
   int s = pl.seq, kvh = 0, rb = 0;
   Seq sq = read_seq(a.batch, s);
   int rows = seq_rows(a, sq);
-  long long at = pl.begin;       // line position
-  long long unit0;               // line position of the unit's first tile
+  long long unit0;  // the unit's first place on the line: V, then its tiles
   Block blk;
   if (rows <= M) {  // one block a head
     blk = row_block(a, sq, rows, 0, M, TK, table);
-    kvh = quotient(at - pl.seq_begin, blk.tiles);
-    unit0 = pl.seq_begin + static_cast<long long>(kvh) * blk.tiles;
+    kvh = quotient(pl.begin - pl.seq_begin, blk.tiles + V);
+    unit0 = pl.seq_begin + static_cast<long long>(kvh) * (blk.tiles + V);
   } else {
-    const long long ht = head_tiles(a, sq, rows, M, TK, table);
-    kvh = quotient(at - pl.seq_begin, ht);
+    const long long ht = head_tiles(a, sq, rows, M, TK, V, table);
+    kvh = quotient(pl.begin - pl.seq_begin, ht);
     unit0 = pl.seq_begin + kvh * ht;
-    rb = find_block(a, sq, rows, M, TK, table, at, unit0);
+    rb = find_block(a, sq, rows, M, TK, V, table, pl.begin, unit0);
     blk = row_block(a, sq, rows, rb, M, TK, table);
   }
 
   while (true) {
-    const int ta = int(at - unit0), tb = int(min(static_cast<long long>(blk.tiles), pl.end - unit0));
+    const int ta = int(max(0LL, pl.begin - unit0 - V)), tb = int(min(static_cast<long long>(blk.tiles), pl.end - unit0 - V));
+    if (tb <= ta) break;  // the part ends before the unit's first tile
     const int r0 = rb * M, rn = min(M, rows - r0);  // rows of the block
     const CT* kbase = static_cast<const CT*>(a.pool.k) + kvh * a.pool.head_stride;
     const CT* vbase = static_cast<const CT*>(a.pool.v) + kvh * a.pool.head_stride;
@@ -876,8 +877,7 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
 
     if (!whole) {
       // the last of the unit's CTAs joins its pieces, in their order
-      const long long u1 = unit0 + blk.tiles - 1;
-      const int c0 = quotient(unit0, pl.per), c1 = quotient(u1, pl.per);
+      const int c0 = quotient(unit0 + V, pl.per), c1 = quotient(unit0 + V + blk.tiles - 1, pl.per);
       __threadfence();
       __syncthreads();
       if (tid == 0) s_last = atomicInc(reinterpret_cast<unsigned*>(a.tickets) + c0, unsigned(c1 - c0)) == unsigned(c1 - c0);
@@ -923,10 +923,9 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
       }
     }
 
-    at = unit0 + tb;
-    if (at >= pl.end) break;
     // next unit
-    unit0 += blk.tiles;
+    unit0 += blk.tiles + V;
+    if (unit0 >= pl.end) break;
     ++rb;
     if (rb * M >= rows) {
       rb = 0;

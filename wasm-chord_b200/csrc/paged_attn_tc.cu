@@ -37,6 +37,7 @@ namespace {
 
 constexpr int TC_THREADS = 448;  // 2 softmax warpgroups, 4 loader warps, 2 issuing warps
 constexpr int TC_M = 256;
+constexpr int UNIT = 3;  // a unit's queries, start and end take about as long as so many tiles of keys
 
 template <int HD>
 struct TcCfg {
@@ -63,8 +64,10 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t sbase = smem_u32(sm);
 
-  const Place pl = find_place<TC_THREADS>(a, TC_M, TC_TK, s_place);
+  const Place pl = find_place<TC_THREADS>(a, TC_M, TC_TK, UNIT, s_place);
   if (pl.begin >= pl.end) return;  // the whole CTA; nothing is held yet
+  Walk<TC_M, UNIT> wk;
+  if (!wk.start(a, pl)) return;    // likewise
 
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
@@ -94,8 +97,6 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
-  Walk<TC_M> wk;
-  wk.start(a, pl);
 
   if (warp >= 12) {
     // ---- issuing warps: products of row tile w --------------------------------
@@ -532,7 +533,7 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
         }
         if (!whole) {
           // the last of the unit's CTAs joins this tile's pieces, in their order
-          const int c0 = quotient(wk.unit0, wk.pl.per), c1 = quotient(wk.unit0 + wk.blk.tiles - 1, wk.pl.per);
+          const int c0 = quotient(wk.unit0 + UNIT, wk.pl.per), c1 = quotient(wk.unit0 + UNIT + wk.blk.tiles - 1, wk.pl.per);
           __threadfence();
           bar_arrive(&sh.piece_full[w]);
           ok = tc_wait_warp(&sh, &sh.piece_full[w], cuts & 1);

@@ -46,6 +46,7 @@ struct Tc32Cfg {
 };
 
 constexpr int EXP_RING = 8;  // tiles
+constexpr int UNIT = 2;      // a unit's queries, start and end take about as long as so many tiles of keys
 
 struct Tc32Shared : TcShared {
   // (read four at a time)
@@ -90,8 +91,10 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t sbase = smem_u32(sm);
 
-  const Place pl = find_place<L::THREADS>(a, M, TC_TK, s_place);
+  const Place pl = find_place<L::THREADS>(a, M, TC_TK, UNIT, s_place);
   if (pl.begin >= pl.end) return;  // the whole CTA; nothing is held yet
+  Walk<M, UNIT> wk;
+  if (!wk.start(a, pl)) return;    // likewise
 
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
@@ -121,8 +124,6 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
-  Walk<M> wk;
-  wk.start(a, pl);
 
   if (warp >= MMA_WARP) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::R_MMA));
@@ -703,7 +704,7 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
         }
         if (!whole) {
           // the last of the unit's CTAs joins this tile's pieces, in their order
-          const int c0 = quotient(wk.unit0, wk.pl.per), c1 = quotient(wk.unit0 + wk.blk.tiles - 1, wk.pl.per);
+          const int c0 = quotient(wk.unit0 + UNIT, wk.pl.per), c1 = quotient(wk.unit0 + UNIT + wk.blk.tiles - 1, wk.pl.per);
           __threadfence();
           bar_arrive(&sh.piece_full[w]);
           ok = tc_wait_warp(&sh, &sh.piece_full[w], cuts & 1);

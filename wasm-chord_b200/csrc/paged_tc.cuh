@@ -139,38 +139,37 @@ __device__ __forceinline__ bool tc_wait_warp(TcShared* sh, uint64_t* bar, uint32
 }
 
 // The units of this CTA, walked by every role by itself.
-template <int M>  // rows of a block: one or two tiles of 128
+template <int M, int V>  // rows of a block: one or two tiles of 128; what a unit costs beside its tiles, in tiles
 struct Walk {
   Place pl;
-  long long at, unit0;
+  long long unit0;  // the unit's first place on the line: V, then its tiles
   int s, kvh, rb, rows, table;
   Seq sq;
   Block blk;
   int ta, tb;  // tiles of the current unit
 
-  // a whole warp
-  __device__ __forceinline__ void start(const AttendArgs& a, const Place& p) {
+  // a whole warp; false: the part ends before its first tile
+  __device__ __forceinline__ bool start(const AttendArgs& a, const Place& p) {
     pl = p;
     table = table_tokens(a.pool, a.batch);
     s = pl.seq;
     sq = read_seq(a.batch, s);
     rows = seq_rows(a, sq);
-    at = pl.begin;
-    const long long ht = head_tiles(a, sq, rows, M, TC_TK, table);
-    kvh = quotient(at - pl.seq_begin, ht);
+    const long long ht = head_tiles(a, sq, rows, M, TC_TK, V, table);
+    kvh = quotient(pl.begin - pl.seq_begin, ht);
     unit0 = pl.seq_begin + kvh * ht;
-    rb = find_block(a, sq, rows, M, TC_TK, table, at, unit0);
+    rb = find_block(a, sq, rows, M, TC_TK, V, table, pl.begin, unit0);
     blk = row_block(a, sq, rows, rb, M, TC_TK, table);
-    cut();
+    return cut();
   }
-  __device__ __forceinline__ void cut() {
-    ta = int(at - unit0);
-    tb = int(min(static_cast<long long>(blk.tiles), pl.end - unit0));
+  __device__ __forceinline__ bool cut() {
+    ta = int(max(0LL, pl.begin - unit0 - V));
+    tb = int(min(static_cast<long long>(blk.tiles), pl.end - unit0 - V));
+    return tb > ta;
   }
   __device__ __forceinline__ bool next(const AttendArgs& a) {
-    at = unit0 + tb;
-    if (at >= pl.end) return false;
-    unit0 += blk.tiles;
+    unit0 += blk.tiles + V;
+    if (unit0 >= pl.end) return false;
     ++rb;
     if (rb * M >= rows) {
       rb = 0;
@@ -184,8 +183,7 @@ struct Walk {
       }
     }
     blk = row_block(a, sq, rows, rb, M, TC_TK, table);
-    cut();
-    return true;
+    return cut();
   }
   // tiles [ta, end) that rows 128 w .. of the block need (those after end see nothing); at least
   // one, so that rows without a key are written too; 0: there are no such rows
