@@ -288,6 +288,18 @@ def test_more_sequences_than_threads(gpu):
     s.check()
 
 
+# units of one, two and many tiles, so many of them that parts begin and end in units of each kind
+@pytest.mark.parametrize("act,cache", PAIRS)
+@pytest.mark.parametrize("dim,chunks", [(64, False), (128, False), (64, True), (128, True)])
+def test_short_and_long_units(gpu, act, cache, dim, chunks):
+    n = 60 if chunks else 300
+    q = [(1, 40, 3, 70, 0, 130, 33)[i % 7] if chunks else 1 for i in range(n)]
+    kv = [x + (0, 100, 20, 250, 60, 1, 700, 127, 128, 64, 900)[i % 11] for i, x in enumerate(q)]
+    s = Step(q, kv, 8, 4, dim, act, cache, 32, False, seed=31)
+    s.attend()
+    s.check()
+
+
 @pytest.mark.parametrize("act,cache,heads,kv_heads,dim", [("f16", "f16", 8, 2, 128), ("f32", "f16", 32, 4, 64), ("bf16", "bf16", 64, 8, 128)])
 def test_long_sequences_and_repeatability(gpu, act, cache, heads, kv_heads, dim):
     s = Step([1, 1], [20011, 3], heads, kv_heads, dim, act, cache, 64, True, seed=10)

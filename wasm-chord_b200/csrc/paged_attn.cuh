@@ -1,6 +1,6 @@
-// Attention of new tokens over a paged cache: the kernel for few rows and for
-// f32 activations (mma.sync; the products of a decode step are far from the
-// tensor cores' rate, its bytes are the bound).
+// Attention of new tokens over a paged cache: the kernel for few rows (mma.sync;
+// the products of a decode step are far from the tensor cores' rate, its bytes are
+// the bound) and for f32 activations over a bf16 cache.
 //
 // o_i = sum_j softmax_j(scale q_i . k_j) v_j over the keys a token sees, in one
 // pass over K and V with a running maximum m and sum l (both f32):
@@ -10,11 +10,12 @@
 //
 // Split: a unit is (sequence, key head, row block); its keys are TK-key tiles.
 // All tiles of all units lie on one line, cut into one equal part per CTA, so
-// that ragged lengths leave no CTA idle and one long sequence fills the GPU. A CTA
-// (a unit counts V tiles more than it has, for its queries, its start and its end) finds its place from the lengths on the device (nothing is planned on the
-// host, so a captured call follows the lengths of its replay). A unit that is
-// cut leaves (o, m, l) pieces in the workspace, at most two a CTA; the CTA that
-// finishes last joins them in their order, so results do not depend on timing.
+// that ragged lengths leave no CTA idle and one long sequence fills the GPU; a unit
+// counts V tiles more than it has, for its queries, its start and its end. A CTA finds
+// its place from the lengths on the device (nothing is planned on the host, so a
+// captured call follows the lengths of its replay). A unit that is cut (those of a few
+// tiles are not) leaves (o, m, l) pieces in the workspace, at most two a CTA; the CTA
+// that finishes last joins them in their order, so results do not depend on timing.
 //
 // Products: transposed, S^T = K Q^T and O^T = V^T P^T, so that keys and dims fill the 16 rows of an
 // mma and the few rows of a decode step its 8 columns (8 rows a key head at most need
@@ -38,6 +39,11 @@
 // in tf32. The tensor cores cut their sums off instead of rounding them, so long sums are
 // kept short: small products have accumulators of their own, and a tile's P V is summed
 // by itself and added to O by an ordinary multiply-add.
+//
+// Measured, single tokens over f16: 64 sequences of up to 8191 keys, 64/8 heads of 128
+// (1.1 GB), 182 us run after run, 93 % of the copy rate; one of 131071 keys (537 MB) 98.5 us, 83 %, the rest is the
+// launch, the first loads and the join; 16 sequences of 1 to 6 tokens over 500 to 2304
+// keys, 32/32 heads (349 MB), 66 us, 81 %; one sequence of 320 keys 8 us, all of it latency.
 #pragma once
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -362,7 +368,8 @@ struct AttnCfg {
   static constexpr bool F32A = std::is_same<AT, float>::value;
   static constexpr bool F32C = std::is_same<CT, float>::value;
   static constexpr int TK = 64;       // keys of a tile
-  static constexpr int V = 1;         // what a unit costs beside its tiles, in tiles
+  static constexpr int V = 2;         // what a unit costs beside its tiles, in tiles (0: the drafts of 66 us take 71, the 182 us 189)
+  static constexpr int SNAP = 2;      // units of so few tiles are not cut
   static constexpr int KW = TK / 4;   // keys of a warp: the rows of one mma
   static constexpr int M = 8 * NB;    // rows of a block
   static constexpr int PANELS = HD * int(sizeof(CT)) / 128;
@@ -387,7 +394,7 @@ __global__ void __launch_bounds__(AT_THREADS, (AttnCfg<AT, CT, HD, NB>::PER_SM))
 attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap kmap,
               const __grid_constant__ CUtensorMap vmap, int box) {
   using L = AttnCfg<AT, CT, HD, NB>;
-  constexpr int TK = L::TK, KW = L::KW, M = L::M, S = L::STAGES, V = L::V;
+  constexpr int TK = L::TK, KW = L::KW, M = L::M, S = L::STAGES, V = L::V, SNAP = L::SNAP;
   constexpr bool F32A = L::F32A, F32C = L::F32C;
   constexpr int MB = HD / 16;                    // 16-dim blocks of the output
   constexpr int CH = HD * int(sizeof(CT)) / 16;  // 16-byte chunks of a row
@@ -444,8 +451,30 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
     blk = row_block(a, sq, rows, rb, M, TK, table);
   }
 
+  auto next_unit = [&] {
+    unit0 += blk.tiles + V;
+    if (unit0 >= pl.end) return false;
+    ++rb;
+    if (rb * M >= rows) {
+      rb = 0;
+      if (++kvh == a.pool.n_kv) {
+        kvh = 0;
+        do {
+          ++s;  // there are units left, so a sequence with rows follows
+          sq = read_seq(a.batch, s);
+          rows = seq_rows(a, sq);
+        } while (rows == 0);
+      }
+    }
+    blk = row_block(a, sq, rows, rb, M, TK, table);
+    return true;
+  };
+  // a small unit is the part's that it begins in
+  if (blk.tiles <= SNAP && unit0 < pl.begin && !next_unit()) return;
+
   while (true) {
-    const int ta = int(max(0LL, pl.begin - unit0 - V)), tb = int(min(static_cast<long long>(blk.tiles), pl.end - unit0 - V));
+    const int ta = blk.tiles <= SNAP ? 0 : int(max(0LL, pl.begin - unit0 - V));
+    const int tb = blk.tiles <= SNAP ? blk.tiles : int(min(static_cast<long long>(blk.tiles), pl.end - unit0 - V));
     if (tb <= ta) break;  // the part ends before the unit's first tile
     const int r0 = rb * M, rn = min(M, rows - r0);  // rows of the block
     const CT* kbase = static_cast<const CT*>(a.pool.k) + kvh * a.pool.head_stride;
@@ -923,22 +952,7 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
       }
     }
 
-    // next unit
-    unit0 += blk.tiles + V;
-    if (unit0 >= pl.end) break;
-    ++rb;
-    if (rb * M >= rows) {
-      rb = 0;
-      if (++kvh == a.pool.n_kv) {
-        kvh = 0;
-        do {
-          ++s;  // there are tiles left, so a sequence with rows follows
-          sq = read_seq(a.batch, s);
-          rows = seq_rows(a, sq);
-        } while (rows == 0);
-      }
-    }
-    blk = row_block(a, sq, rows, rb, M, TK, table);
+    if (!next_unit()) break;
   }
 }
 

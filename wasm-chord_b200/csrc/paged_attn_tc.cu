@@ -5,11 +5,11 @@
 // One CTA per SM holds two tiles of 128 rows (row = token * rep + head), each with
 // a warpgroup for its softmax (one thread a row: no shuffles) and a thread that
 // issues its products; both share the K and V tiles that four loader warps bring
-// into a ring of tiles in shared memory. A tile that every row sees whole comes by
-// TMA, in boxes of gcd(page_size, 128) tokens, which never cross a page; other tiles
-// (the diagonal, the ends, pages whose gcd is below 8) come by 16-byte cp.async,
-// which can leave out single keys (measured: 2100 clocks for a 32 KB tile, against the
-// 2048 that a tile of keys takes the tensor cores). Per tile of keys:
+// into a ring of tiles in shared memory: by TMA, in boxes of gcd(page_size, 128) tokens,
+// which never cross a page. The values of ragged tiles (the diagonal, the ends) and pools
+// whose gcd is below 8 come by 16-byte cp.async, which can leave out single keys (measured:
+// 2100 clocks for a 32 KB tile, against the 2048 that a tile of keys takes the tensor
+// cores). Per tile of keys:
 //   S = Q K^T      tcgen05.mma, both operands from shared memory, S in TMEM (f32)
 //   P = 2^(S - m)  read from TMEM, rounded to 16 bits, written back over S
 //   O += P V       tcgen05.mma, P from TMEM, V as it lies ([key][dim]: N-major)
@@ -23,12 +23,13 @@
 // room for the factor): one vote on the sum instead of 64 comparisons a row.
 // TMEM: S0 | S1 | O0 | O1, 512 columns at head_dim 128.
 //
-// 2047 new tokens over 32767 keys, 64/8 heads of 128, bf16: 2.36 ms, 903 TFLOP/s (54 %
-// of the measured cuBLAS rate). What bounds it: the exponentials of the two softmax warps of
-// a scheduler and what surrounds them (1250 clocks a half with both row tiles; 600 without
-// the exponentials themselves, when the products' 2560 clocks become the bound, 2.0 ms).
-// Part of the exponentials by a polynomial on the multiply-add units (a quarter, an eighth) gained
-// nothing: those pay as many clocks for it.
+// 2047 new tokens over 32767 keys, 64/8 heads of 128, bf16: 2.0 ms run after run, 2.3 ms with
+// pauses in between, 1060 and 925 TFLOP/s (64 and 55 % of the measured cuBLAS rate). What bounds it: the
+// exponentials of the two softmax warps of a scheduler and what surrounds them (1250 clocks a
+// half with both row tiles; without the exponentials themselves 600, and the products' 2560
+// clocks become the bound). Part of the exponentials by a polynomial on the multiply-add units
+// (a quarter, an eighth) gained nothing: those pay as many clocks for it. Short units: 11
+// sequences of 204 tokens 74 us (82 with units that are cut in two for one tile).
 #include "paged_tc.cuh"
 
 namespace wcb {

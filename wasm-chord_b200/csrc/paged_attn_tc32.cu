@@ -17,6 +17,11 @@
 // of a half, so a group's exponent is one warp's affair); those of an f16 cache come by TMA where
 // the tile is whole. head_dim 64: two row tiles of 128 rows; 128: one (Q in two parts and a
 // ring of K and V in two parts fill the shared memory).
+//
+// 46 sequences of 919 tokens, 32/4 heads of 64, f32 cache: 1.26 ms, 126 TFLOP/s of the formula's
+// products, 380 of those made (23 % of the measured cuBLAS rate); nine sequences of 1 to 700 tokens with
+// a window of 511 132 us. What bounds it: the instructions of the splitting, in the softmax (P) and in the loaders
+// (K and V), and at few tiles a unit's start and end.
 #include "paged_tc.cuh"
 
 namespace wcb {

@@ -160,11 +160,17 @@ struct Walk {
     unit0 = pl.seq_begin + kvh * ht;
     rb = find_block(a, sq, rows, M, TC_TK, V, table, pl.begin, unit0);
     blk = row_block(a, sq, rows, rb, M, TC_TK, table);
-    return cut();
+    return cut() || next(a);
   }
+  // units of no more tiles than they cost otherwise are not cut: they are the part's that they begin in
   __device__ __forceinline__ bool cut() {
-    ta = int(max(0LL, pl.begin - unit0 - V));
-    tb = int(min(static_cast<long long>(blk.tiles), pl.end - unit0 - V));
+    if (blk.tiles <= V) {
+      ta = 0;
+      tb = unit0 >= pl.begin ? blk.tiles : 0;
+    } else {
+      ta = int(max(0LL, pl.begin - unit0 - V));
+      tb = int(min(static_cast<long long>(blk.tiles), pl.end - unit0 - V));
+    }
     return tb > ta;
   }
   __device__ __forceinline__ bool next(const AttendArgs& a) {

