@@ -54,11 +54,16 @@ constexpr int EXP_RING = 8;  // tiles
 constexpr int UNIT = 2;      // a unit's queries, start and end take about as long as so many tiles of keys
 
 struct Tc32Shared : TcShared {
-  // (read four at a time)
-  alignas(16) int kexp[EXP_RING][16];
-  alignas(16) int vexp[EXP_RING][16];  // of 8 keys: their numbers are 2^exp times what the tile holds
+  // of 8 keys: their numbers are so many times (a power of two) what the tile holds (read four at a time)
+  alignas(16) float kfac[EXP_RING][16];
+  alignas(16) float vfac[EXP_RING][16];
 };
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((max(-126, min(127, e)) + 127) << 23); }
 // the exponent that brings numbers up to `top` below 2^14; `none` where there are only zeros
 __device__ __forceinline__ int group_exp(float top, int none) {
@@ -333,7 +338,7 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
 #pragma unroll
             for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
             const int ge = group_exp(top, kvi ? -126 : 0);  // zeros among values never make the largest exponent
-            if (lane == 0) (kvi ? sh.vexp : sh.kexp)[tiles % EXP_RING][8 * b + lw] = ge;
+            if (lane == 0) (kvi ? sh.vfac : sh.kfac)[tiles % EXP_RING][8 * b + lw] = pow2(ge);
             const uint64_t f = pack_f32x2(pow2(-ge), pow2(-ge));
             uint8_t* dst = sm + L::RING + ((n + kvi) % NS) * L::SLOT;
 #pragma unroll
@@ -473,7 +478,7 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
 #pragma unroll
             for (int d = LPR / 2; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
             const int ge = group_exp(top, 0);
-            const float f = pow2(-ge), back = pow2(ge);
+            const float f = copysignf(pow2(-ge), a.scale_log2), back = pow2(ge);  // (a negative scale turns the queries)
 #pragma unroll
             for (int i = 0; i < RPI; ++i) {
               const float v = __shfl_sync(0xffffffffu, back, i * LPR);
@@ -496,6 +501,7 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
         float o[HD];
 #pragma unroll
         for (int d = 0; d < HD; ++d) o[d] = 0.0f;
+        const float scale = fabsf(a.scale_log2);
         float due = 0.0f;  // factor of the half whose O' is not added yet
         auto add_half = [&](int b) {
 #pragma unroll
@@ -504,7 +510,9 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
             tmem_ld16(to + HD * b + 16 * q, x);
             tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[16 * q + e] = fmaf(__uint_as_float(x[e]), due, o[16 * q + e]);
+            for (int e = 0; e < 16; e += 2)
+              unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), pack_f32x2(due, due), pack_f32x2(o[16 * q + e], o[16 * q + e + 1])),
+                           o[16 * q + e], o[16 * q + e + 1]);
           }
         };
         for (int i = wk.ta; i < end && ok; ++i) {
@@ -518,38 +526,36 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
             if (!ok) break;
             tc_fence_after();
             const int key0 = (wk.blk.tile0 + i) * TC_TK + 64 * b;
-            const bool mask = cut || (holes[2 * b] | holes[2 * b + 1]) != 0;
             const uint32_t sa = ts + 64 * b;
             uint32_t v[2][16];
             tmem_ld16(sa, v[0]);
             // factors of 8 keys each: of the products, and of P (relative to the half's largest exponent `ref`)
             float kf[8], vf[8];
             // never zero, or a masked product's infinity would become NaN
-            auto factor = [&](float f) { return copysignf(fmaxf(fabsf(a.scale_log2) * f, 1e-37f), a.scale_log2); };
-            int ref = 0;
+            auto factor = [&](float f) { return fmaxf(scale * f, 1e-37f); };
+            float ref = 1.0f;
             if constexpr (F32C) {
-              ref = -126;
 #pragma unroll
               for (int q = 0; q < 2; ++q) {
-                const int4 ke = *reinterpret_cast<const int4*>(&sh.kexp[rt % EXP_RING][8 * b + 4 * q]);
-                const int4 ve = *reinterpret_cast<const int4*>(&sh.vexp[rt % EXP_RING][8 * b + 4 * q]);
-                ref = max(ref, max(max(ve.x, ve.y), max(ve.z, ve.w)));
+                const float4 ke = *reinterpret_cast<const float4*>(&sh.kfac[rt % EXP_RING][8 * b + 4 * q]);
+                const float4 ve = *reinterpret_cast<const float4*>(&sh.vfac[rt % EXP_RING][8 * b + 4 * q]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                  kf[4 * q + j] = factor(qinv * pow2((&ke.x)[j]));
-                  vf[4 * q + j] = float((&ve.x)[j]);
+                  kf[4 * q + j] = factor(qinv * (&ke.x)[j]);
+                  vf[4 * q + j] = (&ve.x)[j];
                 }
               }
+              ref = max3(max3(vf[0], vf[1], vf[2]), max3(vf[3], vf[4], vf[5]), fmaxf(vf[6], vf[7]));
+              const float inv = __uint_as_float((254u << 23) - __float_as_uint(ref));  // 1 / ref
 #pragma unroll
-              for (int q = 0; q < 8; ++q) {
-                const int d = int(vf[q]) - ref;
-                vf[q] = d < -126 ? 0.0f : pow2(d);
-              }
+              for (int q = 0; q < 8; ++q) vf[q] *= inv;
             } else {
               kf[0] = factor(qinv);
             }
+            // which of the keys this row sees; whether some row of the warp does not see all of them
             uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
-            if (mask) {
+            bool mask = false;
+            if (cut || (holes[2 * b] | holes[2 * b + 1]) != 0) {
               const int lo = max(0, min(64, klo - key0)), hi = max(0, min(64, khi - key0));
 #pragma unroll
               for (int q = 0; q < 2; ++q) {
@@ -557,15 +563,15 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
                 const uint32_t below1 = b1 >= 32 ? 0xffffffffu : (1u << b1) - 1u, below0 = b0 >= 32 ? 0xffffffffu : (1u << b0) - 1u;
                 seen[q] = below1 & ~below0 & ~holes[2 * b + q];
               }
+              mask = __any_sync(0xffffffffu, (seen[0] & seen[1]) != 0xffffffffu);
             }
             // S is read twice, 16 keys at a time: for the maximum, then for P, whose two parts take the 16 columns' place
-            const uint32_t none = a.scale_log2 < 0.0f ? 0x7f800000u : 0xff800000u;  // -infinity once scaled
             auto keys = [&](int c, uint32_t (&x)[16]) {  // columns 16 c .. of S, the next ones on their way
               tmem_wait_ld();
               if (mask) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
-                  if (!((seen[c >> 1] >> (16 * (c & 1) + e)) & 1)) x[e] = none;
+                  if (!((seen[c >> 1] >> (16 * (c & 1) + e)) & 1)) x[e] = 0xff800000u;  // -infinity
               }
             };
             float top = -INFINITY;
@@ -577,13 +583,8 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
 #pragma unroll
               for (int q = 0; q < 2; ++q) {
                 const float f = kf[F32C ? 2 * c + q : 0];
-                float hi = __uint_as_float(x[8 * q]), lo = hi;
-#pragma unroll
-                for (int e = 1; e < 8; ++e) {
-                  if (a.scale_log2 >= 0.0f) hi = fmaxf(hi, __uint_as_float(x[8 * q + e]));
-                  else lo = fminf(lo, __uint_as_float(x[8 * q + e]));
-                }
-                top = fmaxf(top, (a.scale_log2 >= 0.0f ? hi : lo) * f);
+                auto at = [&](int e) { return __uint_as_float(x[8 * q + e]); };
+                top = fmaxf(top, max3(max3(at(0), at(1), at(2)), max3(at(3), at(4), at(5)), fmaxf(at(6), at(7))) * f);
               }
             }
             if (__any_sync(0xffffffffu, top > m + SLACK)) {
@@ -634,7 +635,7 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
               add_half(1 - b);
               tc_fence_before();
             }
-            due = pow2(ref);
+            due = ref;
           }
           ++t;
         }
