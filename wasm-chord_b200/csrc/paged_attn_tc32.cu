@@ -18,9 +18,9 @@
 // the tile is whole. head_dim 64: two row tiles of 128 rows; 128: one (Q in two parts and a
 // ring of K and V in two parts fill the shared memory).
 //
-// 46 sequences of 919 tokens, 32/4 heads of 64, f32 cache: 1.26 ms, 126 TFLOP/s of the formula's
-// products, 380 of those made (23 % of the measured cuBLAS rate); nine sequences of 1 to 700 tokens with
-// a window of 511 132 us. What bounds it: the instructions of the splitting, in the softmax (P) and in the loaders
+// 46 sequences of 919 tokens, 32/4 heads of 64, f32 cache: 1.11 ms, 143 TFLOP/s of the formula's
+// products, 430 of those made (26 % of the measured cuBLAS rate); nine sequences of 1 to 700 tokens with
+// a window of 511 118 us; one of 2048 tokens over 16384 keys 1.05 ms, 250 and 740 TFLOP/s (44 %). What bounds it: the instructions of the splitting, in the softmax (P) and in the loaders
 // (K and V), and at few tiles a unit's start and end.
 #include "paged_tc.cuh"
 
@@ -43,10 +43,11 @@ struct Tc32Cfg {
   static constexpr int RING = RT * 2 * PART;
   static constexpr int OFFS = RING + SLOTS * SLOT;   // [2][128] row offsets (f16 cache)
   static constexpr int SMEM = OFFS + 2 * 128 * 8 + 1024;
-  // registers of a thread by role; together no more than the launch's
+  // registers of a thread by role; together no more than the launch's (two row tiles, f32: softmax 168 and loaders 48 took
+  // 1.15 ms for the 2048 tokens over 16384 keys that take 1.05; 152 and 64 more than either at short units)
   static constexpr int LAUNCH = 65536 / THREADS / 8 * 8;
-  static constexpr int R_MMA = 40, R_LOAD = F32C ? (RT == 2 ? 48 : 96) : 80;
-  static constexpr int R_SOFT = RT == 2 ? (F32C ? 168 : 192) : 240;
+  static constexpr int R_MMA = 40, R_LOAD = F32C ? (RT == 2 ? 56 : 96) : 80;
+  static constexpr int R_SOFT = RT == 2 ? (F32C ? 160 : 192) : 240;
   static_assert(RT * R_SOFT + LW / 4 * R_LOAD + R_MMA <= WGS * LAUNCH, "register split");
 };
 
@@ -283,7 +284,7 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
                                   static_cast<const float*>(a.pool.v) + wk.kvh * a.pool.head_stride + 8 * sub};
           // K's halves, V's halves: the next one is on its way while one is split. (A rolled loop, like all that is long here:
           // the roles' code together has to stay in the instruction cache. Unrolled, the kernel took 1.81 ms where
-          // it takes 1.50 ms at 46 sequences of 919 new tokens, 32/4 heads of 64.)
+          // it took 1.50 ms at 46 sequences of 919 new tokens, 32/4 heads of 64.)
           float4 y[IT], ahead[IT];
           auto load = [&](int u) {
             const float* from = u < 2 ? base[0] : base[1];
