@@ -41,7 +41,7 @@
 // by itself and added to O by an ordinary multiply-add.
 //
 // Measured, single tokens over f16: 64 sequences of up to 8191 keys, 64/8 heads of 128
-// (1.1 GB), 182 us run after run, 93 % of the copy rate; one of 131071 keys (537 MB) 98.5 us, 83 %, the rest is the
+// (1.1 GB), 182 us run after run, 93 % of the copy rate; one of 131071 keys (537 MB) 96 us, 86 %, the rest is the
 // launch, the first loads and the join; 16 sequences of 1 to 6 tokens over 500 to 2304
 // keys, 32/32 heads (349 MB), 66 us, 81 %; one sequence of 320 keys 8 us, all of it latency.
 #pragma once
@@ -527,6 +527,7 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
       }
     };
 
+    fence_proxy_async();  // (results went through the ring's memory)
     __syncthreads();  // the ring and offs of the last unit are done with
 #pragma unroll
     for (int i = 0; i < S; ++i)
@@ -905,26 +906,35 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
     }
 
     if (!whole) {
-      // the last of the unit's CTAs joins its pieces, in their order
+      // The last of the unit's CTAs joins its pieces, in their order. More than GROUP pieces: the last of
+      // every `step` of them joins those into the first one's, the last of all the groups (one sequence
+      // of 131071 keys, 75 pieces: in one go 98.1 us, by groups 95.6).
+      constexpr int GROUP = 8;
       const int c0 = quotient(unit0 + V, pl.per), c1 = quotient(unit0 + V + blk.tiles - 1, pl.per);
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) s_last = atomicInc(reinterpret_cast<unsigned*>(a.tickets) + c0, unsigned(c1 - c0)) == unsigned(c1 - c0);
-      __syncthreads();
-      if (s_last) {
+      auto part = [&](int p) { return a.part + (size_t(p) * 2 + (p == c0 ? 1 : 0)) * size_t(M) * (HD + 2); };
+      // whether this CTA is the last of n at a counter (which is left at zero)
+      auto last = [&](int ticket, int n) {
         __threadfence();
+        __syncthreads();
+        if (tid == 0) s_last = n == 1 || atomicInc(reinterpret_cast<unsigned*>(a.tickets) + ticket, unsigned(n - 1)) == unsigned(n - 1);
+        __syncthreads();
+        const bool is = s_last;
+        if (is) __threadfence();
+        return is;
+      };
+      // pieces from, from + step .. of up to `to`; into the first, or the output
+      auto join = [&](int from, int to, int step, bool out) {
         for (int c = tid; c < rn * (HD / 4); c += AT_THREADS) {
           const int r = c / (HD / 4), d = 4 * (c % (HD / 4));
-          auto part = [&](int p) { return a.part + (size_t(p) * 2 + (p == c0 ? 1 : 0)) * size_t(M) * (HD + 2); };
-          // eight pieces at a time: their loads are on the way together
+          // eight at a time: their loads are on the way together
           float m = -INFINITY, l = 0.0f;
           float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          for (int p0 = c0; p0 <= c1; p0 += 8) {
+          for (int p0 = from; p0 <= to; p0 += 8 * step) {
             float2 q[8];
             float4 v[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              const float* pc = part(min(p0 + j, c1));
+              const float* pc = part(p0 + j * step <= to ? p0 + j * step : p0);
               q[j] = __ldcg(reinterpret_cast<const float2*>(pc + size_t(M) * HD + 2 * r));
               v[j] = __ldcg(reinterpret_cast<const float4*>(pc + size_t(r) * HD + d));
             }
@@ -936,18 +946,36 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
             l *= f0;
             x = make_float4(x.x * f0, x.y * f0, x.z * f0, x.w * f0);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float f = p0 + j <= c1 ? fast_exp2(q[j].x - u) : 0.0f;
-              if (p0 + j <= c1) {
+            for (int j = 0; j < 8; ++j)
+              if (p0 + j * step <= to) {
+                const float f = fast_exp2(q[j].x - u);
                 l += f * q[j].y;
                 x.x += f * v[j].x;
                 x.y += f * v[j].y;
                 x.z += f * v[j].z;
                 x.w += f * v[j].w;
               }
-            }
           }
-          finish(r, d, x, m, l);
+          if (out) {
+            finish(r, d, x, m, l);
+          } else {
+            float* to_piece = part(from);
+            __syncwarp(HD == 128 ? 0xffffffffu : 0xffffu << (lane & 16));  // a row's threads have read its m and l before one writes them
+            *reinterpret_cast<float4*>(to_piece + size_t(r) * HD + d) = x;
+            if (d == 0) *reinterpret_cast<float2*>(to_piece + size_t(M) * HD + 2 * r) = make_float2(m, l);
+          }
+        }
+      };
+      const int n = c1 - c0 + 1;
+      if (n <= GROUP) {
+        if (last(c0, n)) join(c0, c1, 1, true);
+      } else {
+        // counters: a group's is its first CTA's; that of the groups is c0 + 1's, a CTA that no other unit begins in
+        const int step = n <= 16 * GROUP ? GROUP : 4 * GROUP;
+        const int me = c0 + (int(blockIdx.x) - c0) / step * step, end = min(c1, me + step - 1);
+        if (last(me, end - me + 1)) {
+          if (end > me) join(me, end, 1, false);
+          if (last(c0 + 1, (n + step - 1) / step)) join(c0, c1, step, true);
         }
       }
     }

@@ -23,13 +23,13 @@
 // room for the factor): one vote on the sum instead of 64 comparisons a row.
 // TMEM: S0 | S1 | O0 | O1, 512 columns at head_dim 128.
 //
-// 2047 new tokens over 32767 keys, 64/8 heads of 128, bf16: 2.0 ms run after run, 2.3 ms with
-// pauses in between, 1060 and 925 TFLOP/s (64 and 55 % of the measured cuBLAS rate). What bounds it: the
+// 2047 new tokens over 32767 keys, 64/8 heads of 128, bf16: 1.96 ms run after run, 2.3 ms with
+// pauses in between, 1090 and 925 TFLOP/s (65 and 55 % of the measured cuBLAS rate). What bounds it: the
 // exponentials of the two softmax warps of a scheduler and what surrounds them (1250 clocks a
 // half with both row tiles; without the exponentials themselves 600, and the products' 2560
 // clocks become the bound). Part of the exponentials by a polynomial on the multiply-add units
 // (a quarter, an eighth) gained nothing: those pay as many clocks for it. Short units: 11
-// sequences of 204 tokens 74 us (82 with units that are cut in two for one tile).
+// sequences of 204 tokens 72 us (82 with units that are cut in two for one tile).
 #include "paged_tc.cuh"
 
 namespace wcb {
@@ -339,10 +339,10 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
             if (!ok) break;
             tc_fence_after();
             const int key0 = (wk.blk.tile0 + i) * TC_TK + 64 * b;
-            const bool mask = cut || (holes[2 * b] | holes[2 * b + 1]) != 0;
-            // bit c: key key0 + c is seen
+            // bit c: key key0 + c is seen; mask: some row of the warp does not see all of them
             uint32_t seen[2];
-            if (mask) {
+            bool mask = false;
+            if (cut || (holes[2 * b] | holes[2 * b + 1]) != 0) {
               const int lo = max(0, min(64, klo - key0)), hi = max(0, min(64, khi - key0));
 #pragma unroll
               for (int q = 0; q < 2; ++q) {
@@ -350,6 +350,7 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
                 const uint32_t below1 = b1 >= 32 ? 0xffffffffu : (1u << b1) - 1u, below0 = b0 >= 32 ? 0xffffffffu : (1u << b0) - 1u;
                 seen[q] = below1 & ~below0 & ~holes[2 * b + q];
               }
+              mask = __any_sync(0xffffffffu, (seen[0] & seen[1]) != 0xffffffffu);
             }
             // the row's 64 products in registers: TMEM is read once
             uint32_t v[64];
@@ -392,13 +393,15 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
             };
             // Most halves need no maximum: the last one still serves as long as the sum shows that no
             // exponential left the range of f16 and of a sound sum (GROWTH); a row's sum is wanted anyway.
-            float part;
-            bool again = __any_sync(0xffffffffu, mask || m == -INFINITY);
-            if (!again) {
+            // A row decides by its own sum alone, so that its result does not depend on what its neighbours see.
+            float part = 0.0f;
+            bool moves = m == -INFINITY;
+            if (!__all_sync(0xffffffffu, moves)) {
               exponentials();
               part = total();
-              again = __any_sync(0xffffffffu, !(part <= GROWTH));
+              moves = moves || !(part <= GROWTH);
             }
+            const bool again = __any_sync(0xffffffffu, moves);
             if (again) {
               float top;
               if (a.scale_log2 >= 0.0f) {
@@ -406,7 +409,7 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
 #pragma unroll
                 for (int e = 0; e < 64; e += 8)
 #pragma unroll
-                  for (int j = 0; j < 4; ++j) x[j] = fmaxf(x[j], fmaxf(__uint_as_float(v[e + 2 * j]), __uint_as_float(v[e + 2 * j + 1])));
+                  for (int j = 0; j < 4; ++j) x[j] = max3(x[j], __uint_as_float(v[e + 2 * j]), __uint_as_float(v[e + 2 * j + 1]));
                 top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * a.scale_log2;
               } else {  // a negative scale turns the order round
                 float x = INFINITY;
@@ -414,8 +417,8 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
                 for (int e = 0; e < 64; ++e) x = fminf(x, __uint_as_float(v[e]));
                 top = x * a.scale_log2;
               }
-              if (__any_sync(0xffffffffu, top > m)) {
-                const float nm = fmaxf(m, top);
+              const float nm = moves ? fmaxf(m, top) : m;
+              if (__any_sync(0xffffffffu, nm > m)) {
                 const float f = m == nm ? 1.0f : fast_exp2(m - (nm == -INFINITY ? 0.0f : nm));
                 if (i > wk.ta || b) {  // after the last product
                   ok = tc_wait_warp(&sh, &sh.o_done[w][1 - b], (b ? t : t - 1) & 1);

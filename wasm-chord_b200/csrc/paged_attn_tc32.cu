@@ -60,11 +60,6 @@ struct Tc32Shared : TcShared {
   alignas(16) float vfac[EXP_RING][16];
 };
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((max(-126, min(127, e)) + 127) << 23); }
 // the exponent that brings numbers up to `top` below 2^14; `none` where there are only zeros
 __device__ __forceinline__ int group_exp(float top, int none) {
