@@ -389,7 +389,8 @@ typedef struct wcb_paged_batch {
  * stored; its attention output is zero). BAD_TOKEN: a drafted token outside the
  * vocabulary (turned down). BAD_PROBS: a row of target probabilities without
  * a positive finite value (the sampled token is -1). ABORTED: a wait inside a
- * kernel ran out; the call's outputs are not valid. */
+ * kernel ran out; the call's outputs are not valid, and its workspace has to be
+ * zeroed again. */
 enum {
   WCB_PAGED_BAD_PAGE = 1,
   WCB_PAGED_BAD_ROWS = 2,
