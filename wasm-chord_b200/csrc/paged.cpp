@@ -107,26 +107,25 @@ uint32_t check_rows(const void* p, uint64_t stride, uint64_t width, uint32_t dty
   return WCB_OK;
 }
 
-// Which kernels a call runs, from what the host knows: the types, the longest sequence's rows
+// Which kernels a call runs, from what the host knows: the longest sequence's rows
 // (new tokens * rep), the number of sequences. Sequences of more than TC_MIN rows go to a tensor-core
-// kernel (f32 activations over a bf16 cache have none), the others of the batch to the mma.sync kernel. Its
-// row block is the smallest that holds the longest sequence's rows, so that no product is spent on rows that
-// are not there. A call that would make no more than TC_UNITS blocks of 32 rows in all stays with the mma.sync
-// kernel: cut into many parts, its small blocks are joined sooner than blocks of 256.
+// kernel, the others of the batch to the mma.sync kernel. Its row block is the smallest that holds the longest
+// sequence's rows, so that no product is spent on rows that are not there. A call that would make no more than
+// TC_UNITS blocks of 32 rows in all stays with the mma.sync kernel: cut into many parts, its small blocks are
+// joined sooner than blocks of 256.
 // Measured (us, tensor cores / mma.sync; 32/4 heads of 64, f16, 4096 keys): 1 sequence of 64 rows (8 blocks) 41 / 21, of
 // 256 (32) 45 / 29, of 512 (64) 33 / 40, of 1024 28 / 64; 32 sequences of 40 rows (256) 70 / 114, of 256 87 / 423;
-// f32 over f32: 1 of 128 rows 41 / 34, of 256 47 / 52, 32 of 40 185 / 290; 64/8 heads of 128, bf16: 1 of 64 rows (16) 46 / 32,
-// of 128 (32) 47 / 45, of 256 (64) 53 / 61.
+// f32 over f32: 1 of 128 rows 41 / 34, of 256 47 / 52, 32 of 40 185 / 290; f32 over bf16: 16 of 612 rows 56 / 92;
+// 64/8 heads of 128, bf16: 1 of 64 rows (16) 46 / 32, of 128 (32) 47 / 45, of 256 (64) 53 / 61.
 constexpr uint64_t TC_MIN = 32, TC_UNITS = 32;
 struct Plan {
   int rows;     // row block of the mma.sync kernel, 0: not run
   bool tc;
   int split;    // sequences of more rows are the tensor-core kernel's
 };
-Plan plan(uint32_t dtype, uint32_t cache, uint64_t n_seqs, uint64_t n_kv, uint64_t max_rows) {
+Plan plan(uint64_t n_seqs, uint64_t n_kv, uint64_t max_rows) {
   Plan p{};
-  p.tc = !(dtype == WCB_KV_F32 && cache == WCB_KV_BF16) && max_rows > TC_MIN &&
-         n_seqs * n_kv * ((max_rows + 31) / 32) > TC_UNITS;
+  p.tc = max_rows > TC_MIN && n_seqs * n_kv * ((max_rows + 31) / 32) > TC_UNITS;
   p.split = p.tc ? (n_seqs == 1 ? 0 : int(TC_MIN)) : INT_MAX;
   const uint64_t r = p.tc ? (n_seqs == 1 ? 0 : TC_MIN) : max_rows;
   p.rows = r == 0 ? 0 : r <= 8 ? 8 : r <= 16 ? 16 : 32;
@@ -214,10 +213,7 @@ uint32_t wcb_paged_attention_workspace(const wcb_paged_kv* kv, const wcb_paged_b
   if (n_heads == 0 || n_heads > 4096 || n_heads % kv->n_kv_heads || n_heads / kv->n_kv_heads > 64)
     return bad("Invalid tensor shape: need n_heads % n_kv_heads == 0 (<= 64 per kv head)");
   const uint64_t rows = uint64_t(batch->max_q_len) * (n_heads / kv->n_kv_heads);
-  // the activations' type is not known here: the larger of the two
-  const size_t x = workspace_bytes(plan(WCB_KV_F32, kv->dtype, batch->n_seqs, kv->n_kv_heads, rows), pool.head_dim);
-  const size_t y = kv->dtype == WCB_KV_F32 ? 0 : workspace_bytes(plan(kv->dtype, kv->dtype, batch->n_seqs, kv->n_kv_heads, rows), pool.head_dim);
-  *bytes = x > y ? x : y;
+  *bytes = workspace_bytes(plan(batch->n_seqs, kv->n_kv_heads, rows), pool.head_dim);
   return WCB_OK;
 }
 
@@ -253,7 +249,7 @@ uint32_t wcb_paged_attention_dev(const wcb_paged_kv* kv, const wcb_paged_batch* 
   a.window = int(window);
   a.tickets = static_cast<int*>(workspace);
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + TICKET_BYTES);
-  const Plan p = plan(dtype, kv->dtype, batch->n_seqs, kv->n_kv_heads, uint64_t(batch->max_q_len) * uint64_t(a.rep));
+  const Plan p = plan(batch->n_seqs, kv->n_kv_heads, uint64_t(batch->max_q_len) * uint64_t(a.rep));
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
   if (p.tc) {

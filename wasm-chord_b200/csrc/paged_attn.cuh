@@ -1,6 +1,6 @@
 // Attention of new tokens over a paged cache: the kernel for few rows (mma.sync;
 // the products of a decode step are far from the tensor cores' rate, its bytes are
-// the bound) and for f32 activations over a bf16 cache.
+// the bound).
 //
 // o_i = sum_j softmax_j(scale q_i . k_j) v_j over the keys a token sees, in one
 // pass over K and V with a running maximum m and sum l (both f32):

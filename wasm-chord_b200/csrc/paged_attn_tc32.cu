@@ -1,10 +1,11 @@
 // Attention of many new rows over a paged cache on the 5th-generation tensor
-// cores, f32 activations over an f32 or f16 cache (the formulas and the line of tiles:
+// cores, f32 activations over a cache of any type (the formulas and the line of tiles:
 // paged_attn.cuh; the 16-bit kernel this one is built like: paged_attn_tc.cu).
 //
 // f32 numbers go to the tensor cores as sums of two f16 numbers, x = 2^e (hi + lo), 22 bits: the
 // exponents are a row's (q) or 8 keys' (k and v), so that the largest of them lies below 2^14 and
-// what is lost of the others is below 2^-38 of it. An f16 cache needs no splitting.
+// what is lost of the others is below 2^-38 of it. An f16 cache needs no splitting; a bf16 cache is widened and split like
+// an f32 one (its range is f32's).
 //   S  = Qlo Khi + Qhi Klo + Qhi Khi             (two products over an f16 cache)
 //   O' = Plo Vhi + Phi Vlo + Phi Vhi             (one half of 64 keys)
 //   O  = O 2^(m - m') + O' 2^e                   in registers, by ordinary f32 arithmetic
@@ -20,7 +21,7 @@
 //
 // 46 sequences of 919 tokens, 32/4 heads of 64, f32 cache: 1.11 ms, 143 TFLOP/s of the formula's
 // products, 430 of those made (26 % of the measured cuBLAS rate); nine sequences of 1 to 700 tokens with
-// a window of 511 118 us; one of 2048 tokens over 16384 keys 1.05 ms, 250 and 740 TFLOP/s (44 %). What bounds it: the instructions of the splitting, in the softmax (P) and in the loaders
+// a window of 511 118 us (over a bf16 cache 117, 353 on mma.sync); one of 2048 tokens over 16384 keys 1.05 ms, 250 and 740 TFLOP/s (44 %). What bounds it: the instructions of the splitting, in the softmax (P) and in the loaders
 // (K and V), and at few tiles a unit's start and end.
 #include "paged_tc.cuh"
 
@@ -30,7 +31,7 @@ namespace {
 
 template <typename CT, int HD>
 struct Tc32Cfg {
-  static constexpr bool F32C = std::is_same<CT, float>::value;
+  static constexpr bool F32C = !std::is_same<CT, __half>::value;  // f32, or bf16 widened to it: not exact in f16
   static constexpr int RT = HD == 64 ? 2 : 1;       // row tiles
   static constexpr int M = 128 * RT;
   static constexpr int LW = F32C ? 8 : 4;           // loader warps: those of an f32 cache have the splitting to do
@@ -275,19 +276,28 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
           constexpr int RPI = 32 / LPR;      // rows of an iteration
           constexpr int IT = 2 * 8 / RPI;    // 16-byte words of a lane: two of each of its rows
           const int sub = lane % LPR, rr = lane / LPR;
-          const float* base[2] = {static_cast<const float*>(a.pool.k) + wk.kvh * a.pool.head_stride + 8 * sub,
-                                  static_cast<const float*>(a.pool.v) + wk.kvh * a.pool.head_stride + 8 * sub};
+          const CT* base[2] = {static_cast<const CT*>(a.pool.k) + wk.kvh * a.pool.head_stride + 8 * sub,
+                                  static_cast<const CT*>(a.pool.v) + wk.kvh * a.pool.head_stride + 8 * sub};
           // K's halves, V's halves: the next one is on its way while one is split. (A rolled loop, like all that is long here:
           // the roles' code together has to stay in the instruction cache. Unrolled, the kernel took 1.81 ms where
           // it took 1.50 ms at 46 sequences of 919 new tokens, 32/4 heads of 64.)
           float4 y[IT], ahead[IT];
           auto load = [&](int u) {
-            const float* from = u < 2 ? base[0] : base[1];
+            const CT* from = u < 2 ? base[0] : base[1];
 #pragma unroll
             for (int j = 0; j < IT; j += 2) {
               const long long o = __shfl_sync(0xffffffffu, off, 8 * (u & 1) + RPI * (j / 2) + rr);
-              ahead[j] = o >= 0 ? __ldg(reinterpret_cast<const float4*>(from + o)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-              ahead[j + 1] = o >= 0 ? __ldg(reinterpret_cast<const float4*>(from + o) + 1) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              if constexpr (std::is_same<CT, float>::value) {
+                ahead[j] = o >= 0 ? __ldg(reinterpret_cast<const float4*>(from + o)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                ahead[j + 1] = o >= 0 ? __ldg(reinterpret_cast<const float4*>(from + o) + 1) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              } else {
+                const uint4 w = o >= 0 ? __ldg(reinterpret_cast<const uint4*>(from + o)) : make_uint4(0, 0, 0, 0);
+                auto widen = [](uint32_t x, uint32_t y) {  // (a bf16 is the upper half of its f32)
+                  return make_float4(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u), __uint_as_float(y << 16), __uint_as_float(y & 0xffff0000u));
+                };
+                ahead[j] = widen(w.x, w.y);
+                ahead[j + 1] = widen(w.z, w.w);
+              }
             }
           };
 #pragma unroll 1
@@ -777,6 +787,7 @@ cudaError_t run_tc32(const AttendArgs& a, cudaStream_t s) {
 
 cudaError_t launch_attend_tc32(const AttendArgs& a, int cache, cudaStream_t s) {
   if (cache == E_F16) return a.pool.head_dim == 64 ? run_tc32<__half, 64>(a, s) : run_tc32<__half, 128>(a, s);
+  if (cache == E_BF16) return a.pool.head_dim == 64 ? run_tc32<__nv_bfloat16, 64>(a, s) : run_tc32<__nv_bfloat16, 128>(a, s);
   return a.pool.head_dim == 64 ? run_tc32<float, 64>(a, s) : run_tc32<float, 128>(a, s);
 }
 
