@@ -300,6 +300,18 @@ def test_short_and_long_units(gpu, act, cache, dim, chunks):
     s.check()
 
 
+# one sequence cut into about 7, 8, 9, 16, 17, 127 .. 130 and 256 pieces: joined in one go, by groups, by large groups
+@pytest.mark.parametrize("act,cache,dim", [("f16", "f16", 128), ("f32", "f32", 64), ("f32", "bf16", 64)])
+@pytest.mark.parametrize("kv", [448, 512, 513, 1024, 1025, 8128, 8192, 8256, 8257, 16384])
+def test_pieces_and_groups(gpu, act, cache, dim, kv):
+    s = Step([1], [kv], 8, 2, dim, act, cache, 64, True, seed=32)
+    room = s.attend()
+    s.check()
+    first = s.out.clone()
+    s.attend(room=room)
+    assert torch.equal(first, s.out) and (room[:4096] == 0).all()
+
+
 @pytest.mark.parametrize("act,cache,heads,kv_heads,dim", [("f16", "f16", 8, 2, 128), ("f32", "f16", 32, 4, 64), ("bf16", "bf16", 64, 8, 128)])
 def test_long_sequences_and_repeatability(gpu, act, cache, heads, kv_heads, dim):
     s = Step([1, 1], [20011, 3], heads, kv_heads, dim, act, cache, 64, True, seed=10)
