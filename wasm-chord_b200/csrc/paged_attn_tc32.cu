@@ -19,10 +19,11 @@
 // the tile is whole. head_dim 64: two row tiles of 128 rows; 128: one (Q in two parts and a
 // ring of K and V in two parts fill the shared memory).
 //
-// 46 sequences of 919 tokens, 32/4 heads of 64, f32 cache: 1.11 ms, 143 TFLOP/s of the formula's
-// products, 430 of those made (26 % of the measured cuBLAS rate); nine sequences of 1 to 700 tokens with
-// a window of 511 118 us (over a bf16 cache 117, 353 on mma.sync); one of 2048 tokens over 16384 keys 1.05 ms, 250 and 740 TFLOP/s (44 %). What bounds it: the instructions of the splitting, in the softmax (P) and in the loaders
-// (K and V), and at few tiles a unit's start and end.
+// 46 sequences of 919 tokens, 32/4 heads of 64, f32 cache: 1.13 ms, 141 TFLOP/s of the formula's
+// products, 423 of those made (25 % of the measured cuBLAS rate); one of 2048 tokens over 16384 keys
+// 1.05 ms, 250 and 740 TFLOP/s (44 %); nine of 1 to 700 tokens with a window of 511 120 us (over a bf16
+// cache 117; 353 on mma.sync). What bounds it: the instructions of the splitting, in the softmax (P) and in
+// the loaders (K and V), and at few tiles a unit's start and end.
 #include "paged_tc.cuh"
 
 namespace wcb {
@@ -528,7 +529,7 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
 #pragma unroll 1
           for (int b = 0; b < 2; ++b) {
             ok = tc_wait_warp(&sh, &sh.s_full[w][b], t & 1);
-            if (F32C && b == 0) ok = ok && tc_wait_warp(&sh, &sh.full[(2 * rt + 1) % NS], ((2 * rt + 1) / NS) & 1);  // the values' exponents
+            if (F32C && b == 0) ok = ok && tc_wait_warp(&sh, &sh.full[(2 * rt + 1) % NS], ((2 * rt + 1) / NS) & 1);  // the values' factors
             if (!ok) break;
             tc_fence_after();
             const int key0 = (wk.blk.tile0 + i) * TC_TK + 64 * b;
@@ -594,7 +595,7 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
               }
             }
             if (__any_sync(0xffffffffu, top > m + SLACK)) {
-              const float nm = fmaxf(m, top);
+              const float nm = top > m + SLACK ? top : m;  // (a row by itself: not by what its neighbours see)
               const float f = m == nm ? 1.0f : fast_exp2(m - (nm == -INFINITY ? 0.0f : nm));
 #pragma unroll
               for (int d = 0; d < HD; ++d) o[d] *= f;
