@@ -1,0 +1,171 @@
+"""Paged attention over numbers of very different sizes: large finite keys and values that a row does not see or
+gives no weight, a key that takes most of the weight, and the low-order parts of f32 numbers. Held to bounds near the
+kernels' own errors, row by row, against 64 bits.
+
+Bound for f32 activations. Each weight p_j carries a relative error of its score's error, of the exponential and
+of the splits and short sums: with numbers kept to 22 bits and sums to 2^-24 a step, 2^-20 together at scores of
+a few units; a score's own part grows with its size: its products, of signs of their own, scale sqrt(sum_d q_d^2 k_d^2) to
+2^-22; and where they all have one sign, |s| itself, which the tensor cores sum in d / 16 steps, cutting the sum off below
+its 24 bits (up to 2^-23 of it) at each: d / 16 2^-23 |s|. Errors
+that all weights share cancel in the quotient or change a row by that part of itself; the others have signs of
+their own, so that a row's error is at most about rel ||(sum_j p_j^2 v_j^2)^(1/2)|| + rel ||o||. A product that is
+left out (hi x lo) would be an error of 2^-11 in the weights, a thousand times more."""
+import math
+
+import pytest
+
+import test_gpu_paged as paged
+import wcb
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+TOP = {"f32": torch.finfo(torch.float32).max, "f16": torch.finfo(torch.float16).max, "bf16": torch.finfo(torch.bfloat16).max}
+
+
+def exact(s, window=0, scale=0.0):
+    """Of each row and head: the output in 64 bits, the bound's 2-norm for f32 activations (above), ln of the sum, and the
+    bound of that."""
+    scale = scale or 1 / math.sqrt(s.d)
+    rep = s.h // s.hk
+    q = s.q[:, :s.h * s.d].double().cpu().view(-1, s.h, s.d)
+    kt, vt = s.by_token(s.k.cpu().double()), s.by_token(s.v.cpu().double())
+    out, lse = torch.zeros_like(q), torch.full(q.shape[:2], -math.inf, dtype=torch.float64)
+    tol, ltol = torch.zeros(q.shape[:2], dtype=torch.float64), torch.zeros(q.shape[:2], dtype=torch.float64)
+    for i, (nq, nk) in enumerate(zip(s.q_len, s.kv_len)):
+        if nq == 0 or nk <= 0:
+            continue
+        sl = s.slots(i)
+        k, v = kt[sl], vt[sl]
+        pos, j = torch.arange(nk - nq, nk)[:, None], torch.arange(nk)[None]
+        seen = (j <= pos) & ((j > pos - window) if window else True)
+        r = slice(s.start[i], s.start[i] + nq)
+        for h in range(s.h):
+            kk, vv, qq = k[:, h // rep], v[:, h // rep], q[r, h]
+            a = (qq @ kk.T * scale).masked_fill(~seen, -math.inf)
+            l = a.logsumexp(-1)
+            p = torch.where(seen, (a - l[:, None]).exp(), 0.0)
+            part = (qq.square() @ kk.square().T).sqrt() * abs(scale) + s.d / 32 * a.abs()
+            live = p > 2.0 ** -30 * p.amax(-1, keepdim=True)
+            rel = 2.0 ** -20 + 2.0 ** -22 * torch.where(live, part, 0.0).amax(-1)
+            o = p @ vv
+            out[r, h], lse[r, h] = o, l
+            tol[r, h] = rel * (o.norm(dim=-1) + (p.square() @ vv.square()).sqrt().norm(dim=-1)) + 1e-37
+            ltol[r, h] = rel + 2.0 ** -23 * l.abs().nan_to_num(0, 0, 0)
+    return out, tol, lse, ltol
+
+
+def check(s, rows=None, window=0, scale=0.0):
+    """f32 activations: the rows' 2-norm errors, and their lse."""
+    out, tol, lse, ltol = exact(s, window, scale)
+    rows = [r for i, n in enumerate(s.q_len) for r in range(s.start[i], s.start[i] + n)] if rows is None else rows
+    got = s.out[:, :s.h * s.d].double().cpu().view(out.shape)[rows]
+    assert torch.isfinite(got).all()
+    far = (got - out[rows]).norm(dim=-1) / tol[rows]
+    assert far.max() <= 1, (float(far.max()), rows[int(far.amax(-1).argmax())])
+    assert ((s.lse.double().cpu()[rows] - lse[rows]).abs() <= ltol[rows]).all()
+
+
+def put(s, i, key, k=None, v=None):
+    """Key `key` of sequence i, all its heads."""
+    page, slot = int(s.table[i, key // s.page]), key % s.page
+    for pool, x in ((s.k, k), (s.v, v)):
+        if x is not None:
+            (pool[page, :, slot] if s.by_head else pool[page, slot])[:] = x
+
+
+F32 = [("f32", "f32"), ("f32", "bf16"), ("f32", "f16")]
+
+
+# many rows (the tensor cores), and few (mma.sync)
+@pytest.mark.parametrize("act,cache", F32)
+@pytest.mark.parametrize("heads,kv_heads,dim,q", [(8, 2, 64, [70, 3]), (8, 8, 128, [70, 3]), (4, 4, 64, [6, 3])])
+@pytest.mark.parametrize("size", [1e3, 1e6, 1e9, 1e30])
+@pytest.mark.parametrize("where", ["k", "v", "kv"])
+def test_large_keys_and_values_that_a_row_does_not_see(gpu, act, cache, heads, kv_heads, dim, q, size, where):
+    kv, window = [140, 30], 60
+    s = paged.Step(q, kv, heads, kv_heads, dim, act, cache, 16, seed=50)
+    size = TOP[cache] if size == "largest" else min(size, TOP[cache])
+    first = kv[0] - q[0]  # the first new token's position; it alone sees the key that leaves the window after it
+    for i, key in ((0, 139), (0, first - window + 1), (1, 29)):
+        put(s, i, key, size if "k" in where else None, -size if "v" in where else None)
+    s.attend(window=window)
+    assert int(s.status.item()) == 0
+    check(s, [*range(1, q[0] - 1), *range(q[0], q[0] + q[1] - 1)], window=window)
+
+
+@pytest.mark.parametrize("act,cache", [("f32", "f32"), ("f32", "bf16")])
+@pytest.mark.parametrize("heads,kv_heads,dim,q", [(8, 2, 64, 80), (8, 8, 128, 80), (4, 4, 64, 6)])
+@pytest.mark.parametrize("spread", [20, 40, 80])
+def test_keys_and_values_of_many_sizes(gpu, act, cache, heads, kv_heads, dim, q, spread):
+    """Every value has a size of its own between 1 and 2^spread, by its position: late rows see what early ones do not. Every
+    eighth key is as much smaller, so that its score vanishes and is no less exact."""
+    kv = 400
+    s = paged.Step([q], [kv], heads, kv_heads, dim, act, cache, 16, seed=51)
+    for j in range(kv):
+        page, slot = int(s.table[0, j // 16]), j % 16
+        s.v[page, slot] *= 2.0 ** (spread * j / kv)
+        if j % 8 == 3:
+            s.k[page, slot] *= 2.0 ** -spread
+    s.attend()
+    check(s)
+
+
+@pytest.mark.parametrize("act,cache", [("f32", "f32"), ("f32", "bf16")])
+@pytest.mark.parametrize("heads,kv_heads,dim,q", [(8, 2, 64, 80), (8, 8, 128, 80)])
+def test_large_values_without_weight(gpu, act, cache, heads, kv_heads, dim, q):
+    """Seen values of 1e9 whose keys lie 70 nats below the others: no less exact for the rest."""
+    s = paged.Step([q], [300], heads, kv_heads, dim, act, cache, 16, seed=52)
+    base = torch.randn(dim, generator=torch.Generator().manual_seed(1)).cuda()
+    base *= math.sqrt(dim) / base.norm()
+    s.q[:, :heads * dim] = (s.q[:, :heads * dim].view(-1, heads, dim) * 0.3 + base).view(s.tokens, -1)
+    for j in (5, 77, 78, 150, 219):
+        put(s, 0, j, (base * -70 / math.sqrt(dim)).to(s.ct), 1e9)
+    s.attend()
+    check(s)
+
+
+@pytest.mark.parametrize("act,cache", F32)
+@pytest.mark.parametrize("heads,kv_heads,dim,q", [(4, 2, 64, 70), (4, 4, 128, 70), (4, 4, 64, 2)])
+@pytest.mark.parametrize("gap", [13.0, 17.4, 25.0])
+def test_a_key_that_takes_most_of_the_weight(gpu, act, cache, heads, kv_heads, dim, q, gap):
+    """The first key stands `gap` nats above 12000 others and its value is zero, so that the others are the whole output."""
+    s = paged.Step([q], [12000], heads, kv_heads, dim, act, cache, 64, seed=53)
+    base = torch.ones(dim, device="cuda")
+    s.q[:, :heads * dim] = (s.q[:, :heads * dim].view(-1, heads, dim) * 0.05 + base).view(s.tokens, -1)
+    put(s, 0, 0, gap / math.sqrt(dim) * 1.0, 0.0)
+    s.attend()
+    check(s)
+
+
+@pytest.mark.parametrize("act,cache", F32)
+@pytest.mark.parametrize("heads,kv_heads,dim,q", [(8, 2, 64, 80), (8, 8, 128, 80), (4, 4, 64, 6), (8, 2, 64, 1)])
+@pytest.mark.parametrize("kv", [130, 900])
+def test_f32_keeps_its_low_bits(gpu, act, cache, heads, kv_heads, dim, q, kv):
+    s = paged.Step([q], [kv], heads, kv_heads, dim, act, cache, 16, seed=54)
+    s.attend()
+    check(s)
+    # one head's output over all rows, not only row by row
+    out, tol, _, _ = exact(s)
+    err = (s.out[:q, :s.h * s.d].double().cpu().view(q, heads, dim) - out[:q]).norm()
+    assert err <= 2.0 ** -19 * out[:q].norm()
+
+
+@pytest.mark.parametrize("act,cache", F32)
+@pytest.mark.parametrize("heads,kv_heads,dim,q", [(4, 2, 64, 80), (4, 4, 128, 80), (4, 4, 64, 6)])
+@pytest.mark.parametrize("part", ["q", "k", "p", "v"])
+def test_each_low_part_counts(gpu, act, cache, heads, kv_heads, dim, q, part):
+    """Numbers whose low parts all have one sign: 1 + 2^-12 (2^-10 too coarse for bf16's 8 bits: left out there) rounds to 1 in
+    f16 and tf32, so that a product without its low part is off by 2^-12 of itself, and nothing averages out."""
+    fine = 1 + 2.0 ** -12
+    if (part in "kv" and cache != "f32"):
+        pytest.skip("the cache's type has no low part")
+    s = paged.Step([q], [260], heads, kv_heads, dim, act, cache, 16, seed=55)
+    sign = torch.where(s.q[:, :heads * dim] < 0, -1.0, 1.0)
+    s.q[:, :heads * dim] = sign * (fine if part == "q" else 1.0)
+    s.k.copy_(torch.where(s.k.float() < 0, -1.0, 1.0) * (fine if part == "k" else 1.0))
+    s.v.copy_(fine if part == "v" else 1.0 + (torch.arange(dim, device="cuda") % 5 == 0).float())
+    if part == "p":  # two kinds of keys, weights that are no f16 numbers
+        s.v[..., :dim // 2] *= torch.where(s.k.float().sum(-1, keepdim=True) > 0, 1.0, -1.0)
+    s.attend(scale=0.31)
+    check(s, scale=0.31)

@@ -4,8 +4,11 @@
 //
 // f32 numbers go to the tensor cores as sums of two f16 numbers, x = 2^e (hi + lo), 22 bits: the
 // exponents are a row's (q) or 8 keys' (k and v), so that the largest of them lies below 2^14 and
-// what is lost of the others is below 2^-38 of it. An f16 cache needs no splitting; a bf16 cache is widened and split like
-// an f32 one (its range is f32's).
+// what is lost of the others is below 2^-38 of it. 8 keys that are farther apart than 2^16 stay out of the products:
+// each row that sees one adds it in ordinary f32 arithmetic, so that a large key or value, of a later token for instance,
+// takes no bits from what other rows see. P is split with an exponent of each row's own for 64 keys, that of
+// the largest weight times the size of its values among the keys that the row sees. An f16 cache needs no
+// splitting; a bf16 cache is widened and split like an f32 one (its range is f32's).
 //   S  = Qlo Khi + Qhi Klo + Qhi Khi             (two products over an f16 cache)
 //   O' = Plo Vhi + Phi Vlo + Phi Vhi             (one half of 64 keys)
 //   O  = O 2^(m - m') + O' 2^e                   in registers, by ordinary f32 arithmetic
@@ -19,11 +22,12 @@
 // the tile is whole. head_dim 64: two row tiles of 128 rows; 128: one (Q in two parts and a
 // ring of K and V in two parts fill the shared memory).
 //
-// 46 sequences of 919 tokens, 32/4 heads of 64, f32 cache: 1.13 ms, 141 TFLOP/s of the formula's
-// products, 423 of those made (25 % of the measured cuBLAS rate); one of 2048 tokens over 16384 keys
-// 1.05 ms, 250 and 740 TFLOP/s (44 %); nine of 1 to 700 tokens with a window of 511 120 us (over a bf16
-// cache 117; 353 on mma.sync). What bounds it: the instructions of the splitting, in the softmax (P) and in
-// the loaders (K and V), and at few tiles a unit's start and end.
+// 46 sequences of 919 tokens, 32/4 heads of 64, f32 cache: 1.16 ms, 137 TFLOP/s of the formula's
+// products, 412 of those made (25 % of the measured cuBLAS rate); one of 2048 tokens over 16384 keys
+// 1.08 ms, 243 and 720 TFLOP/s (43 %). The rows' own exponents of P and the search for keys that are far apart are 2 to
+// 5 % of that (an exponent for each key instead, read by a second way through the softmax: 10 %). What bounds it: the
+// instructions of the splitting, in the softmax (P) and in the loaders (K and V), about 500 bytes of registers that
+// spill in each kernel, and at few tiles a unit's start and end.
 #include "paged_tc.cuh"
 
 namespace wcb {
@@ -46,7 +50,7 @@ struct Tc32Cfg {
   static constexpr int OFFS = RING + SLOTS * SLOT;   // [2][128] row offsets (f16 cache)
   static constexpr int SMEM = OFFS + 2 * 128 * 8 + 1024;
   // registers of a thread by role; together no more than the launch's (two row tiles, f32: softmax 168 and loaders 48 took
-  // 1.15 ms for the 2048 tokens over 16384 keys that take 1.05; 152 and 64 more than either at short units)
+  // a tenth more for 2048 tokens over 16384 keys; 152 and 64 more than either at short units)
   static constexpr int LAUNCH = 65536 / THREADS / 8 * 8;
   static constexpr int R_MMA = 40, R_LOAD = F32C ? (RT == 2 ? 56 : 96) : 80;
   static constexpr int R_SOFT = RT == 2 ? (F32C ? 160 : 192) : 240;
@@ -56,17 +60,21 @@ struct Tc32Cfg {
 constexpr int EXP_RING = 8;  // tiles
 constexpr int UNIT = 2;      // a unit's queries, start and end take about as long as so many tiles of keys
 
+constexpr float WIDE = 1.0f / 65536;  // 8 keys whose numbers are farther apart than this do not share an exponent
+
 struct Tc32Shared : TcShared {
-  // of 8 keys: their numbers are so many times (a power of two) what the tile holds (read four at a time)
+  // of 8 keys: their numbers are so many times (a power of two, of values its exponent too) what the tile holds (read four at a time)
   alignas(16) float kfac[EXP_RING][16];
   alignas(16) float vfac[EXP_RING][16];
+  alignas(16) float vexp[EXP_RING][16];
+  uint32_t apart[HOLE_RING][4];  // keys that the products leave out for that
 };
 
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((max(-126, min(127, e)) + 127) << 23); }
 // the exponent that brings numbers up to `top` below 2^14; `none` where there are only zeros
 __device__ __forceinline__ int group_exp(float top, int none) {
   const int e = int(__float_as_uint(top) >> 23) - 127;  // top in [2^e, 2^(e + 1)); below 2^-126: -127
-  return top > 0.0f ? max(-100, min(120, e - 13)) : none;
+  return top > 0.0f ? max(-126, min(120, e - 13)) : none;
 }
 // (two f32 operations in one instruction)
 __device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
@@ -266,6 +274,8 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
             uint8_t* h = reinterpret_cast<uint8_t*>(sh.holes[tiles % HOLE_RING]);  // by 8 keys
             h[lw] = uint8_t(hb);
             h[8 + lw] = uint8_t(hb >> 8);
+            uint8_t* x = reinterpret_cast<uint8_t*>(sh.apart[tiles % HOLE_RING]);
+            x[lw] = x[8 + lw] = 0;
           } else {
             sh.holes[tiles % HOLE_RING][lw] = hb;
           }
@@ -312,11 +322,24 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
               ok = ok && room(n + kvi);
               if (!ok) break;
             }
-            float top = 0.0f;
+            // the largest number of the 8 keys, and the smallest of the nonzero maxima of 8 numbers each
+            float top = 0.0f, low = INFINITY;
             uint64_t zero = 0;  // NaN where a number is not finite
+            auto largest = [&](int j) {
+              float t = 0.0f;
+#pragma unroll
+              for (int i = j; i < j + 2; ++i)
+                t = fmaxf(fmaxf(t, fmaxf(fabsf(y[i].x), fabsf(y[i].y))), fmaxf(fabsf(y[i].z), fabsf(y[i].w)));
+              return t;
+            };
+#pragma unroll
+            for (int j = 0; j < IT; j += 2) {
+              const float t = largest(j);
+              top = fmaxf(top, t);
+              if (t > 0.0f) low = fminf(low, t);
+            }
 #pragma unroll
             for (int j = 0; j < IT; ++j) {
-              top = fmaxf(fmaxf(top, fmaxf(fabsf(y[j].x), fabsf(y[j].y))), fmaxf(fabsf(y[j].z), fabsf(y[j].w)));
               zero = fma_f32x2(pack_f32x2(y[j].x, y[j].y), 0, zero);
               zero = fma_f32x2(pack_f32x2(y[j].z, y[j].w), 0, zero);
             }
@@ -327,6 +350,7 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
               // infinities and NaN take no part in the exponent; a value's is added to O at the end, to the
               // rows that see it
               top = 0.0f;
+              low = INFINITY;
               bool odd = false;
 #pragma unroll
               for (int j = 0; j < IT; ++j)
@@ -335,6 +359,7 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
                   float& v = (&y[j].x)[e];
                   if (fabsf(v) <= FLT_MAX) {
                     top = fmaxf(top, fabsf(v));
+                    if (v != 0.0f) low = fminf(low, fabsf(v));
                   } else if (kvi) {
                     odd = true;
                     v = 0.0f;
@@ -342,10 +367,28 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
                 }
               if (odd) sh.odd[item % ODD_RING] = 1;
             }
-#pragma unroll
-            for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            const int ge = group_exp(top, kvi ? -126 : 0);  // zeros among values never make the largest exponent
-            if (lane == 0) (kvi ? sh.vfac : sh.kfac)[tiles % EXP_RING][8 * b + lw] = pow2(ge);
+            // (the bits of numbers that are not negative are in their order)
+            top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+            low = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(low)));
+            const int none = kvi ? -126 : 0;  // zeros among values never make the largest exponent
+            const int ge = group_exp(top, none);
+            if (lane == 0) {
+              const int at = 8 * b + lw, r = tiles % EXP_RING;
+              if (kvi) {
+                sh.vfac[r][at] = pow2(ge);
+                sh.vexp[r][at] = float(ge);
+              } else {
+                sh.kfac[r][at] = pow2(ge);
+              }
+              if (low < top * WIDE) {
+                // what is large in one key, seen or not, would take the others' bits: the rows that see
+                // these keys add them by themselves (those without a page are left out already)
+                uint8_t* h = reinterpret_cast<uint8_t*>(sh.holes[tiles % HOLE_RING]) + at;
+                uint8_t* x = reinterpret_cast<uint8_t*>(sh.apart[tiles % HOLE_RING]) + at;
+                *x |= uint8_t(~*h);
+                *h = 0xff;
+              }
+            }
             const uint64_t f = pack_f32x2(pow2(-ge), pow2(-ge));
             uint8_t* dst = sm + L::RING + ((n + kvi) % NS) * L::SLOT;
 #pragma unroll
@@ -536,29 +579,31 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
             const uint32_t sa = ts + 64 * b;
             uint32_t v[2][16];
             tmem_ld16(sa, v[0]);
-            // factors of 8 keys each: of the products, and of P (relative to the half's largest exponent `ref`)
-            float kf[8], vf[8];
-            // never zero, or a masked product's infinity would become NaN
-            auto factor = [&](float f) { return fmaxf(scale * f, 1e-37f); };
-            float ref = 1.0f;
+            // factors of the products: of 8 keys, or of all; never zero, or a masked product's infinity would become NaN
+            float kf[8];
+            auto factor = [&](float f) { return fmaxf(scale * qinv * f, 1e-37f); };
             if constexpr (F32C) {
 #pragma unroll
               for (int q = 0; q < 2; ++q) {
                 const float4 ke = *reinterpret_cast<const float4*>(&sh.kfac[rt % EXP_RING][8 * b + 4 * q]);
-                const float4 ve = *reinterpret_cast<const float4*>(&sh.vfac[rt % EXP_RING][8 * b + 4 * q]);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  kf[4 * q + j] = factor(qinv * (&ke.x)[j]);
-                  vf[4 * q + j] = (&ve.x)[j];
-                }
+                for (int j = 0; j < 4; ++j) kf[4 * q + j] = factor((&ke.x)[j]);
               }
-              ref = max3(max3(vf[0], vf[1], vf[2]), max3(vf[3], vf[4], vf[5]), fmaxf(vf[6], vf[7]));
-              const float inv = __uint_as_float((254u << 23) - __float_as_uint(ref));  // 1 / ref
-#pragma unroll
-              for (int q = 0; q < 8; ++q) vf[q] *= inv;
             } else {
-              kf[0] = factor(qinv);
+              kf[0] = factor(1.0f);
             }
+            auto rescale = [&](float top) {
+              if (__any_sync(0xffffffffu, top > m + SLACK)) {
+                // (a row by itself: not by what its neighbours see). Over an f16 cache a whole number, so that m - lift is exact
+                const float nm = top > m + SLACK ? (F32C ? top : ceilf(top)) : m;
+                const float f = m == nm ? 1.0f : fast_exp2(m - (nm == -INFINITY ? 0.0f : nm));
+#pragma unroll
+                for (int d = 0; d < HD; ++d) o[d] *= f;
+                due *= f;
+                l *= f;
+                m = nm;
+              }
+            };
             // which of the keys this row sees; whether some row of the warp does not see all of them
             uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
             bool mask = false;
@@ -571,8 +616,37 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
                 seen[q] = below1 & ~below0 & ~holes[2 * b + q];
               }
               mask = __any_sync(0xffffffffu, (seen[0] & seen[1]) != 0xffffffffu);
+              if constexpr (F32C) {
+                // keys that the products leave out: q k and p v by ordinary arithmetic, one key after another (rare, and
+                // short code rather than fast)
+                const uint32_t* apart = sh.apart[rt % HOLE_RING];
+#pragma unroll 1
+                for (uint64_t left = uint64_t(apart[2 * b]) | uint64_t(apart[2 * b + 1]) << 32; left; left &= left - 1) {
+                  const int c = __ffsll(static_cast<long long>(left)) - 1;
+                  bool hole;
+                  const long long off = wk.key_offset(a, key0 + c, hole);
+                  if (off < 0) continue;
+                  const CT* kp = static_cast<const CT*>(a.pool.k) + wk.kvh * a.pool.head_stride + off;
+                  const CT* vp = static_cast<const CT*>(a.pool.v) + wk.kvh * a.pool.head_stride + off;
+                  const float* qp = static_cast<const float*>(a.q) + q_at;
+                  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+                  for (int d = 0; d < HD; d += 4)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum[e] = fmaf(__ldg(qp + d + e), to_f32(kp[d + e]), sum[e]);
+                  const float x = c >= lo && c < hi ? ((sum[0] + sum[1]) + (sum[2] + sum[3])) * a.scale_log2 : -INFINITY;
+                  rescale(x);
+                  const float p = fast_exp2(x - (m == -INFINITY ? 0.0f : m));
+                  l += p;
+#pragma unroll
+                  for (int d = 0; d < HD; ++d) {
+                    const float y = to_f32(vp[d]);
+                    o[d] = fmaf(p, fabsf(y) <= FLT_MAX ? y : 0.0f, o[d]);  // (the others are added at the unit's end)
+                  }
+                }
+              }
             }
-            // S is read twice, 16 keys at a time: for the maximum, then for P, whose two parts take the 16 columns' place
+            // S is read twice, 16 keys at a time: for the maxima, then for P, whose two parts take the 16 columns' place
             auto keys = [&](int c, uint32_t (&x)[16]) {  // columns 16 c .. of S, the next ones on their way
               tmem_wait_ld();
               if (mask) {
@@ -581,7 +655,14 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
                   if (!((seen[c >> 1] >> (16 * (c & 1) + e)) & 1)) x[e] = 0xff800000u;  // -infinity
               }
             };
-            float top = -INFINITY;
+            // the largest score, and the largest of a score and its values' exponent, of what the row sees
+            float top = -INFINITY, top_v = -INFINITY;
+            float ve[8];
+            if constexpr (F32C) {
+#pragma unroll
+              for (int q = 0; q < 2; ++q)
+                *reinterpret_cast<float4*>(ve + 4 * q) = *reinterpret_cast<const float4*>(&sh.vexp[rt % EXP_RING][8 * b + 4 * q]);
+            }
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               uint32_t (&x)[16] = v[c & 1];
@@ -591,19 +672,27 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
               for (int q = 0; q < 2; ++q) {
                 const float f = kf[F32C ? 2 * c + q : 0];
                 auto at = [&](int e) { return __uint_as_float(x[8 * q + e]); };
-                top = fmaxf(top, max3(max3(at(0), at(1), at(2)), max3(at(3), at(4), at(5)), fmaxf(at(6), at(7))) * f);
+                const float t = max3(max3(at(0), at(1), at(2)), max3(at(3), at(4), at(5)), fmaxf(at(6), at(7))) * f;
+                top = fmaxf(top, t);
+                if constexpr (F32C) top_v = fmaxf(top_v, t + ve[2 * c + q]);
               }
             }
-            if (__any_sync(0xffffffffu, top > m + SLACK)) {
-              const float nm = top > m + SLACK ? top : m;  // (a row by itself: not by what its neighbours see)
-              const float f = m == nm ? 1.0f : fast_exp2(m - (nm == -INFINITY ? 0.0f : nm));
-#pragma unroll
-              for (int d = 0; d < HD; ++d) o[d] *= f;
-              due *= f;
-              l *= f;
-              m = nm;
-            }
+            rescale(top);
             const float use = m == -INFINITY ? 0.0f : m;
+            // P goes to the products times 2^lift, which brings the row's largest weight (times the size of its values) near
+            // 2^14: two f16 numbers end at 2^-24, 2^-38 of that. Only what the row sees counts, and with its weight.
+            const int lift = 14 - int(fminf(fmaxf(ceilf((F32C ? top_v : top) - use), -112.0f), 140.0f));
+            float vf[8];  // of P
+            if constexpr (F32C) {
+              const float up = pow2(lift);
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                const float4 x = *reinterpret_cast<const float4*>(&sh.vfac[rt % EXP_RING][8 * b + 4 * q]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) vf[4 * q + j] = fminf((&x.x)[j] * up, 0x1p126f);  // (finite, for weights of zero)
+              }
+            }
+            const float from = F32C ? use : use - float(lift);
             uint64_t s2[2] = {0, 0};
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
@@ -615,7 +704,7 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
               for (int e = 0; e < 8; ++e) {
                 const int gq = F32C ? 2 * c + e / 4 : 0;
                 float y0, y1;
-                unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), pack_f32x2(kf[gq], kf[gq]), pack_f32x2(-use, -use)), y0, y1);
+                unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), pack_f32x2(kf[gq], kf[gq]), pack_f32x2(-from, -from)), y0, y1);
                 uint64_t z = pack_f32x2(fast_exp2(y0), fast_exp2(y1));
                 s2[e & 1] = add_f32x2(s2[e & 1], z);
                 if (F32C) z = mul_f32x2(z, pack_f32x2(vf[gq], vf[gq]));
@@ -628,7 +717,7 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
               float x0, y0, x1, y1;
               unpack_f32x2(s2[0], x0, y0);
               unpack_f32x2(s2[1], x1, y1);
-              l += (x0 + y0) + (x1 + y1);
+              l += ((x0 + y0) + (x1 + y1)) * (F32C ? 1.0f : pow2(-lift));
             }
             tmem_wait_st();
             tc_fence_before();
@@ -642,7 +731,7 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
               add_half(1 - b);
               tc_fence_before();
             }
-            due = ref;
+            due = pow2(-lift);
           }
           ++t;
         }
