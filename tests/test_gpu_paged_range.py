@@ -80,7 +80,7 @@ F32 = [("f32", "f32"), ("f32", "bf16"), ("f32", "f16")]
 # many rows (the tensor cores), and few (mma.sync)
 @pytest.mark.parametrize("act,cache", F32)
 @pytest.mark.parametrize("heads,kv_heads,dim,q", [(8, 2, 64, [70, 3]), (8, 8, 128, [70, 3]), (4, 4, 64, [6, 3])])
-@pytest.mark.parametrize("size", [1e3, 1e6, 1e9, 1e30])
+@pytest.mark.parametrize("size", [1e3, 1e6, 1e9, 1e30, "largest"])
 @pytest.mark.parametrize("where", ["k", "v", "kv"])
 def test_large_keys_and_values_that_a_row_does_not_see(gpu, act, cache, heads, kv_heads, dim, q, size, where):
     kv, window = [140, 30], 60

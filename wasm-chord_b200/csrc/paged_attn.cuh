@@ -105,6 +105,14 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) 
   const float l = x - __uint_as_float(hi);
   lo = fabsf(x) <= FLT_MAX ? tf32_of(l) : 0u;
 }
+// The same for a cache's numbers, with hi cut off instead of rounded: 21 bits as well (lo has a bit more to hold), numbers
+// near FLT_MAX do not become infinite, so that a value that is not seen is 0 times a number, and the mask is the
+// cheaper instruction (64 sequences of up to 4191 keys, 64/8 heads of 128, f32 over f32: 470 -> 418 us).
+__device__ __forceinline__ void split_tf32_cut(float x, uint32_t& hi, uint32_t& lo) {
+  hi = __float_as_uint(x) & 0xffffe000u;
+  const float l = x - __uint_as_float(hi);
+  lo = fabsf(x) <= FLT_MAX ? tf32_of(l) : 0u;
+}
 __device__ __forceinline__ float fast_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -654,7 +662,7 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
             uint32_t x[4], h[4], l[4];
             ldsm4(x, ks + uint32_t((k >> 2) * L::PANEL) + (lane_k ^ uint32_t((k & 3) * 32)));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) split_tf32(__uint_as_float(x[j]), h[j], l[j]);
+            for (int j = 0; j < 4; ++j) split_tf32_cut(__uint_as_float(x[j]), h[j], l[j]);
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
               const uint4 q = qfrag[(nb * (HD / 8) + k) * 32 + lane];
@@ -815,7 +823,7 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
               uint32_t h[4], l[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e)  // (dim g, key t), (dim g + 8, key t), (.., key t + 4)
-                split_tf32(ldsf(vs + elem_at(kw0 + 8 * j + t + 4 * (e >> 1), 16 * mb + g + 8 * (e & 1))), h[e], l[e]);
+                split_tf32_cut(ldsf(vs + elem_at(kw0 + 8 * j + t + 4 * (e >> 1), 16 * mb + g + 8 * (e & 1))), h[e], l[e]);
 #pragma unroll
               for (int nb = 0; nb < NB; ++nb) {
                 mma8(x[nb], l, ph[j][nb][0], ph[j][nb][1]);
