@@ -169,3 +169,25 @@ def test_each_low_part_counts(gpu, act, cache, heads, kv_heads, dim, q, part):
         s.v[..., :dim // 2] *= torch.where(s.k.float().sum(-1, keepdim=True) > 0, 1.0, -1.0)
     s.attend(scale=0.31)
     check(s, scale=0.31)
+
+
+@pytest.mark.parametrize("act,cache", paged.PAIRS)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 64), (4, 4, 128)])
+@pytest.mark.parametrize("late", [[70], [130, 190], [400, 401, 520, 700, 701]])
+def test_maxima_that_move_late_and_for_some_rows(gpu, act, cache, heads, kv_heads, dim, late):
+    """Keys that lie far above all before them, for every third row only: those rows' weights are made again, the others' of the
+    same warp are not."""
+    s = paged.Step([100], [900], heads, kv_heads, dim, act, cache, 16, seed=56)
+    base = torch.randn(dim, generator=torch.Generator().manual_seed(2)).cuda()
+    base /= base.norm()
+    q = s.q[:, :heads * dim].view(-1, heads, dim)
+    q[::3] += (3 * base).to(s.at)
+    for n, j in enumerate(late):
+        put(s, 0, j, (base * (6 + 5 * n) * math.sqrt(dim)).to(s.ct))
+    room = s.attend()
+    s.check()
+    first = s.out.clone()
+    for _ in range(3):
+        s.out.fill_(7.0)
+        s.attend(room=room)
+        assert torch.equal(first, s.out)

@@ -437,6 +437,7 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
                 l *= f;
                 m = nm;
               }
+              tmem_wait_st();  // the first P lies in the same columns: two stores have no order of their own
               exponentials();
               part = total();
             }
