@@ -191,3 +191,28 @@ def test_maxima_that_move_late_and_for_some_rows(gpu, act, cache, heads, kv_head
         s.out.fill_(7.0)
         s.attend(room=room)
         assert torch.equal(first, s.out)
+
+
+# so many sequences that most are one CTA's from the first key to the last (a part without the first key has a maximum of its own)
+@pytest.mark.parametrize("act", ["f16", "bf16"])
+@pytest.mark.parametrize("n,heads,kv_heads,dim,q,kv", [(12, 16, 16, 64, 40, 1500), (12, 16, 16, 128, 40, 1500), (40, 16, 16, 64, 1, 600), (40, 16, 16, 128, 1, 600),
+                                                       (40, 32, 16, 64, 6, 600), (40, 32, 16, 64, 14, 600)])
+@pytest.mark.parametrize("gap", [14.0, 17.7, 18.5])
+def test_small_weights_beside_a_large_one(gpu, act, n, heads, kv_heads, dim, q, kv, gap):
+    """A first key `gap` nats above the others (17.7: 2^-25.5), with a value of zero: the others are the whole output, and the
+    sum that divides it counts them. Bound: P rounds to half a step of its type, and in f16 ends at 2^-24, which is 2^-31 of the
+    largest weight: half of that a key; the scores as for f32 (their products are exact in 32 bits); one rounding."""
+    s = paged.Step([q] * n, [kv] * n, heads, kv_heads, dim, act, act, 64, seed=57)
+    s.q[:, :heads * dim] = (s.q[:, :heads * dim].view(-1, heads, dim) * 0.05 + 1.0).view(s.tokens, -1)
+    s.k *= 0.1
+    s.v.copy_(1000.0 + 100.0 * s.v.float())
+    for i in range(n):
+        put(s, i, 0, gap / math.sqrt(dim), 0.0)
+    s.attend()
+    out, tol, lse, ltol = exact(s)
+    e, t = paged.half_step(s.at), n * q
+    got = s.out[:t, :heads * dim].double().cpu().view(t, heads, dim)
+    # (the values lie between 400 and 1600, so that o is also the sum of p |v|; the largest weight is at most 1)
+    bound = out[:t] * 2.02 * e + tol[:t, :, None] + (kv * 2.0 ** -32 * 1600 + 2.0 ** -25 if act == "f16" else 0)
+    assert ((got - out[:t]).abs() <= bound).all(), ((got - out[:t]).abs() / bound).max()
+    assert ((s.lse.double().cpu()[:t] - lse[:t]).abs() <= ltol[:t]).all()

@@ -21,7 +21,8 @@
 // mma and the few rows of a decode step its 8 columns (8 rows a key head at most need
 // half the products, registers and exponentials of the other way round). The 4 warps share
 // a tile's keys, each with its own m, l and O, joined at a unit's end. m moves only where some
-// score passes it by 2^8 (sums in f32 and P have room for that), by one vote a tile.
+// score passes it by 2^8 (sums in f32 and P have room for that; 2^15 where P is f16, and m then lies 2^7 below the
+// largest score), by one vote a tile.
 //
 // Tile: K and V
 // arrive in rows of 128-byte panels, swizzled, through STAGES buffers: whole tiles by
@@ -370,6 +371,11 @@ __device__ __forceinline__ int quotient(long long x, long long y) {
 // ---- the kernel -------------------------------------------------------------
 
 constexpr float SLACK = 8.0f;  // how far (in powers of two) a score may pass the maximum before it moves
+// What O and l are scaled by lies below the maximum by so much where P is held in f16, which ends at 2^-24: weights down
+// to 2^-31 of the largest count (2^-24 dropped 1.8e-3 of the weight at 60000 keys 2^-25 below one key, and l counted it).
+// P stays below 2^15. bf16 and tf32 have f32's exponents and need none.
+template <typename T>
+constexpr float LIFT = std::is_same<T, __half>::value ? 7.0f : 0.0f;
 
 template <typename AT, typename CT, int HD, int NB>
 struct AttnCfg {
@@ -692,7 +698,7 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
             if (!seen) v = -INFINITY;
           }
           sc[nb][e] = v;
-          grow |= v > mx[nb][e & 1] + SLACK;
+          grow |= v > mx[nb][e & 1] + (SLACK + LIFT<AT>);
         }
       }
       const bool moved = __any_sync(0xffffffffu, grow);
@@ -702,7 +708,7 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            float top = fmaxf(mx[nb][h], fmaxf(sc[nb][h], sc[nb][h + 2]));
+            float top = fmaxf(mx[nb][h], fmaxf(sc[nb][h], sc[nb][h + 2]) - LIFT<AT>);
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
             fac[nb][h] = mx[nb][h] == top ? 1.0f : fast_exp2(mx[nb][h] - top);

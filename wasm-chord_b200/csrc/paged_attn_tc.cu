@@ -38,6 +38,12 @@ namespace {
 
 constexpr int TC_THREADS = 448;  // 2 softmax warpgroups, 4 loader warps, 2 issuing warps
 constexpr int TC_M = 256;
+// A half's sum of exponentials may grow to this before the maximum is taken anew, and m then lies so many powers of two below
+// it. f16: sums of P up to 2^15, and weights down to 2^-32 of the largest count (P in f16 ends at 2^-24); bf16 has f32's range.
+template <typename T>
+constexpr float GROWTH = std::is_same<T, __half>::value ? 32768.0f : 8192.0f;
+template <typename T>
+constexpr float BELOW = std::is_same<T, __half>::value ? 8.0f : 0.0f;
 constexpr int UNIT = 3;  // a unit's queries, start and end take about as long as so many tiles of keys
 
 template <int HD>
@@ -392,14 +398,14 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
               return (x0 + y0) + (x1 + y1);
             };
             // Most halves need no maximum: the last one still serves as long as the sum shows that no
-            // exponential left the range of f16 and of a sound sum (GROWTH); a row's sum is wanted anyway.
+            // exponential left the range of f16 and of a sound sum; a row's sum is wanted anyway.
             // A row decides by its own sum alone, so that its result does not depend on what its neighbours see.
             float part = 0.0f;
             bool moves = m == -INFINITY;
             if (!__all_sync(0xffffffffu, moves)) {
               exponentials();
               part = total();
-              moves = moves || !(part <= GROWTH);
+              moves = moves || !(part <= GROWTH<T>);
             }
             const bool again = __any_sync(0xffffffffu, moves);
             if (again) {
@@ -417,7 +423,7 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
                 for (int e = 0; e < 64; ++e) x = fminf(x, __uint_as_float(v[e]));
                 top = x * a.scale_log2;
               }
-              const float nm = moves ? fmaxf(m, top) : m;
+              const float nm = moves ? fmaxf(m, top - BELOW<T>) : m;
               if (__any_sync(0xffffffffu, nm > m)) {
                 const float f = m == nm ? 1.0f : fast_exp2(m - (nm == -INFINITY ? 0.0f : nm));
                 if (i > wk.ta || b) {  // after the last product

@@ -10,7 +10,6 @@ namespace {
 
 constexpr int TC_TK = 128;
 constexpr int TILE_PANEL = 128 * 128;  // bytes of 128 rows x 64 dims
-constexpr float GROWTH = 8192.0f;  // a half's sum of exponentials may grow to this before the maximum is taken anew
 constexpr int HOLE_RING = 8;   // tiles: the loaders are at most 4 ahead of the softmax
 constexpr int ODD_RING = 16;   // units, likewise
 
