@@ -6,6 +6,7 @@
 #include <climits>
 #include <cmath>
 #include <cstdint>
+#include <cstdlib>
 #include <string>
 
 #include "../../include/wcb.h"
@@ -249,6 +250,10 @@ uint32_t wcb_paged_attention_dev(const wcb_paged_kv* kv, const wcb_paged_batch* 
   a.window = int(window);
   a.tickets = static_cast<int*>(workspace);
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + TICKET_BYTES);
+  // test hook for the bounded waits (unset in normal use, read once): tiles wait for bytes that do not come
+  static const bool withhold = std::getenv("WCB_TEST_WITHHOLD_COPY") != nullptr;
+  a.withheld = withhold ? 16 : 0;
+  a.wait_ns = withhold ? 20000000ull : 2000000000ull;
   const Plan p = plan(batch->n_seqs, kv->n_kv_heads, uint64_t(batch->max_q_len) * uint64_t(a.rep));
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;

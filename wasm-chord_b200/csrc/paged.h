@@ -54,6 +54,8 @@ struct AttendArgs {
   int row_lo, row_hi;  // sequences with row_lo < rows (new tokens * rep) <= row_hi are this launch's
   int* tickets;      // one per CTA, zero between calls
   float* part;       // partial results, two pieces per CTA
+  uint64_t wait_ns;  // a wait for a copy or a product ends after so long
+  uint32_t withheld; // bytes that a tile by TMA waits for and that do not come (test hook; 0)
 };
 
 struct VerifyArgs {

@@ -120,6 +120,30 @@ __device__ __forceinline__ float fast_exp2(float x) {
   return y;
 }
 
+// Bounded wait for one phase of an mbarrier: until so many ns have passed (or 2^24 polls), or until `gone`, where there is
+// one, says that another thread has given up.
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, uint64_t ns, const volatile int* gone = nullptr) {
+  const uint32_t addr = smem_u32(bar);
+  uint64_t start = 0;
+  for (uint32_t it = 0; it < (1u << 24); ++it) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((it & 63) == 63) {
+      uint64_t now;
+      asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
+      if (start == 0) start = now;
+      if (now - start > ns || (gone && *gone)) return false;
+    }
+  }
+  return false;
+}
+constexpr uint64_t DRAIN_NS = 10000000;  // for copies and products still on their way when a CTA gives up
+
 // an 8 x 8 block of 16-bit values, a row (2t, 2t + 1) in lane 4 g + t, transposed
 __device__ __forceinline__ uint32_t transposed8(uint32_t x) {
   uint32_t y;
@@ -421,6 +445,7 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
   __shared__ PlaceShared<AT_THREADS> s_place;
   __shared__ int s_last;
   __shared__ uint64_t s_full[S];  // a stage's bytes are there (tiles by TMA)
+  __shared__ int s_late[2];       // a tile did not come
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
@@ -430,10 +455,10 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
   if (pl.begin >= pl.end) return;
   if (tid == 0) {
     for (int i = 0; i < S; ++i) mbar_init(&s_full[i], 1);
+    s_late[0] = s_late[1] = 0;
     mbar_fence_init();
   }
   uint32_t phase = 0;  // bit i: of s_full[i]
-  bool landed = true;
 
   // byte offset of 16-byte chunk c of row r in a stage's K or V; elements by row and dim
   auto chunk_at = [](int r, int c) { return uint32_t((c >> 3) * L::PANEL + r * 128 + (((c & 7) ^ (r & 7)) << 4)); };
@@ -517,7 +542,7 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
       const uint32_t dst = sbase + uint32_t((i % S) * L::STAGE);
       const long long* ro = offs + (i % (S + 1)) * TK;
       if (whole_tile(i)) {
-        if (tid == 0) mbar_expect_tx(&s_full[i % S], L::STAGE);
+        if (tid == 0) mbar_expect_tx(&s_full[i % S], L::STAGE + a.withheld);
         if (tid < TK && tid % box == 0) {
           const long long page = ro[tid];
           const int at_page = page < 0 ? a.pool.n_pages : int(page);  // a page that is not there: past the last one, zeros
@@ -606,13 +631,13 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
     bool hole_seen = false;
     for (int i = ta; i < tb; ++i) {
       if (whole_tile(i)) {
-        landed &= mbar_wait(&s_full[i % S], (phase >> (i % S)) & 1);
-        phase ^= 1u << (i % S);
+        if (!bar_wait(&s_full[i % S], (phase >> (i % S)) & 1, a.wait_ns)) s_late[i & 1] = 1;
       } else {
         cp_wait<S - 2>();
         fence_proxy_async();  // the stage may be TMA's next
       }
       __syncthreads();
+      const bool late = s_late[i & 1] != 0;  // (the next tile's flag is another, so that every thread reads the same)
       // offs of tile i + S - 1 were written before this barrier; its stage was read before it
       if (i + S - 1 < tb) request(i + S - 1);
       cp_commit();
@@ -763,6 +788,16 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
         }
       }
 
+      if (late) {
+        // give up, once the copies on their way have landed: those of this tile and of the ones requested after it
+        for (int j = i; j < tb && j < i + S; ++j)
+          if (whole_tile(j)) bar_wait(&s_full[j % S], (phase >> (j % S)) & 1, DRAIN_NS);
+        cp_wait<0>();
+        if (tid == 0) report(a.batch, ST_ABORTED);
+        return;
+      }
+      if (whole_tile(i)) phase ^= 1u << (i % S);
+
       // O^T += V^T P^T
       if constexpr (!F32A) {
         uint32_t ph[NB][2], pw[NB][2];  // keys 2t, 2t + 1 (and + 8) of row g: S^T's blocks transposed
@@ -846,7 +881,6 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
       }
     }
     cp_wait<0>();
-    if (!landed) report(a.batch, ST_ABORTED);
     if (hole_seen && tid == 0) report(a.batch, ST_BAD_PAGE);
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)

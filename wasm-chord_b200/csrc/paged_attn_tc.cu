@@ -92,7 +92,9 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
       mbar_init(&sh.last_full[w], 1);
     }
     mbar_init(&sh.offs_full, 128);
+    for (int w = 0; w < 2; ++w) mbar_init(&sh.drained[w], 1);
     sh.abort = 0;
+    sh.wait_ns = a.wait_ns;
     mbar_fence_init();
   }
   if (tid < ODD_RING) sh.odd[tid] = 0;
@@ -195,12 +197,17 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
           }
         }
       } while (ok && wk.next(a));
+      // the memory of S, P and O is given back after the last product, whether or not the roles came to their ends
+      if (one) tc_commit(&sh.drained[w]);
+      __syncwarp();
+      bar_wait(&sh.drained[w], 0, DRAIN_NS);
     }
   } else if (warp >= 8) {
     // ---- loaders --------------------------------------------------------------
     const int lt = tid - 256;
     long long* offs = reinterpret_cast<long long*>(sm + L::OFFS);
     uint32_t n = 0, tiles = 0, item = 0, by_copy = 0;
+    uint32_t issued = 0;  // ring tiles up to the last that came by TMA
     bool ok = true, holes_seen = false;
     // the page of this thread's key of tile i; -1: none
     auto page_of = [&](int i) {
@@ -233,8 +240,9 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
             ok = room(n + kvi);
             if (!ok) break;
             uint64_t* bar = &sh.full[(n + kvi) % NS];
+            issued = n + kvi + 1;
             if (lane == 0) {  // warp 8's arrival brings the bytes to wait for
-              if (warp == 8) mbar_expect_tx(bar, L::TILE);
+              if (warp == 8) mbar_expect_tx(bar, L::TILE + a.withheld);
               else bar_arrive(bar);
             }
             if (lt % box == 0) {
@@ -298,6 +306,8 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
       ++item;
     } while (ok && wk.next(a));
     cp_wait<0>();
+    // nor does the CTA leave before its boxes have landed: those of the last tiles, if a role gave up
+    for (uint32_t m = n > NS ? n - NS : 0; m < issued; ++m) bar_wait(&sh.full[m % NS], (m / NS) & 1, DRAIN_NS);
     if (holes_seen && lane == 0) report(a.batch, ST_BAD_PAGE);
   } else {
     // ---- softmax of row tile w: thread = row ----------------------------------
@@ -593,6 +603,8 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
       tiles += uint32_t(wk.tb - wk.ta);
       ++item;
     } while (ok && wk.next(a));
+    tmem_wait_ld();
+    tmem_wait_st();
   }
   tc_fence_before();
   __syncthreads();

@@ -128,7 +128,9 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
       mbar_init(&sh.last_full[w], 1);
     }
     mbar_init(&sh.offs_full, 128);
+    for (int w = 0; w < RT; ++w) mbar_init(&sh.drained[w], 1);
     sh.abort = 0;
+    sh.wait_ns = a.wait_ns;
     mbar_fence_init();
   }
   if (tid < ODD_RING) sh.odd[tid] = 0;
@@ -240,6 +242,10 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
           }
         }
       } while (ok && wk.next(a));
+      // the memory of S, P and O is given back after the last product, whether or not the roles came to their ends
+      if (one) tc_commit(&sh.drained[w]);
+      __syncwarp();
+      bar_wait(&sh.drained[w], 0, DRAIN_NS);
     }
   } else if (warp >= 4 * RT) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::R_LOAD));
@@ -247,6 +253,7 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
     const int lt = tid - 128 * RT, lw = warp - 4 * RT;
     long long* offs = reinterpret_cast<long long*>(sm + L::OFFS);
     uint32_t n = 0, tiles = 0, item = 0, by_copy = 0;
+    uint32_t issued = 0;  // ring tiles up to the last that came by TMA
     bool ok = true, holes_seen = false;
     // this thread's key of a tile. f32: 8 keys of each half are one warp's (lanes 0 .. 7, 8 .. 15; the others have none)
     const int my_key = F32C ? 64 * ((lane >> 3) & 1) + 8 * lw + (lane & 7) : lt;
@@ -422,8 +429,9 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
               ok = room(n + kvi);
               if (!ok) break;
               uint64_t* bar = &sh.full[(n + kvi) % NS];
+              issued = n + kvi + 1;
               if (lane == 0) {  // the first warp's arrival brings the bytes to wait for
-                if (lw == 0) mbar_expect_tx(bar, L::SLOT);
+                if (lw == 0) mbar_expect_tx(bar, L::SLOT + a.withheld);
                 else bar_arrive(bar);
               }
               if (lt % box == 0) {
@@ -488,6 +496,8 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
       ++item;
     } while (ok && wk.next(a));
     cp_wait<0>();
+    // nor does the CTA leave before its boxes have landed: those of the last tiles, if a role gave up
+    for (uint32_t m = n > NS ? n - NS : 0; m < issued; ++m) bar_wait(&sh.full[m % NS], (m / NS) & 1, DRAIN_NS);
     if (holes_seen && lane == 0) report(a.batch, ST_BAD_PAGE);
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::R_SOFT));
@@ -844,6 +854,8 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
       tiles += uint32_t(wk.tb - wk.ta);
       ++item;
     } while (ok && wk.next(a));
+    tmem_wait_ld();
+    tmem_wait_st();
   }
   tc_fence_before();
   __syncthreads();

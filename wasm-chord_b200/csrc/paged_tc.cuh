@@ -114,6 +114,8 @@ struct TcShared {
   uint64_t full[8], empty[8];  // ring slots
   uint64_t q_full[2], s_full[2][2], p_full[2][2], o_done[2][2];  // [row tile][half of the keys]
   uint64_t offs_full, piece_full[2], last_full[2];
+  uint64_t drained[2];           // all products of a row tile are done
+  uint64_t wait_ns;
   uint32_t tmem;
   int abort;                     // a wait ran out: everybody leaves
   uint32_t holes[HOLE_RING][4];  // keys of a tile without a page
@@ -121,19 +123,9 @@ struct TcShared {
   int last[2];
 };
 
-// Bounded wait: about 2^24 polls, or until another thread has given up.
+// A role's wait; one that gives up takes the others with it.
 __device__ __forceinline__ bool tc_wait(TcShared* sh, uint64_t* bar, uint32_t parity) {
-  const uint32_t addr = smem_u32(bar);
-  for (uint32_t it = 0; it < (1u << 24); ++it) {
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(ok)
-        : "r"(addr), "r"(parity)
-        : "memory");
-    if (ok) return true;
-    if ((it & 63) == 63 && *reinterpret_cast<volatile int*>(&sh->abort)) return false;
-  }
+  if (bar_wait(bar, parity, sh->wait_ns, &sh->abort)) return true;
   *reinterpret_cast<volatile int*>(&sh->abort) = 1;
   return false;
 }
