@@ -868,13 +868,16 @@ template <typename CT, int HD>
 cudaError_t run_tc32(const AttendArgs& a, cudaStream_t s) {
   using L = Tc32Cfg<CT, HD>;
   static_assert(L::SMEM + sizeof(Tc32Shared) + sizeof(PlaceShared<L::THREADS>) <= 227 * 1024, "shared memory");
-  // the register split draws on what the kernel is launched with
-  static const bool fits = [] {
+  // the register split draws on what the kernel is launched with (looked up until it is known: a call that fails, for want
+  // of a device for instance, says why and leaves nothing behind)
+  static std::atomic<int> regs{0};
+  if (regs.load(std::memory_order_relaxed) == 0) {
     cudaFuncAttributes at;
-    return cudaFuncGetAttributes(&at, attend_tc32_kernel<CT, HD>) == cudaSuccess &&
-           L::WGS * at.numRegs >= L::RT * L::R_SOFT + L::LW / 4 * L::R_LOAD + L::R_MMA;
-  }();
-  if (!fits) return cudaErrorInvalidKernelImage;
+    const cudaError_t found = cudaFuncGetAttributes(&at, attend_tc32_kernel<CT, HD>);
+    if (found != cudaSuccess) return found;
+    regs.store(at.numRegs, std::memory_order_relaxed);
+  }
+  if (L::WGS * regs.load(std::memory_order_relaxed) < L::RT * L::R_SOFT + L::LW / 4 * L::R_LOAD + L::R_MMA) return cudaErrorInvalidKernelImage;
   static std::atomic<uint64_t> done{0};
   const cudaError_t e = allow_shared(attend_tc32_kernel<CT, HD>, L::SMEM, done);
   if (e != cudaSuccess) return e;
