@@ -234,3 +234,19 @@ def test_small_weights_beside_a_large_one_f32(gpu, cache, n, heads, kv_heads, di
         put(s, i, 0, gap / math.sqrt(dim), 0.0)
     s.attend()
     check(s, more=64 * 2.0 ** -37 * 1600 * math.sqrt(dim))
+
+
+@pytest.mark.parametrize("act", ["f32", "f16"])
+@pytest.mark.parametrize("n,q,window", [(1, 1, 63), (4, 40, 88), (1, 100, 28), (1, 3, 61), (1, 1, 1), (1, 1, 1 << 30)])
+def test_the_longest_sequence_past_its_table(gpu, act, n, q, window):
+    """kv_len of 2^31 - 1 with a window that begins where the table has ended (at 2^30 keys): no key is there, so zeros and
+    -infinity, whatever the places' last bits."""
+    s = paged.Step([q] * n, [q] * n, 8, 2, 64, act, "f16", 16, seed=59)
+    s.dev[1].fill_(2 ** 31 - 1)
+    s.kv = wcb.PagedKV(s.k.data_ptr(), s.v.data_ptr(), wcb.KV_F16, 1, 1 << 30, 2, 64, 0, 0, 0)
+    table = torch.zeros(n, 1, dtype=torch.int32, device="cuda") - 1  # were a key looked up, it would have no page
+    s.batch = wcb.PagedBatch(s.dev[0].data_ptr(), s.dev[1].data_ptr(), table.data_ptr(), n, s.tokens, q, 1, s.status.data_ptr())
+    s.attend(window=window)
+    assert int(s.status.item()) == wcb.PAGED_BAD_PAGE
+    assert (s.out[:n * q] == 0).all() and (s.lse[:n * q] == -math.inf).all()
+    assert (s.out[n * q:] == 7).all() and (s.lse[n * q:] == 7).all()

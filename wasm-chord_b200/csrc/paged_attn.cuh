@@ -237,7 +237,7 @@ __device__ __forceinline__ Block row_block(const AttendArgs& a, const Seq& q, in
   b.pos0 = q.kv - q.n + token_of(a, r0);
   b.pos1 = q.kv - q.n + token_of(a, r1 - 1);
   b.hi = min(b.pos1 + 1, table);
-  b.lo = a.window > 0 ? max(0, b.pos0 - a.window + 1) : 0;
+  b.lo = a.window > 0 ? min(max(0, b.pos0 - a.window + 1), max(0, b.hi)) : 0;  // (no tile past the table: its end counts in 32 bits)
   b.tile0 = b.lo / TK;
   // rows that see nothing still have their zeros written
   b.tiles = b.hi > b.lo ? (b.hi + TK - 1) / TK - b.tile0 : 1;
