@@ -250,3 +250,22 @@ def test_the_longest_sequence_past_its_table(gpu, act, n, q, window):
     assert int(s.status.item()) == wcb.PAGED_BAD_PAGE
     assert (s.out[:n * q] == 0).all() and (s.lse[:n * q] == -math.inf).all()
     assert (s.out[n * q:] == 7).all() and (s.lse[n * q:] == 7).all()
+
+
+@pytest.mark.parametrize("act,cache", paged.PAIRS)
+@pytest.mark.parametrize("q", [100, 2])
+@pytest.mark.parametrize("far", [1e4, 1e6, 3e7, -3e7])
+def test_scores_far_from_zero(gpu, act, cache, q, far):
+    """Scores of one size, far from zero and all equal: plain means of the values, and every row of the same one."""
+    s = paged.Step([q], [700], 8, 2, 64, act, cache, 16, seed=60)
+    s.q[:, :512] = 1.0
+    s.k[:] = 1.0
+    s.v.copy_(torch.where(s.v.float() < 0, 1.0, 3.0))
+    scale = far / 64
+    s.attend(scale=scale)
+    got = s.out[:q, :512].double().cpu().view(q, 8, 64)
+    vt = s.by_token(s.v.double().cpu())[s.slots(0)].repeat_interleave(4, 1)
+    for r in range(0, q, 7):
+        want = vt[:700 - q + r + 1].mean(0)
+        # equal weights: sums of 1 and 3 are exact, so the quotient's rounding (2^-22) and the output's are left
+        assert ((got[r] - want).abs() <= 3 * (paged.half_step(s.at) + 2.0 ** -22)).all(), r

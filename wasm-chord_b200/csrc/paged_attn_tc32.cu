@@ -691,7 +691,8 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
             const float use = m == -INFINITY ? 0.0f : m;
             // P goes to the products times 2^lift, which brings the row's largest weight (times the size of its values) near
             // 2^14: two f16 numbers end at 2^-24, 2^-38 of that. Only what the row sees counts, and with its weight.
-            const int lift = 14 - int(fminf(fmaxf(ceilf((F32C ? top_v : top) - use), -112.0f), 140.0f));
+            int lift = 14 - int(fminf(fmaxf(ceilf((F32C ? top_v : top) - use), -112.0f), 140.0f));
+            if (!F32C && fabsf(use) > 8388608.0f) lift = 0;  // (scores that are whole numbers at best)
             float vf[8];  // of P
             if constexpr (F32C) {
               const float up = pow2(lift);
@@ -702,7 +703,7 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
                 for (int j = 0; j < 4; ++j) vf[4 * q + j] = fminf((&x.x)[j] * up, 0x1p126f);  // (finite, for weights of zero)
               }
             }
-            const float from = F32C ? use : use - float(lift);
+            const float from = F32C ? use : use - float(lift);  // (exact: whole numbers below 2^24)
             uint64_t s2[2] = {0, 0};
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
