@@ -345,8 +345,8 @@ uint32_t wcb_attention_dev_noalloc(const float* q, const float* k_cache, const f
 
 /* A pool of pages. Key (and value) of head h of the token in slot t of page p
  * starts at element p * page_stride + t * token_stride + h * head_stride of k
- * (and v); head_dim elements follow. A model's contiguous cache
- * [slot][n_kv_heads][max_seq][head_dim] is the pool with page_size = max_seq.
+ * (and v); head_dim elements follow. A contiguous cache [slot][n_kv_heads][max_seq][head_dim]
+ * (wcb_attention_dev's, for one slot) is the pool with page_size = max_seq.
  * Strides in elements, multiples of 16 bytes; k and v 16-byte aligned. All
  * strides 0: [page][slot][head][head_dim] without gaps. */
 typedef struct wcb_paged_kv {
@@ -385,7 +385,8 @@ typedef struct wcb_paged_batch {
 /* Status bits. BAD_PAGE: a page id outside the pool, or a position outside the
  * page table's row (the token is not stored, the key takes no part in the
  * attention). BAD_ROWS: q_start outside 0 .. n_tokens or descending (the
- * sequence is skipped). BAD_LEN: a new token's position is negative (not
+ * sequence is skipped; rows that others of such a batch share hold the results of one of them, or a
+ * mixture). BAD_LEN: a new token's position is negative (not
  * stored; its attention output is zero). BAD_TOKEN: a drafted token outside the
  * vocabulary (turned down). BAD_PROBS: a row of target probabilities without
  * a positive finite value (the sampled token is -1). ABORTED: a wait inside a
@@ -441,7 +442,9 @@ uint32_t wcb_paged_attention_workspace(const wcb_paged_kv* kv, const wcb_paged_b
 /* compute_attention (attention.rs:332-435) over pages: for each new token at
  * position p of its sequence, softmax(scale * q . k_j) v_j over the keys j <= p,
  * and j > p - window where window > 0 (at most 2^30); n_heads / n_kv_heads query heads share
- * a key head (any whole ratio up to 64). q and out: [n_tokens][n_heads][head_dim]
+ * a key head (any whole ratio up to 64). Scores and sums are kept in 32 bits; with 16-bit activations the weights are
+ * rounded once to their type before they multiply the values (not for up to 8 rows a key head), with F32 ones they, the
+ * queries, keys and values keep 21 bits or more (of the largest of 8 neighbouring numbers). q and out: [n_tokens][n_heads][head_dim]
  * with their strides between tokens (elements, multiples of 16 bytes), types as
  * for wcb_paged_append_dev. scale 0: 1 / sqrt(head_dim). lse (device f32
  * [n_tokens][n_heads], or NULL): the natural logarithm of the softmax's sum,

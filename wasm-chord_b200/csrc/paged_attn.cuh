@@ -222,7 +222,8 @@ int make_maps(CUtensorMap* k, CUtensorMap* v, const Pool& p, int TK) {
 
 // ---- the line of tiles ------------------------------------------------------
 
-// row / rep and row % rep, exact for rows below 2^33 (2^40 / rep + 1 is too large by at most rep <= 64 parts in 2^40)
+// row / rep and row % rep: rep_inv is above 2^40 / rep by at most 1, which is exact as long as the product fits in 64 bits,
+// up to 2^24 tokens (the most a call takes)
 __device__ __forceinline__ int token_of(const AttendArgs& a, int row) { return int((uint64_t(uint32_t(row)) * a.rep_inv) >> 40); }
 __device__ __forceinline__ int head_of(const AttendArgs& a, int row) { return row - token_of(a, row) * a.rep; }
 

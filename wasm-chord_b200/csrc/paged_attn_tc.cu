@@ -23,13 +23,15 @@
 // room for the factor): one vote on the sum instead of 64 comparisons a row.
 // TMEM: S0 | S1 | O0 | O1, 512 columns at head_dim 128.
 //
-// 2047 new tokens over 32767 keys, 64/8 heads of 128, bf16: 1.96 ms run after run, 2.3 ms with
-// pauses in between, 1090 and 925 TFLOP/s (65 and 55 % of the measured cuBLAS rate). What bounds it: the
-// exponentials of the two softmax warps of a scheduler and what surrounds them (1250 clocks a
-// half with both row tiles; without the exponentials themselves 600, and the products' 2560
-// clocks become the bound). Part of the exponentials by a polynomial on the multiply-add units
-// (a quarter, an eighth) gained nothing: those pay as many clocks for it. Short units: 11
+// 2047 new tokens over 32767 keys, 64/8 heads of 128, bf16: 2.3 ms with new inputs from call to call, 925 TFLOP/s (55 % of
+// the measured cuBLAS rate); 1.98 ms at best, run after run. What bounds it: the
+// chain within a half, S to registers, exponentials, P back, products, none of which is near its limit by itself (tensor
+// pipe 47 %, exponentials 49 %, issue 36 % busy): 1250 clocks a half with both row tiles; without the
+// exponentials 600, and the products' 2560 clocks become the bound. Part of the exponentials by a polynomial on the
+// multiply-add units (a quarter, an eighth) gained nothing. About 120 bytes of registers spill. Short units: 11
 // sequences of 204 tokens 72 us (82 with units that are cut in two for one tile).
+// P is rounded once to the 16-bit type: kept in two parts, as for few rows, P V would be two products, and a bf16 output would
+// still be off by its own rounding (relative error 1.7e-3 in place of 2.3e-3 at the size above).
 #include "paged_tc.cuh"
 
 namespace wcb {

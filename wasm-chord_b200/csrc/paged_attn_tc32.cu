@@ -22,10 +22,10 @@
 // the tile is whole. head_dim 64: two row tiles of 128 rows; 128: one (Q in two parts and a
 // ring of K and V in two parts fill the shared memory).
 //
-// 46 sequences of 919 tokens, 32/4 heads of 64, f32 cache: 1.16 ms, 137 TFLOP/s of the formula's
-// products, 412 of those made (25 % of the measured cuBLAS rate); one of 2048 tokens over 16384 keys
-// 1.08 ms, 243 and 720 TFLOP/s (43 %). The rows' own exponents of P and the search for keys that are far apart are 2 to
-// 5 % of that (an exponent for each key instead, read by a second way through the softmax: 10 %). What bounds it: the
+// 46 sequences of 919 tokens, 32/4 heads of 64, f32 cache: 1.17 ms, 136 TFLOP/s of the formula's
+// products, 408 of those made (24 % of the measured cuBLAS rate); one of 2048 tokens over 16384 keys
+// 1.09 ms, 241 and 713 TFLOP/s (43 %). The rows' own exponents of P and the search for keys that are far apart are 2 to
+// 6 % of that (an exponent for each key instead, read by a second way through the softmax: 10 %). What bounds it: the
 // instructions of the splitting, in the softmax (P) and in the loaders (K and V), about 500 bytes of registers that
 // spill in each kernel, and at few tiles a unit's start and end.
 #include "paged_tc.cuh"

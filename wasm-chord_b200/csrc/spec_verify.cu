@@ -3,16 +3,16 @@
 // Token i is accepted while u_i q(x_i) < p(x_i) (the product of two 24-bit
 // numbers is exact in 64 bits). At the first token turned down the next one is
 // drawn from r_j = max(p_j - q_j, 0), after the last accepted one from p: the
-// lowest j with r_0 + .. + r_j > u S. One or two rows of vocab floats of each
-// sequence are read once: memory bound for large batches, latency bound for
-// one sequence. A cluster of C CTAs shares one sequence's row in C slices: each
+// lowest j with r_0 + .. + r_j > u S. The target's row of each sequence is read, and the draft's where a token was
+// turned down (where nothing is left of the target above the draft, the target's again): memory bound for
+// large batches, latency bound for one sequence. A cluster of C CTAs shares one sequence's row in C slices: each
 // sums its slice by chunks of 256 (64-bit sums, which keep the order of the
 // chunks), the CTAs exchange their sums through distributed shared memory, and
 // the one whose slice holds u S searches its chunks, then the chunk again.
 //
-// 192 sequences of 100003, both distributions read (154 MB): 36 us, 65 % of the copy rate: each CTA has three
-// steps that wait for one another (the count, the sums, the search), and the loads of one row are
-// too few to fill them. One sequence of 32000: 5.7 us.
+// 192 sequences of 100003, a token turned down in 66 % of them (127 MB): 36 us, 54 % of the copy rate: each CTA has three
+// steps that wait for one another (the count, the sums, the search), the loads of one row are
+// too few to fill them, and 384 CTAs leave some SMs with three and others with two. One sequence of 32000: 5.7 us.
 #include <cooperative_groups.h>
 
 #include "paged_common.cuh"
