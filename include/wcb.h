@@ -444,7 +444,7 @@ uint32_t wcb_paged_attention_workspace(const wcb_paged_kv* kv, const wcb_paged_b
  * and j > p - window where window > 0 (at most 2^30); n_heads / n_kv_heads query heads share
  * a key head (any whole ratio up to 64). Scores and sums are kept in 32 bits; with 16-bit activations the weights are
  * rounded once to their type before they multiply the values (not for up to 8 rows a key head), with F32 ones they, the
- * queries, keys and values keep 21 bits or more (of the largest of 8 neighbouring numbers). q and out: [n_tokens][n_heads][head_dim]
+ * queries, keys and values keep 21 bits or more (of the largest number of their head). q and out: [n_tokens][n_heads][head_dim]
  * with their strides between tokens (elements, multiples of 16 bytes), types as
  * for wcb_paged_append_dev. scale 0: 1 / sqrt(head_dim). lse (device f32
  * [n_tokens][n_heads], or NULL): the natural logarithm of the softmax's sum,

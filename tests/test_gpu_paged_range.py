@@ -269,3 +269,16 @@ def test_scores_far_from_zero(gpu, act, cache, q, far):
         want = vt[:700 - q + r + 1].mean(0)
         # equal weights: sums of 1 and 3 are exact, so the quotient's rounding (2^-22) and the output's are left
         assert ((got[r] - want).abs() <= 3 * (paged.half_step(s.at) + 2.0 ** -22)).all(), r
+
+
+@pytest.mark.parametrize("cache", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,dim,q", [(8, 2, 64, 80), (8, 8, 128, 80)])
+@pytest.mark.parametrize("small", [1e-6, 1e-12, 1e-30])
+def test_dimensions_of_many_sizes(gpu, cache, heads, kv_heads, dim, q, small):
+    """Half of the dimensions are `small` times the others, 8 by 8: a head's numbers share what they are measured by."""
+    s = paged.Step([q], [300], heads, kv_heads, dim, "f32", cache, 16, seed=61)
+    thin = (torch.arange(dim, device="cuda") // 8) % 2 == 1
+    for x in (s.q[:, :heads * dim].view(-1, heads, dim), s.k, s.v):
+        x[..., thin] *= small
+    s.attend()
+    check(s)

@@ -4,7 +4,7 @@
 //
 // f32 numbers go to the tensor cores as sums of two f16 numbers, x = 2^e (hi + lo), 22 bits: the
 // exponents are a row's (q) or 8 keys' (k and v), so that the largest of them lies below 2^14 and
-// what is lost of the others is below 2^-38 of it. 8 keys that are farther apart than 2^16 stay out of the products:
+// what is lost of the others is below 2^-38 of it. 8 keys whose largest numbers are farther apart than 2^16 stay out of the products:
 // each row that sees one adds it in ordinary f32 arithmetic, so that a large key or value, of a later token for instance,
 // takes no bits from what other rows see. P is split with an exponent of each row's own for 64 keys, that of
 // the largest weight times the size of its values among the keys that the row sees. An f16 cache needs no
@@ -22,10 +22,11 @@
 // the tile is whole. head_dim 64: two row tiles of 128 rows; 128: one (Q in two parts and a
 // ring of K and V in two parts fill the shared memory).
 //
-// 46 sequences of 919 tokens, 32/4 heads of 64, f32 cache: 1.17 ms, 136 TFLOP/s of the formula's
-// products, 408 of those made (24 % of the measured cuBLAS rate); one of 2048 tokens over 16384 keys
-// 1.09 ms, 241 and 713 TFLOP/s (43 %). The rows' own exponents of P and the search for keys that are far apart are 2 to
-// 6 % of that (an exponent for each key instead, read by a second way through the softmax: 10 %). What bounds it: the
+// 46 sequences of 919 tokens, 32/4 heads of 64, f32 cache: 1.19 ms, 134 TFLOP/s of the formula's
+// products, 402 of those made (24 % of the measured cuBLAS rate); one of 2048 tokens over 16384 keys
+// 1.09 ms, 241 and 713 TFLOP/s (43 %). The rows' own exponents of P and the search for keys that are far apart are 1 to
+// 7 % of that (an exponent for each key instead, read by a second way through the softmax: 10 %); a call all of whose
+// keys are far apart takes a hundred times as long. What bounds it: the
 // instructions of the splitting, in the softmax (P) and in the loaders (K and V), about 500 bytes of registers that
 // spill in each kernel, and at few tiles a unit's start and end.
 #include "paged_tc.cuh"
@@ -67,7 +68,7 @@ struct Tc32Shared : TcShared {
   alignas(16) float kfac[EXP_RING][16];
   alignas(16) float vfac[EXP_RING][16];
   alignas(16) float vexp[EXP_RING][16];
-  uint32_t apart[HOLE_RING][4];  // keys that the products leave out for that
+  alignas(8) uint32_t apart[HOLE_RING][4];  // keys that the products leave out for that
 };
 
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((max(-126, min(127, e)) + 127) << 23); }
@@ -329,24 +330,13 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
               ok = ok && room(n + kvi);
               if (!ok) break;
             }
-            // the largest number of the 8 keys, and the smallest of the nonzero maxima of 8 numbers each
-            float top = 0.0f, low = INFINITY;
+            // the largest of 8 numbers each, of all 8 keys, and the smallest of the former that is not zero
+            float top = 0.0f, low = INFINITY, t8[IT / 2];
             uint64_t zero = 0;  // NaN where a number is not finite
-            auto largest = [&](int j) {
-              float t = 0.0f;
-#pragma unroll
-              for (int i = j; i < j + 2; ++i)
-                t = fmaxf(fmaxf(t, fmaxf(fabsf(y[i].x), fabsf(y[i].y))), fmaxf(fabsf(y[i].z), fabsf(y[i].w)));
-              return t;
-            };
-#pragma unroll
-            for (int j = 0; j < IT; j += 2) {
-              const float t = largest(j);
-              top = fmaxf(top, t);
-              if (t > 0.0f) low = fminf(low, t);
-            }
 #pragma unroll
             for (int j = 0; j < IT; ++j) {
+              const float t = fmaxf(fmaxf(fabsf(y[j].x), fabsf(y[j].y)), fmaxf(fabsf(y[j].z), fabsf(y[j].w)));
+              t8[j / 2] = j % 2 ? fmaxf(t8[j / 2], t) : t;
               zero = fma_f32x2(pack_f32x2(y[j].x, y[j].y), 0, zero);
               zero = fma_f32x2(pack_f32x2(y[j].z, y[j].w), 0, zero);
             }
@@ -356,29 +346,46 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
             if (bad) {
               // infinities and NaN take no part in the exponent; a value's is added to O at the end, to the
               // rows that see it
-              top = 0.0f;
-              low = INFINITY;
               bool odd = false;
 #pragma unroll
-              for (int j = 0; j < IT; ++j)
+              for (int j = 0; j < IT; ++j) {
+                if (j % 2 == 0) t8[j / 2] = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                   float& v = (&y[j].x)[e];
                   if (fabsf(v) <= FLT_MAX) {
-                    top = fmaxf(top, fabsf(v));
-                    if (v != 0.0f) low = fminf(low, fabsf(v));
+                    t8[j / 2] = fmaxf(t8[j / 2], fabsf(v));
                   } else if (kvi) {
                     odd = true;
                     v = 0.0f;
                   }
                 }
+              }
               if (odd) sh.odd[item % ODD_RING] = 1;
+            }
+#pragma unroll
+            for (int j = 0; j < IT / 2; ++j) {
+              top = fmaxf(top, t8[j]);
+              if (t8[j] > 0.0f) low = fminf(low, t8[j]);
             }
             // (the bits of numbers that are not negative are in their order)
             top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
             low = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(low)));
             const int none = kvi ? -126 : 0;  // zeros among values never make the largest exponent
             const int ge = group_exp(top, none);
+            // Farther apart than WIDE, a key against the others? (The first look takes 8 numbers by themselves, which is cheap; a key's
+            // own small ones lose nothing that shows beside its large ones.)
+            if (low < top * WIDE) {
+              low = INFINITY;
+#pragma unroll
+              for (int j = 0; j < IT / 2; ++j) {
+                float t = t8[j];
+#pragma unroll
+                for (int d = LPR / 2; d > 0; d >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, d));
+                if (t > 0.0f) low = fminf(low, t);
+              }
+              low = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(low)));
+            }
             if (lane == 0) {
               const int at = 8 * b + lw, r = tiles % EXP_RING;
               if (kvi) {
@@ -575,14 +582,66 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
                            o[16 * q + e], o[16 * q + e + 1]);
           }
         };
+        auto rescale = [&](float top) {
+          if (__any_sync(0xffffffffu, top > m + SLACK)) {
+            // (a row by itself: not by what its neighbours see). Over an f16 cache a whole number, so that m - lift is exact
+            const float nm = top > m + SLACK ? (F32C ? top : ceilf(top)) : m;
+            const float f = m == nm ? 1.0f : fast_exp2(m - (nm == -INFINITY ? 0.0f : nm));
+#pragma unroll
+            for (int d = 0; d < HD; ++d) o[d] *= f;
+            due *= f;
+            l *= f;
+            m = nm;
+          }
+        };
         for (int i = wk.ta; i < end && ok; ++i) {
           const uint32_t rt = tiles + (i - wk.ta);  // ring tile pair
           const uint32_t* holes = sh.holes[rt % HOLE_RING];
           const bool cut = wk.ragged(a, i);
+          if constexpr (F32C) {
+            ok = tc_wait_warp(&sh, &sh.full[(2 * rt + 1) % NS], ((2 * rt + 1) / NS) & 1);  // the values' factors
+            if (!ok) break;
+            // keys that the products leave out: q k and p v by ordinary arithmetic, one key after another (rare, and
+            // short code rather than fast)
+            const uint64_t* apart = reinterpret_cast<const uint64_t*>(sh.apart[rt % HOLE_RING]);
+            if ((apart[0] | apart[1]) != 0) {
+#pragma unroll 1
+              for (int b = 0; b < 2; ++b)
+#pragma unroll 1
+                for (uint64_t left = apart[b]; left; left &= left - 1) {
+                  const int key = (wk.blk.tile0 + i) * TC_TK + 64 * b + __ffsll(static_cast<long long>(left)) - 1;
+                  bool hole;
+                  const long long off = wk.key_offset(a, key, hole);
+                  if (off < 0) continue;
+                  const CT* kp = static_cast<const CT*>(a.pool.k) + wk.kvh * a.pool.head_stride + off;
+                  const CT* vp = static_cast<const CT*>(a.pool.v) + wk.kvh * a.pool.head_stride + off;
+                  const float* qp = static_cast<const float*>(a.q) + q_at;
+                  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+                  for (int d = 0; d < HD; d += 8) {
+                    float x[8], y[8];
+                    load_vec<float, 8>(qp + d, x);
+                    load_vec<CT, 8>(kp + d, y);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sum[e & 3] = fmaf(x[e], y[e], sum[e & 3]);
+                  }
+                  const float x = key >= klo && key < khi ? ((sum[0] + sum[1]) + (sum[2] + sum[3])) * a.scale_log2 : -INFINITY;
+                  rescale(x);
+                  const float p = fast_exp2(x - (m == -INFINITY ? 0.0f : m));
+                  l += p;
+#pragma unroll
+                  for (int d = 0; d < HD; d += 8) {
+                    float y[8];
+                    load_vec<CT, 8>(vp + d, y);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) o[d + e] = fmaf(p, fabsf(y[e]) <= FLT_MAX ? y[e] : 0.0f, o[d + e]);  // (the others are added at the unit's end)
+                  }
+                }
+            }
+          }
 #pragma unroll 1
           for (int b = 0; b < 2; ++b) {
             ok = tc_wait_warp(&sh, &sh.s_full[w][b], t & 1);
-            if (F32C && b == 0) ok = ok && tc_wait_warp(&sh, &sh.full[(2 * rt + 1) % NS], ((2 * rt + 1) / NS) & 1);  // the values' factors
             if (!ok) break;
             tc_fence_after();
             const int key0 = (wk.blk.tile0 + i) * TC_TK + 64 * b;
@@ -602,18 +661,6 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
             } else {
               kf[0] = factor(1.0f);
             }
-            auto rescale = [&](float top) {
-              if (__any_sync(0xffffffffu, top > m + SLACK)) {
-                // (a row by itself: not by what its neighbours see). Over an f16 cache a whole number, so that m - lift is exact
-                const float nm = top > m + SLACK ? (F32C ? top : ceilf(top)) : m;
-                const float f = m == nm ? 1.0f : fast_exp2(m - (nm == -INFINITY ? 0.0f : nm));
-#pragma unroll
-                for (int d = 0; d < HD; ++d) o[d] *= f;
-                due *= f;
-                l *= f;
-                m = nm;
-              }
-            };
             // which of the keys this row sees; whether some row of the warp does not see all of them
             uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
             bool mask = false;
@@ -626,35 +673,6 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
                 seen[q] = below1 & ~below0 & ~holes[2 * b + q];
               }
               mask = __any_sync(0xffffffffu, (seen[0] & seen[1]) != 0xffffffffu);
-              if constexpr (F32C) {
-                // keys that the products leave out: q k and p v by ordinary arithmetic, one key after another (rare, and
-                // short code rather than fast)
-                const uint32_t* apart = sh.apart[rt % HOLE_RING];
-#pragma unroll 1
-                for (uint64_t left = uint64_t(apart[2 * b]) | uint64_t(apart[2 * b + 1]) << 32; left; left &= left - 1) {
-                  const int c = __ffsll(static_cast<long long>(left)) - 1;
-                  bool hole;
-                  const long long off = wk.key_offset(a, key0 + c, hole);
-                  if (off < 0) continue;
-                  const CT* kp = static_cast<const CT*>(a.pool.k) + wk.kvh * a.pool.head_stride + off;
-                  const CT* vp = static_cast<const CT*>(a.pool.v) + wk.kvh * a.pool.head_stride + off;
-                  const float* qp = static_cast<const float*>(a.q) + q_at;
-                  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 1
-                  for (int d = 0; d < HD; d += 4)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) sum[e] = fmaf(__ldg(qp + d + e), to_f32(kp[d + e]), sum[e]);
-                  const float x = c >= lo && c < hi ? ((sum[0] + sum[1]) + (sum[2] + sum[3])) * a.scale_log2 : -INFINITY;
-                  rescale(x);
-                  const float p = fast_exp2(x - (m == -INFINITY ? 0.0f : m));
-                  l += p;
-#pragma unroll
-                  for (int d = 0; d < HD; ++d) {
-                    const float y = to_f32(vp[d]);
-                    o[d] = fmaf(p, fabsf(y) <= FLT_MAX ? y : 0.0f, o[d]);  // (the others are added at the unit's end)
-                  }
-                }
-              }
             }
             // S is read twice, 16 keys at a time: for the maxima, then for P, whose two parts take the 16 columns' place
             auto keys = [&](int c, uint32_t (&x)[16]) {  // columns 16 c .. of S, the next ones on their way
