@@ -599,7 +599,9 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
           const uint32_t* holes = sh.holes[rt % HOLE_RING];
           const bool cut = wk.ragged(a, i);
           if constexpr (F32C) {
-            ok = tc_wait_warp(&sh, &sh.full[(2 * rt + 1) % NS], ((2 * rt + 1) / NS) & 1);  // the values' factors
+            // the values' factors, after S: the loaders are in this tile then, and the slot's barrier in this phase or past it (a row
+            // tile that sees few keys would else be here two phases early, where the parity is the same)
+            ok = tc_wait_warp(&sh, &sh.s_full[w][0], t & 1) && tc_wait_warp(&sh, &sh.full[(2 * rt + 1) % NS], ((2 * rt + 1) / NS) & 1);
             if (!ok) break;
             // keys that the products leave out: q k and p v by ordinary arithmetic, one key after another (rare, and
             // short code rather than fast)
@@ -641,7 +643,7 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
           }
 #pragma unroll 1
           for (int b = 0; b < 2; ++b) {
-            ok = tc_wait_warp(&sh, &sh.s_full[w][b], t & 1);
+            if (!F32C || b) ok = tc_wait_warp(&sh, &sh.s_full[w][b], t & 1);
             if (!ok) break;
             tc_fence_after();
             const int key0 = (wk.blk.tile0 + i) * TC_TK + 64 * b;
