@@ -24,7 +24,7 @@
 //
 // 46 sequences of 919 tokens, 32/4 heads of 64, f32 cache: 1.19 ms, 134 TFLOP/s of the formula's
 // products, 402 of those made (24 % of the measured cuBLAS rate); one of 2048 tokens over 16384 keys
-// 1.09 ms, 241 and 713 TFLOP/s (43 %). The rows' own exponents of P and the search for keys that are far apart are 1 to
+// 1.12 ms, 234 and 694 TFLOP/s (42 %). The rows' own exponents of P and the search for keys that are far apart are 1 to
 // 7 % of that (an exponent for each key instead, read by a second way through the softmax: 10 %); a call all of whose
 // keys are far apart takes a hundred times as long. What bounds it: the
 // instructions of the splitting, in the softmax (P) and in the loaders (K and V), about 500 bytes of registers that
