@@ -391,14 +391,17 @@ typedef struct wcb_paged_batch {
  * vocabulary (turned down). BAD_PROBS: a row of target probabilities without
  * a positive finite value (the sampled token is -1). ABORTED: a wait inside a
  * kernel ran out; the call's outputs are not valid, and its workspace has to be
- * zeroed again. */
+ * zeroed again. BAD_TREE: a
+ * parent that is no earlier token of its sequence (the token cannot be reached),
+ * or a path that does not ascend within the new tokens (nothing is moved). */
 enum {
   WCB_PAGED_BAD_PAGE = 1,
   WCB_PAGED_BAD_ROWS = 2,
   WCB_PAGED_BAD_LEN = 4,
   WCB_PAGED_BAD_TOKEN = 8,
   WCB_PAGED_BAD_PROBS = 16,
-  WCB_PAGED_ABORTED = 32
+  WCB_PAGED_ABORTED = 32,
+  WCB_PAGED_BAD_TREE = 64
 };
 
 /* Rotation of a head's first rot_dim dimensions (attention.rs:230-262 rotates
@@ -478,6 +481,107 @@ uint32_t wcb_spec_verify_dev(const int32_t* draft, const int32_t* draft_len, con
                              uint32_t max_draft, uint32_t vocab, int32_t* tokens, int32_t* accepted,
                              uint64_t target_seq_stride, uint64_t target_row_stride, uint64_t draft_seq_stride,
                              uint64_t draft_row_stride, uint32_t* status, void* stream);
+
+/* ---- Trees of drafted tokens ----------------------------------------------
+ * No counterpart in the reference. The new tokens of a sequence may be a tree
+ * instead of a chain: the first one is the root (the last token that is certain),
+ * each other one a guess at what follows an earlier one. A step is:
+ * wcb_paged_tree_append_dev and wcb_paged_tree_attention_dev in every layer,
+ * wcb_sample_dev (a token of the target's at every node), wcb_tree_accept_dev
+ * (the way down the tree along the target's tokens), wcb_paged_keep_dev (the
+ * nodes on it move to the slots behind the context, in every layer). The tokens
+ * that come out are draws from the target's distribution, whatever was drafted.
+ * What the head of "Paged serving" says holds here too.
+ */
+
+/* The shape of the new tokens. depth[row]: how far row's token lies below its
+ * sequence's root, so that its position is kv_len[s] - (new tokens of s) + depth;
+ * its slot is that of wcb_paged_append_dev, one after another. mask: bit i % 32 of
+ * word mask[row * mask_words + i / 32] is set if row's token sees the i-th new
+ * token of its sequence; of a tree, its ancestors and itself. The mask need not
+ * be a tree's; tokens that 32 * mask_words bits do not reach are not seen.
+ * Rows of no sequence may hold anything. */
+typedef struct wcb_paged_tree {
+  uint32_t struct_size; /* sizeof(wcb_paged_tree) */
+  uint32_t mask_words;  /* 32-bit words of a row's mask */
+  const int32_t* depth; /* device, [n_tokens] */
+  const uint32_t* mask; /* device, [n_tokens][mask_words] */
+} wcb_paged_tree;
+
+/* depth [n] and mask [n][mask_words] of one tree from parent [n], all on the
+ * host: parent[i] < i is the i-th token's parent (parent[0] is not read). */
+uint32_t wcb_paged_tree_fill(const int32_t* parent, uint32_t n, uint32_t mask_words, int32_t* depth, uint32_t* mask);
+
+/* wcb_paged_append_dev with positions by depth: queries and keys turn by
+ * context + depth. tree->mask is not used and may be NULL. */
+uint32_t wcb_paged_tree_append_dev(const wcb_paged_kv* kv, const wcb_paged_batch* batch, const wcb_paged_tree* tree,
+                                   const wcb_rope* rope, const void* q, const void* k, const void* v, void* q_out,
+                                   uint32_t dtype, uint32_t n_heads, uint64_t q_stride, uint64_t k_stride,
+                                   uint64_t v_stride, uint64_t q_out_stride, const float* q_norm, const float* k_norm,
+                                   float eps, void* stream);
+
+/* wcb_paged_attention_dev over the context and, among the new tokens, those
+ * that the mask names. window > 0: of the context, the keys j > position - window,
+ * position = context + depth, depth held to 0 .. new tokens - 1 (the mask alone
+ * decides on the new tokens); depth may be NULL without a window. A row that sees
+ * nothing gives zeros and -infinity. Workspace: wcb_paged_attention_workspace's. */
+uint32_t wcb_paged_tree_attention_dev(const wcb_paged_kv* kv, const wcb_paged_batch* batch, const wcb_paged_tree* tree,
+                                      const void* q, void* out, uint32_t dtype, uint32_t n_heads, uint64_t q_stride,
+                                      uint64_t out_stride, void* workspace, size_t workspace_bytes, float scale,
+                                      uint32_t window, float* lse, void* stream);
+
+/* The way down each sequence's tree: node 0, then as long as there is one the
+ * lowest node whose parent is the last one on the way and whose token equals what
+ * was sampled there. Of batch, q_start (and n_seqs, n_tokens, status) are used. parent [n_tokens]: a
+ * token's parent among its sequence's new tokens (-1: none; the first one's is
+ * not read), token [n_tokens]: the drafted tokens, sampled [n_tokens]: the
+ * target's token after each (negative: none, the way ends there). path
+ * [n_seqs][max_path]: the nodes of the way, at most max_path of them, then -1;
+ * tokens [n_seqs][max_path]: sampled at each of them, which are the tokens to
+ * put out, then -1; count [n_seqs]: the nodes of the way (0 without new tokens). */
+uint32_t wcb_tree_accept_dev(const wcb_paged_batch* batch, const int32_t* parent, const int32_t* token,
+                             const int32_t* sampled, uint32_t max_path, int32_t* path, int32_t* tokens, int32_t* count,
+                             void* stream);
+
+/* Keys and values of the nodes on the way, in every layer: new token
+ * path[s * max_path + i] of sequence s moves to the place of its i-th new token,
+ * i < count[s] (held to 0 .. max_path). A path has to ascend. The sequence then
+ * has kv_len[s] - (new tokens of s) + count[s] tokens; what lies in the slots after
+ * them is left as it is. layers: n_layers pools that differ in k and v alone
+ * and do not overlap. One launch for up to 128 layers. */
+uint32_t wcb_paged_keep_dev(const wcb_paged_kv* const* layers, uint32_t n_layers, const wcb_paged_batch* batch,
+                            const int32_t* path, uint32_t max_path, const int32_t* count, void* stream);
+
+/* Settings of each row of a wcb_sample_dev call, device arrays of n_rows values;
+ * NULL switches one off for all rows. temperature (NULL: 1): not above zero means
+ * the largest logit's token. top_k: 0 or less is off. top_p: 1 or more is off.
+ * min_p: 0 or less is off, above 1 counts as 1. (NaN: off.) */
+typedef struct wcb_sampling {
+  uint32_t struct_size; /* sizeof(wcb_sampling) */
+  uint32_t reserved;    /* 0 */
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+} wcb_sampling;
+
+/* One token of each row of logits [n_rows][vocab] (row_stride elements apart,
+ * 0: vocab; F32, F16 or BF16), by given random numbers u [n_rows] in [0, 1)
+ * (held to that). Token j weighs exp((l_j - max l) / temperature). In the order of
+ * falling logits, the lowest index first among equal ones, top_k keeps the first
+ * k tokens, top_p of those the ones before which less than top_p of their sum
+ * lies, min_p those that weigh at least min_p (the largest weighs 1). The token
+ * is the lowest index at which the sum of the kept weights, in the order of
+ * indices, exceeds u times the sum of all. Weights and sums are kept in 64 bits.
+ * sampling NULL: all of the row at temperature 1. probs
+ * (or NULL): [n_rows][vocab] f32 (probs_stride apart, 0: vocab), the
+ * probabilities that the draw went by, zero for what was not kept: the input of
+ * wcb_spec_verify_dev, for instance. NaN and -infinity are no candidates; if
+ * there are infinities, only they are weighed (all the same). A row without
+ * candidates gives -1, zeros, and WCB_PAGED_BAD_PROBS in status (or NULL). */
+uint32_t wcb_sample_dev(const void* logits, uint32_t dtype, uint32_t n_rows, uint32_t vocab, uint64_t row_stride,
+                        const wcb_sampling* sampling, const float* u, int32_t* tokens, float* probs,
+                        uint64_t probs_stride, uint32_t* status, void* stream);
 
 /* Device stream a model handle launches on (a cudaStream_t), for callers that
  * time or order work against it. */

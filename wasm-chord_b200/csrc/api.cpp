@@ -235,6 +235,14 @@ size_t wcb_struct_layout(const char* s, const char* f) {
     if (!f) return sizeof(wcb_rope);
     WCB_FIELD(wcb_rope, struct_size) WCB_FIELD(wcb_rope, rot_dim) WCB_FIELD(wcb_rope, halves)
     WCB_FIELD(wcb_rope, reserved) WCB_FIELD(wcb_rope, inv_freq)
+  } else if (st == "wcb_paged_tree") {
+    if (!f) return sizeof(wcb_paged_tree);
+    WCB_FIELD(wcb_paged_tree, struct_size) WCB_FIELD(wcb_paged_tree, mask_words) WCB_FIELD(wcb_paged_tree, depth)
+    WCB_FIELD(wcb_paged_tree, mask)
+  } else if (st == "wcb_sampling") {
+    if (!f) return sizeof(wcb_sampling);
+    WCB_FIELD(wcb_sampling, struct_size) WCB_FIELD(wcb_sampling, reserved) WCB_FIELD(wcb_sampling, temperature)
+    WCB_FIELD(wcb_sampling, top_k) WCB_FIELD(wcb_sampling, top_p) WCB_FIELD(wcb_sampling, min_p)
   }
 #undef WCB_FIELD
   return SIZE_MAX;

@@ -3,6 +3,7 @@
 // before the first CUDA call.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -124,9 +125,9 @@ struct Plan {
   bool tc;
   int split;    // sequences of more rows are the tensor-core kernel's
 };
-Plan plan(uint64_t n_seqs, uint64_t n_kv, uint64_t max_rows) {
+Plan plan(uint64_t n_seqs, uint64_t n_kv, uint64_t max_rows, bool tree) {
   Plan p{};
-  p.tc = max_rows > TC_MIN && n_seqs * n_kv * ((max_rows + 31) / 32) > TC_UNITS;
+  p.tc = !tree && max_rows > TC_MIN && n_seqs * n_kv * ((max_rows + 31) / 32) > TC_UNITS;
   p.split = p.tc ? (n_seqs == 1 ? 0 : int(TC_MIN)) : INT_MAX;
   const uint64_t r = p.tc ? (n_seqs == 1 ? 0 : TC_MIN) : max_rows;
   p.rows = r == 0 ? 0 : r <= 8 ? 8 : r <= 16 ? 16 : 32;
@@ -140,27 +141,22 @@ size_t workspace_bytes(const Plan& p, int head_dim) {
   return TICKET_BYTES + (x > y ? x : y);
 }
 
-}  // namespace
+constexpr uint32_t MAX_WORDS = 1u << 19;  // of a row's mask: 2^24 new tokens
 
-extern "C" {
-
-uint32_t wcb_rope_init(wcb_rope* r, uint32_t rot_dim, double theta, uint32_t halves) {
-  if (!r) return bad("Invalid argument: null pointer");
-  if (rot_dim % 16 || rot_dim > 128 || halves > 1 || !(theta > 0.0) || std::isinf(theta))
-    return bad("Invalid argument: need rot_dim a multiple of 16 up to 128, theta > 0, halves 0|1");
-  r->struct_size = sizeof(wcb_rope);
-  r->rot_dim = rot_dim;
-  r->halves = halves;
-  r->reserved = 0;
-  for (uint32_t i = 0; i < 64; ++i)
-    r->inv_freq[i] = i < rot_dim / 2 ? std::pow(theta, -2.0 * double(i) / double(rot_dim)) : 0.0;
+uint32_t check_tree(const wcb_paged_tree* tree) {
+  if (!tree) return bad("Invalid argument: null pointer");
+  if (tree->struct_size < sizeof(wcb_paged_tree)) return bad("Invalid argument: wcb_paged_tree.struct_size");
+  if (tree->mask && (tree->mask_words == 0 || tree->mask_words > MAX_WORDS))
+    return bad("Invalid tensor shape: need 1 <= mask_words <= 2^19");
+  if ((reinterpret_cast<uintptr_t>(tree->depth) | reinterpret_cast<uintptr_t>(tree->mask)) & 3)
+    return bad("Invalid argument: depth and mask must be 4-byte aligned");
   return WCB_OK;
 }
 
-uint32_t wcb_paged_append_dev(const wcb_paged_kv* kv, const wcb_paged_batch* batch, const wcb_rope* rope,
-                              const void* q, const void* k, const void* v, void* q_out, uint32_t dtype,
-                              uint32_t n_heads, uint64_t q_stride, uint64_t k_stride, uint64_t v_stride,
-                              uint64_t q_out_stride, const float* q_norm, const float* k_norm, float eps, void* stream) {
+uint32_t append(const wcb_paged_kv* kv, const wcb_paged_batch* batch, const int32_t* depth, const wcb_rope* rope,
+                const void* q, const void* k, const void* v, void* q_out, uint32_t dtype, uint32_t n_heads,
+                uint64_t q_stride, uint64_t k_stride, uint64_t v_stride, uint64_t q_out_stride, const float* q_norm,
+                const float* k_norm, float eps, void* stream) {
   AppendArgs a;
   uint32_t rc = check_pool(kv, &a.pool);
   if (rc == WCB_OK) rc = check_batch(batch, &a.batch);
@@ -199,29 +195,14 @@ uint32_t wcb_paged_append_dev(const wcb_paged_kv* kv, const wcb_paged_batch* bat
   a.n_heads = int(n_heads);
   a.rot = rope ? int(rope->rot_dim) : 0;
   a.halves = rope ? int(rope->halves) : 0;
+  a.depth = depth;
   for (int i = 0; i < 64; ++i) a.turns[i] = i < a.rot / 2 ? rope->inv_freq[i] * 0.15915494309189533577 : 0.0;
   return cuda_result(launch_append(a, int(dtype), int(kv->dtype), static_cast<cudaStream_t>(stream)), "paged append");
 }
 
-uint32_t wcb_paged_attention_workspace(const wcb_paged_kv* kv, const wcb_paged_batch* batch, uint32_t n_heads,
-                                       size_t* bytes) {
-  if (!bytes) return bad("Invalid argument: null pointer");
-  Pool pool;
-  Batch b;
-  uint32_t rc = check_pool(kv, &pool);
-  if (rc == WCB_OK) rc = check_batch(batch, &b);
-  if (rc != WCB_OK) return rc;
-  if (n_heads == 0 || n_heads > 4096 || n_heads % kv->n_kv_heads || n_heads / kv->n_kv_heads > 64)
-    return bad("Invalid tensor shape: need n_heads % n_kv_heads == 0 (<= 64 per kv head)");
-  const uint64_t rows = uint64_t(batch->max_q_len) * (n_heads / kv->n_kv_heads);
-  *bytes = workspace_bytes(plan(batch->n_seqs, kv->n_kv_heads, rows), pool.head_dim);
-  return WCB_OK;
-}
-
-uint32_t wcb_paged_attention_dev(const wcb_paged_kv* kv, const wcb_paged_batch* batch, const void* q, void* out,
-                                 uint32_t dtype, uint32_t n_heads, uint64_t q_stride, uint64_t out_stride,
-                                 void* workspace, size_t workspace_bytes_given, float scale, uint32_t window,
-                                 float* lse, void* stream) {
+uint32_t attend(const wcb_paged_kv* kv, const wcb_paged_batch* batch, const wcb_paged_tree* tree, const void* q,
+                void* out, uint32_t dtype, uint32_t n_heads, uint64_t q_stride, uint64_t out_stride, void* workspace,
+                size_t workspace_bytes_given, float scale, uint32_t window, float* lse, void* stream) {
   AttendArgs a;
   size_t need = 0;
   uint32_t rc = wcb_paged_attention_workspace(kv, batch, n_heads, &need);
@@ -248,13 +229,16 @@ uint32_t wcb_paged_attention_dev(const wcb_paged_kv* kv, const wcb_paged_batch* 
   a.rep = int(n_heads / kv->n_kv_heads);
   a.rep_inv = (uint64_t(1) << 40) / uint64_t(a.rep) + 1;
   a.window = int(window);
+  a.depth = tree ? tree->depth : nullptr;
+  a.mask = tree ? tree->mask : nullptr;
+  a.mask_words = tree ? int(tree->mask_words) : 0;
   a.tickets = static_cast<int*>(workspace);
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + TICKET_BYTES);
   // test hook for the bounded waits (unset in normal use, read once): tiles wait for bytes that do not come
   static const bool withhold = std::getenv("WCB_TEST_WITHHOLD_COPY") != nullptr;
   a.withheld = withhold ? 16 : 0;
   a.wait_ns = withhold ? 20000000ull : 2000000000ull;
-  const Plan p = plan(batch->n_seqs, kv->n_kv_heads, uint64_t(batch->max_q_len) * uint64_t(a.rep));
+  const Plan p = plan(batch->n_seqs, kv->n_kv_heads, uint64_t(batch->max_q_len) * uint64_t(a.rep), tree != nullptr);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
   if (p.tc) {
@@ -265,9 +249,199 @@ uint32_t wcb_paged_attention_dev(const wcb_paged_kv* kv, const wcb_paged_batch* 
   if (p.rows && e == cudaSuccess) {
     a.row_lo = 0;
     a.row_hi = p.split;
-    e = dtype == WCB_KV_F32 ? launch_attend_32(a, int(kv->dtype), p.rows, s) : launch_attend_16(a, int(dtype), p.rows, s);
+    if (tree) e = dtype == WCB_KV_F32 ? launch_tree_32(a, int(kv->dtype), p.rows, s) : launch_tree_16(a, int(dtype), p.rows, s);
+    else e = dtype == WCB_KV_F32 ? launch_attend_32(a, int(kv->dtype), p.rows, s) : launch_attend_16(a, int(dtype), p.rows, s);
   }
   return cuda_result(e, "paged attention");
+}
+
+}  // namespace
+
+extern "C" {
+
+uint32_t wcb_rope_init(wcb_rope* r, uint32_t rot_dim, double theta, uint32_t halves) {
+  if (!r) return bad("Invalid argument: null pointer");
+  if (rot_dim % 16 || rot_dim > 128 || halves > 1 || !(theta > 0.0) || std::isinf(theta))
+    return bad("Invalid argument: need rot_dim a multiple of 16 up to 128, theta > 0, halves 0|1");
+  r->struct_size = sizeof(wcb_rope);
+  r->rot_dim = rot_dim;
+  r->halves = halves;
+  r->reserved = 0;
+  for (uint32_t i = 0; i < 64; ++i)
+    r->inv_freq[i] = i < rot_dim / 2 ? std::pow(theta, -2.0 * double(i) / double(rot_dim)) : 0.0;
+  return WCB_OK;
+}
+
+uint32_t wcb_paged_append_dev(const wcb_paged_kv* kv, const wcb_paged_batch* batch, const wcb_rope* rope,
+                              const void* q, const void* k, const void* v, void* q_out, uint32_t dtype,
+                              uint32_t n_heads, uint64_t q_stride, uint64_t k_stride, uint64_t v_stride,
+                              uint64_t q_out_stride, const float* q_norm, const float* k_norm, float eps, void* stream) {
+  return append(kv, batch, nullptr, rope, q, k, v, q_out, dtype, n_heads, q_stride, k_stride, v_stride, q_out_stride,
+                q_norm, k_norm, eps, stream);
+}
+
+uint32_t wcb_paged_tree_append_dev(const wcb_paged_kv* kv, const wcb_paged_batch* batch, const wcb_paged_tree* tree,
+                                   const wcb_rope* rope, const void* q, const void* k, const void* v, void* q_out,
+                                   uint32_t dtype, uint32_t n_heads, uint64_t q_stride, uint64_t k_stride,
+                                   uint64_t v_stride, uint64_t q_out_stride, const float* q_norm, const float* k_norm,
+                                   float eps, void* stream) {
+  const uint32_t rc = check_tree(tree);
+  if (rc != WCB_OK) return rc;
+  if (!tree->depth) return bad("Invalid argument: null pointer (wcb_paged_tree.depth)");
+  return append(kv, batch, tree->depth, rope, q, k, v, q_out, dtype, n_heads, q_stride, k_stride, v_stride,
+                q_out_stride, q_norm, k_norm, eps, stream);
+}
+
+uint32_t wcb_paged_attention_workspace(const wcb_paged_kv* kv, const wcb_paged_batch* batch, uint32_t n_heads,
+                                       size_t* bytes) {
+  if (!bytes) return bad("Invalid argument: null pointer");
+  Pool pool;
+  Batch b;
+  uint32_t rc = check_pool(kv, &pool);
+  if (rc == WCB_OK) rc = check_batch(batch, &b);
+  if (rc != WCB_OK) return rc;
+  if (n_heads == 0 || n_heads > 4096 || n_heads % kv->n_kv_heads || n_heads / kv->n_kv_heads > 64)
+    return bad("Invalid tensor shape: need n_heads % n_kv_heads == 0 (<= 64 per kv head)");
+  const uint64_t rows = uint64_t(batch->max_q_len) * (n_heads / kv->n_kv_heads);
+  *bytes = std::max(workspace_bytes(plan(batch->n_seqs, kv->n_kv_heads, rows, false), pool.head_dim),
+                    workspace_bytes(plan(batch->n_seqs, kv->n_kv_heads, rows, true), pool.head_dim));
+  return WCB_OK;
+}
+
+uint32_t wcb_paged_attention_dev(const wcb_paged_kv* kv, const wcb_paged_batch* batch, const void* q, void* out,
+                                 uint32_t dtype, uint32_t n_heads, uint64_t q_stride, uint64_t out_stride,
+                                 void* workspace, size_t workspace_bytes_given, float scale, uint32_t window,
+                                 float* lse, void* stream) {
+  return attend(kv, batch, nullptr, q, out, dtype, n_heads, q_stride, out_stride, workspace, workspace_bytes_given,
+                scale, window, lse, stream);
+}
+
+uint32_t wcb_paged_tree_attention_dev(const wcb_paged_kv* kv, const wcb_paged_batch* batch, const wcb_paged_tree* tree,
+                                      const void* q, void* out, uint32_t dtype, uint32_t n_heads, uint64_t q_stride,
+                                      uint64_t out_stride, void* workspace, size_t workspace_bytes_given, float scale,
+                                      uint32_t window, float* lse, void* stream) {
+  const uint32_t rc = check_tree(tree);
+  if (rc != WCB_OK) return rc;
+  if (!tree->mask) return bad("Invalid argument: null pointer (wcb_paged_tree.mask)");
+  if (window && !tree->depth) return bad("Invalid argument: a window needs wcb_paged_tree.depth");
+  return attend(kv, batch, tree, q, out, dtype, n_heads, q_stride, out_stride, workspace, workspace_bytes_given, scale,
+                window, lse, stream);
+}
+
+uint32_t wcb_paged_tree_fill(const int32_t* parent, uint32_t n, uint32_t mask_words, int32_t* depth, uint32_t* mask) {
+  if (!parent || !depth || !mask) return bad("Invalid argument: null pointer");
+  if (n == 0 || n > (1u << 24) || mask_words == 0 || mask_words > MAX_WORDS || uint64_t(mask_words) * 32 < n)
+    return bad("Invalid tensor shape: need 1 <= n <= 2^24, 32 * mask_words >= n");
+  for (uint32_t i = 1; i < n; ++i)
+    if (parent[i] < 0 || uint32_t(parent[i]) >= i)
+      return bad("Invalid argument: a node's parent must be an earlier one (the first node is the root)");
+  for (uint32_t i = 0; i < n; ++i) {
+    uint32_t* row = mask + size_t(i) * mask_words;
+    if (i == 0) {
+      depth[0] = 0;
+      std::fill(row, row + mask_words, 0u);
+    } else {
+      depth[i] = depth[parent[i]] + 1;
+      std::copy_n(mask + size_t(parent[i]) * mask_words, mask_words, row);
+    }
+    row[i / 32] |= 1u << (i % 32);
+  }
+  return WCB_OK;
+}
+
+uint32_t wcb_tree_accept_dev(const wcb_paged_batch* batch, const int32_t* parent, const int32_t* token,
+                             const int32_t* sampled, uint32_t max_path, int32_t* path, int32_t* tokens, int32_t* count,
+                             void* stream) {
+  AcceptArgs a;
+  const uint32_t rc = check_batch(batch, &a.batch);
+  if (rc != WCB_OK) return rc;
+  if (!parent || !token || !sampled || !path || !tokens || !count) return bad("Invalid argument: null pointer");
+  if (max_path == 0 || max_path > (1u << 24)) return bad("Invalid tensor shape: need 1 <= max_path <= 2^24");
+  if ((reinterpret_cast<uintptr_t>(parent) | reinterpret_cast<uintptr_t>(token) | reinterpret_cast<uintptr_t>(sampled) |
+       reinterpret_cast<uintptr_t>(path) | reinterpret_cast<uintptr_t>(tokens) | reinterpret_cast<uintptr_t>(count)) & 3)
+    return bad("Invalid argument: pointers must be 4-byte aligned");
+  a.parent = parent;
+  a.token = token;
+  a.sampled = sampled;
+  a.max_path = int(max_path);
+  a.path = path;
+  a.tokens = tokens;
+  a.count = count;
+  return cuda_result(launch_accept(a, static_cast<cudaStream_t>(stream)), "tree acceptance");
+}
+
+uint32_t wcb_paged_keep_dev(const wcb_paged_kv* const* layers, uint32_t n_layers, const wcb_paged_batch* batch,
+                            const int32_t* path, uint32_t max_path, const int32_t* count, void* stream) {
+  if (!layers || !path || !count) return bad("Invalid argument: null pointer");
+  if (n_layers == 0 || n_layers > 4096 || max_path == 0 || max_path > (1u << 24))
+    return bad("Invalid tensor shape: need 1 <= n_layers <= 4096, 1 <= max_path <= 2^24");
+  KeepArgs a;
+  uint32_t rc = check_batch(batch, &a.batch);
+  for (uint32_t i = 0; i < n_layers && rc == WCB_OK; ++i) {
+    Pool p;
+    rc = check_pool(layers[i], &p);
+    if (rc != WCB_OK) break;
+    if (i == 0) a.pool = p;
+    if (layers[i]->dtype != layers[0]->dtype || p.n_kv != a.pool.n_kv || p.head_dim != a.pool.head_dim ||
+        p.page_size != a.pool.page_size || p.n_pages != a.pool.n_pages || p.page_stride != a.pool.page_stride ||
+        p.token_stride != a.pool.token_stride || p.head_stride != a.pool.head_stride)
+      return bad("Invalid argument: the layers' pools differ in more than k and v");
+  }
+  if (rc != WCB_OK) return rc;
+  if ((reinterpret_cast<uintptr_t>(path) | reinterpret_cast<uintptr_t>(count)) & 3)
+    return bad("Invalid argument: pointers must be 4-byte aligned");
+  a.path = path;
+  a.count = count;
+  a.max_path = int(max_path);
+  a.size = size_of(layers[0]->dtype);
+  for (uint32_t first = 0; first < n_layers; first += KEEP_LAYERS) {
+    a.n_layers = int(n_layers - first < KEEP_LAYERS ? n_layers - first : KEEP_LAYERS);
+    for (int i = 0; i < a.n_layers; ++i) {
+      a.pools[2 * i] = layers[first + i]->k;
+      a.pools[2 * i + 1] = layers[first + i]->v;
+    }
+    const cudaError_t e = launch_keep(a, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_result(e, "keeping accepted tokens");
+  }
+  return WCB_OK;
+}
+
+uint32_t wcb_sample_dev(const void* logits, uint32_t dtype, uint32_t n_rows, uint32_t vocab, uint64_t row_stride,
+                        const wcb_sampling* sampling, const float* u, int32_t* tokens, float* probs,
+                        uint64_t probs_stride, uint32_t* status, void* stream) {
+  SampleArgs a{};
+  if (!logits || !u || !tokens) return bad("Invalid argument: null pointer");
+  if (dtype > WCB_KV_BF16) return bad("Unsupported data type: logits are F32, F16 or BF16");
+  if (n_rows == 0 || n_rows > (1u << 20) || vocab == 0 || vocab > (1u << 20))
+    return bad("Invalid tensor shape: need 1 <= n_rows <= 2^20, 1 <= vocab <= 2^20");
+  if (sampling) {
+    if (sampling->struct_size < sizeof(wcb_sampling)) return bad("Invalid argument: wcb_sampling.struct_size");
+    if (sampling->reserved != 0) return bad("Invalid argument: wcb_sampling.reserved must be 0");
+    a.temperature = sampling->temperature;
+    a.top_k = sampling->top_k;
+    a.top_p = sampling->top_p;
+    a.min_p = sampling->min_p;
+  }
+  if ((reinterpret_cast<uintptr_t>(a.temperature) | reinterpret_cast<uintptr_t>(a.top_k) |
+       reinterpret_cast<uintptr_t>(a.top_p) | reinterpret_cast<uintptr_t>(a.min_p) | reinterpret_cast<uintptr_t>(u) |
+       reinterpret_cast<uintptr_t>(tokens) | reinterpret_cast<uintptr_t>(probs) | reinterpret_cast<uintptr_t>(status)) & 3)
+    return bad("Invalid argument: pointers must be 4-byte aligned");
+  if (reinterpret_cast<uintptr_t>(logits) % uintptr_t(size_of(dtype)))
+    return bad("Invalid argument: logits must be aligned to their type");
+  const uint64_t l_row = row_stride ? row_stride : vocab, p_row = probs_stride ? probs_stride : vocab;
+  if (l_row < vocab || p_row < vocab || l_row > MAX_STRIDE || p_row > MAX_STRIDE)
+    return bad("Invalid argument: a row stride is shorter than the vocabulary, or above 2^40");
+  if (static_cast<const void*>(probs) == logits) return bad("Invalid argument: probs must not be logits");
+  a.logits = logits;
+  a.stride = int64_t(l_row);
+  a.probs_stride = int64_t(p_row);
+  a.n_rows = int(n_rows);
+  a.vocab = int(vocab);
+  a.u = u;
+  a.tokens = tokens;
+  a.probs = probs;
+  a.status = status;
+  return cuda_result(launch_sample(a, int(dtype), static_cast<cudaStream_t>(stream)), "sampling");
 }
 
 uint32_t wcb_spec_verify_dev(const int32_t* draft, const int32_t* draft_len, const float* target,

@@ -10,7 +10,7 @@ namespace wcb {
 namespace paged {
 
 enum { E_F32 = 0, E_F16 = 1, E_BF16 = 2 };  // element types (WCB_KV_*)
-enum { ST_BAD_PAGE = 1, ST_BAD_ROWS = 2, ST_BAD_LEN = 4, ST_BAD_TOKEN = 8, ST_BAD_PROBS = 16, ST_ABORTED = 32 };
+enum { ST_BAD_PAGE = 1, ST_BAD_ROWS = 2, ST_BAD_LEN = 4, ST_BAD_TOKEN = 8, ST_BAD_PROBS = 16, ST_ABORTED = 32, ST_BAD_TREE = 64 };
 
 // pool and batch as the kernels see them (wcb_paged_kv, wcb_paged_batch)
 struct Pool {
@@ -37,6 +37,7 @@ struct AppendArgs {
   const float *q_norm, *k_norm;
   float eps;
   int n_heads, rot, halves;
+  const int32_t* depth;  // of a tree's tokens (position: context + depth); NULL: one after another
   double turns[64];  // inv_freq / 2 pi
 };
 
@@ -56,6 +57,10 @@ struct AttendArgs {
   float* part;       // partial results, two pieces per CTA
   uint64_t wait_ns;  // a wait for a copy or a product ends after so long
   uint32_t withheld; // bytes that a tile by TMA waits for and that do not come (test hook; 0)
+  // trees: each new token's depth (NULL where no window asks for it) and, as bits, the new tokens that it sees (NULL: no trees)
+  const int32_t* depth;
+  const uint32_t* mask;
+  int mask_words;
 };
 
 struct VerifyArgs {
@@ -64,6 +69,33 @@ struct VerifyArgs {
   int n_seqs, max_draft, vocab;
   int32_t *tokens, *accepted;
   int64_t t_seq, t_row, d_seq, d_row;
+  uint32_t* status;
+};
+
+struct AcceptArgs {
+  Batch batch;
+  const int32_t *parent, *token, *sampled;
+  int max_path;
+  int32_t *path, *tokens, *count;
+};
+
+constexpr int KEEP_LAYERS = 128;  // of one launch
+struct KeepArgs {
+  Pool pool;  // strides and sizes of all layers
+  Batch batch;
+  const int32_t *path, *count;
+  int max_path, n_layers, size;  // size: bytes of an element
+  void* pools[2 * KEEP_LAYERS];  // keys and values of each layer
+};
+
+struct SampleArgs {
+  const void* logits;
+  int64_t stride, probs_stride;
+  int n_rows, vocab;
+  const float *temperature, *top_p, *min_p, *u;
+  const int32_t* top_k;
+  int32_t* tokens;
+  float* probs;
   uint32_t* status;
 };
 
@@ -81,6 +113,11 @@ cudaError_t launch_attend_16(const AttendArgs& a, int act, int rows, cudaStream_
 cudaError_t launch_attend_32(const AttendArgs& a, int cache, int rows, cudaStream_t s);
 cudaError_t launch_attend_tc(const AttendArgs& a, int act, cudaStream_t s);
 cudaError_t launch_attend_tc32(const AttendArgs& a, int cache, cudaStream_t s);
+cudaError_t launch_tree_16(const AttendArgs& a, int act, int rows, cudaStream_t s);
+cudaError_t launch_tree_32(const AttendArgs& a, int cache, int rows, cudaStream_t s);
+cudaError_t launch_accept(const AcceptArgs& a, cudaStream_t s);
+cudaError_t launch_keep(const KeepArgs& a, cudaStream_t s);
+cudaError_t launch_sample(const SampleArgs& a, int kind, cudaStream_t s);
 cudaError_t launch_verify(const VerifyArgs& a, cudaStream_t s);
 
 }  // namespace paged

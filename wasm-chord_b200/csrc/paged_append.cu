@@ -60,7 +60,8 @@ __global__ void __launch_bounds__(AP_THREADS, AP_PER_SM) append_kernel(const __g
   }
   if (bad && tid == 0 && blockIdx.y == 0) report(a.batch, bad);
   if (tid < a.rot / 2) {
-    const double turn = double(pos) * a.turns[tid];
+    const double at = a.depth ? double(sq.kv - sq.n) + double(__ldg(a.depth + row)) : double(pos);
+    const double turn = at * a.turns[tid];
     const float f = float(2.0 * (turn - rint(turn)));  // half turns in [-1, 1]
     float sn, cs;
     sincospif(f, &sn, &cs);

@@ -228,17 +228,24 @@ __device__ __forceinline__ int token_of(const AttendArgs& a, int row) { return i
 __device__ __forceinline__ int head_of(const AttendArgs& a, int row) { return row - token_of(a, row) * a.rep; }
 
 // Keys of rows [r0, r1) of a sequence's key head: lo <= key < hi (in the cache's
-// table), first and last token's positions.
+// table), first and last token's positions (of a tree: every key up to pos0 is seen by all rows, none after pos1 by any).
 struct Block {
   int lo, hi, pos0, pos1, tile0, tiles;
 };
+template <bool TREE = false>
 __device__ __forceinline__ Block row_block(const AttendArgs& a, const Seq& q, int rows, int rb, int M, int TK, int table) {
   Block b;
   const int r0 = rb * M, r1 = min(rows, r0 + M);
-  b.pos0 = q.kv - q.n + token_of(a, r0);
-  b.pos1 = q.kv - q.n + token_of(a, r1 - 1);
+  if constexpr (TREE) {
+    // a row may see any of the new tokens; all that lies before them, but for the window (no row stands before the first of them)
+    b.pos0 = q.kv - q.n - 1;
+    b.pos1 = q.kv - 1;
+  } else {
+    b.pos0 = q.kv - q.n + token_of(a, r0);
+    b.pos1 = q.kv - q.n + token_of(a, r1 - 1);
+  }
   b.hi = min(b.pos1 + 1, table);
-  b.lo = a.window > 0 ? min(max(0, b.pos0 - a.window + 1), max(0, b.hi)) : 0;  // (no tile past the table: its end counts in 32 bits)
+  b.lo = a.window > 0 ? min(max(0, b.pos0 + (TREE ? 1 : 0) - a.window + 1), max(0, b.hi)) : 0;  // (no tile past the table: its end counts in 32 bits)
   b.tile0 = b.lo / TK;
   // rows that see nothing still have their zeros written
   b.tiles = b.hi > b.lo ? (b.hi + TK - 1) / TK - b.tile0 : 1;
@@ -248,23 +255,34 @@ __device__ __forceinline__ int seq_rows(const AttendArgs& a, const Seq& q) {
   const long long r = static_cast<long long>(q.n) * a.rep;
   return r > a.row_lo && r <= a.row_hi ? int(r) : 0;
 }
+// A tree's masks: the new token's depth (held to what a tree of so many can have), whether its bit for another is set
+// (bits past the mask's words are not).
+__device__ __forceinline__ int tree_depth(const AttendArgs& a, const Seq& q, int token) {
+  return a.depth ? max(0, min(q.n - 1, __ldg(a.depth + q.r0 + token))) : 0;
+}
+__device__ __forceinline__ bool tree_bit(const AttendArgs& a, const uint32_t* bits, int i) {
+  const int w = i >> 5;
+  return w < a.mask_words && ((__ldg(bits + w) >> (i & 31)) & 1u) != 0;
+}
 // Places on the line of one key head of a sequence, its tiles and V for each unit; a whole warp, its lanes over the row blocks (a chunk
 // of a few thousand tokens has dozens, and every CTA of a call counts them).
+template <bool TREE = false>
 __device__ __forceinline__ long long head_tiles(const AttendArgs& a, const Seq& q, int rows, int M, int TK, int V, int table) {
   long long n = 0;
-  for (int rb = threadIdx.x & 31; rb * M < rows; rb += 32) n += row_block(a, q, rows, rb, M, TK, table).tiles + V;
+  for (int rb = threadIdx.x & 31; rb * M < rows; rb += 32) n += row_block<TREE>(a, q, rows, rb, M, TK, table).tiles + V;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
   return n;
 }
 // The same for 32 sequences, one of each lane: those of one or two row blocks by their lane, the
 // others one after the other by the warp.
+template <bool TREE = false>
 __device__ __forceinline__ long long lane_tiles(const AttendArgs& a, const Seq& q, int M, int TK, int V, int table) {
   const int rows = seq_rows(a, q);
   long long n = 0;
   if (rows > 0 && rows <= 2 * M) {
-    n = row_block(a, q, rows, 0, M, TK, table).tiles + V;
-    if (rows > M) n += row_block(a, q, rows, 1, M, TK, table).tiles + V;
+    n = row_block<TREE>(a, q, rows, 0, M, TK, table).tiles + V;
+    if (rows > M) n += row_block<TREE>(a, q, rows, 1, M, TK, table).tiles + V;
   }
   for (unsigned left = __ballot_sync(0xffffffffu, rows > 2 * M); left; left &= left - 1) {
     const int src = __ffs(int(left)) - 1;
@@ -273,18 +291,19 @@ __device__ __forceinline__ long long lane_tiles(const AttendArgs& a, const Seq& 
     w.kv = __shfl_sync(0xffffffffu, q.kv, src);
     w.r0 = 0;
     w.sound = true;
-    const long long sum = head_tiles(a, w, __shfl_sync(0xffffffffu, rows, src), M, TK, V, table);
+    const long long sum = head_tiles<TREE>(a, w, __shfl_sync(0xffffffffu, rows, src), M, TK, V, table);
     if (int(threadIdx.x & 31) == src) n = sum;
   }
   return n;
 }
 // Row block of line position `at` in a key head whose tiles begin at unit0 (moved to the block's
 // first tile); a whole warp.
+template <bool TREE = false>
 __device__ __forceinline__ int find_block(const AttendArgs& a, const Seq& q, int rows, int M, int TK, int V, int table, long long at, long long& unit0) {
   const int lane = threadIdx.x & 31;
   for (int rb0 = 0;; rb0 += 32) {
     const int rb = rb0 + lane;
-    const long long n = rb * M < rows ? row_block(a, q, rows, rb, M, TK, table).tiles + V : 0;
+    const long long n = rb * M < rows ? row_block<TREE>(a, q, rows, rb, M, TK, table).tiles + V : 0;
     long long inc = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -317,7 +336,7 @@ struct PlaceShared {
   long long warp[THREADS / 32];
   long long found[2];
 };
-template <int THREADS>
+template <int THREADS, bool TREE = false>
 __device__ __forceinline__ Place find_place(const AttendArgs& a, int M, int TK, int V, PlaceShared<THREADS>& sh) {
   constexpr int NW = THREADS / 32;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -331,7 +350,7 @@ __device__ __forceinline__ Place find_place(const AttendArgs& a, int M, int TK, 
     Seq q{0, 0, 0, true};
     if (s < n) q = read_seq(a.batch, s);
     unsound |= !q.sound;
-    sh.count[slot] = lane_tiles(a, q, M, TK, V, table) * a.pool.n_kv;
+    sh.count[slot] = lane_tiles<TREE>(a, q, M, TK, V, table) * a.pool.n_kv;
     __syncthreads();
     mine = sh.count[tid];
     long long inc = mine;
@@ -428,7 +447,7 @@ struct AttnCfg {
   static constexpr int PER_SM = FIT < 1 ? 1 : FIT < WANT ? FIT : WANT;
 };
 
-template <typename AT, typename CT, int HD, int NB>
+template <typename AT, typename CT, int HD, int NB, bool TREE>
 __global__ void __launch_bounds__(AT_THREADS, (AttnCfg<AT, CT, HD, NB>::PER_SM))
 attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap kmap,
               const __grid_constant__ CUtensorMap vmap, int box) {
@@ -452,7 +471,7 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
   const int g = lane >> 2, t = lane & 3;
   const uint32_t sbase = smem_u32(sm);
   const int table = table_tokens(a.pool, a.batch);
-  const Place pl = find_place<AT_THREADS>(a, M, TK, V, s_place);
+  const Place pl = find_place<AT_THREADS, TREE>(a, M, TK, V, s_place);
   if (pl.begin >= pl.end) return;
   if (tid == 0) {
     for (int i = 0; i < S; ++i) mbar_init(&s_full[i], 1);
@@ -480,15 +499,15 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
   long long unit0;  // the unit's first place on the line: V, then its tiles
   Block blk;
   if (rows <= M) {  // one block a head
-    blk = row_block(a, sq, rows, 0, M, TK, table);
+    blk = row_block<TREE>(a, sq, rows, 0, M, TK, table);
     kvh = quotient(pl.begin - pl.seq_begin, blk.tiles + V);
     unit0 = pl.seq_begin + static_cast<long long>(kvh) * (blk.tiles + V);
   } else {
-    const long long ht = head_tiles(a, sq, rows, M, TK, V, table);
+    const long long ht = head_tiles<TREE>(a, sq, rows, M, TK, V, table);
     kvh = quotient(pl.begin - pl.seq_begin, ht);
     unit0 = pl.seq_begin + kvh * ht;
-    rb = find_block(a, sq, rows, M, TK, V, table, pl.begin, unit0);
-    blk = row_block(a, sq, rows, rb, M, TK, table);
+    rb = find_block<TREE>(a, sq, rows, M, TK, V, table, pl.begin, unit0);
+    blk = row_block<TREE>(a, sq, rows, rb, M, TK, table);
   }
 
   auto next_unit = [&] {
@@ -506,7 +525,7 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
         } while (rows == 0);
       }
     }
-    blk = row_block(a, sq, rows, rb, M, TK, table);
+    blk = row_block<TREE>(a, sq, rows, rb, M, TK, table);
     return true;
   };
   // a small unit is the part's that it begins in
@@ -620,14 +639,31 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
     // position (rows past the block see what its last row sees; nothing of theirs is kept)
     float mx[NB][2], ls[NB][2];
     int pos[NB][2];
+    const uint32_t* bits[NB][2];  // of a tree: the new tokens that the row sees
+    const int context = sq.kv - sq.n;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         mx[nb][h] = -INFINITY;
         ls[nb][h] = 0.0f;
-        pos[nb][h] = sq.kv - sq.n + token_of(a, r0 + min(8 * nb + 2 * t + h, rn - 1));
+        const int token = token_of(a, r0 + min(8 * nb + 2 * t + h, rn - 1));
+        if constexpr (TREE) {
+          pos[nb][h] = context + tree_depth(a, sq, token);
+          bits[nb][h] = a.mask + int64_t(sq.r0 + token) * a.mask_words;
+        } else {
+          pos[nb][h] = context + token;
+        }
       }
+    // whether this lane's row sees a key between blk.lo and blk.hi
+    auto sees = [&](int nb, int h, int key) {
+      if constexpr (TREE) {
+        if (key >= context) return tree_bit(a, bits[nb][h], key - context);
+      } else {
+        if (key > pos[nb][h]) return false;
+      }
+      return a.window <= 0 || key > pos[nb][h] - a.window;
+    };
 
     bool hole_seen = false;
     for (int i = ta; i < tb; ++i) {
@@ -718,9 +754,8 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
         for (int e = 0; e < 4; ++e) {
           float v = sc[nb][e] * a.scale_log2;
           if (ragged) {
-            const int kk = kw0 + g + 8 * (e >> 1), key = key0 + kk, p = pos[nb][e & 1];
-            const bool seen = key <= p && key < blk.hi && key >= blk.lo && (a.window <= 0 || key > p - a.window) &&
-                              (!hole || offs[(i % (S + 1)) * TK + kk] >= 0);
+            const int kk = kw0 + g + 8 * (e >> 1), key = key0 + kk;
+            const bool seen = key < blk.hi && key >= blk.lo && sees(nb, e & 1, key) && (!hole || offs[(i % (S + 1)) * TK + kk] >= 0);
             if (!seen) v = -INFINITY;
           }
           sc[nb][e] = v;
@@ -775,8 +810,7 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                   const float v = to_f32(val(kk, 16 * mb + g + 8 * (e >> 1)));
-                  const int p = pos[nb][e & 1];
-                  if (!(fabsf(v) <= FLT_MAX) && key <= p && (a.window <= 0 || key > p - a.window)) o[mb][nb][e] += v;
+                  if (!(fabsf(v) <= FLT_MAX) && sees(nb, e & 1, key)) o[mb][nb][e] += v;
                 }
           }
           __syncthreads();
@@ -890,7 +924,7 @@ attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUte
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) ls[nb][h] += __shfl_xor_sync(0xffffffffu, ls[nb][h], d);
     if (tid == 0 && blk.pos1 >= table) report(a.batch, ST_BAD_PAGE);
-    if (tid == 0 && blk.pos0 < 0) report(a.batch, ST_BAD_LEN);
+    if (tid == 0 && (TREE ? context : blk.pos0) < 0) report(a.batch, ST_BAD_LEN);
 
     // four results of row r from dim d on, l and m of the row
     auto finish = [&](int r, int d, float4 x, float m, float l) {
@@ -1047,24 +1081,24 @@ cudaError_t allow_shared(K kernel, int bytes, std::atomic<uint64_t>& done) {
   return e;
 }
 
-template <typename AT, typename CT, int HD, int NB>
+template <typename AT, typename CT, int HD, int NB, bool TREE>
 cudaError_t run_attend(const AttendArgs& a, cudaStream_t st) {
   using L = AttnCfg<AT, CT, HD, NB>;
   static_assert(L::SMEM <= 227 * 1024, "shared memory");
   static std::atomic<uint64_t> done{0};
-  const cudaError_t e = allow_shared(attend_kernel<AT, CT, HD, NB>, L::SMEM, done);
+  const cudaError_t e = allow_shared(attend_kernel<AT, CT, HD, NB, TREE>, L::SMEM, done);
   if (e != cudaSuccess) return e;
   CUtensorMap km{}, vm{};
   const int box = make_maps<CT>(&km, &vm, a.pool, L::TK);
-  attend_kernel<AT, CT, HD, NB><<<SMS * L::PER_SM, AT_THREADS, L::SMEM, st>>>(a, km, vm, box);
+  attend_kernel<AT, CT, HD, NB, TREE><<<SMS * L::PER_SM, AT_THREADS, L::SMEM, st>>>(a, km, vm, box);
   return cudaGetLastError();
 }
 
-template <typename AT, typename CT>
+template <typename AT, typename CT, bool TREE>
 cudaError_t run_attend_rows(const AttendArgs& a, int rows, cudaStream_t st) {
   if (a.pool.head_dim == 64)
-    return rows == 8 ? run_attend<AT, CT, 64, 1>(a, st) : rows == 16 ? run_attend<AT, CT, 64, 2>(a, st) : run_attend<AT, CT, 64, 4>(a, st);
-  return rows == 8 ? run_attend<AT, CT, 128, 1>(a, st) : rows == 16 ? run_attend<AT, CT, 128, 2>(a, st) : run_attend<AT, CT, 128, 4>(a, st);
+    return rows == 8 ? run_attend<AT, CT, 64, 1, TREE>(a, st) : rows == 16 ? run_attend<AT, CT, 64, 2, TREE>(a, st) : run_attend<AT, CT, 64, 4, TREE>(a, st);
+  return rows == 8 ? run_attend<AT, CT, 128, 1, TREE>(a, st) : rows == 16 ? run_attend<AT, CT, 128, 2, TREE>(a, st) : run_attend<AT, CT, 128, 4, TREE>(a, st);
 }
 
 }  // namespace

@@ -5,8 +5,8 @@ namespace wcb {
 namespace paged {
 
 cudaError_t launch_attend_16(const AttendArgs& a, int act, int rows, cudaStream_t s) {
-  return act == E_F16 ? run_attend_rows<__half, __half>(a, rows, s)
-                      : run_attend_rows<__nv_bfloat16, __nv_bfloat16>(a, rows, s);
+  return act == E_F16 ? run_attend_rows<__half, __half, false>(a, rows, s)
+                      : run_attend_rows<__nv_bfloat16, __nv_bfloat16, false>(a, rows, s);
 }
 
 }  // namespace paged

@@ -1,0 +1,114 @@
+// The accepted tokens of a tree move to the slots behind their sequence's context, in every layer: slot
+// context + i takes the key and value of slot context + path[i].
+//
+// path ascends, so path[i] >= i: what a move overwrites was read by an earlier one or is not wanted. A thread
+// owns 16 bytes of a token in one layer's keys or values and moves them for i = 0, 1 .., several at a time,
+// all loads before the first store; no thread reads what another writes. A CTA finds the moves of its sequence (those
+// with path[i] > i) once, then each of its threads goes through them.
+//
+// Bound by latency: lengths, path, page table and the tokens are four loads that wait for one another.
+#include "paged_common.cuh"
+
+namespace wcb {
+namespace paged {
+namespace {
+
+constexpr int KP_THREADS = 128;
+constexpr int KP_MOVES = 128;  // moves that are looked up at a time
+constexpr int KP_AHEAD = 8;    // loads of a thread before its stores
+
+__global__ void __launch_bounds__(KP_THREADS) keep_kernel(const __grid_constant__ KeepArgs a) {
+  __shared__ int64_t s_of[KP_MOVES], s_to[KP_MOVES];
+  __shared__ int s_moves[KP_THREADS / 32];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, s = blockIdx.x;
+  const bool says = blockIdx.y == 0;  // one CTA of a sequence reports
+  const Seq q = read_seq(a.batch, s);
+  if (!q.sound && says && tid == 0) report(a.batch, ST_BAD_ROWS);
+  const int count = q.n > 0 ? min(max(__ldg(a.count + s), 0), a.max_path) : 0;
+  const int32_t* path = a.path + int64_t(s) * a.max_path;
+  // a path that does not ascend, or leaves the new tokens, is not followed
+  bool bad = false;
+  for (int i = tid; i < count; i += KP_THREADS) {
+    const int p = __ldg(path + i), before = i ? __ldg(path + i - 1) : -1;
+    bad |= p <= before || p >= q.n;
+  }
+  if (__syncthreads_or(bad)) {
+    if (says && tid == 0) report(a.batch, ST_BAD_TREE);
+    return;
+  }
+  const int context = q.kv - q.n, table = table_tokens(a.pool, a.batch);
+  const int per_head = a.pool.head_dim * a.size / 16;
+  const int words = a.pool.n_kv * per_head;  // 16-byte words of a token in one layer's keys or values
+  const int items = words * 2 * a.n_layers;
+  uint32_t wrong = 0;
+  auto slot = [&](int pos) -> int64_t {
+    if (pos < 0) {
+      wrong |= ST_BAD_LEN;
+      return -1;
+    }
+    const int page = pos < table ? __ldg(a.batch.page_table + int64_t(s) * a.batch.max_pages + pos / a.pool.page_size) : -1;
+    if (page < 0 || page >= a.pool.n_pages) {
+      wrong |= ST_BAD_PAGE;
+      return -1;
+    }
+    return (page * a.pool.page_stride + int64_t(pos % a.pool.page_size) * a.pool.token_stride) * a.size;
+  };
+  for (int i0 = 0; i0 < count; i0 += KP_MOVES) {
+    // the moves, in their order
+    const int i = i0 + tid;
+    int64_t of = -1, to = -1;
+    if (i < count) {
+      const int p = __ldg(path + i);
+      if (p > i) {
+        of = slot(context + p);
+        to = slot(context + i);
+      }
+    }
+    const bool move = of >= 0 && to >= 0;
+    const unsigned some = __ballot_sync(0xffffffffu, move);
+    if (lane == 0) s_moves[warp] = __popc(some);
+    __syncthreads();
+    int at = __popc(some & ((1u << lane) - 1u)), moves = 0;
+#pragma unroll
+    for (int w = 0; w < KP_THREADS / 32; ++w) {
+      if (w < warp) at += s_moves[w];
+      moves += s_moves[w];
+    }
+    if (move) {
+      s_of[at] = of;
+      s_to[at] = to;
+    }
+    __syncthreads();
+    if (moves > 0) {
+      for (int it = blockIdx.y * KP_THREADS + tid; it < items; it += gridDim.y * KP_THREADS) {
+        const int pool = it / words, w = it % words;
+        uint8_t* base = static_cast<uint8_t*>(a.pools[pool]) + (w / per_head) * a.pool.head_stride * a.size + (w % per_head) * 16;
+        for (int m0 = 0; m0 < moves; m0 += KP_AHEAD) {
+          uint4 x[KP_AHEAD];
+#pragma unroll
+          for (int m = 0; m < KP_AHEAD; ++m)
+            if (m0 + m < moves) x[m] = *reinterpret_cast<const uint4*>(base + s_of[m0 + m]);
+#pragma unroll
+          for (int m = 0; m < KP_AHEAD; ++m)
+            if (m0 + m < moves) *reinterpret_cast<uint4*>(base + s_to[m0 + m]) = x[m];
+        }
+      }
+    }
+    __syncthreads();  // the moves are done with
+  }
+  if (says) report(a.batch, wrong);
+}
+
+}  // namespace
+
+cudaError_t launch_keep(const KeepArgs& a, cudaStream_t s) {
+  const int words = a.pool.n_kv * a.pool.head_dim * a.size / 16;
+  const long long items = static_cast<long long>(words) * 2 * a.n_layers;
+  long long y = (items + KP_THREADS - 1) / KP_THREADS;
+  if (y > 65535) y = 65535;
+  keep_kernel<<<dim3(a.batch.n_seqs, unsigned(y)), KP_THREADS, 0, s>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace paged
+}  // namespace wcb

@@ -36,6 +36,7 @@ PAGED_BAD_LEN = 4
 PAGED_BAD_TOKEN = 8
 PAGED_BAD_PROBS = 16
 PAGED_ABORTED = 32
+PAGED_BAD_TREE = 64
 
 EXPORTED = [
     "wcb_gen_config_default", "wcb_model_load", "wcb_model_free", "wcb_model_config_get", "wcb_forward",
@@ -47,7 +48,8 @@ EXPORTED = [
     "wcb_attention_dev",
     "wcb_attention_dev_noalloc", "wcb_tp_id", "wcb_model_tp_handle", "wcb_model_tp_connect", "wcb_model_tp_abort",
     "wcb_load_opts_init", "wcb_struct_layout", "wcb_rope_init", "wcb_paged_append_dev",
-    "wcb_paged_attention_workspace", "wcb_paged_attention_dev", "wcb_spec_verify_dev",
+    "wcb_paged_attention_workspace", "wcb_paged_attention_dev", "wcb_spec_verify_dev", "wcb_paged_tree_fill",
+    "wcb_paged_tree_append_dev", "wcb_paged_tree_attention_dev", "wcb_tree_accept_dev", "wcb_paged_keep_dev", "wcb_sample_dev",
 ]
 
 # the ctypes mirrors of include/wcb.h's structs, checked against the library's
@@ -100,8 +102,18 @@ class _Rope(C.Structure):
                 ("reserved", C.c_uint32), ("inv_freq", C.c_double * 64)]
 
 
+class _PagedTree(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("mask_words", C.c_uint32), ("depth", C.c_void_p), ("mask", C.c_void_p)]
+
+
+class _Sampling(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("reserved", C.c_uint32), ("temperature", C.c_void_p),
+                ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p)]
+
+
 STRUCTS.update({"wcb_load_opts": _LoadOpts, "wcb_model_config": _ModelConfig, "wcb_gen_config": _GenConfig,
-                "wcb_paged_kv": _PagedKV, "wcb_paged_batch": _PagedBatch, "wcb_rope": _Rope})
+                "wcb_paged_kv": _PagedKV, "wcb_paged_batch": _PagedBatch, "wcb_rope": _Rope,
+                "wcb_paged_tree": _PagedTree, "wcb_sampling": _Sampling})
 
 _LIB = None
 
@@ -175,6 +187,12 @@ def lib() -> C.CDLL:
     L.wcb_paged_attention_workspace.argtypes = [vp, vp, u32, C.POINTER(sz)]
     L.wcb_paged_attention_dev.argtypes = [vp, vp, vp, vp, u32, u32, u64, u64, vp, sz, f32, u32, vp, vp]
     L.wcb_spec_verify_dev.argtypes = [vp, vp, vp, vp, vp, vp, u32, u32, u32, vp, vp, u64, u64, u64, u64, vp, vp]
+    L.wcb_paged_tree_fill.argtypes = [vp, u32, u32, vp, vp]
+    L.wcb_paged_tree_append_dev.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, u32, u32, u64, u64, u64, u64, vp, vp, f32, vp]
+    L.wcb_paged_tree_attention_dev.argtypes = [vp, vp, vp, vp, vp, u32, u32, u64, u64, vp, sz, f32, u32, vp, vp]
+    L.wcb_tree_accept_dev.argtypes = [vp, vp, vp, vp, u32, vp, vp, vp, vp]
+    L.wcb_paged_keep_dev.argtypes = [vp, u32, vp, vp, u32, vp, vp]
+    L.wcb_sample_dev.argtypes = [vp, u32, u32, u32, u64, vp, vp, vp, vp, u64, vp, vp]
     L.wcb_tp_id.argtypes = [vp]
     L.wcb_model_tp_handle.argtypes = [u32, vp]
     L.wcb_model_tp_connect.argtypes = [u32, vp, u32]
@@ -647,6 +665,91 @@ def spec_verify_dev(draft_ptr: int, draft_len_ptr: int, target_ptr: int, draft_p
     _check(lib().wcb_spec_verify_dev(draft_ptr, draft_len_ptr, target_ptr, draft_probs_ptr, u_accept_ptr, u_sample_ptr,
                                      n_seqs, max_draft, vocab, tokens_ptr, accepted_ptr, target_seq_stride,
                                      target_row_stride, draft_seq_stride, draft_row_stride, status_ptr, stream))
+
+
+# ---- trees of drafted tokens, sampling --------------------------------------
+class PagedTree:
+    """The shape of a step's new tokens (wcb_paged_tree): device arrays depth [n_tokens]
+    (int32) and mask [n_tokens][mask_words] (32-bit words, bit i: the i-th new token of the
+    sequence is seen). depth_ptr 0: for attention without a window; mask_ptr 0: for append."""
+
+    def __init__(self, depth_ptr: int, mask_ptr: int, mask_words: int):
+        self._c = _PagedTree(C.sizeof(_PagedTree), mask_words, depth_ptr or None, mask_ptr or None)
+        self._at = C.addressof(self._c)
+
+
+def paged_tree_fill(parent: Sequence[int], mask_words: int = 0) -> Tuple[np.ndarray, np.ndarray]:
+    """depth (int32 [n]) and mask (uint32 [n][mask_words]) of one tree, on the host. parent[i] < i:
+    the i-th token's parent; the first is the root. mask_words 0: as many as the tree needs."""
+    p = np.ascontiguousarray(parent, dtype=np.int32)
+    words = mask_words or max(1, -(-p.size // 32))
+    depth, mask = np.empty(p.size, dtype=np.int32), np.empty((p.size, words), dtype=np.uint32)
+    _check(lib().wcb_paged_tree_fill(p.ctypes.data, p.size, words, depth.ctypes.data, mask.ctypes.data))
+    return depth, mask
+
+
+def paged_tree_append_dev(kv: PagedKV, batch: PagedBatch, tree: PagedTree, rope: Optional[Rope], q_ptr: int, k_ptr: int,
+                          v_ptr: int, q_out_ptr: int, dtype: int, n_heads: int, q_stride: int, k_stride: int,
+                          v_stride: int, q_out_stride: int, q_norm_ptr: int = 0, k_norm_ptr: int = 0, eps: float = 1e-5,
+                          stream: int = 0) -> None:
+    """wcb_paged_tree_append_dev: paged_append_dev whose tokens turn by the context's length
+    plus their depth in the tree."""
+    _check(lib().wcb_paged_tree_append_dev(kv._at, batch._at, tree._at, rope._at if rope else None, q_ptr, k_ptr, v_ptr,
+                                          q_out_ptr, dtype, n_heads, q_stride, k_stride, v_stride, q_out_stride,
+                                          q_norm_ptr, k_norm_ptr, eps, stream))
+
+
+def paged_tree_attention_dev(kv: PagedKV, batch: PagedBatch, tree: PagedTree, q_ptr: int, out_ptr: int, dtype: int,
+                             n_heads: int, q_stride: int, out_stride: int, workspace_ptr: int, workspace_bytes: int,
+                             scale: float = 0.0, window: int = 0, lse_ptr: int = 0, stream: int = 0) -> None:
+    """wcb_paged_tree_attention_dev: the new tokens attend to their sequences' context and
+    to those new tokens that the tree's mask names; the rest as in paged_attention_dev."""
+    _check(lib().wcb_paged_tree_attention_dev(kv._at, batch._at, tree._at, q_ptr, out_ptr, dtype, n_heads, q_stride,
+                                             out_stride, workspace_ptr, workspace_bytes, scale, window, lse_ptr,
+                                             stream))
+
+
+def tree_accept_dev(batch: PagedBatch, parent_ptr: int, token_ptr: int, sampled_ptr: int, max_path: int, path_ptr: int,
+                    tokens_ptr: int, count_ptr: int, stream: int = 0) -> None:
+    """wcb_tree_accept_dev: the way down each tree along the sampled tokens: its nodes
+    (path), the tokens sampled at them (tokens, both [n_seqs][max_path], then -1), how many (count)."""
+    _check(lib().wcb_tree_accept_dev(batch._at, parent_ptr, token_ptr, sampled_ptr, max_path, path_ptr, tokens_ptr,
+                                    count_ptr, stream))
+
+
+class PagedLayers:
+    """The pools of a model's layers, alike in all but k and v, for paged_keep_dev."""
+
+    def __init__(self, layers: Sequence[PagedKV]):
+        self._layers = list(layers)
+        self._c = (C.c_void_p * max(1, len(self._layers)))(*[kv._at for kv in self._layers])
+        self._at = C.addressof(self._c)
+
+
+def paged_keep_dev(layers: PagedLayers, batch: PagedBatch, path_ptr: int, max_path: int, count_ptr: int,
+                   stream: int = 0) -> None:
+    """wcb_paged_keep_dev: in every layer, new token path[s][i] moves to the place of the
+    i-th new token of sequence s, i < count[s]."""
+    _check(lib().wcb_paged_keep_dev(layers._at, len(layers._layers), batch._at, path_ptr, max_path, count_ptr, stream))
+
+
+class Sampling:
+    """Each row's settings (wcb_sampling): device arrays temperature, top_p, min_p (float32)
+    and top_k (int32); 0 switches one off."""
+
+    def __init__(self, temperature_ptr: int = 0, top_k_ptr: int = 0, top_p_ptr: int = 0, min_p_ptr: int = 0):
+        self._c = _Sampling(C.sizeof(_Sampling), 0, temperature_ptr or None, top_k_ptr or None, top_p_ptr or None,
+                            min_p_ptr or None)
+        self._at = C.addressof(self._c)
+
+
+def sample_dev(logits_ptr: int, dtype: int, n_rows: int, vocab: int, sampling: Optional[Sampling], u_ptr: int,
+               tokens_ptr: int, row_stride: int = 0, probs_ptr: int = 0, probs_stride: int = 0, status_ptr: int = 0,
+               stream: int = 0) -> None:
+    """wcb_sample_dev: a token of each row of logits (KV_* type) by temperature, top-k, top-p and
+    min-p from given random numbers u; probs_ptr: the probabilities it was drawn from, f32."""
+    _check(lib().wcb_sample_dev(logits_ptr, dtype, n_rows, vocab, row_stride, sampling._at if sampling else None, u_ptr,
+                               tokens_ptr, probs_ptr, probs_stride, status_ptr, stream))
 
 
 def tp_unique_id() -> bytes:
