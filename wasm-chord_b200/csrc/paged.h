@@ -115,6 +115,8 @@ cudaError_t launch_attend_tc(const AttendArgs& a, int act, cudaStream_t s);
 cudaError_t launch_attend_tc32(const AttendArgs& a, int cache, cudaStream_t s);
 cudaError_t launch_tree_16(const AttendArgs& a, int act, int rows, cudaStream_t s);
 cudaError_t launch_tree_32(const AttendArgs& a, int cache, int rows, cudaStream_t s);
+cudaError_t launch_tree_tc(const AttendArgs& a, int act, cudaStream_t s);
+cudaError_t launch_tree_tc32(const AttendArgs& a, int cache, cudaStream_t s);
 cudaError_t launch_accept(const AcceptArgs& a, cudaStream_t s);
 cudaError_t launch_keep(const KeepArgs& a, cudaStream_t s);
 cudaError_t launch_sample(const SampleArgs& a, int kind, cudaStream_t s);

@@ -136,7 +136,7 @@ __device__ __forceinline__ bool tc_wait_warp(TcShared* sh, uint64_t* bar, uint32
 }
 
 // The units of this CTA, walked by every role by itself.
-template <int M, int V>  // rows of a block: one or two tiles of 128; what a unit costs beside its tiles, in tiles
+template <int M, int V, bool TREE>  // rows of a block: one or two tiles of 128; what a unit costs beside its tiles, in tiles
 struct Walk {
   Place pl;
   long long unit0;  // the unit's first place on the line: V, then its tiles
@@ -152,11 +152,11 @@ struct Walk {
     s = pl.seq;
     sq = read_seq(a.batch, s);
     rows = seq_rows(a, sq);
-    const long long ht = head_tiles(a, sq, rows, M, TC_TK, V, table);
+    const long long ht = head_tiles<TREE>(a, sq, rows, M, TC_TK, V, table);
     kvh = quotient(pl.begin - pl.seq_begin, ht);
     unit0 = pl.seq_begin + kvh * ht;
-    rb = find_block(a, sq, rows, M, TC_TK, V, table, pl.begin, unit0);
-    blk = row_block(a, sq, rows, rb, M, TC_TK, table);
+    rb = find_block<TREE>(a, sq, rows, M, TC_TK, V, table, pl.begin, unit0);
+    blk = row_block<TREE>(a, sq, rows, rb, M, TC_TK, table);
     return cut() || next(a);
   }
   // units of no more tiles than they cost otherwise are not cut: they are the part's that they begin in
@@ -185,7 +185,7 @@ struct Walk {
         } while (rows == 0);
       }
     }
-    blk = row_block(a, sq, rows, rb, M, TC_TK, table);
+    blk = row_block<TREE>(a, sq, rows, rb, M, TC_TK, table);
     return cut();
   }
   // tiles [ta, end) that rows 128 w .. of the block need (those after end see nothing); at least
@@ -193,6 +193,7 @@ struct Walk {
   __device__ __forceinline__ int end_of(const AttendArgs& a, int w) const {
     const int r0 = rb * M + 128 * w;
     if (r0 >= rows) return ta;
+    if constexpr (TREE) return tb;
     const int r1 = min(rows, r0 + 128);
     const int hi = min(sq.kv - sq.n + token_of(a, r1 - 1) + 1, table);
     const int t = (max(hi, 0) + TC_TK - 1) / TC_TK - blk.tile0;
@@ -213,6 +214,49 @@ struct Walk {
     }
     return page * a.pool.page_stride + int64_t(key % a.pool.page_size) * a.pool.token_stride;
   }
+};
+
+// What a row sees: of a chain the keys [lo, hi); of a tree those of its context [lo, context) and, below hi, the new tokens that its mask names.
+template <bool TREE>
+struct Sight {
+  int lo, hi, context;
+  const uint32_t* bits;
+  __device__ __forceinline__ Sight(const AttendArgs& a, const Seq& q, int token, int table) {
+    const int first = q.kv - q.n;
+    if constexpr (TREE) {
+      context = first;
+      hi = min(q.kv, table);
+      lo = a.window > 0 ? max(0, first + tree_depth(a, q, token) - a.window + 1) : 0;
+      bits = a.mask + int64_t(q.r0 + token) * a.mask_words;
+    } else {
+      hi = min(first + token + 1, table);
+      lo = a.window > 0 ? max(0, first + token - a.window + 1) : 0;
+    }
+  }
+  // bit c: key + c is seen
+  __device__ __forceinline__ uint32_t of32(const AttendArgs& a, int key) const {
+    auto below = [&](int to) {  // keys below `to`
+      const int n = max(0, min(32, to - key));
+      return n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+    };
+    if constexpr (TREE) {
+      const int at = key - context, w = at >> 5;
+      auto word = [&](int i) { return i >= 0 && i < a.mask_words ? __ldg(bits + i) : 0u; };
+      return ((below(context) & ~below(lo)) | (~below(context) & __funnelshift_r(word(w), word(w + 1), at & 31))) & below(hi);
+    } else {
+      return below(hi) & ~below(lo);
+    }
+  }
+  __device__ __forceinline__ bool has(const AttendArgs& a, int key) const {
+    if constexpr (TREE) {
+      if (key >= context) return key < hi && tree_bit(a, bits, key - context);
+      return key >= lo && key < hi;
+    } else {
+      return key >= lo && key < hi;
+    }
+  }
+  // the first key from `key` on that may be seen
+  __device__ __forceinline__ int from(int key) const { return TREE ? key : max(key, lo); }
 };
 
 // byte offset of 16-byte chunk ch of row r in a swizzled tile
