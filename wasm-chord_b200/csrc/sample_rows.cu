@@ -32,36 +32,41 @@ namespace {
 constexpr int SR_THREADS = 512;
 constexpr int SR_WARPS = SR_THREADS / 32;
 constexpr int SR_CLUSTER = 8;
-constexpr int SR_CACHE = 190 * 1024;     // bytes of a slice in shared memory at most
-constexpr int SR_CACHE_TWO = 82 * 1024;  // so that an SM holds two
-constexpr int FIX = 43;  // bits after the point
+constexpr int SR_CACHE = 176 * 1024;     // bytes of a slice in shared memory at most
+constexpr int SR_CACHE_TWO = 66 * 1024;  // so that an SM holds two
+constexpr int FIX = 43;                  // bits after the point
+constexpr int BINS = 2048;
+constexpr float REACH = 20.0f;  // the bins' width is REACH / BINS; what lies farther from the largest logit is in the last one
+constexpr float SLACK = 2e-5f;  // of a bin's weights: its ends are rounded, and sums of 32 bits
+constexpr float BIN0 = 8388608.0f;  // 2^23: bins as floats, BIN0 + number, so that adding BIN0 rounds to a whole one
+constexpr int DIGITS = 1024;
+constexpr int LIST = 4096;  // tokens that a row's list holds, an equal part for each CTA
+constexpr int CHUNK = 256;  // logits of one warp's round, 8 a lane
 
-// order-preserving bits; 0: no candidate (NaN, -infinity)
+// order-preserving bits of a number (-0 is 0)
 __device__ __forceinline__ uint32_t key_of(float l) {
-  if (!(l >= -FLT_MAX)) return 0;
-  const uint32_t b = __float_as_uint(l + 0.0f);  // (-0 is 0)
+  const uint32_t b = __float_as_uint(l + 0.0f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
-// What is left after a filter: keys above `key`, and those at it up to index `last`.
-struct Kept {
-  uint32_t key;
+// What a filter leaves: logits above `at`, and those at it up to index `last`.
+struct Cut {
+  float at;
   int last;
-  __device__ __forceinline__ bool has(uint32_t k, int i) const { return k > key || (k == key && i <= last); }
+  __device__ __forceinline__ bool has(float l, int i) const { return l > at || (l == at && i <= last); }
 };
-__device__ __forceinline__ Kept stricter(const Kept& a, const Kept& b) {
-  return a.key != b.key ? (a.key > b.key ? a : b) : (a.last < b.last ? a : b);
+__device__ __forceinline__ Cut stricter(const Cut& a, const Cut& b) {
+  return a.at != b.at ? (a.at > b.at ? a : b) : (a.last < b.last ? a : b);
 }
 
 struct Weights {
   double top, rate;  // the largest logit; log2(e) / T
-  // a logit of at most `top`
+  // a logit of at most `top` and at least 60 / rate below it. (Without branches: several of them are computed side by side.)
   __device__ __forceinline__ double of(float l) const {
-    if (double(l) == top) return 1.0;  // (infinities too)
-    const double d = double(l) - top;
     constexpr double BIG = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are the nearest whole number
+    const double d = double(fminf(l, FLT_MAX)) - top;
     const double z = fma(d, rate, BIG);
-    if (!(z >= BIG - 60.0)) return 0.0;  // far below a step (and where infinities are the largest)
     const double f = fma(d, rate, BIG - z);
     double p = 1.0205905413765595794e-7;
     p = fma(p, f, 1.325964524488711024e-6);
@@ -72,7 +77,7 @@ struct Weights {
     p = fma(p, f, 5.5504108664651672007e-2);
     p = fma(p, f, 0.2402265069564033974);
     p = fma(p, f, 0.69314718055994615897);
-    p = fma(p, f, 1.0000000000000134868);
+    p = fma(p, f, 1.0);
     return __hiloint2double(__double2hiint(p) + (__double2loint(z) << 20), __double2loint(p));
   }
 };
@@ -81,27 +86,12 @@ __device__ __forceinline__ unsigned long long fixed(double e) {
   return static_cast<unsigned long long>(__double_as_longlong(e + one) - __double_as_longlong(one));
 }
 
-constexpr int BINS = 2048;
-constexpr float REACH = 20.0f;    // the bins' width is REACH / BINS; what lies farther from the largest logit is in the last one
-constexpr float SLACK = 2e-5f;    // of a bin's weights: its ends are rounded, and sums of 32 bits
-constexpr int DIGITS = 1024;
-constexpr int LIST = 2048;        // tokens that a row's list holds
-constexpr int CHUNK = 256;        // logits of one warp's round
-
 struct SampleShared {
+  uint2 list[LIST];  // logit, index
+  unsigned count[DIGITS], hi[DIGITS];  // of a digit: tokens, the halves of their sum
   union {
-    unsigned bins[BINS];
-    struct {
-      uint32_t key[LIST];
-      int at[LIST];
-    } list;
-  };
-  unsigned count[DIGITS];  // of a digit: tokens, the two halves of their sum
-  union {
-    struct {
-      unsigned lo[DIGITS], hi[DIGITS];
-    };
-    int mine[LIST];  // this CTA's part of the list, until it is gathered
+    unsigned lo[DIGITS];
+    unsigned bins[BINS / 2];  // two counts of 16 bits in a word
   };
   unsigned long long sum[2][3][SR_CLUSTER];  // exchanged
   unsigned long long warp_sum[3][SR_WARPS];
@@ -109,8 +99,14 @@ struct SampleShared {
   unsigned long long pick_before;
   unsigned pick, pick_count;
   int first, last;  // bins between which top-p ends
-  int found, listed;
+  int listed;
 };
+
+// Places of a slice in shared memory: as far behind a multiple of 16 bytes as in memory, filled up with -infinity to whole chunks.
+template <typename T>
+__host__ __device__ constexpr int places(int per) {
+  return (per + 16 / int(sizeof(T)) - 1 + CHUNK - 1) / CHUNK * CHUNK;
+}
 
 // CACHED: the slice fits into shared memory; else it is read again and again
 template <typename T, bool CACHED>
@@ -119,19 +115,34 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
   cg::cluster_group cluster = cg::this_cluster();
   const int C = int(cluster.num_blocks()), rank = int(cluster.block_rank());
   const int row = blockIdx.x / C, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  extern __shared__ __align__(16) unsigned long long chunk_sum[];  // of each CHUNK of the slice; then the slice
+  extern __shared__ __align__(16) unsigned long long chunk_sum[];  // of each chunk of the slice; then the slice
   __shared__ SampleShared sh;
-  const int start = rank * per, mine = max(0, min(per, a.vocab - start));
-  const int chunks = (mine + CHUNK - 1) / CHUNK;
-  const T* logits = static_cast<const T*>(a.logits) + row * a.stride + start;
-  // the slice lies in shared memory as far behind a multiple of 16 bytes as in memory
   constexpr int V = 16 / int(sizeof(T));
-  T* cache = reinterpret_cast<T*>(chunk_sum + ((per + CHUNK - 1) / CHUNK + 1) / 2 * 2) + int((reinterpret_cast<uintptr_t>(logits) & 15) / sizeof(T));
+  const int begin = rank * per, mine = max(0, min(per, a.vocab - begin));
+  const T* slice = static_cast<const T*>(a.logits) + row * a.stride + begin;
+  const int shift = int((reinterpret_cast<uintptr_t>(slice) & 15) / sizeof(T));
+  const int chunks = mine > 0 ? (shift + mine + CHUNK - 1) / CHUNK : 0;
+  const int start = begin - shift;  // index of place 0
+  T* cache = reinterpret_cast<T*>(chunk_sum + (places<T>(per) / CHUNK + 1) / 2 * 2);
   // every CTA of the cluster runs before any writes into another's shared memory
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-  auto logit = [&](int i) {
-    if constexpr (CACHED) return to_f32(cache[i]);
-    else return to_f32(logits[i]);
+  auto logit = [&](int at) {
+    if constexpr (CACHED) return to_f32(cache[at]);
+    else return at >= shift && at < shift + mine ? to_f32(slice[at - shift]) : -INFINITY;
+  };
+  // a lane's 8 logits of a chunk, and where they lie
+  auto place = [&](int c, int j) { return c * CHUNK + (sizeof(T) == 4 ? 128 * (j / 4) + 4 * lane + j % 4 : 8 * lane + j); };
+  auto eight = [&](int c, float (&l)[8]) {
+    if constexpr (CACHED) {
+      alignas(16) T e[8];
+#pragma unroll
+      for (int j = 0; j < 8; j += V) *reinterpret_cast<uint4*>(e + j) = *reinterpret_cast<const uint4*>(cache + place(c, j));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) l[j] = to_f32(e[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) l[j] = logit(place(c, j));
+    }
   };
 
   // A number of each CTA to all CTAs of the cluster (three at a time). What others may still read of the exchange before is the
@@ -156,102 +167,115 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
     for (int r = 0; r < upto; ++r) all += sh.sum[swap][i][r];
     return all;
   };
-
-  // the slice, and the row's largest key with the lowest index that has it
-  uint32_t best = 0;
-  int best_at = 0;
-  auto look = [&](float l, int i) {
-    const uint32_t k = key_of(l);
-    if (k > best || (k == best && i < best_at)) {
-      best = k;
-      best_at = i;
-    }
-  };
-  {
-    const int head = min(mine, int((16 - (reinterpret_cast<uintptr_t>(logits) & 15)) & 15) / int(sizeof(T)));
-    const int words = (mine - head) / V, tail = head + words * V;
-    for (int i = tid; i < head + (mine - tail); i += SR_THREADS) {
-      const int at = i < head ? i : tail + i - head;
-      const T x = logits[at];
-      if constexpr (CACHED) cache[at] = x;
-      look(to_f32(x), at);
-    }
-    const uint4* from = reinterpret_cast<const uint4*>(logits + head);
-    for (int i0 = tid; i0 < words; i0 += 4 * SR_THREADS) {
-      uint4 x[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (i0 + j * SR_THREADS < words) x[j] = __ldg(from + i0 + j * SR_THREADS);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int i = i0 + j * SR_THREADS;
-        if (i < words) {
-          if constexpr (CACHED) *reinterpret_cast<uint4*>(cache + head + i * V) = x[j];
-          alignas(16) T e[V];
-          *reinterpret_cast<uint4*>(e) = x[j];
-#pragma unroll
-          for (int q = 0; q < V; ++q) look(to_f32(e[q]), head + i * V + q);
-        }
-      }
-    }
-    // larger keys first, then lower indices
-    unsigned long long v = (static_cast<unsigned long long>(best) << 32) | uint32_t(~(start + best_at));
+  auto block_max = [&](unsigned long long v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       const unsigned long long x = __shfl_xor_sync(0xffffffffu, v, o);
       v = x > v ? x : v;
     }
     if (lane == 0) sh.warp_sum[0][warp] = v;
-    for (int i = tid; i < BINS; i += SR_THREADS) sh.bins[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < SR_WARPS; ++w) v = sh.warp_sum[0][w] > v ? sh.warp_sum[0][w] : v;
+    return v;
+  };
+
+  // ---- the slice, and the row's largest logit ----
+  float top = -INFINITY;
+  {
+    const int head = shift ? min(mine, V - shift) : 0, words = (mine - head) / V, tail = head + words * V;
+    for (int i = tid; i < head + (mine - tail); i += SR_THREADS) {
+      const int at = i < head ? i : tail + i - head;
+      const T x = slice[at];
+      if constexpr (CACHED) cache[shift + at] = x;
+      top = fmaxf(top, to_f32(x));  // (the number, where the other is NaN)
+    }
+    if constexpr (CACHED) {
+      for (int at = tid; at < shift + chunks * CHUNK - (shift + mine); at += SR_THREADS)
+        cache[at < shift ? at : mine + at] = from_f32<T>(-INFINITY);
+    }
+    const uint4* from = reinterpret_cast<const uint4*>(slice + head);
+    constexpr int AHEAD = 8;
+    for (int i0 = tid; i0 < words; i0 += AHEAD * SR_THREADS) {
+      uint4 x[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j)
+        if (i0 + j * SR_THREADS < words) x[j] = __ldg(from + i0 + j * SR_THREADS);
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const int i = i0 + j * SR_THREADS;
+        if (i < words) {
+          if constexpr (CACHED) *reinterpret_cast<uint4*>(cache + shift + head + i * V) = x[j];
+          alignas(16) T e[V];
+          *reinterpret_cast<uint4*>(e) = x[j];
+#pragma unroll
+          for (int q = 0; q < V; ++q) top = fmaxf(top, to_f32(e[q]));
+        }
+      }
+    }
+    for (int i = tid; i < BINS / 2; i += SR_THREADS) sh.bins[i] = 0;
     if (tid == 0) {
       sh.first = sh.last = BINS - 1;
       sh.listed = 0;
       sh.pick = BINS;
     }
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < SR_WARPS; ++w) v = sh.warp_sum[0][w] > v ? sh.warp_sum[0][w] : v;
+    const unsigned long long v = block_max(key_of(top));
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     exchange(0, v);
     cluster.sync();
-    for (int r = 0; r < C; ++r) v = sh.sum[swap][0][r] > v ? sh.sum[swap][0][r] : v;
-    best = uint32_t(v >> 32);
-    best_at = int(~uint32_t(v));
+    unsigned long long best = v;
+    for (int r = 0; r < C; ++r) best = sh.sum[swap][0][r] > best ? sh.sum[swap][0][r] : best;
+    top = value_of(uint32_t(best));
   }
   float* probs = a.probs ? a.probs + row * a.probs_stride + start : nullptr;
+  const bool some = top > -INFINITY;
   const float temp = a.temperature ? __ldg(a.temperature + row) : 1.0f;
-  if (best == 0 || !(temp > 0.0f)) {  // no candidates, or the largest logit's token
+  if (!some || !(temp > 0.0f)) {  // no candidates, or the largest logit's token: the lowest index that has it
+    int at = INT_MAX;
+    if (some)
+      for (int c = warp; c < chunks; c += SR_WARPS) {
+        float l[8];
+        eight(c, l);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (l[j] == top) at = min(at, start + place(c, j));
+      }
+    __syncthreads();
+    const unsigned long long v = block_max(~uint32_t(at));
+    swap ^= 1;
+    exchange(0, v);
+    cluster.sync();
+    unsigned long long lowest = v;
+    for (int r = 0; r < C; ++r) lowest = sh.sum[swap][0][r] > lowest ? sh.sum[swap][0][r] : lowest;
+    const int token = some ? int(~uint32_t(lowest)) : -1;
     if (rank == 0 && tid == 0) {
-      a.tokens[row] = best == 0 ? -1 : best_at;
-      if (best == 0 && a.status) atomicOr(a.status, uint32_t(ST_BAD_PROBS));
+      a.tokens[row] = token;
+      if (!some && a.status) atomicOr(a.status, uint32_t(ST_BAD_PROBS));
     }
     if (probs)
-      for (int i = tid; i < mine; i += SR_THREADS) probs[i] = best != 0 && start + i == best_at ? 1.0f : 0.0f;
+      for (int i = shift + tid; i < shift + mine; i += SR_THREADS) probs[i] = start + i == token ? 1.0f : 0.0f;
     return;
   }
-  const float top = __uint_as_float(best & 0x80000000u ? best & 0x7fffffffu : ~best);
-  const Weights w{double(top), 1.4426950408889634074 / double(temp)};
+  const float ceiling = fminf(top, FLT_MAX);
+  const Weights w{double(ceiling), 1.4426950408889634074 / double(temp)};
   const int top_k = a.top_k ? __ldg(a.top_k + row) : 0;
   const float top_p = a.top_p ? __ldg(a.top_p + row) : 1.0f, min_p = a.min_p ? __ldg(a.min_p + row) : 0.0f;
   const bool by_k = top_k > 0 && top_k < a.vocab, by_p = top_p < 1.0f;
   const double least = min_p > 0.0f ? fmin(double(min_p), 1.0) : 0.0;
-  const float per_bin = float(BINS) / REACH / temp;
-  // (infinite logits: all others are in the last bin; a temperature without end: all in the first)
-  auto bin_of = [&](float l) { return l == top ? 0 : int(fminf((top - l) * per_bin, float(BINS - 1))); };
-  // the last bin in which min-p leaves something
-  const int least_bin = least > 0.0 ? int(fminf(-logf(float(least)) * (float(BINS) / REACH) * (1.0f + SLACK), float(BINS - 1))) + 1 : BINS;
+  // candidates (NaN is none): where there are infinities, only they; weights below 2^-59 count as none
+  const float lowest = top > FLT_MAX ? INFINITY : -FLT_MAX;
+  const float faint = fmaxf(lowest, ceiling - 41.0f * temp);
+  // A logit's bin, as BIN0 + number: one that is larger is in the same bin or an earlier one.
+  const float per_bin = fminf(float(BINS) / REACH / temp, 1e30f), of_top = ceiling * per_bin;
+  auto bin_of = [&](float l) { return fminf(fmaf(-l, per_bin, of_top), float(BINS - 1)) + BIN0; };
+  auto number = [](float bin) { return int(__float_as_uint(bin) & (BINS - 1)); };
+  // (16 bits count a slice's; of_top's rounding is to be far below a bin)
+  const bool binned = per < 65536 && top <= FLT_MAX && fabsf(of_top) <= 65536.0f;
 
-  // What is kept: `kept`, of bins up to max_bin. Bins below sure are kept whole.
-  Kept kept{1u, INT_MAX};
-  int max_bin = BINS - 1, sure = BINS;
-  auto weight = [&](int i) {
-    const float l = logit(i);
-    const uint32_t k = key_of(l);
-    const int b = bin_of(l);
-    if (!k || b > max_bin || b > least_bin || !(b < sure || kept.has(k, start + i))) return 0.0;
-    const double e = w.of(l);
-    return e >= least ? e : 0.0;
-  };
+  // What is kept: bins up to sure (as bin_of gives them), and what cut has; of both, what min-p leaves.
+  float sure = 2.0f * BIN0;  // all
+  Cut cut{INFINITY, -1};     // none
+  auto keeps = [&](float l, int at) { return l >= faint && (bin_of(l) <= sure || cut.has(l, start + at)); };
 
   // Digits, counted (and summed) here or over all CTAs: the first from the top with which they reach the goal, into sh.pick ..
   auto pick = [&](bool over_all, bool by_weight, unsigned long long before, double goal) {
@@ -287,7 +311,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
     for (int x = 0; x < warp; ++x) prev += sh.warp_sum[0][x];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      if (double(prev) < goal && double(prev + mass[j]) >= goal) {  // one digit: the goal lies above what is before and not above all
+      if (mass[j] > 0 && double(prev) < goal && double(prev + mass[j]) >= goal) {  // one digit: the goal lies above what is before and not above all
         sh.pick = unsigned(d + 1 - j);
         sh.pick_count = cnt[j];
         sh.pick_before = prev;
@@ -296,33 +320,31 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
     }
     __syncthreads();
   };
-
   // Among keys that each() goes through, `bits` of them not known to be the same (the others: prefix), the one with which, from the largest
   // on, the count or the sum of `before` and theirs reaches the goal; in sh.pick_before what comes before it, in sh.pick_count how many there are.
   auto select = [&](auto&& each, bool over_all, uint32_t prefix, int bits, bool by_weight, unsigned long long before, double goal) {
     for (int known = 32 - bits; known < 32;) {
-      const int shift = max(0, 32 - known - 10);
+      const int low = max(0, 32 - known - 10);
       const uint32_t above = known ? ~0u << (32 - known) : 0u;
       if (over_all) cluster.sync();  // the counts before were read
       else __syncthreads();
       for (int i = tid; i < DIGITS; i += SR_THREADS) sh.count[i] = sh.lo[i] = sh.hi[i] = 0;
       __syncthreads();
-      each([&](uint32_t k, float l) {
+      each([&](uint32_t k, unsigned long long f) {
         if ((k & above) != prefix) return;
-        const unsigned d = (k & ~above) >> shift;
+        const unsigned d = (k & ~above) >> low;
         atomicAdd(&sh.count[d], 1u);
         if (by_weight) {
-          const unsigned long long f = fixed(w.of(l));
-          const unsigned lo = unsigned(f), old = atomicAdd(&sh.lo[d], lo);
-          atomicAdd(&sh.hi[d], unsigned(f >> 32) + (old + lo < old ? 1u : 0u));
+          const unsigned x = unsigned(f), old = atomicAdd(&sh.lo[d], x);
+          atomicAdd(&sh.hi[d], unsigned(f >> 32) + (old + x < old ? 1u : 0u));
         }
       });
       if (over_all) cluster.sync();
       else __syncthreads();
       pick(over_all, by_weight, before, goal);
-      prefix |= sh.pick << shift;
+      prefix |= sh.pick << low;
       before = sh.pick_before;
-      known = 32 - shift;
+      known = 32 - low;
     }
     return prefix;
   };
@@ -330,9 +352,8 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
   auto take_of = [&](uint32_t key, bool by_weight, double goal) {
     const double left = goal - double(sh.pick_before);
     if (!by_weight) return unsigned(left);
-    const double e = double(fixed(w.of(__uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key))));
-    const double need = ceil(left / e);
-    return need >= double(sh.pick_count) || !(e > 0.0) ? sh.pick_count : need > 1.0 ? unsigned(need) : 1u;
+    const double need = ceil(left / double(fixed(w.of(value_of(key)))));
+    return need >= double(sh.pick_count) ? sh.pick_count : need > 1.0 ? unsigned(need) : 1u;
   };
 
   // ---- bins: where top-k and top-p end ----
@@ -340,21 +361,26 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
   bool whole = true;              // all of that bin is kept
   int first = BINS, last = -1;    // top-p ends in these bins
   const double p = fmax(double(top_p), 0.0);
-  if (by_k || by_p) {
-    for (int i = tid; i < mine; i += SR_THREADS) {
-      const float l = logit(i);
-      if (key_of(l)) atomicAdd(&sh.bins[bin_of(l)], 1u);
+  if ((by_k || by_p) && binned) {
+    for (int c = warp; c < chunks; c += SR_WARPS) {
+      float l[8];
+      eight(c, l);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int b = number(bin_of(l[j]));
+        if (l[j] >= lowest) atomicAdd(&sh.bins[b >> 1], 1u << (16 * (b & 1)));
+      }
     }
     cluster.sync();
     constexpr int PER = BINS / SR_THREADS;
     static_assert(PER == 4, "four bins a thread");
     unsigned cnt[PER] = {0, 0, 0, 0};
     for (int r = 0; r < C; ++r) {
-      const uint4 n = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(sh.bins, r) + PER * tid);
-      cnt[0] += n.x;
-      cnt[1] += n.y;
-      cnt[2] += n.z;
-      cnt[3] += n.w;
+      const uint2 n = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(sh.bins, r) + 2 * tid);
+      cnt[0] += n.x & 0xffffu;
+      cnt[1] += n.x >> 16;
+      cnt[2] += n.y & 0xffffu;
+      cnt[3] += n.y >> 16;
     }
     if (by_k) {
       const unsigned own = cnt[0] + cnt[1] + cnt[2] + cnt[3];
@@ -382,7 +408,6 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
       if (k_bin < BINS) {
         above_k = int(sh.pick_before);
         whole = above_k + int(sh.pick_count) == top_k;
-        max_bin = k_bin;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
           if (PER * tid + j > k_bin) cnt[j] = 0;
@@ -396,9 +421,9 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
       const float width = REACH / float(BINS) * 1.44269504f;
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
-        const int b = PER * tid + j;
-        up[j] = float(cnt[j]) * exp2f(-width * float(b)) * (1.0f + SLACK);
-        low[j] = b == BINS - 1 ? 0.0f : float(cnt[j]) * exp2f(-width * float(b + 1)) * (1.0f - SLACK);
+        const int b = PER * tid + j;  // logits of b - 1/2 to b + 1/2 widths
+        up[j] = float(cnt[j]) * exp2f(-width * fmaxf(float(b) - 0.5f, 0.0f)) * (1.0f + SLACK);
+        low[j] = b == BINS - 1 ? 0.0f : float(cnt[j]) * exp2f(-width * (float(b) + 0.5f)) * (1.0f - SLACK);
         low_inc += low[j];
         up_inc += up[j];
       }
@@ -443,183 +468,270 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
         atomicMin(&sh.last, must);
       }
       __syncthreads();
-      last = min(sh.last, max_bin);
+      last = min(sh.last, k_bin);
       first = min(sh.first, last);
     }
-    sure = by_p ? first : whole ? max_bin + 1 : k_bin;
+    const int end = by_p ? first : whole ? min(k_bin + 1, BINS) : k_bin;  // bins before it are kept whole
+    sure = BIN0 + float(end - 1);
   }
 
   // ---- one pass: weights, sums of the sure tokens by chunks, the others listed ----
-  unsigned long long sum_above = 0, sum_between = 0;  // above top-p's bins; between them and top-k's end
-  for (int c = warp; c < chunks; c += SR_WARPS) {
-    unsigned long long v = 0;
-#pragma unroll 4
-    for (int e = 0; e < CHUNK / 32; ++e) {
-      const int i = c * CHUNK + 32 * e + lane;
-      if (i >= mine) continue;
-      const float l = logit(i);
-      const int b = bin_of(l);
-      if (!key_of(l) || b > max_bin) continue;
-      if ((b >= first && b <= last) || (b == k_bin && !whole)) {
-        const int at = atomicAdd(&sh.listed, 1);
-        if (at < LIST) sh.mine[at] = i;
-      } else if (by_p || b <= least_bin) {
-        const double x = w.of(l);
-        const unsigned long long f = fixed(x);
-        if (b < sure && x >= least) v += f;
-        if (b < first) sum_above += f;
-        else sum_between += f;
-      }
-    }
+  const bool lists = (by_p || !whole) && binned;
+  const int room = LIST / C;
+  unsigned long long sum_all = 0, sum_above = 0;  // of what is not listed; of that, above top-p's bins
+  if (binned || !(by_k || by_p)) {
+    uint2* list = sh.list + rank * room;
+    const float k_at = BIN0 + float(k_bin), k_end = by_k && k_bin < BINS ? k_at : 2.0f * BIN0;
+    const float list_from = by_p ? BIN0 + float(first) : k_at, list_to = by_p ? BIN0 + float(last) : whole ? 0.0f : k_at;
+    const float k_list = !whole ? k_at : 0.0f;
+    // the last bin whose weights are wanted: of the sure ones, those that min-p may leave; with top-p all
+    const float least_bin = least > 0.0 ? fminf(BIN0 + ceilf(-logf(float(least)) * (float(BINS) / REACH) * (1.0f + SLACK)) + 2.0f, 2.0f * BIN0) : 2.0f * BIN0;
+    const float wanted = !binned ? 2.0f * BIN0 : by_p ? k_end : fminf(sure, least_bin);
+    for (int c = warp; c < chunks; c += SR_WARPS) {
+      unsigned long long v = 0;
+      float l[8];
+      eight(c, l);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if (lane == 0) chunk_sum[c] = v;
+      for (int half = 0; half < 8; half += 4) {
+        bool on[4], sures[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float x = l[half + j], b = bin_of(x);
+          bool listed = false;
+          if (lists) listed = x >= lowest && ((b >= list_from && b <= list_to) || b == k_list);
+          if (listed) {
+            const int at = atomicAdd(&sh.listed, 1);
+            if (at < room) list[at] = make_uint2(__float_as_uint(x), unsigned(start + place(c, half + j)));
+          }
+          on[j] = x >= faint && b <= wanted && !listed;
+          sures[j] = b <= sure;
+        }
+        if (__any_sync(0xffffffffu, on[0] || on[1] || on[2] || on[3])) {
+          double x[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[j] = w.of(l[half + j]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const unsigned long long f = on[j] ? fixed(x[j]) : 0;
+            sum_all += f;
+            if (sures[j]) {
+              if (least > 0.0) {  // (for all threads alike)
+                sum_above += f;
+                if (x[j] >= least) v += f;
+              } else {
+                v += f;
+              }
+            }
+          }
+        }
+      }
+      if (!(least > 0.0)) sum_above += v;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (lane == 0) chunk_sum[c] = v;
+    }
   }
 
-  if (by_p || !whole) {
+  bool fits = binned || !(by_k || by_p);
+  if (lists) {
     block_sum(0, sum_above);
-    block_sum(1, sum_between);
+    block_sum(1, sum_all);
     __syncthreads();
-    const int listed = sh.listed;
+    // sums and lists to every CTA
+    const int listed = min(sh.listed, room);
     swap ^= 1;
     exchange(0, of_warps(0));
     exchange(1, of_warps(1));
-    exchange(2, listed);
+    exchange(2, sh.listed);
+    for (int j = tid; j < listed; j += SR_THREADS) {
+      const uint2 x = sh.list[rank * room + j];
+      for (int r = 1; r < C; ++r) cluster.map_shared_rank(sh.list, (rank + r) % C)[rank * room + j] = x;
+    }
     cluster.sync();
     sum_above = of_cluster(0, C);
-    sum_between = of_cluster(1, C);
-    const unsigned long long total = of_cluster(2, C);
-    bool fits = total <= LIST;
+    sum_all = of_cluster(1, C);
+    int n = 0;
+    for (int r = 0; r < C; ++r) {
+      n += int(sh.sum[swap][2][r]);
+      fits = fits && sh.sum[swap][2][r] <= unsigned(room);
+    }
     if (fits) {
-      // the lists to every CTA, one behind the other
-      const int before = int(of_cluster(2, rank)), n = int(total);
-      for (int j = tid; j < listed; j += SR_THREADS) {
-        const int i = sh.mine[j];
-        const uint32_t k = key_of(logit(i));
-        for (int r = 0; r < C; ++r) {
-          cluster.map_shared_rank(sh.list.key, r)[before + j] = k;
-          cluster.map_shared_rank(sh.list.at, r)[before + j] = start + i;
-        }
-      }
-      cluster.sync();
-      auto value = [](uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); };
-      auto each_listed = [&](int from, int to, auto&& f) {
-        for (int j = tid; j < n; j += SR_THREADS) {
-          const uint32_t k = sh.list.key[j];
-          const float l = value(k);
-          const int b = bin_of(l);
-          if (b >= from && b <= to && (b != k_bin || kept.has(k, sh.list.at[j]))) f(k, l);
+      struct Item {
+        float l;
+        int at, bin;
+        unsigned long long weight;
+      };
+      auto item = [&](int j) {
+        int r = 0;
+        for (; j >= int(sh.sum[swap][2][r]); ++r) j -= int(sh.sum[swap][2][r]);
+        const uint2 x = sh.list[r * room + j];
+        const float l = __uint_as_float(x.x);
+        return Item{l, int(x.y), number(bin_of(l)), l >= faint ? fixed(w.of(l)) : 0};
+      };
+      const Item own = tid < n ? item(tid) : Item{0.0f, 0, 0, 0};
+      auto each_listed = [&](auto&& f) {
+        if (tid < n && (own.bin != k_bin || whole || cut.has(own.l, own.at))) f(own);
+        for (int j = tid + SR_THREADS; j < n; j += SR_THREADS) {
+          const Item x = item(j);
+          if (x.bin != k_bin || whole || cut.has(x.l, x.at)) f(x);
         }
       };
-      // the end among those of bins from .. to
-      auto end_in = [&](int from, int to, bool by_weight, unsigned long long done, double goal) {
-        // bits that are not the same in all of them
+      // the end among those of bins from .. to; same: the bits that are in all of their keys, and those that are in any
+      auto end_in = [&](int from, int to, unsigned long long same, bool by_weight, unsigned long long done, double goal) {
+        const uint32_t any1 = uint32_t(same);
+        const int bits = max(1, 32 - __clz(int(uint32_t(same >> 32) ^ any1)));
+        const uint32_t key = select(
+            [&](auto&& f) {
+              each_listed([&](const Item& x) {
+                if (x.bin >= from && x.bin <= to) f(key_of(x.l), x.weight);
+              });
+            },
+            false, bits == 32 ? 0u : any1 & (~0u << bits), bits, by_weight, done, goal);
+        const unsigned take = take_of(key, by_weight, goal);
+        Cut end{value_of(key), INT_MAX};
+        if (take < sh.pick_count)  // equal logits: those of the lowest indices, which are the largest when turned round
+          end.last = int(~select(
+              [&](auto&& f) {
+                each_listed([&](const Item& x) {
+                  if (x.l == end.at) f(~uint32_t(x.at), 0ull);
+                });
+              },
+              false, ~0u << 20, 20, false, 0, double(take)));
+        return end;
+      };
+      // the sum of the listed, of those in bins from .. to, and the bits of the latter's keys
+      unsigned long long sum_listed = 0, sum_in = 0, same = 0;
+      auto look_at = [&](int from, int to) {
+        unsigned long long v = 0, in = 0;
         uint32_t all1 = ~0u, any1 = 0;
-        each_listed(from, to, [&](uint32_t k, float) {
-          all1 &= k;
-          any1 |= k;
+        each_listed([&](const Item& x) {
+          v += x.weight;
+          if (x.bin >= from && x.bin <= to) {
+            in += x.weight;
+            all1 &= key_of(x.l);
+            any1 |= key_of(x.l);
+          }
         });
         all1 = __reduce_and_sync(0xffffffffu, all1);
         any1 = __reduce_or_sync(0xffffffffu, any1);
         __syncthreads();
-        if (lane == 0) sh.warp_sum[0][warp] = (static_cast<unsigned long long>(all1) << 32) | any1;
+        block_sum(0, v);
+        block_sum(1, in);
+        if (lane == 0) sh.warp_sum[2][warp] = (static_cast<unsigned long long>(all1) << 32) | any1;
         __syncthreads();
+        sum_listed = of_warps(0);
+        sum_in = of_warps(1);
 #pragma unroll
         for (int x = 0; x < SR_WARPS; ++x) {
-          all1 &= uint32_t(sh.warp_sum[0][x] >> 32);
-          any1 |= uint32_t(sh.warp_sum[0][x]);
+          all1 &= uint32_t(sh.warp_sum[2][x] >> 32);
+          any1 |= uint32_t(sh.warp_sum[2][x]);
         }
-        const int bits = max(1, 32 - __clz(int(all1 ^ any1)));
-        const uint32_t key = select([&](auto&& f) { each_listed(from, to, f); }, false, bits == 32 ? 0u : any1 & (~0u << bits), bits, by_weight, done, goal);
-        const unsigned take = take_of(key, by_weight, goal);
-        Kept end{key, INT_MAX};
-        if (take < sh.pick_count) {  // equal logits: those of the lowest indices, which are the largest when turned round
-          end.last = int(~select(
-              [&](auto&& f) {
-                for (int j = tid; j < n; j += SR_THREADS)
-                  if (sh.list.key[j] == key && kept.has(key, sh.list.at[j])) f(~uint32_t(sh.list.at[j]), 0.0f);
-              },
-              false, ~0u << 20, 20, false, 0, double(take)));
-        }
-        return end;
+        same = (static_cast<unsigned long long>(all1) << 32) | any1;
       };
-      if (!whole) kept = end_in(k_bin, k_bin, false, above_k, double(top_k));
+      if (!whole) {
+        cut = Cut{-INFINITY, -1};
+        look_at(k_bin, k_bin);
+        const Cut end = end_in(k_bin, k_bin, same, false, above_k, double(top_k));
+        __syncthreads();
+        cut = end;
+      }
       if (by_p) {
-        unsigned long long v = 0, in_bins = 0;
-        each_listed(0, BINS - 1, [&](uint32_t, float l) { v += fixed(w.of(l)); });
-        if (k_bin > last) each_listed(first, last, [&](uint32_t, float l) { in_bins += fixed(w.of(l)); });
-        __syncthreads();
-        block_sum(0, v);
-        block_sum(1, in_bins);
-        __syncthreads();
-        v = of_warps(0);
-        in_bins = k_bin > last ? of_warps(1) : v;
-        const double goal = fmax(1.0, p * double(sum_above + sum_between + v));
-        if (double(sum_above) < goal && double(sum_above + in_bins) >= goal)
-          kept = stricter(kept, end_in(first, last, true, sum_above, goal));
-        else
-          fits = false;
+        look_at(first, last);
+        const double goal = fmax(1.0, p * double(sum_all + sum_listed));
+        fits = double(sum_above) < goal && double(sum_above + sum_in) >= goal;
+        if (fits) {
+          const Cut end = end_in(first, last, same, true, sum_above, goal);
+          cut = whole ? end : stricter(cut, end);
+        }
       }
       if (fits) {  // what is kept of the CTA's own to its chunks
-        __syncthreads();
-        for (int j = before + tid; j < before + listed; j += SR_THREADS) {
-          const uint32_t k = sh.list.key[j];
-          const int at = sh.list.at[j];
-          if (!kept.has(k, at)) continue;
-          const double x = w.of(value(k));
-          if (x >= least) atomicAdd(&chunk_sum[(at - start) / CHUNK], fixed(x));
-        }
-        __syncthreads();
+        each_listed([&](const Item& x) {
+          const int at = x.at - start;
+          if (at >= shift && at < shift + mine && cut.has(x.l, x.at) && x.l >= faint && (!(least > 0.0) || w.of(x.l) >= least))
+            atomicAdd(&chunk_sum[at / CHUNK], x.weight);
+        });
       }
     }
-    if (!fits) {
-      // the whole row, digit by digit, then its chunks again
-      kept = Kept{1u, INT_MAX};
-      max_bin = BINS - 1;
-      sure = 0;
-      auto each_of_slice = [&](auto&& f) {
-        for (int i = tid; i < mine; i += SR_THREADS) {
-          const float l = logit(i);
-          const uint32_t k = key_of(l);
-          if (k && kept.has(k, start + i)) f(k, l);
-        }
-      };
-      auto end_of_row = [&](bool by_weight, double goal) {
-        const uint32_t key = select(each_of_slice, true, 0u, 32, by_weight, 0, goal);
-        const unsigned take = take_of(key, by_weight, goal);
-        Kept end{key, INT_MAX};
-        if (take < sh.pick_count)
-          end.last = int(~select(
-              [&](auto&& f) {
-                for (int i = tid; i < mine; i += SR_THREADS)
-                  if (key_of(logit(i)) == key && kept.has(key, start + i)) f(~uint32_t(start + i), 0.0f);
-              },
-              true, ~0u << 20, 20, false, 0, double(take)));
-        return end;
-      };
-      if (k_bin < BINS) kept = end_of_row(false, double(top_k));
-      if (by_p) {
-        unsigned long long v = 0;
-        each_of_slice([&](uint32_t, float l) { v += fixed(w.of(l)); });
-        __syncthreads();
-        block_sum(0, v);
-        __syncthreads();
-        swap ^= 1;
-        exchange(0, of_warps(0));
-        cluster.sync();
-        kept = stricter(kept, end_of_row(true, fmax(1.0, p * double(of_cluster(0, C)))));
-      }
-      for (int c = warp; c < chunks; c += SR_WARPS) {
-        unsigned long long v = 0;
-#pragma unroll 4
-        for (int e = 0; e < CHUNK / 32; ++e) {
-          const int i = c * CHUNK + 32 * e + lane;
-          if (i < mine) v += fixed(weight(i));
-        }
+  }
+  // the weights of four logits that are kept, 32 places apart; a whole warp
+  auto weights = [&](int at, double (&x)[4]) {
+    float l[4];
+    bool on[4];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (lane == 0) chunk_sum[c] = v;
+    for (int j = 0; j < 4; ++j) {
+      l[j] = logit(at + 32 * j);
+      on[j] = keeps(l[j], at + 32 * j);
+      x[j] = 0.0;
+    }
+    if (__any_sync(0xffffffffu, on[0] || on[1] || on[2] || on[3])) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const double e = w.of(l[j]);
+        x[j] = on[j] && e >= least ? e : 0.0;
       }
+    }
+  };
+  if (!fits) {
+    // the whole row, digit by digit, then its chunks
+    cut = Cut{-INFINITY, -1};
+    auto each_of_slice = [&](auto&& f) {
+      for (int at = shift + tid; at < shift + mine; at += SR_THREADS) {
+        const float l = logit(at);
+        if (l >= lowest && cut.has(l, start + at)) f(l);
+      }
+    };
+    // the sum of a number over all CTAs' threads
+    auto sum_of_all = [&](unsigned long long v) {
+      __syncthreads();
+      block_sum(0, v);
+      __syncthreads();
+      swap ^= 1;
+      exchange(0, of_warps(0));
+      cluster.sync();
+      return of_cluster(0, C);
+    };
+    auto weight = [&](float l) { return l >= faint ? fixed(w.of(l)) : 0ull; };
+    auto end_of_row = [&](bool by_weight, double goal) {
+      const uint32_t key = select(
+          [&](auto&& f) {
+            each_of_slice([&](float l) { f(key_of(l), by_weight ? weight(l) : 0ull); });
+          },
+          true, 0u, 32, by_weight, 0, goal);
+      const unsigned take = take_of(key, by_weight, goal);
+      Cut end{value_of(key), INT_MAX};
+      if (take < sh.pick_count)
+        end.last = int(~select(
+            [&](auto&& f) {
+              for (int at = shift + tid; at < shift + mine; at += SR_THREADS)
+                if (logit(at) == end.at && cut.has(end.at, start + at)) f(~uint32_t(start + at), 0ull);
+            },
+            true, ~0u << 20, 20, false, 0, double(take)));
+      return end;
+    };
+    if (by_k) {
+      unsigned long long v = 0;
+      each_of_slice([&](float) { ++v; });
+      if (static_cast<unsigned long long>(top_k) < sum_of_all(v)) cut = end_of_row(false, double(top_k));
+    }
+    if (by_p) {
+      unsigned long long v = 0;
+      each_of_slice([&](float l) { v += weight(l); });
+      const double goal = fmax(1.0, p * double(sum_of_all(v)));
+      cut = stricter(cut, end_of_row(true, goal));
+    }
+    sure = NAN;  // no bins: all is the cut's
+    __syncthreads();
+    for (int c = warp; c < chunks; c += SR_WARPS) {
+      unsigned long long v = 0;
+      for (int half = 0; half < CHUNK; half += 128) {
+        double x[4];
+        weights(c * CHUNK + half + lane, x);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v += fixed(x[j]);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (lane == 0) chunk_sum[c] = v;
     }
   }
 
@@ -654,8 +766,11 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
       base += __shfl_sync(0xffffffffu, hit ? inc - v : inc, at);
     }
     for (int e = 0; e < CHUNK / 32; ++e) {
-      const int i = chunk * CHUNK + 32 * e + lane;
-      unsigned long long inc = i < mine ? fixed(weight(i)) : 0;
+      const int at = chunk * CHUNK + 32 * e + lane;
+      const float l = logit(at);
+      double x = keeps(l, at) ? w.of(l) : 0.0;
+      if (x < least) x = 0.0;
+      unsigned long long inc = fixed(x);
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const unsigned long long t = __shfl_up_sync(0xffffffffu, inc, o);
@@ -671,23 +786,30 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
   }
   if (probs) {
     const double inv = 1.0 / (double(all) * (1.0 / double(1ull << FIX)));
-    for (int i = tid; i < mine; i += SR_THREADS) probs[i] = float(weight(i) * inv);
+    for (int c = warp; c < chunks; c += SR_WARPS) {
+      for (int half = 0; half < CHUNK; half += 128) {
+        const int at = c * CHUNK + half + lane;
+        double x[4];
+        weights(at, x);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (at + 32 * j >= shift && at + 32 * j < shift + mine) probs[at + 32 * j] = float(x[j] * inv);
+      }
+    }
   }
 }
 
 template <typename T, bool CACHED>
 cudaError_t run_sample(const SampleArgs& a, int c, int per, size_t shared, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
-  if (CACHED) {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (!(done.load(std::memory_order_acquire) & bit)) {
+    e = cudaFuncSetAttribute(sample_kernel<T, CACHED>, cudaFuncAttributeMaxDynamicSharedMemorySize, SR_CACHE);
     if (e != cudaSuccess) return e;
-    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
-    if (!(done.load(std::memory_order_acquire) & bit)) {
-      e = cudaFuncSetAttribute(sample_kernel<T, CACHED>, cudaFuncAttributeMaxDynamicSharedMemorySize, SR_CACHE);
-      if (e != cudaSuccess) return e;
-      done.fetch_or(bit, std::memory_order_release);
-    }
+    done.fetch_or(bit, std::memory_order_release);
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(a.n_rows) * unsigned(c));
@@ -705,10 +827,10 @@ cudaError_t run_sample(const SampleArgs& a, int c, int per, size_t shared, cudaS
 
 template <typename T>
 cudaError_t run_sample(const SampleArgs& a, cudaStream_t s) {
-  // bytes of a CTA's chunk sums, and of its slice (which may begin up to 16 bytes late)
+  // bytes of a CTA's chunk sums, and of its slice with them
   auto slice = [&](int c) { return (a.vocab + c - 1) / c; };
-  auto sums = [&](int c) { return sizeof(unsigned long long) * size_t(((slice(c) + CHUNK - 1) / CHUNK + 1) / 2 * 2); };
-  auto bytes = [&](int c) { return sums(c) + size_t(slice(c)) * sizeof(T) + 16; };
+  auto sums = [&](int c) { return sizeof(unsigned long long) * size_t((places<T>(slice(c)) / CHUNK + 1) / 2 * 2); };
+  auto bytes = [&](int c) { return sums(c) + size_t(places<T>(slice(c))) * sizeof(T); };
   // CTAs of a row: until there are two for each SM, with slices of at least 1024 logits; more where an SM does not hold two slices
   int c = 1;
   while (c < SR_CLUSTER && ((a.n_rows * c < 2 * SMS && a.vocab / (2 * c) >= 1024) || bytes(c) > size_t(SR_CACHE_TWO))) c *= 2;
