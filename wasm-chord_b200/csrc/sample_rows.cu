@@ -22,6 +22,7 @@
 
 #include <atomic>
 #include <climits>
+#include <type_traits>
 
 #include "paged_common.cuh"
 
@@ -32,14 +33,14 @@ namespace {
 constexpr int SR_THREADS = 512;
 constexpr int SR_WARPS = SR_THREADS / 32;
 constexpr int SR_CLUSTER = 8;
-constexpr int SR_CACHE = 176 * 1024;     // bytes of a slice in shared memory at most
-constexpr int SR_CACHE_TWO = 66 * 1024;  // so that an SM holds two
-constexpr int FIX = 43;                  // bits after the point
+constexpr int SR_CACHE = 66 * 1024;  // bytes of a slice in shared memory at most: an SM holds two
+constexpr int FIX = 43;              // bits after the point
 constexpr int BINS = 2048;
 constexpr float REACH = 20.0f;  // the bins' width is REACH / BINS; what lies farther from the largest logit is in the last one
 constexpr float SLACK = 2e-5f;  // of a bin's weights: its ends are rounded, and sums of 32 bits
 constexpr float BIN0 = 8388608.0f;  // 2^23: bins as floats, BIN0 + number, so that adding BIN0 rounds to a whole one
 constexpr int DIGITS = 1024;
+constexpr int CONTROL = 256;  // threads that go through bins, digits and lists: what they do is no less for being shared by more
 constexpr int LIST = 4096;  // tokens that a row's list holds, an equal part for each CTA
 constexpr int CHUNK = 256;  // logits of one warp's round, 8 a lane
 
@@ -86,20 +87,32 @@ __device__ __forceinline__ unsigned long long fixed(double e) {
   return static_cast<unsigned long long>(__double_as_longlong(e + one) - __double_as_longlong(one));
 }
 
+// the sum over a warp of whole numbers below 2^50
+__device__ __forceinline__ unsigned long long warp_sum50(unsigned long long v) {
+  const unsigned lo = __reduce_add_sync(0xffffffffu, unsigned(v) & 0x1ffffffu);
+  const unsigned hi = __reduce_add_sync(0xffffffffu, unsigned(v >> 25));
+  return (static_cast<unsigned long long>(hi) << 25) + lo;
+}
+
 struct SampleShared {
   uint2 list[LIST];  // logit, index
-  unsigned count[DIGITS], hi[DIGITS];  // of a digit: tokens, the halves of their sum
+  unsigned count[DIGITS];  // of a digit: tokens, the halves of their sum
   union {
-    unsigned lo[DIGITS];
-    unsigned bins[BINS / 2];  // two counts of 16 bits in a word
+    struct {
+      unsigned lo[DIGITS], hi[DIGITS];
+    };
+    unsigned bins[BINS];  // or, packed, two counts of 16 bits in each of half as many words
   };
   unsigned long long sum[2][3][SR_CLUSTER];  // exchanged
   unsigned long long warp_sum[3][SR_WARPS];
-  float warp_low[SR_WARPS], warp_up[SR_WARPS];
+  float warp_low[CONTROL / 32], warp_up[CONTROL / 32];
   unsigned long long pick_before;
   unsigned pick, pick_count;
-  int first, last;  // bins between which top-p ends
-  int listed;
+  uint32_t found;
+  int k_bin, above_k, whole;  // top-k's bin (BINS: there are fewer tokens), tokens above it, whether all of it is kept
+  int first, last;            // bins between which top-p ends
+  int listed, fits;
+  Cut end;
 };
 
 // Places of a slice in shared memory: as far behind a multiple of 16 bytes as in memory, filled up with -infinity to whole chunks.
@@ -139,45 +152,51 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
       for (int j = 0; j < 8; j += V) *reinterpret_cast<uint4*>(e + j) = *reinterpret_cast<const uint4*>(cache + place(c, j));
 #pragma unroll
       for (int j = 0; j < 8; ++j) l[j] = to_f32(e[j]);
+    } else if (c * CHUNK >= shift && (c + 1) * CHUNK <= shift + mine) {
+      alignas(16) T e[8];
+#pragma unroll
+      for (int j = 0; j < 8; j += V) *reinterpret_cast<uint4*>(e + j) = __ldg(reinterpret_cast<const uint4*>(slice - shift + place(c, j)));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) l[j] = to_f32(e[j]);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) l[j] = logit(place(c, j));
     }
   };
 
-  // A number of each CTA to all CTAs of the cluster (three at a time). What others may still read of the exchange before is the
-  // other half of sh.sum.
+  // Numbers of each thread, summed by CTA, to all CTAs of the cluster (three at a time). What others may still read of the exchange before is
+  // the other half of sh.sum.
   int swap = 0;
-  auto exchange = [&](int i, unsigned long long v) {  // every thread the same v
-    if (tid < C) cluster.map_shared_rank(&sh.sum[swap][i][0], tid)[rank] = v;
-  };
   auto block_sum = [&](int i, unsigned long long v) {  // (a barrier follows)
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (lane == 0) sh.warp_sum[i][warp] = v;
   };
-  auto of_warps = [&](int i) {
-    unsigned long long all = 0;
+  auto of_warps = [&](int i) {  // one warp
+    unsigned long long v = lane < SR_WARPS ? sh.warp_sum[i][lane] : 0;
 #pragma unroll
-    for (int w = 0; w < SR_WARPS; ++w) all += sh.warp_sum[i][w];
-    return all;
+    for (int o = SR_WARPS / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  };
+  auto exchange = [&](int i, unsigned long long v) {  // one warp, every lane the same v
+    if (lane < C) cluster.map_shared_rank(&sh.sum[swap][i][0], lane)[rank] = v;
   };
   auto of_cluster = [&](int i, int upto) {
     unsigned long long all = 0;
     for (int r = 0; r < upto; ++r) all += sh.sum[swap][i][r];
     return all;
   };
-  auto block_max = [&](unsigned long long v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const unsigned long long x = __shfl_xor_sync(0xffffffffu, v, o);
-      v = x > v ? x : v;
-    }
+  auto control_sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(CONTROL) : "memory"); };
+  // the largest of a number (above zero) over all CTAs' threads
+  auto max_of_all = [&](uint32_t v) {
+    v = __reduce_max_sync(0xffffffffu, v);
     if (lane == 0) sh.warp_sum[0][warp] = v;
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < SR_WARPS; ++w) v = sh.warp_sum[0][w] > v ? sh.warp_sum[0][w] : v;
-    return v;
+    if (warp == 0) exchange(0, __reduce_max_sync(0xffffffffu, lane < SR_WARPS ? uint32_t(sh.warp_sum[0][lane]) : 0u));
+    cluster.sync();
+    uint32_t best = 0;
+    for (int r = 0; r < C; ++r) best = max(best, uint32_t(sh.sum[swap][0][r]));
+    return best;
   };
 
   // ---- the slice, and the row's largest logit ----
@@ -213,19 +232,15 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
         }
       }
     }
-    for (int i = tid; i < BINS / 2; i += SR_THREADS) sh.bins[i] = 0;
+    for (int i = tid; i < BINS; i += SR_THREADS) sh.bins[i] = 0;
     if (tid == 0) {
       sh.first = sh.last = BINS - 1;
       sh.listed = 0;
-      sh.pick = BINS;
+      sh.k_bin = BINS;
+      sh.whole = 1;
     }
-    const unsigned long long v = block_max(key_of(top));
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-    exchange(0, v);
-    cluster.sync();
-    unsigned long long best = v;
-    for (int r = 0; r < C; ++r) best = sh.sum[swap][0][r] > best ? sh.sum[swap][0][r] : best;
-    top = value_of(uint32_t(best));
+    top = value_of(max_of_all(key_of(top)));
   }
   float* probs = a.probs ? a.probs + row * a.probs_stride + start : nullptr;
   const bool some = top > -INFINITY;
@@ -240,14 +255,8 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
         for (int j = 0; j < 8; ++j)
           if (l[j] == top) at = min(at, start + place(c, j));
       }
-    __syncthreads();
-    const unsigned long long v = block_max(~uint32_t(at));
     swap ^= 1;
-    exchange(0, v);
-    cluster.sync();
-    unsigned long long lowest = v;
-    for (int r = 0; r < C; ++r) lowest = sh.sum[swap][0][r] > lowest ? sh.sum[swap][0][r] : lowest;
-    const int token = some ? int(~uint32_t(lowest)) : -1;
+    const int first_at = int(~max_of_all(~uint32_t(at))), token = some ? first_at : -1;
     if (rank == 0 && tid == 0) {
       a.tokens[row] = token;
       if (!some && a.status) atomicOr(a.status, uint32_t(ST_BAD_PROBS));
@@ -269,36 +278,45 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
   const float per_bin = fminf(float(BINS) / REACH / temp, 1e30f), of_top = ceiling * per_bin;
   auto bin_of = [&](float l) { return fminf(fmaf(-l, per_bin, of_top), float(BINS - 1)) + BIN0; };
   auto number = [](float bin) { return int(__float_as_uint(bin) & (BINS - 1)); };
-  // (16 bits count a slice's; of_top's rounding is to be far below a bin)
-  const bool binned = per < 65536 && top <= FLT_MAX && fabsf(of_top) <= 65536.0f;
+  // (of_top's rounding is to be far below a bin)
+  const bool binned = top <= FLT_MAX && fabsf(of_top) <= 65536.0f;
 
   // What is kept: bins up to sure (as bin_of gives them), and what cut has; of both, what min-p leaves.
   float sure = 2.0f * BIN0;  // all
   Cut cut{INFINITY, -1};     // none
   auto keeps = [&](float l, int at) { return l >= faint && (bin_of(l) <= sure || cut.has(l, start + at)); };
 
-  // Digits, counted (and summed) here or over all CTAs: the first from the top with which they reach the goal, into sh.pick ..
-  auto pick = [&](bool over_all, bool by_weight, unsigned long long before, double goal) {
-    static_assert(DIGITS == 2 * SR_THREADS, "two digits a thread");
-    const int d = DIGITS - 2 - 2 * tid;  // the thread's second one
-    unsigned cnt[2] = {0, 0};
-    unsigned long long mass[2] = {0, 0};
+  // Digits, counted (and summed) here or over all CTAs: the first from the top with which they reach the goal, into sh.pick ..; the
+  // control threads.
+  auto pick = [&](bool over_all, bool by_weight, unsigned long long before, unsigned long long goal) {
+    constexpr int PER = DIGITS / CONTROL;
+    const int d = DIGITS - PER - PER * tid;  // the thread's last one
+    unsigned cnt[PER];
+    unsigned long long mass[PER], own = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      cnt[j] = 0;
+      mass[j] = 0;
+    }
     for (int r = over_all ? 0 : rank; r < (over_all ? C : rank + 1); ++r) {
-      const uint2 n = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(sh.count, r) + d);
-      cnt[0] += n.y;
-      cnt[1] += n.x;
-      if (by_weight) {
-        const uint2 lo = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(sh.lo, r) + d);
-        const uint2 hi = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(sh.hi, r) + d);
-        mass[0] += (static_cast<unsigned long long>(hi.y) << 32) + lo.y;
-        mass[1] += (static_cast<unsigned long long>(hi.x) << 32) + lo.x;
+#pragma unroll
+      for (int j = 0; j < PER; j += 4) {
+        const uint4 n = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(sh.count, r) + d + j);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) cnt[j + q] += (&n.x)[q];
+        if (by_weight) {
+          const uint4 lo = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(sh.lo, r) + d + j);
+          const uint4 hi = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(sh.hi, r) + d + j);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) mass[j + q] += (static_cast<unsigned long long>((&hi.x)[q]) << 32) + (&lo.x)[q];
+        }
       }
     }
-    if (!by_weight) {
-      mass[0] = cnt[0];
-      mass[1] = cnt[1];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      if (!by_weight) mass[j] = cnt[j];
+      own += mass[j];
     }
-    const unsigned long long own = mass[0] + mass[1];
     unsigned long long inc = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -306,30 +324,36 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
       if (lane >= o) inc += t;
     }
     if (lane == 31) sh.warp_sum[0][warp] = inc;
-    __syncthreads();
+    control_sync();
     unsigned long long prev = before + inc - own;
     for (int x = 0; x < warp; ++x) prev += sh.warp_sum[0][x];
+    if (own > 0 && prev < goal && prev + own >= goal) {  // one thread: the goal lies above what is before and not above all
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      if (mass[j] > 0 && double(prev) < goal && double(prev + mass[j]) >= goal) {  // one digit: the goal lies above what is before and not above all
-        sh.pick = unsigned(d + 1 - j);
-        sh.pick_count = cnt[j];
-        sh.pick_before = prev;
+      for (int j = PER - 1; j >= 0; --j) {
+        if (prev < goal && prev + mass[j] >= goal) {
+          sh.pick = unsigned(d + j);
+          sh.pick_count = cnt[j];
+          sh.pick_before = prev;
+        }
+        prev += mass[j];
       }
-      prev += mass[j];
     }
-    __syncthreads();
+    control_sync();
   };
   // Among keys that each() goes through, `bits` of them not known to be the same (the others: prefix), the one with which, from the largest
-  // on, the count or the sum of `before` and theirs reaches the goal; in sh.pick_before what comes before it, in sh.pick_count how many there are.
-  auto select = [&](auto&& each, bool over_all, uint32_t prefix, int bits, bool by_weight, unsigned long long before, double goal) {
+  // on, the count or the sum of `before` and theirs reaches the goal; in sh.pick_before what comes before it, in sh.pick_count how many there
+  // are. Over all CTAs every thread, else the control threads.
+  auto select = [&](auto over_all, auto&& each, uint32_t prefix, int bits, bool by_weight, unsigned long long before, unsigned long long goal) {
+    constexpr bool ALL = decltype(over_all)::value;
     for (int known = 32 - bits; known < 32;) {
       const int low = max(0, 32 - known - 10);
       const uint32_t above = known ? ~0u << (32 - known) : 0u;
-      if (over_all) cluster.sync();  // the counts before were read
-      else __syncthreads();
-      for (int i = tid; i < DIGITS; i += SR_THREADS) sh.count[i] = sh.lo[i] = sh.hi[i] = 0;
-      __syncthreads();
+      if constexpr (ALL) cluster.sync();  // the counts before were read
+      else control_sync();
+      for (int i = 4 * tid; i < DIGITS; i += 4 * (ALL ? SR_THREADS : CONTROL))
+        *reinterpret_cast<uint4*>(sh.count + i) = *reinterpret_cast<uint4*>(sh.lo + i) = *reinterpret_cast<uint4*>(sh.hi + i) = make_uint4(0, 0, 0, 0);
+      if constexpr (ALL) __syncthreads();
+      else control_sync();
       each([&](uint32_t k, unsigned long long f) {
         if ((k & above) != prefix) return;
         const unsigned d = (k & ~above) >> low;
@@ -339,135 +363,188 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
           atomicAdd(&sh.hi[d], unsigned(f >> 32) + (old + x < old ? 1u : 0u));
         }
       });
-      if (over_all) cluster.sync();
-      else __syncthreads();
-      pick(over_all, by_weight, before, goal);
+      if constexpr (ALL) {
+        cluster.sync();
+        if (tid < CONTROL) pick(true, by_weight, before, goal);
+        __syncthreads();
+      } else {
+        control_sync();
+        pick(false, by_weight, before, goal);
+      }
       prefix |= sh.pick << low;
       before = sh.pick_before;
       known = 32 - low;
+      if (!ALL && known < 32 && sh.pick_count == 1) {  // only one has these digits
+        each([&](uint32_t k, unsigned long long) {
+          if ((k & (~0u << low)) == prefix) sh.found = k;
+        });
+        control_sync();
+        prefix = sh.found;
+        break;
+      }
     }
     return prefix;
   };
   // of the tokens at that key, how many it takes
-  auto take_of = [&](uint32_t key, bool by_weight, double goal) {
-    const double left = goal - double(sh.pick_before);
+  auto take_of = [&](uint32_t key, bool by_weight, unsigned long long goal) {
+    const unsigned long long left = goal - sh.pick_before;
     if (!by_weight) return unsigned(left);
-    const double need = ceil(left / double(fixed(w.of(value_of(key)))));
-    return need >= double(sh.pick_count) ? sh.pick_count : need > 1.0 ? unsigned(need) : 1u;
+    const unsigned long long e = fixed(w.of(value_of(key)));
+    return unsigned(min(static_cast<unsigned long long>(sh.pick_count), (left + e - 1) / e));
   };
+  // top-p's goal
+  auto goal_of = [&](unsigned long long sum) { return max(1ull, static_cast<unsigned long long>(ceil(fmax(double(top_p), 0.0) * double(sum)))); };
 
   // ---- bins: where top-k and top-p end ----
-  int k_bin = BINS, above_k = 0;  // top-k's bin, tokens above it
-  bool whole = true;              // all of that bin is kept
-  int first = BINS, last = -1;    // top-p ends in these bins
-  const double p = fmax(double(top_p), 0.0);
+  int k_bin = BINS, above_k = 0;
+  bool whole = true;
+  int first = BINS, last = -1;
   if ((by_k || by_p) && binned) {
+    // (one CTA reads the counts of many: 16 bits a count there)
+    const bool packed = C >= 4 && per < 65536;
+    int far = 0;  // in the last bin
     for (int c = warp; c < chunks; c += SR_WARPS) {
       float l[8];
       eight(c, l);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int b = number(bin_of(l[j]));
-        if (l[j] >= lowest) atomicAdd(&sh.bins[b >> 1], 1u << (16 * (b & 1)));
+        const float b = bin_of(l[j]);
+        if (b < BIN0 + float(BINS - 1)) atomicAdd(&sh.bins[packed ? number(b) >> 1 : number(b)], packed && (number(b) & 1) ? 0x10000u : 1u);
+        else far += l[j] >= lowest ? 1 : 0;
       }
     }
+    far = int(__reduce_add_sync(0xffffffffu, unsigned(far)));
+    if (lane == 0 && far) atomicAdd(&sh.bins[packed ? BINS / 2 - 1 : BINS - 1], packed ? unsigned(far) << 16 : unsigned(far));
     cluster.sync();
-    constexpr int PER = BINS / SR_THREADS;
-    static_assert(PER == 4, "four bins a thread");
-    unsigned cnt[PER] = {0, 0, 0, 0};
-    for (int r = 0; r < C; ++r) {
-      const uint2 n = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(sh.bins, r) + 2 * tid);
-      cnt[0] += n.x & 0xffffu;
-      cnt[1] += n.x >> 16;
-      cnt[2] += n.y & 0xffffu;
-      cnt[3] += n.y >> 16;
-    }
-    if (by_k) {
-      const unsigned own = cnt[0] + cnt[1] + cnt[2] + cnt[3];
-      unsigned inc = own;
+    if (tid < CONTROL) {
+      constexpr int PER = BINS / CONTROL, WORDS = PER / 4;
+      static_assert(PER == 8, "a 16-byte word of packed counts a thread");
+      unsigned cnt[PER];
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const unsigned t = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += t;
-      }
-      if (lane == 31) sh.warp_sum[0][warp] = inc;
-      __syncthreads();
-      unsigned prev = inc - own;
-      for (int x = 0; x < warp; ++x) prev += unsigned(sh.warp_sum[0][x]);
+      for (int j = 0; j < PER; ++j) cnt[j] = 0;
+      // (the loads of eight, or four, CTAs are on their way together)
+      if (packed) {
+        uint4 theirs[SR_CLUSTER];
 #pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        if (prev < unsigned(top_k) && prev + cnt[j] >= unsigned(top_k)) {
-          sh.pick = unsigned(PER * tid + j);
-          sh.pick_before = prev;
-          sh.pick_count = cnt[j];
+        for (int r = 0; r < SR_CLUSTER; ++r) theirs[r] = r < C ? reinterpret_cast<const uint4*>(cluster.map_shared_rank(sh.bins, r))[tid] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < SR_CLUSTER; ++r)
+#pragma unroll
+          for (int j = 0; j < PER; j += 2) {
+            cnt[j] += (&theirs[r].x)[j / 2] & 0xffffu;
+            cnt[j + 1] += (&theirs[r].x)[j / 2] >> 16;
+          }
+      } else {
+#pragma unroll
+        for (int r0 = 0; r0 < SR_CLUSTER; r0 += 4) {
+          if (r0 >= C) break;
+          uint4 theirs[4][WORDS];
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int q = 0; q < WORDS; ++q)
+              theirs[r][q] = r0 + r < C ? reinterpret_cast<const uint4*>(cluster.map_shared_rank(sh.bins, r0 + r))[WORDS * tid + q] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < PER; ++j) cnt[j] += (&theirs[r][j / 4].x)[j % 4];
         }
-        prev += cnt[j];
       }
-      __syncthreads();
-      k_bin = int(sh.pick);  // BINS: there are fewer tokens
-      if (k_bin < BINS) {
-        above_k = int(sh.pick_before);
-        whole = above_k + int(sh.pick_count) == top_k;
+      if (by_k) {
+        unsigned own = 0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) own += cnt[j];
+        unsigned inc = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const unsigned t = __shfl_up_sync(0xffffffffu, inc, o);
+          if (lane >= o) inc += t;
+        }
+        if (lane == 31) sh.warp_sum[0][warp] = inc;
+        control_sync();
+        unsigned prev = inc - own;
+        for (int x = 0; x < warp; ++x) prev += unsigned(sh.warp_sum[0][x]);
+        if (prev < unsigned(top_k) && prev + own >= unsigned(top_k)) {
+#pragma unroll
+          for (int j = 0; j < PER; ++j) {
+            if (prev < unsigned(top_k) && prev + cnt[j] >= unsigned(top_k)) {
+              sh.k_bin = PER * tid + j;
+              sh.above_k = int(prev);
+              sh.whole = prev + cnt[j] == unsigned(top_k);
+            }
+            prev += cnt[j];
+          }
+        }
+        control_sync();
+        if (by_p && sh.k_bin < BINS) {
+#pragma unroll
+          for (int j = 0; j < PER; ++j) {
+            if (PER * tid + j > sh.k_bin) cnt[j] = 0;
+            if (PER * tid + j == sh.k_bin) cnt[j] = unsigned(top_k - sh.above_k);
+          }
+        }
+      }
+      if (by_p) {
+        // lower and upper bounds of the weights up to and with each bin, and of those after it
+        constexpr float STEP = REACH / float(BINS) * 1.44269504f;
+        const float half = exp2f(-0.5f * STEP), unit = half * half;
+        float at = exp2f(-STEP * float(PER * tid)), low_inc = 0.0f, up_inc = 0.0f;
+        float low[PER], up[PER];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {  // logits of b - 1/2 to b + 1/2 widths
+          up[j] = float(cnt[j]) * (at / half);
+          low[j] = PER * tid + j == BINS - 1 ? 0.0f : float(cnt[j]) * (at * half);
+          at *= unit;
+          low_inc += low[j];
+          up_inc += up[j];
+        }
+        float low_sum = low_inc, up_sum = up_inc;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const float x = __shfl_up_sync(0xffffffffu, low_sum, o), y = __shfl_up_sync(0xffffffffu, up_sum, o);
+          if (lane >= o) {
+            low_sum += x;
+            up_sum += y;
+          }
+        }
+        if (lane == 31) {
+          sh.warp_low[warp] = low_sum;
+          sh.warp_up[warp] = up_sum;
+        }
+        control_sync();
+        float low_all = 0.0f, up_all = 0.0f, l = low_sum - low_inc, u = up_sum - up_inc;
+#pragma unroll
+        for (int x = 0; x < CONTROL / 32; ++x) {
+          if (x < warp) {
+            l += sh.warp_low[x];
+            u += sh.warp_up[x];
+          }
+          low_all += sh.warp_low[x];
+          up_all += sh.warp_up[x];
+        }
+        // the end is in the first bin at which (sum so far) (1 - p) >= p (sum after it)
+        const float q = fmaxf(top_p, 0.0f), q1 = 1.0f - q;
+        unsigned may = BINS - 1, must = BINS - 1;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-          if (PER * tid + j > k_bin) cnt[j] = 0;
-          if (PER * tid + j == k_bin) cnt[j] = unsigned(top_k - above_k);
+          l += low[j];
+          u += up[j];
+          if (u * q1 * (1.0f + SLACK) >= q * fmaxf(low_all - l, 0.0f) * (1.0f - SLACK)) may = min(may, unsigned(PER * tid + j));
+          if (l * q1 * (1.0f - SLACK) >= q * fmaxf(up_all - u, 0.0f) * (1.0f + SLACK) + SLACK * up_all) must = min(must, unsigned(PER * tid + j));
+        }
+        may = __reduce_min_sync(0xffffffffu, may);
+        must = __reduce_min_sync(0xffffffffu, must);
+        if (lane == 0) {
+          atomicMin(&sh.first, int(may));
+          atomicMin(&sh.last, int(must));
         }
       }
     }
+    __syncthreads();
+    k_bin = sh.k_bin;
+    above_k = sh.above_k;
+    whole = sh.whole != 0;
     if (by_p) {
-      // lower and upper bounds of the weights up to and with each bin, and of those after it
-      float low[PER], up[PER], low_inc = 0.0f, up_inc = 0.0f;
-      const float width = REACH / float(BINS) * 1.44269504f;
-#pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        const int b = PER * tid + j;  // logits of b - 1/2 to b + 1/2 widths
-        up[j] = float(cnt[j]) * exp2f(-width * fmaxf(float(b) - 0.5f, 0.0f)) * (1.0f + SLACK);
-        low[j] = b == BINS - 1 ? 0.0f : float(cnt[j]) * exp2f(-width * (float(b) + 0.5f)) * (1.0f - SLACK);
-        low_inc += low[j];
-        up_inc += up[j];
-      }
-      float low_sum = low_inc, up_sum = up_inc;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const float x = __shfl_up_sync(0xffffffffu, low_sum, o), y = __shfl_up_sync(0xffffffffu, up_sum, o);
-        if (lane >= o) {
-          low_sum += x;
-          up_sum += y;
-        }
-      }
-      if (lane == 31) {
-        sh.warp_low[warp] = low_sum;
-        sh.warp_up[warp] = up_sum;
-      }
-      __syncthreads();
-      float low_all = 0.0f, up_all = 0.0f, l = low_sum - low_inc, u = up_sum - up_inc;
-#pragma unroll
-      for (int x = 0; x < SR_WARPS; ++x) {
-        if (x < warp) {
-          l += sh.warp_low[x];
-          u += sh.warp_up[x];
-        }
-        low_all += sh.warp_low[x];
-        up_all += sh.warp_up[x];
-      }
-      // the end is in the first bin at which (sum so far) (1 - p) >= p (sum after it)
-      const float q = float(p), q1 = float(1.0 - p);
-      int may = BINS - 1, must = BINS - 1;
-#pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        l += low[j];
-        u += up[j];
-        if (u * q1 * (1.0f + SLACK) >= q * fmaxf(low_all - l, 0.0f) * (1.0f - SLACK)) may = min(may, PER * tid + j);
-        if (l * q1 * (1.0f - SLACK) >= q * fmaxf(up_all - u, 0.0f) * (1.0f + SLACK) + SLACK * up_all) must = min(must, PER * tid + j);
-      }
-      may = int(__reduce_min_sync(0xffffffffu, unsigned(may)));
-      must = int(__reduce_min_sync(0xffffffffu, unsigned(must)));
-      if (lane == 0) {
-        atomicMin(&sh.first, may);
-        atomicMin(&sh.last, must);
-      }
-      __syncthreads();
       last = min(sh.last, k_bin);
       first = min(sh.first, last);
     }
@@ -493,41 +570,50 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
       eight(c, l);
 #pragma unroll
       for (int half = 0; half < 8; half += 4) {
-        bool on[4], sures[4];
+        bool on[4], sures[4], listed[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float x = l[half + j], b = bin_of(x);
-          bool listed = false;
-          if (lists) listed = x >= lowest && ((b >= list_from && b <= list_to) || b == k_list);
-          if (listed) {
-            const int at = atomicAdd(&sh.listed, 1);
-            if (at < room) list[at] = make_uint2(__float_as_uint(x), unsigned(start + place(c, half + j)));
-          }
-          on[j] = x >= faint && b <= wanted && !listed;
+          listed[j] = lists && x >= lowest && ((b >= list_from && b <= list_to) || b == k_list);
+          on[j] = x >= faint && b <= wanted && !listed[j];
           sures[j] = b <= sure;
+        }
+        if (listed[0] || listed[1] || listed[2] || listed[3]) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (listed[j]) {
+              const int at = atomicAdd(&sh.listed, 1);
+              if (at < room) list[at] = make_uint2(__float_as_uint(l[half + j]), unsigned(start + place(c, half + j)));
+            }
         }
         if (__any_sync(0xffffffffu, on[0] || on[1] || on[2] || on[3])) {
           double x[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) x[j] = w.of(l[half + j]);
+          if (least > 0.0) {  // (for all threads alike)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const unsigned long long f = on[j] ? fixed(x[j]) : 0;
-            sum_all += f;
-            if (sures[j]) {
-              if (least > 0.0) {  // (for all threads alike)
-                sum_above += f;
-                if (x[j] >= least) v += f;
-              } else {
-                v += f;
-              }
+            for (int j = 0; j < 4; ++j) {
+              const unsigned long long f = on[j] ? fixed(x[j]) : 0;
+              sum_all += f;
+              if (sures[j]) sum_above += f;
+              if (sures[j] && x[j] >= least) v += f;
             }
+          } else if (by_p) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const unsigned long long f = on[j] ? fixed(x[j]) : 0;
+              sum_all += f;
+              if (sures[j]) v += f;
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (on[j]) v += fixed(x[j]);
           }
         }
       }
       if (!(least > 0.0)) sum_above += v;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      v = warp_sum50(v);
       if (lane == 0) chunk_sum[c] = v;
     }
   }
@@ -540,22 +626,21 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
     // sums and lists to every CTA
     const int listed = min(sh.listed, room);
     swap ^= 1;
-    exchange(0, of_warps(0));
-    exchange(1, of_warps(1));
-    exchange(2, sh.listed);
+    if (warp < 2) exchange(warp, of_warps(warp));
+    if (warp == 2) exchange(2, sh.listed);
     for (int j = tid; j < listed; j += SR_THREADS) {
       const uint2 x = sh.list[rank * room + j];
       for (int r = 1; r < C; ++r) cluster.map_shared_rank(sh.list, (rank + r) % C)[rank * room + j] = x;
     }
     cluster.sync();
-    sum_above = of_cluster(0, C);
-    sum_all = of_cluster(1, C);
-    int n = 0;
-    for (int r = 0; r < C; ++r) {
-      n += int(sh.sum[swap][2][r]);
-      fits = fits && sh.sum[swap][2][r] <= unsigned(room);
-    }
-    if (fits) {
+    if (tid < CONTROL) {
+      sum_above = of_cluster(0, C);
+      sum_all = of_cluster(1, C);
+      int n = 0;
+      for (int r = 0; r < C; ++r) {
+        n += int(sh.sum[swap][2][r]);
+        fits = fits && sh.sum[swap][2][r] <= unsigned(room);
+      }
       struct Item {
         float l;
         int at, bin;
@@ -568,109 +653,142 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
         const float l = __uint_as_float(x.x);
         return Item{l, int(x.y), number(bin_of(l)), l >= faint ? fixed(w.of(l)) : 0};
       };
-      const Item own = tid < n ? item(tid) : Item{0.0f, 0, 0, 0};
-      auto each_listed = [&](auto&& f) {
-        if (tid < n && (own.bin != k_bin || whole || cut.has(own.l, own.at))) f(own);
-        for (int j = tid + SR_THREADS; j < n; j += SR_THREADS) {
-          const Item x = item(j);
-          if (x.bin != k_bin || whole || cut.has(x.l, x.at)) f(x);
+      if (fits && n <= 32) {
+        // few: sorted, a lane each (every warp by itself). Both ends are places in that order.
+        const Item own = lane < n ? item(lane) : Item{-INFINITY, INT_MAX, BINS, 0};
+        float l = own.l;
+        int at = own.at;
+        unsigned long long f = own.weight;
+#pragma unroll
+        for (int k = 2; k <= 32; k *= 2)
+#pragma unroll
+          for (int j = k / 2; j > 0; j /= 2) {
+            const float ol = __shfl_xor_sync(0xffffffffu, l, j);
+            const int oat = __shfl_xor_sync(0xffffffffu, at, j);
+            const unsigned long long of = __shfl_xor_sync(0xffffffffu, f, j);
+            // the larger logit, or of equal ones the lower index, to the front (to the back in every other run)
+            const bool mine_first = l > ol || (l == ol && at < oat), front = ((lane & j) == 0) == ((lane & k) == 0);
+            if (mine_first != front) {
+              l = ol;
+              at = oat;
+              f = of;
+            }
+          }
+        const int bin = number(bin_of(l));
+        const int in_p = __popc(__ballot_sync(0xffffffffu, lane < n && bin <= last)), above = __popc(__ballot_sync(0xffffffffu, lane < n && bin < k_bin));
+        int end = whole ? n : above + (top_k - above_k);  // what top-k leaves of the list
+        if (by_p) {
+          unsigned long long inc = f;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const unsigned long long t = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += t;
+          }
+          const unsigned long long sum_listed = __shfl_sync(0xffffffffu, inc, max(end - 1, 0));
+          const unsigned long long goal = goal_of(sum_all + (end > 0 ? sum_listed : 0));
+          // the first with which the sum reaches the goal
+          const unsigned reached = __ballot_sync(0xffffffffu, lane < min(in_p, end) && sum_above + inc >= goal);
+          fits = sum_above < goal && reached != 0;
+          end = fits ? __ffs(int(reached)) : 1;
         }
-      };
-      // the end among those of bins from .. to; same: the bits that are in all of their keys, and those that are in any
-      auto end_in = [&](int from, int to, unsigned long long same, bool by_weight, unsigned long long done, double goal) {
-        const uint32_t any1 = uint32_t(same);
-        const int bits = max(1, 32 - __clz(int(uint32_t(same >> 32) ^ any1)));
-        const uint32_t key = select(
-            [&](auto&& f) {
-              each_listed([&](const Item& x) {
-                if (x.bin >= from && x.bin <= to) f(key_of(x.l), x.weight);
-              });
-            },
-            false, bits == 32 ? 0u : any1 & (~0u << bits), bits, by_weight, done, goal);
-        const unsigned take = take_of(key, by_weight, goal);
-        Cut end{value_of(key), INT_MAX};
-        if (take < sh.pick_count)  // equal logits: those of the lowest indices, which are the largest when turned round
-          end.last = int(~select(
+        cut = Cut{__shfl_sync(0xffffffffu, l, end - 1), __shfl_sync(0xffffffffu, at, end - 1)};
+      } else if (fits) {
+        const Item own = tid < n ? item(tid) : Item{0.0f, 0, 0, 0};
+        auto each_listed = [&](auto&& f) {
+          if (tid < n && (own.bin != k_bin || whole || cut.has(own.l, own.at))) f(own);
+          for (int j = tid + CONTROL; j < n; j += CONTROL) {
+            const Item x = item(j);
+            if (x.bin != k_bin || whole || cut.has(x.l, x.at)) f(x);
+          }
+        };
+        // the end among those of bins from .. to; same: the bits that are in all of their keys, and those that are in any
+        auto end_in = [&](int from, int to, unsigned long long same, bool by_weight, unsigned long long done, unsigned long long goal) {
+          const uint32_t any1 = uint32_t(same);
+          const int bits = max(1, 32 - __clz(int(uint32_t(same >> 32) ^ any1)));
+          const uint32_t key = select(
+              std::false_type(),
               [&](auto&& f) {
                 each_listed([&](const Item& x) {
-                  if (x.l == end.at) f(~uint32_t(x.at), 0ull);
+                  if (x.bin >= from && x.bin <= to) f(key_of(x.l), x.weight);
                 });
               },
-              false, ~0u << 20, 20, false, 0, double(take)));
-        return end;
-      };
-      // the sum of the listed, of those in bins from .. to, and the bits of the latter's keys
-      unsigned long long sum_listed = 0, sum_in = 0, same = 0;
-      auto look_at = [&](int from, int to) {
-        unsigned long long v = 0, in = 0;
-        uint32_t all1 = ~0u, any1 = 0;
-        each_listed([&](const Item& x) {
-          v += x.weight;
-          if (x.bin >= from && x.bin <= to) {
-            in += x.weight;
-            all1 &= key_of(x.l);
-            any1 |= key_of(x.l);
-          }
-        });
-        all1 = __reduce_and_sync(0xffffffffu, all1);
-        any1 = __reduce_or_sync(0xffffffffu, any1);
-        __syncthreads();
-        block_sum(0, v);
-        block_sum(1, in);
-        if (lane == 0) sh.warp_sum[2][warp] = (static_cast<unsigned long long>(all1) << 32) | any1;
-        __syncthreads();
-        sum_listed = of_warps(0);
-        sum_in = of_warps(1);
+              bits == 32 ? 0u : any1 & (~0u << bits), bits, by_weight, done, goal);
+          const unsigned take = take_of(key, by_weight, goal);
+          Cut end{value_of(key), INT_MAX};
+          if (take < sh.pick_count)  // equal logits: those of the lowest indices, which are the largest when turned round
+            end.last = int(~select(
+                std::false_type(),
+                [&](auto&& f) {
+                  each_listed([&](const Item& x) {
+                    if (x.l == end.at) f(~uint32_t(x.at), 0ull);
+                  });
+                },
+                ~0u << 20, 20, false, 0, take));
+          return end;
+        };
+        // the sum of the listed, of those in bins from .. to, and the bits of the latter's keys
+        unsigned long long sum_listed = 0, sum_in = 0, same = 0;
+        auto look_at = [&](int from, int to) {
+          unsigned long long v = 0, in = 0;
+          uint32_t all1 = ~0u, any1 = 0;
+          each_listed([&](const Item& x) {
+            v += x.weight;
+            if (x.bin >= from && x.bin <= to) {
+              in += x.weight;
+              all1 &= key_of(x.l);
+              any1 |= key_of(x.l);
+            }
+          });
+          all1 = __reduce_and_sync(0xffffffffu, all1);
+          any1 = __reduce_or_sync(0xffffffffu, any1);
+          control_sync();
+          block_sum(0, v);
+          block_sum(1, in);
+          if (lane == 0) sh.warp_sum[2][warp] = (static_cast<unsigned long long>(all1) << 32) | any1;
+          control_sync();
+          sum_listed = sum_in = 0;
 #pragma unroll
-        for (int x = 0; x < SR_WARPS; ++x) {
-          all1 &= uint32_t(sh.warp_sum[2][x] >> 32);
-          any1 |= uint32_t(sh.warp_sum[2][x]);
+          for (int x = 0; x < CONTROL / 32; ++x) {
+            sum_listed += sh.warp_sum[0][x];
+            sum_in += sh.warp_sum[1][x];
+            all1 &= uint32_t(sh.warp_sum[2][x] >> 32);
+            any1 |= uint32_t(sh.warp_sum[2][x]);
+          }
+          same = (static_cast<unsigned long long>(all1) << 32) | any1;
+        };
+        if (!whole) {
+          cut = Cut{-INFINITY, -1};
+          look_at(k_bin, k_bin);
+          cut = end_in(k_bin, k_bin, same, false, above_k, top_k);
         }
-        same = (static_cast<unsigned long long>(all1) << 32) | any1;
-      };
-      if (!whole) {
-        cut = Cut{-INFINITY, -1};
-        look_at(k_bin, k_bin);
-        const Cut end = end_in(k_bin, k_bin, same, false, above_k, double(top_k));
-        __syncthreads();
-        cut = end;
-      }
-      if (by_p) {
-        look_at(first, last);
-        const double goal = fmax(1.0, p * double(sum_all + sum_listed));
-        fits = double(sum_above) < goal && double(sum_above + sum_in) >= goal;
-        if (fits) {
-          const Cut end = end_in(first, last, same, true, sum_above, goal);
-          cut = whole ? end : stricter(cut, end);
+        if (by_p) {
+          look_at(first, last);
+          const unsigned long long goal = goal_of(sum_all + sum_listed);
+          fits = sum_above < goal && sum_above + sum_in >= goal;
+          if (fits) {
+            const Cut end = end_in(first, last, same, true, sum_above, goal);
+            cut = whole ? end : stricter(cut, end);
+          }
         }
       }
-      if (fits) {  // what is kept of the CTA's own to its chunks
-        each_listed([&](const Item& x) {
-          const int at = x.at - start;
-          if (at >= shift && at < shift + mine && cut.has(x.l, x.at) && x.l >= faint && (!(least > 0.0) || w.of(x.l) >= least))
-            atomicAdd(&chunk_sum[at / CHUNK], x.weight);
-        });
+      if (tid == 0) {
+        sh.fits = fits;
+        sh.end = cut;
+      }
+    }
+    __syncthreads();
+    fits = sh.fits != 0;
+    cut = sh.end;
+    if (fits) {  // what is kept of the CTA's own to its chunks
+      for (int j = tid; j < listed; j += SR_THREADS) {
+        const uint2 x = sh.list[rank * room + j];
+        const float l = __uint_as_float(x.x);
+        if (!cut.has(l, int(x.y)) || l < faint) continue;
+        const double e = w.of(l);
+        if (e >= least) atomicAdd(&chunk_sum[(int(x.y) - start) / CHUNK], fixed(e));
       }
     }
   }
-  // the weights of four logits that are kept, 32 places apart; a whole warp
-  auto weights = [&](int at, double (&x)[4]) {
-    float l[4];
-    bool on[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      l[j] = logit(at + 32 * j);
-      on[j] = keeps(l[j], at + 32 * j);
-      x[j] = 0.0;
-    }
-    if (__any_sync(0xffffffffu, on[0] || on[1] || on[2] || on[3])) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const double e = w.of(l[j]);
-        x[j] = on[j] && e >= least ? e : 0.0;
-      }
-    }
-  };
   if (!fits) {
     // the whole row, digit by digit, then its chunks
     cut = Cut{-INFINITY, -1};
@@ -686,51 +804,53 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
       block_sum(0, v);
       __syncthreads();
       swap ^= 1;
-      exchange(0, of_warps(0));
+      if (warp == 0) exchange(0, of_warps(0));
       cluster.sync();
       return of_cluster(0, C);
     };
     auto weight = [&](float l) { return l >= faint ? fixed(w.of(l)) : 0ull; };
-    auto end_of_row = [&](bool by_weight, double goal) {
+    auto end_of_row = [&](bool by_weight, unsigned long long goal) {
       const uint32_t key = select(
+          std::true_type(),
           [&](auto&& f) {
             each_of_slice([&](float l) { f(key_of(l), by_weight ? weight(l) : 0ull); });
           },
-          true, 0u, 32, by_weight, 0, goal);
+          0u, 32, by_weight, 0, goal);
       const unsigned take = take_of(key, by_weight, goal);
       Cut end{value_of(key), INT_MAX};
       if (take < sh.pick_count)
         end.last = int(~select(
+            std::true_type(),
             [&](auto&& f) {
               for (int at = shift + tid; at < shift + mine; at += SR_THREADS)
                 if (logit(at) == end.at && cut.has(end.at, start + at)) f(~uint32_t(start + at), 0ull);
             },
-            true, ~0u << 20, 20, false, 0, double(take)));
+            ~0u << 20, 20, false, 0, take));
       return end;
     };
     if (by_k) {
       unsigned long long v = 0;
       each_of_slice([&](float) { ++v; });
-      if (static_cast<unsigned long long>(top_k) < sum_of_all(v)) cut = end_of_row(false, double(top_k));
+      if (static_cast<unsigned long long>(top_k) < sum_of_all(v)) cut = end_of_row(false, top_k);
     }
     if (by_p) {
       unsigned long long v = 0;
       each_of_slice([&](float l) { v += weight(l); });
-      const double goal = fmax(1.0, p * double(sum_of_all(v)));
-      cut = stricter(cut, end_of_row(true, goal));
+      cut = stricter(cut, end_of_row(true, goal_of(sum_of_all(v))));
     }
     sure = NAN;  // no bins: all is the cut's
     __syncthreads();
     for (int c = warp; c < chunks; c += SR_WARPS) {
       unsigned long long v = 0;
-      for (int half = 0; half < CHUNK; half += 128) {
-        double x[4];
-        weights(c * CHUNK + half + lane, x);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v += fixed(x[j]);
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      float l[8];
+      eight(c, l);
+#pragma unroll 1
+      for (int j = 0; j < 8; ++j)
+        if (keeps(l[j], place(c, j))) {
+          const double e = w.of(l[j]);
+          if (e >= least) v += fixed(e);
+        }
+      v = warp_sum50(v);
       if (lane == 0) chunk_sum[c] = v;
     }
   }
@@ -742,14 +862,14 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
   block_sum(0, acc);
   __syncthreads();
   swap ^= 1;
-  exchange(0, of_warps(0));
+  if (warp == 0) exchange(0, of_warps(0));
   cluster.sync();
   const unsigned long long before = of_cluster(0, rank), own = sh.sum[swap][0][rank], all = of_cluster(0, C);
   float u = __ldg(a.u + row);
   u = u > 0.0f ? fminf(u, 0.99999994f) : 0.0f;
-  const double goal = double(u) * double(all);
-  // the CTA whose slice passes the goal (the sum of all does), in it the chunk, in it the token
-  if (warp == 0 && double(before) <= goal && double(before + own) > goal) {
+  const unsigned long long goal = static_cast<unsigned long long>(double(u) * double(all)) + 1;  // the sum that exceeds u times all
+  // the CTA whose slice reaches the goal (the sum of all does), in it the chunk, in it the token
+  if (warp == 0 && before < goal && before + own >= goal) {
     unsigned long long base = before;
     int chunk = -1;
     for (int c0 = 0; chunk < 0; c0 += 32) {
@@ -760,7 +880,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
         const unsigned long long t = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += t;
       }
-      const unsigned hit = __ballot_sync(0xffffffffu, double(base + inc) > goal);
+      const unsigned hit = __ballot_sync(0xffffffffu, base + inc >= goal);
       const int at = hit ? __ffs(int(hit)) - 1 : 31;
       if (hit) chunk = c0 + at;
       base += __shfl_sync(0xffffffffu, hit ? inc - v : inc, at);
@@ -776,7 +896,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
         const unsigned long long t = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += t;
       }
-      const unsigned hit = __ballot_sync(0xffffffffu, double(base + inc) > goal);
+      const unsigned hit = __ballot_sync(0xffffffffu, base + inc >= goal);
       if (hit) {
         if (lane == 0) a.tokens[row] = start + chunk * CHUNK + 32 * e + __ffs(int(hit)) - 1;
         break;
@@ -786,14 +906,33 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
   }
   if (probs) {
     const double inv = 1.0 / (double(all) * (1.0 / double(1ull << FIX)));
+    // 16 bytes at a time where the rows allow it
+    const bool wide = (reinterpret_cast<uintptr_t>(probs) & 15) == 0;
     for (int c = warp; c < chunks; c += SR_WARPS) {
-      for (int half = 0; half < CHUNK; half += 128) {
-        const int at = c * CHUNK + half + lane;
-        double x[4];
-        weights(at, x);
+      const bool inside = c * CHUNK >= shift && (c + 1) * CHUNK <= shift + mine;
+      float l[8];
+      eight(c, l);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (at + 32 * j >= shift && at + 32 * j < shift + mine) probs[at + 32 * j] = float(x[j] * inv);
+      for (int half = 0; half < 8; half += 4) {
+        bool on[4];
+        float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) on[j] = keeps(l[half + j], place(c, half + j));
+        if (__any_sync(0xffffffffu, on[0] || on[1] || on[2] || on[3])) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const double e = w.of(l[half + j]);
+            y[j] = on[j] && e >= least ? float(e * inv) : 0.0f;
+          }
+        }
+        float* to = probs + place(c, half);
+        if (wide && inside) {
+          *reinterpret_cast<float4*>(to) = make_float4(y[0], y[1], y[2], y[3]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (inside || (place(c, half + j) >= shift && place(c, half + j) < shift + mine)) to[j] = y[j];
+        }
       }
     }
   }
@@ -827,15 +966,15 @@ cudaError_t run_sample(const SampleArgs& a, int c, int per, size_t shared, cudaS
 
 template <typename T>
 cudaError_t run_sample(const SampleArgs& a, cudaStream_t s) {
-  // bytes of a CTA's chunk sums, and of its slice with them
-  auto slice = [&](int c) { return (a.vocab + c - 1) / c; };
-  auto sums = [&](int c) { return sizeof(unsigned long long) * size_t((places<T>(slice(c)) / CHUNK + 1) / 2 * 2); };
-  auto bytes = [&](int c) { return sums(c) + size_t(places<T>(slice(c))) * sizeof(T); };
-  // CTAs of a row: until there are two for each SM, with slices of at least 1024 logits; more where an SM does not hold two slices
+  // CTAs of a row: until there are two for each SM, with slices of at least 1024 logits. What a CTA does beside its logits
+  // costs as much as some ten thousand of them, so that many rows are not cut further to fit into shared memory: (192 rows of 100003, f32,
+  // top-p 0.95) 2 CTAs that read their slices again 107 us, 8 with slices in shared memory 167, 4 of either kind 129 to 170.
   int c = 1;
-  while (c < SR_CLUSTER && ((a.n_rows * c < 2 * SMS && a.vocab / (2 * c) >= 1024) || bytes(c) > size_t(SR_CACHE_TWO))) c *= 2;
-  if (bytes(c) <= size_t(SR_CACHE)) return run_sample<T, true>(a, c, slice(c), bytes(c), s);
-  return run_sample<T, false>(a, c, slice(c), sums(c), s);
+  while (c < SR_CLUSTER && a.n_rows * c < 2 * SMS && a.vocab / (2 * c) >= 1024) c *= 2;
+  const int per = (a.vocab + c - 1) / c;
+  const size_t sums = sizeof(unsigned long long) * size_t((places<T>(per) / CHUNK + 1) / 2 * 2), slice = size_t(places<T>(per)) * sizeof(T);
+  if (sums + slice <= size_t(SR_CACHE)) return run_sample<T, true>(a, c, per, sums + slice, s);
+  return run_sample<T, false>(a, c, per, sums, s);
 }
 
 }  // namespace
