@@ -125,11 +125,12 @@ struct Plan {
   bool tc;
   int split;    // sequences of more rows are the tensor-core kernel's
 };
-Plan plan(uint64_t n_seqs, uint64_t n_kv, uint64_t max_rows) {
+Plan plan(uint64_t n_seqs, uint64_t n_kv, uint64_t max_rows, bool tree) {
   Plan p{};
   p.tc = max_rows > TC_MIN && n_seqs * n_kv * ((max_rows + 31) / 32) > TC_UNITS;
-  p.split = p.tc ? (n_seqs == 1 ? 0 : int(TC_MIN)) : INT_MAX;
-  const uint64_t r = p.tc ? (n_seqs == 1 ? 0 : TC_MIN) : max_rows;
+  const int few = n_seqs == 1 || tree ? 0 : int(TC_MIN);
+  p.split = p.tc ? few : INT_MAX;
+  const uint64_t r = p.tc ? uint64_t(few) : max_rows;
   p.rows = r == 0 ? 0 : r <= 8 ? 8 : r <= 16 ? 16 : 32;
   return p;
 }
@@ -238,7 +239,7 @@ uint32_t attend(const wcb_paged_kv* kv, const wcb_paged_batch* batch, const wcb_
   static const bool withhold = std::getenv("WCB_TEST_WITHHOLD_COPY") != nullptr;
   a.withheld = withhold ? 16 : 0;
   a.wait_ns = withhold ? 20000000ull : 2000000000ull;
-  const Plan p = plan(batch->n_seqs, kv->n_kv_heads, uint64_t(batch->max_q_len) * uint64_t(a.rep));
+  const Plan p = plan(batch->n_seqs, kv->n_kv_heads, uint64_t(batch->max_q_len) * uint64_t(a.rep), tree != nullptr);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
   if (p.tc) {
@@ -304,7 +305,8 @@ uint32_t wcb_paged_attention_workspace(const wcb_paged_kv* kv, const wcb_paged_b
   if (n_heads == 0 || n_heads > 4096 || n_heads % kv->n_kv_heads || n_heads / kv->n_kv_heads > 64)
     return bad("Invalid tensor shape: need n_heads % n_kv_heads == 0 (<= 64 per kv head)");
   const uint64_t rows = uint64_t(batch->max_q_len) * (n_heads / kv->n_kv_heads);
-  *bytes = workspace_bytes(plan(batch->n_seqs, kv->n_kv_heads, rows), pool.head_dim);
+  // (a tree's call needs no more than a chain's)
+  *bytes = workspace_bytes(plan(batch->n_seqs, kv->n_kv_heads, rows, false), pool.head_dim);
   return WCB_OK;
 }
 
