@@ -466,10 +466,11 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
         if (!ok) break;
         tc_fence_after();
 
-        // results: normalised, or a piece [HD][256] + m [256] + l [256]
+        // results: normalised, or a piece [HD / 4][256][4] + m [256] + l [256]
         const bool whole = wk.ta == 0 && wk.tb == wk.blk.tiles;
         constexpr size_t PIECE = size_t(TC_M) * (HD + 2);
-        float* piece = a.part + (size_t(blockIdx.x) * 2 + (wk.ta == 0 ? 1 : 0)) * PIECE + 128 * w + row;
+        float* piece = a.part + (size_t(blockIdx.x) * 2 + (wk.ta == 0 ? 1 : 0)) * PIECE;
+        const int pr = 128 * w + row;  // the row in a piece
         const bool odd = *reinterpret_cast<volatile int*>(&sh.odd[item % ODD_RING]) != 0;
         const int64_t tok = wk.sq.r0 + token_of(a, gr);
         const int hh = wk.kvh * a.rep + head_of(a, gr);
@@ -531,7 +532,8 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
             stage(x, q);
           } else if (row < rn) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) piece[size_t(32 * q + e) * TC_M] = __uint_as_float(v[e]);
+            for (int e = 0; e < 32; e += 4)
+              reinterpret_cast<uint4*>(piece)[size_t(8 * q + e / 4) * TC_M + pr] = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
           }
         }
         tc_fence_before();
@@ -540,8 +542,8 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
           if (whole) {
             if (a.lse) a.lse[tok * a.n_heads + hh] = some ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
           } else {
-            piece[size_t(HD) * TC_M] = m;
-            piece[size_t(HD + 1) * TC_M] = l;
+            piece[size_t(HD) * TC_M + pr] = m;
+            piece[size_t(HD + 1) * TC_M + pr] = l;
           }
         }
         if (row == 0 && w == 0) {
@@ -566,13 +568,13 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
           ++cuts;
           if (sh.last[w]) {
             __threadfence();
-            auto part = [&](int p) { return a.part + (size_t(p) * 2 + (p == c0 ? 1 : 0)) * PIECE + 128 * w + row; };
+            auto part = [&](int p) { return a.part + (size_t(p) * 2 + (p == c0 ? 1 : 0)) * PIECE; };
             float jm = -INFINITY, jl = 0.0f;
             if (row < rn)
-              for (int p = c0; p <= c1; ++p) jm = fmaxf(jm, __ldcg(part(p) + size_t(HD) * TC_M));
+              for (int p = c0; p <= c1; ++p) jm = fmaxf(jm, __ldcg(part(p) + size_t(HD) * TC_M + pr));
             const float u = jm == -INFINITY ? 0.0f : jm;
             if (row < rn)
-              for (int p = c0; p <= c1; ++p) jl += fast_exp2(__ldcg(part(p) + size_t(HD) * TC_M) - u) * __ldcg(part(p) + size_t(HD + 1) * TC_M);
+              for (int p = c0; p <= c1; ++p) jl += fast_exp2(__ldcg(part(p) + size_t(HD) * TC_M + pr) - u) * __ldcg(part(p) + size_t(HD + 1) * TC_M + pr);
             const bool any = jl > 0.0f || jl != jl;
             const float jinv = any ? 1.0f / jl : 0.0f;
 #pragma unroll 1
@@ -584,9 +586,15 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
 #pragma unroll 2
                 for (int p = c0; p <= c1; ++p) {
                   const float* pp = part(p);
-                  const float f = fast_exp2(__ldcg(pp + size_t(HD) * TC_M) - u);
+                  const float f = fast_exp2(__ldcg(pp + size_t(HD) * TC_M + pr) - u);
 #pragma unroll
-                  for (int e = 0; e < 32; ++e) x[e] = fmaf(f, __ldcg(pp + size_t(32 * q + e) * TC_M), x[e]);
+                  for (int e = 0; e < 32; e += 4) {
+                    const float4 y = __ldcg(reinterpret_cast<const float4*>(pp) + size_t(8 * q + e / 4) * TC_M + pr);
+                    x[e] = fmaf(f, y.x, x[e]);
+                    x[e + 1] = fmaf(f, y.y, x[e + 1]);
+                    x[e + 2] = fmaf(f, y.z, x[e + 2]);
+                    x[e + 3] = fmaf(f, y.w, x[e + 3]);
+                  }
                 }
               }
 #pragma unroll

@@ -788,11 +788,12 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
             }
           }
         }
-        // results: normalised, or a piece [HD][M] + m [M] + l [M]
+        // results: normalised, or a piece [HD / 4][M][4] + m [M] + l [M]
         const bool whole = wk.ta == 0 && wk.tb == wk.blk.tiles;
         const int64_t tok = wk.sq.r0 + token_of(a, gr);
         const int hh = wk.kvh * a.rep + head_of(a, gr);
         constexpr size_t PIECE = size_t(M) * (HD + 2);
+        const int pr = 128 * w + row;  // the row in a piece
         // rows leave through shared memory, each warp its own: a thread's row by itself would be 32 lines a store
         auto send = [&] {
           const bool some = (l > 0.0f && m > -INFINITY) || l != l;
@@ -819,11 +820,11 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
         if (whole) {
           send();
         } else if (row < rn) {
-          float* piece = a.part + (size_t(blockIdx.x) * 2 + (wk.ta == 0 ? 1 : 0)) * PIECE + 128 * w + row;
+          float* piece = a.part + (size_t(blockIdx.x) * 2 + (wk.ta == 0 ? 1 : 0)) * PIECE;
 #pragma unroll
-          for (int d = 0; d < HD; ++d) piece[size_t(d) * M] = o[d];
-          piece[size_t(HD) * M] = m;
-          piece[size_t(HD + 1) * M] = l;
+          for (int d = 0; d < HD; d += 4) reinterpret_cast<float4*>(piece)[size_t(d / 4) * M + pr] = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
+          piece[size_t(HD) * M + pr] = m;
+          piece[size_t(HD + 1) * M + pr] = l;
         }
         if (row == 0 && w == 0) {
           uint32_t bits = 0;
@@ -852,16 +853,22 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
 #pragma unroll
             for (int d = 0; d < HD; ++d) o[d] = 0.0f;
             if (row < rn) {
-              auto part = [&](int p) { return a.part + (size_t(p) * 2 + (p == c0 ? 1 : 0)) * PIECE + 128 * w + row; };
-              for (int p = c0; p <= c1; ++p) m = fmaxf(m, __ldcg(part(p) + size_t(HD) * M));
+              auto part = [&](int p) { return a.part + (size_t(p) * 2 + (p == c0 ? 1 : 0)) * PIECE; };
+              for (int p = c0; p <= c1; ++p) m = fmaxf(m, __ldcg(part(p) + size_t(HD) * M + pr));
               const float u = m == -INFINITY ? 0.0f : m;
 #pragma unroll 1
               for (int p = c0; p <= c1; ++p) {
                 const float* pp = part(p);
-                const float f = fast_exp2(__ldcg(pp + size_t(HD) * M) - u);
-                l += f * __ldcg(pp + size_t(HD + 1) * M);
+                const float f = fast_exp2(__ldcg(pp + size_t(HD) * M + pr) - u);
+                l += f * __ldcg(pp + size_t(HD + 1) * M + pr);
 #pragma unroll
-                for (int d = 0; d < HD; ++d) o[d] = fmaf(f, __ldcg(pp + size_t(d) * M), o[d]);
+                for (int d = 0; d < HD; d += 4) {
+                  const float4 y = __ldcg(reinterpret_cast<const float4*>(pp) + size_t(d / 4) * M + pr);
+                  o[d] = fmaf(f, y.x, o[d]);
+                  o[d + 1] = fmaf(f, y.y, o[d + 1]);
+                  o[d + 2] = fmaf(f, y.z, o[d + 2]);
+                  o[d + 3] = fmaf(f, y.w, o[d + 3]);
+                }
               }
             }
             send();
