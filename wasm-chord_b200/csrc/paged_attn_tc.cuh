@@ -332,17 +332,15 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
         // a row's places in q and out, in its thread; other lanes ask for them
         const long long q_at = (wk.sq.r0 + token_of(a, gr)) * a.q_stride + (wk.kvh * a.rep + head_of(a, gr)) * HD;
         const long long o_at = (wk.sq.r0 + token_of(a, gr)) * a.out_stride + (wk.kvh * a.rep + head_of(a, gr)) * HD;
-        {
-          uint4 x[32 / RPI];
+        // (by cp.async: all of them are on their way at once, where loads to registers came one after another, 12000 clocks a unit)
 #pragma unroll
-          for (int j = 0; j < 32 / RPI; ++j) {
-            const int r = RPI * j + lane / CH;
-            const long long from = __shfl_sync(0xffffffffu, q_at, r);
-            x[j] = r32 + r < rn ? __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + from) + lane % CH) : make_uint4(0, 0, 0, 0);
-          }
-#pragma unroll
-          for (int j = 0; j < 32 / RPI; ++j) *reinterpret_cast<uint4*>(qt + tile_at(r32 + RPI * j + lane / CH, lane % CH)) = x[j];
+        for (int j = 0; j < 32 / RPI; ++j) {
+          const int r = RPI * j + lane / CH;
+          const long long from = __shfl_sync(0xffffffffu, q_at, r);
+          cp16(sbase + uint32_t(L::Q + w * L::TILE) + tile_at(r32 + r, lane % CH), static_cast<const T*>(a.q) + from + 8 * (lane % CH), r32 + r < rn);
         }
+        cp_commit();
+        cp_wait<0>();
         fence_proxy_async();
         bar_arrive(&sh.q_full[w]);
 
@@ -490,7 +488,7 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
         };
         auto send = [&] {
           __syncwarp();
-#pragma unroll 4
+#pragma unroll 8
           for (int j = 0; j < 32 / RPI; ++j) {
             const int r = RPI * j + lane / CH;
             const long long to_at = __shfl_sync(0xffffffffu, o_at, r);
@@ -569,12 +567,29 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
           if (sh.last[w]) {
             __threadfence();
             auto part = [&](int p) { return a.part + (size_t(p) * 2 + (p == c0 ? 1 : 0)) * PIECE; };
-            float jm = -INFINITY, jl = 0.0f;
-            if (row < rn)
-              for (int p = c0; p <= c1; ++p) jm = fmaxf(jm, __ldcg(part(p) + size_t(HD) * TC_M + pr));
+            // maxima and sums of up to eight pieces at a time, then 32 dimensions of two: their loads are on the way together
+            float jm = -INFINITY, jl = 0.0f, pm[8], pl[8];
+            auto sums = [&](int p0) {
+#pragma unroll
+              for (int p = 0; p < 8; ++p) {
+                const float* pp = part(min(p0 + p, c1));
+                const bool there = row < rn && p0 + p <= c1;
+                pm[p] = there ? __ldcg(pp + size_t(HD) * TC_M + pr) : -INFINITY;
+                pl[p] = there ? __ldcg(pp + size_t(HD + 1) * TC_M + pr) : 0.0f;
+              }
+            };
+            for (int p0 = c0; p0 <= c1; p0 += 8) {
+              sums(p0);
+#pragma unroll
+              for (int p = 0; p < 8; ++p) jm = fmaxf(jm, pm[p]);
+            }
             const float u = jm == -INFINITY ? 0.0f : jm;
-            if (row < rn)
-              for (int p = c0; p <= c1; ++p) jl += fast_exp2(__ldcg(part(p) + size_t(HD) * TC_M + pr) - u) * __ldcg(part(p) + size_t(HD + 1) * TC_M + pr);
+            for (int p0 = c0; p0 <= c1; p0 += 8) {
+              if (c1 - c0 >= 8) sums(p0);
+#pragma unroll
+              for (int p = 0; p < 8; ++p)
+                if (p0 + p <= c1) jl += fast_exp2(pm[p] - u) * pl[p];
+            }
             const bool any = jl > 0.0f || jl != jl;
             const float jinv = any ? 1.0f / jl : 0.0f;
 #pragma unroll 1
@@ -583,18 +598,29 @@ attend_tc_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ C
 #pragma unroll
               for (int e = 0; e < 32; ++e) x[e] = 0.0f;
               if (row < rn) {
-#pragma unroll 2
-                for (int p = c0; p <= c1; ++p) {
-                  const float* pp = part(p);
-                  const float f = fast_exp2(__ldcg(pp + size_t(HD) * TC_M + pr) - u);
+#pragma unroll 1
+                for (int p = c0; p <= c1; p += 2) {
+                  float4 y[2][8];
+                  float f[2];
 #pragma unroll
-                  for (int e = 0; e < 32; e += 4) {
-                    const float4 y = __ldcg(reinterpret_cast<const float4*>(pp) + size_t(8 * q + e / 4) * TC_M + pr);
-                    x[e] = fmaf(f, y.x, x[e]);
-                    x[e + 1] = fmaf(f, y.y, x[e + 1]);
-                    x[e + 2] = fmaf(f, y.z, x[e + 2]);
-                    x[e + 3] = fmaf(f, y.w, x[e + 3]);
+                  for (int h = 0; h < 2; ++h) {
+                    const float* pp = part(min(p + h, c1));
+                    f[h] = __ldcg(pp + size_t(HD) * TC_M + pr);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[h][e] = __ldcg(reinterpret_cast<const float4*>(pp) + size_t(8 * q + e) * TC_M + pr);
                   }
+#pragma unroll
+                  for (int h = 0; h < 2; ++h)
+                    if (p + h <= c1) {
+                      const float g = fast_exp2(f[h] - u);
+#pragma unroll
+                      for (int e = 0; e < 8; ++e) {
+                        x[4 * e] = fmaf(g, y[h][e].x, x[4 * e]);
+                        x[4 * e + 1] = fmaf(g, y[h][e].y, x[4 * e + 1]);
+                        x[4 * e + 2] = fmaf(g, y[h][e].z, x[4 * e + 2]);
+                        x[4 * e + 3] = fmaf(g, y[h][e].w, x[4 * e + 3]);
+                      }
+                    }
                 }
               }
 #pragma unroll
