@@ -30,7 +30,12 @@ constexpr int AP_PER_SM = 12;
 template <typename AT, typename CT>
 __global__ void __launch_bounds__(AP_THREADS, AP_PER_SM) append_kernel(const __grid_constant__ AppendArgs a) {
   __shared__ int s_seq;
-  __shared__ float2 s_turn[64];
+  // Two turns, or four weights of a norm, in 16 bytes; laid out so that neighbouring threads read neighbouring words (pairs
+  // that are neighbours: turns in their order, which is no slower). 64 trees with norms and halves: 33 -> 30 us.
+  __shared__ float4 s_turn[32], s_norm[2][32];
+  float2* const turns = reinterpret_cast<float2*>(s_turn);
+  auto turn_at = [](int i) { return (i & 3) * 8 + (i >> 2); };   // turns 2i, 2i + 1 of halves
+  auto norm_at = [](int i) { return (i & 1) * 16 + (i >> 1); };  // weights 4i ..
   const int tid = threadIdx.x, row = blockIdx.x;
   const int hd = a.pool.head_dim, nkv = a.pool.n_kv;
   if (tid == 0) s_seq = -1;
@@ -65,7 +70,12 @@ __global__ void __launch_bounds__(AP_THREADS, AP_PER_SM) append_kernel(const __g
     const float f = float(2.0 * (turn - rint(turn)));  // half turns in [-1, 1]
     float sn, cs;
     sincospif(f, &sn, &cs);
-    s_turn[tid] = make_float2(cs, sn);
+    turns[a.halves ? 2 * turn_at(tid >> 1) + (tid & 1) : tid] = make_float2(cs, sn);
+  }
+  if (tid >= 64) {  // (the second half of the threads)
+    const int i = (tid - 64) & 31, which = (tid - 64) >> 5;
+    const float* w = which ? a.k_norm : a.q_norm;
+    if (w && i < hd / 4) s_norm[which][norm_at(i)] = __ldg(reinterpret_cast<const float4*>(w) + i);
   }
   __syncthreads();
 
@@ -112,9 +122,12 @@ __global__ void __launch_bounds__(AP_THREADS, AP_PER_SM) append_kernel(const __g
       for (int o = lph / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       if (on && (is_q || is_k) && w) {
         const float inv = rsqrtf(sum / float(hd) + a.eps);
-        float wx[8], wy[8];
-        load_vec<float, 8>(w + c0, wx);
-        load_vec<float, 8>(w + c1, wy);
+        alignas(16) float wx[8], wy[8];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          *reinterpret_cast<float4*>(wx + 4 * e) = s_norm[is_q ? 0 : 1][norm_at(c0 / 4 + e)];
+          *reinterpret_cast<float4*>(wy + 4 * e) = s_norm[is_q ? 0 : 1][norm_at(c1 / 4 + e)];
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           x[e] = x[e] * inv * wx[e];
@@ -126,18 +139,22 @@ __global__ void __launch_bounds__(AP_THREADS, AP_PER_SM) append_kernel(const __g
     if (a.halves) {
       if (turn0) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float2 t = s_turn[8 * sub + e];
-          const float p = x[e], q = y[e];
+        for (int e = 0; e < 8; e += 2) {
+          const float4 t = s_turn[turn_at(4 * sub + e / 2)];
+          float p = x[e], q = y[e];
           x[e] = p * t.x - q * t.y;
           y[e] = p * t.y + q * t.x;
+          p = x[e + 1];
+          q = y[e + 1];
+          x[e + 1] = p * t.z - q * t.w;
+          y[e + 1] = p * t.w + q * t.z;
         }
       }
     } else {
       auto turn = [&](float (&z)[8], int c) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float2 t = s_turn[c / 2 + e];
+          const float2 t = turns[c / 2 + e];
           const float p = z[2 * e], q = z[2 * e + 1];
           z[2 * e] = p * t.x - q * t.y;
           z[2 * e + 1] = p * t.y + q * t.x;
