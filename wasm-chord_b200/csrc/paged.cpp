@@ -119,7 +119,7 @@ uint32_t check_rows(const void* p, uint64_t stride, uint64_t width, uint32_t dty
 // 256 (32) 45 / 29, of 512 (64) 33 / 40, of 1024 28 / 64; 32 sequences of 40 rows (256) 70 / 114, of 256 87 / 423;
 // f32 over f32: 1 of 128 rows 41 / 34, of 256 47 / 52, 32 of 40 185 / 290; f32 over bf16: 16 of 612 rows 56 / 92;
 // 64/8 heads of 128, bf16: 1 of 64 rows (16) 46 / 32, of 128 (32) 47 / 45, of 256 (64) 53 / 61.
-constexpr uint64_t TC_MIN = 32, TC_UNITS = 32;
+constexpr uint64_t TC_MIN = 32, TC_UNITS = 32, TREE_UNITS = 104;
 struct Plan {
   int rows;     // row block of the mma.sync kernel, 0: not run
   bool tc;
@@ -132,6 +132,10 @@ Plan plan(uint64_t n_seqs, uint64_t n_kv, uint64_t max_rows, bool tree) {
   p.split = p.tc ? few : INT_MAX;
   const uint64_t r = p.tc ? uint64_t(few) : max_rows;
   p.rows = r == 0 ? 0 : r <= 8 ? 8 : r <= 16 ? 16 : 32;
+  // A tree's call that leaves SMs without a block of its own takes smaller blocks, whose tiles take less time each: 208 rows
+  // of 4 key heads over 333 keys in blocks of 32 17.3 us, of 16 17.0, of 8 14.7, over 2000 keys 33, 25 and 25; 26 rows of 32 key heads
+  // over 1000 keys (32 blocks, 64, 128) 24.1, 18.8, 21.4.
+  while (tree && p.rows > 8 && n_seqs * n_kv * ((r + p.rows / 2 - 1) / (p.rows / 2)) <= TREE_UNITS) p.rows /= 2;
   return p;
 }
 

@@ -536,9 +536,11 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
           for (int j = 0; j < 8; ++j) {
             const int r = RPI * (j0 + j) + lane / LPR;
             const long long from = __shfl_sync(0xffffffffu, q_at, r);
-            x[j] = r32 + r < rn ? __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + from) + lane % LPR)
-                                : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            x[j] = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + from) + lane % LPR);  // (of the last row where there is none)
           }
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (r32 + RPI * (j0 + j) + lane / LPR >= rn) x[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             // (a row with an infinity or NaN gives NaN)

@@ -17,6 +17,34 @@ constexpr int KP_THREADS = 128;
 constexpr int KP_MOVES = 128;  // moves that are looked up at a time
 constexpr int KP_AHEAD = 8;    // loads of a thread before its stores
 
+// The moves of this CTA's words, WIDE of them at a time: all loads before the first store
+template <int WIDE>
+__device__ __forceinline__ void move_words(const KeepArgs& a, const int64_t* of, const int64_t* to, int moves, int words, int per_head, int items) {
+  constexpr int AHEAD = KP_AHEAD / WIDE;
+  const int step = gridDim.y * KP_THREADS;
+  for (int it = blockIdx.y * KP_THREADS + threadIdx.x; it < items; it += WIDE * step) {
+    uint8_t* base[WIDE];
+#pragma unroll
+    for (int i = 0; i < WIDE; ++i) {
+      const int at = min(it + i * step, items - 1), pool = at / words, w = at % words;
+      base[i] = static_cast<uint8_t*>(a.pools[pool]) + (w / per_head) * a.pool.head_stride * a.size + (w % per_head) * 16;
+    }
+    for (int m0 = 0; m0 < moves; m0 += AHEAD) {
+      uint4 x[WIDE][AHEAD];
+#pragma unroll
+      for (int i = 0; i < WIDE; ++i)
+#pragma unroll
+        for (int m = 0; m < AHEAD; ++m)
+          if (m0 + m < moves && it + i * step < items) x[i][m] = *reinterpret_cast<const uint4*>(base[i] + of[m0 + m]);
+#pragma unroll
+      for (int i = 0; i < WIDE; ++i)
+#pragma unroll
+        for (int m = 0; m < AHEAD; ++m)
+          if (m0 + m < moves && it + i * step < items) *reinterpret_cast<uint4*>(base[i] + to[m0 + m]) = x[i][m];
+    }
+  }
+}
+
 __global__ void __launch_bounds__(KP_THREADS) keep_kernel(const __grid_constant__ KeepArgs a) {
   __shared__ int64_t s_of[KP_MOVES], s_to[KP_MOVES];
   __shared__ int s_moves[KP_THREADS / 32];
@@ -79,21 +107,10 @@ __global__ void __launch_bounds__(KP_THREADS) keep_kernel(const __grid_constant_
       s_to[at] = to;
     }
     __syncthreads();
-    if (moves > 0) {
-      for (int it = blockIdx.y * KP_THREADS + tid; it < items; it += gridDim.y * KP_THREADS) {
-        const int pool = it / words, w = it % words;
-        uint8_t* base = static_cast<uint8_t*>(a.pools[pool]) + (w / per_head) * a.pool.head_stride * a.size + (w % per_head) * 16;
-        for (int m0 = 0; m0 < moves; m0 += KP_AHEAD) {
-          uint4 x[KP_AHEAD];
-#pragma unroll
-          for (int m = 0; m < KP_AHEAD; ++m)
-            if (m0 + m < moves) x[m] = *reinterpret_cast<const uint4*>(base + s_of[m0 + m]);
-#pragma unroll
-          for (int m = 0; m < KP_AHEAD; ++m)
-            if (m0 + m < moves) *reinterpret_cast<uint4*>(base + s_to[m0 + m]) = x[m];
-        }
-      }
-    }
+    // KP_AHEAD loads of a thread are on their way together: of one word where there are many moves, else of several
+    if (moves > 4) move_words<1>(a, s_of, s_to, moves, words, per_head, items);
+    else if (moves > 2) move_words<2>(a, s_of, s_to, moves, words, per_head, items);
+    else if (moves > 0) move_words<4>(a, s_of, s_to, moves, words, per_head, items);
     __syncthreads();  // the moves are done with
   }
   if (says) report(a.batch, wrong);
@@ -104,8 +121,11 @@ __global__ void __launch_bounds__(KP_THREADS) keep_kernel(const __grid_constant_
 cudaError_t launch_keep(const KeepArgs& a, cudaStream_t s) {
   const int words = a.pool.n_kv * a.pool.head_dim * a.size / 16;
   const long long items = static_cast<long long>(words) * 2 * a.n_layers;
+  // one word of each thread, as far as all CTAs run at once; then more of a thread, so that the lookups are made once for them
   long long y = (items + KP_THREADS - 1) / KP_THREADS;
-  if (y > 65535) y = 65535;
+  // (32 sequences, 80 layers: short paths 11.7 us with 4 CTAs an SM, 12.6 with 8; paths of up to 32 tokens 38 and 35)
+  const long long most = (a.max_path <= 16 ? 4 : 8) * SMS / a.batch.n_seqs;
+  if (y > most) y = most < 1 ? 1 : most;
   keep_kernel<<<dim3(a.batch.n_seqs, unsigned(y)), KP_THREADS, 0, s>>>(a);
   return cudaGetLastError();
 }

@@ -564,33 +564,93 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
     // the last bin whose weights are wanted: of the sure ones, those that min-p may leave; with top-p all
     const float least_bin = least > 0.0 ? fminf(BIN0 + ceilf(-logf(float(least)) * (float(BINS) / REACH) * (1.0f + SLACK)) + 2.0f, 2.0f * BIN0) : 2.0f * BIN0;
     const float wanted = !binned ? 2.0f * BIN0 : by_p ? k_end : fminf(sure, least_bin);
-    for (int c = warp; c < chunks; c += SR_WARPS) {
-      unsigned long long v = 0;
-      float l[8];
-      eight(c, l);
+    auto enlist = [&](float x, int at) {
+      const int n = atomicAdd(&sh.listed, 1);
+      if (n < room) list[n] = make_uint2(__float_as_uint(x), unsigned(start + at));
+    };
+    // what the integer units do for each logit is the bound beside the 64-bit ones, so rows without filters, and with top-p alone, have loops of their own
+    if (!by_k && !by_p && !(least > 0.0)) {
+      for (int c = warp; c < chunks; c += SR_WARPS) {
+        unsigned long long v = 0;
+        float l[8];
+        eight(c, l);
 #pragma unroll
-      for (int half = 0; half < 8; half += 4) {
-        bool on[4], sures[4], listed[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float x = l[half + j], b = bin_of(x);
-          listed[j] = lists && x >= lowest && ((b >= list_from && b <= list_to) || b == k_list);
-          on[j] = x >= faint && b <= wanted && !listed[j];
-          sures[j] = b <= sure;
-        }
-        if (listed[0] || listed[1] || listed[2] || listed[3]) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (listed[j]) {
-              const int at = atomicAdd(&sh.listed, 1);
-              if (at < room) list[at] = make_uint2(__float_as_uint(l[half + j]), unsigned(start + place(c, half + j)));
-            }
-        }
-        if (__any_sync(0xffffffffu, on[0] || on[1] || on[2] || on[3])) {
+        for (int half = 0; half < 8; half += 4) {
           double x[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) x[j] = w.of(l[half + j]);
-          if (least > 0.0) {  // (for all threads alike)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (l[half + j] >= faint) v += fixed(x[j]);
+        }
+        v = warp_sum50(v);
+        if (lane == 0) chunk_sum[c] = v;
+      }
+    } else if (by_p && !by_k && !(least > 0.0)) {
+      for (int c = warp; c < chunks; c += SR_WARPS) {
+        unsigned long long v = 0;
+        float l[8];
+        eight(c, l);
+#pragma unroll
+        for (int half = 0; half < 8; half += 4) {
+          float b[4];
+          double x[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            b[j] = bin_of(l[half + j]);
+            x[j] = w.of(l[half + j]);
+          }
+          bool some = false;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const bool listed = b[j] >= list_from && b[j] <= list_to;
+            some |= listed;
+            if (l[half + j] >= faint && !listed) {
+              const unsigned long long f = fixed(x[j]);
+              sum_all += f;
+              if (b[j] < list_from) v += f;
+            }
+          }
+          if (some) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (b[j] >= list_from && b[j] <= list_to && l[half + j] >= lowest) enlist(l[half + j], place(c, half + j));
+          }
+        }
+        sum_above += v;
+        v = warp_sum50(v);
+        if (lane == 0) chunk_sum[c] = v;
+      }
+    } else {
+      // (past the last bin of interest nothing is done: nearly everywhere, with top-k)
+      const float reach = fmaxf(wanted, fmaxf(list_to, k_list)) - BIN0 + 1.0f;
+      for (int c = warp; c < chunks; c += SR_WARPS) {
+        unsigned long long v = 0;
+        float l[8];
+        eight(c, l);
+#pragma unroll
+        for (int half = 0; half < 8; half += 4) {
+          bool near = false;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) near |= !(fmaf(-l[half + j], per_bin, of_top) > reach);
+          if (!__any_sync(0xffffffffu, near)) continue;
+          bool on[4], sures[4], listed[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float x = l[half + j], b = bin_of(x);
+            listed[j] = lists && x >= lowest && ((b >= list_from && b <= list_to) || b == k_list);
+            on[j] = x >= faint && b <= wanted && !listed[j];
+            sures[j] = b <= sure;
+          }
+          if (listed[0] || listed[1] || listed[2] || listed[3]) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (listed[j]) enlist(l[half + j], place(c, half + j));
+          }
+          if (__any_sync(0xffffffffu, on[0] || on[1] || on[2] || on[3])) {
+            double x[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = w.of(l[half + j]);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const unsigned long long f = on[j] ? fixed(x[j]) : 0;
@@ -598,23 +658,11 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
               if (sures[j]) sum_above += f;
               if (sures[j] && x[j] >= least) v += f;
             }
-          } else if (by_p) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const unsigned long long f = on[j] ? fixed(x[j]) : 0;
-              sum_all += f;
-              if (sures[j]) v += f;
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (on[j]) v += fixed(x[j]);
           }
         }
+        v = warp_sum50(v);
+        if (lane == 0) chunk_sum[c] = v;
       }
-      if (!(least > 0.0)) sum_above += v;
-      v = warp_sum50(v);
-      if (lane == 0) chunk_sum[c] = v;
     }
   }
 
