@@ -243,3 +243,46 @@ def test_two_calls_at_once(gpu):
             wcb.sample_dev(x.data_ptr(), wcb.KV_F32, 64, 20011, s, u.data_ptr(), o.data_ptr(), stream=st.cuda_stream)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(alone, both))
+
+
+# more equal logits than a list holds: found over the whole row, by one CTA a row (300 rows) and by eight (3 rows); fewer: in the list
+@pytest.mark.parametrize("n,v", [(300, 9001), (3, 70001), (300, 700), (3, 20000)])
+@pytest.mark.parametrize("step", [0.0, 0.25])
+def test_many_equal_logits(gpu, n, v, step):
+    r = np.random.RandomState(n + v)
+    l = np.floor(r.rand(n, v) * 6).astype(np.float32) * step
+    kinds = [(1.0, 0, 0.5, 0.0), (0.7, v // 3, 1.0, 0.0), (1.0, v // 2, 0.9, 0.0), (0.5, v - 1, 0.99, 0.2), (1.0, 33, 0.7, 0.0), (1.0, 0, 2.0 ** -10, 0.0)]
+    t, k, p, m = (list(x) for x in zip(*[kinds[i % len(kinds)] for i in range(n)]))
+    check(l, "f32", t, k, p, m, r.rand(n).tolist())
+
+
+# logits far from zero, temperatures so low that a bin is no more than their rounding: without bins
+@pytest.mark.parametrize("offset,t", [(1e5, 1.0), (-3e6, 50.0), (0.0, 1e-3), (2000.0, 0.3)])
+@pytest.mark.parametrize("v", [500, 30001])
+def test_logits_far_from_zero(gpu, offset, t, v):
+    r = np.random.RandomState(v)
+    l = (r.randn(6, v) * 2.5 + offset).astype(np.float32)
+    check(l, "f32", [t] * 6, [0, 40, 0, 900, 0, 5], [0.9, 1.0, 1.0, 0.95, 0.3, 0.5], [0.0, 0.0, 0.05, 0.0, 0.01, 0.0], r.rand(6).tolist())
+
+
+def test_flat_rows(gpu):
+    # next to no differences: every weight counts
+    r = np.random.RandomState(3)
+    l = (r.randn(4, 131072) * 0.05).astype(np.float32)
+    check(l, "f32", [1.0, 2.0, 0.7, 1.0], [0, 0, 100000, 50], [0.9, 0.99, 0.5, 1.0], [0.0] * 4, r.rand(4).tolist())
+
+
+def test_rows_far_apart(gpu):
+    # offsets past 32 bits: the second row begins 5 GB behind the first (of one buffer)
+    v, stride = 1001, 1_300_000_000
+    if torch.cuda.mem_get_info()[0] < 12e9:
+        pytest.skip("needs 11 GB")
+    rows = torch.empty(2 * stride, dtype=torch.float32, device="cuda")
+    r = np.random.RandomState(4)
+    l = r.randn(2, v).astype(np.float32)
+    for i in range(2):
+        rows[i * stride:i * stride + v] = torch.tensor(l[i], device="cuda")
+    u = torch.tensor([0.3, 0.8], device="cuda")
+    out = torch.empty(2, dtype=torch.int32, device="cuda")
+    wcb.sample_dev(rows.data_ptr(), wcb.KV_F32, 2, v, None, u.data_ptr(), out.data_ptr(), row_stride=stride)
+    assert out.tolist() == sample_plain(l.astype(np.float64), [1.0] * 2, [0] * 2, [1.0] * 2, [0.0] * 2, u.double().cpu().numpy())[0]

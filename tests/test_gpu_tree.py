@@ -593,3 +593,109 @@ def test_steps_with_trees(gpu, act, cache):
         for x in steps:
             x.kv_len = s.kv_len
     assert accepted >= 4 and int(s.status.item()) == 0
+
+
+# ---- calls side by side -----------------------------------------------------------------
+
+def test_trees_and_chains_share_a_workspace(gpu):
+    a = Tree([40, 3], [3000, 500], 8, 2, 128, "f16", "f16", 16, seed=80)
+    b = Step([4, 1, 200], [900, 2500, 800], 8, 2, 128, "f16", "f16", 16, seed=81)
+    room = max((a.workspace(), b.workspace()), key=lambda w: w.numel())
+    graphs = []
+    for s in (a, b):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            s.attend(room=room, stream=torch.cuda.current_stream().cuda_stream)
+        graphs.append(g)
+    for order in ((0, 1), (1, 0), (0, 0, 1, 1)):
+        for s in (a, b):
+            s.out.fill_(7.0)
+            s.lse.fill_(7.0)
+        for i in order:
+            graphs[i].replay()
+        a.check()
+        b.check()
+    assert (room[:4096] == 0).all()
+
+
+def test_two_streams(gpu):
+    s = [Tree([30, 1, 64], [3000, 500, 900], 8, 2, 64, *pair, 16, seed=82 + i) for i, pair in enumerate([("f16", "f16"), ("f32", "f32")])]
+    rooms, streams = [x.workspace() for x in s], [torch.cuda.Stream() for _ in s]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for x, r, st in zip(s, rooms, streams):
+            x.attend(room=r, stream=st.cuda_stream)
+    torch.cuda.synchronize()
+    for x in s:
+        x.check()
+
+
+def _run(code, env=None):
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = code.format(pkg=os.path.join(os.path.dirname(here), "wasm-chord_b200"), tests=here)
+    return subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, env=dict(os.environ, **(env or {})))
+
+
+FIRST_CALLS = """
+import sys
+sys.path.insert(0, {pkg!r}); sys.path.insert(0, {tests!r})
+import torch, wcb, numpy as np
+import test_gpu_tree as t
+for act, cache in t.PAIRS:
+    for q_len in ([5, 2], [90, 3]):
+        s = t.Tree(q_len, [300, 40], 8, 2, 64, act, cache, 16, seed=40)
+        room, graph = s.workspace(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            s.attend(room=room, stream=torch.cuda.current_stream().cuda_stream)
+        graph.replay()
+        graph.replay()
+        s.check()
+from test_gpu_sample import sample_plain, KIND
+for kind in KIND:
+    for n, v in ((2, 5000), (1, 900001)):
+        l = torch.randn(n, v, device="cuda").to(KIND[kind][0])
+        u, out, p = torch.rand(n, device="cuda"), torch.empty(n, dtype=torch.int32, device="cuda"), torch.full((n,), 0.9, device="cuda")
+        settings, graph = wcb.Sampling(0, 0, p.data_ptr(), 0), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            wcb.sample_dev(l.data_ptr(), KIND[kind][1], n, v, settings, u.data_ptr(), out.data_ptr(), stream=torch.cuda.current_stream().cuda_stream)
+        graph.replay()
+        assert out.tolist() == sample_plain(l.double().cpu().numpy(), [1.0] * n, [0] * n, [float(p[0])] * n, [0.0] * n, u.double().cpu().numpy())[0]
+print("captured first")
+"""
+
+
+def test_the_first_calls_may_be_captured_ones(gpu):
+    r = _run(FIRST_CALLS)
+    assert r.returncode == 0 and "captured first" in r.stdout, r.stdout[-500:] + r.stderr[-2000:]
+
+
+WAITS = """
+import sys
+sys.path.insert(0, {pkg!r}); sys.path.insert(0, {tests!r})
+import time, torch, wcb
+import test_gpu_tree as t
+for act, cache in (("bf16", "bf16"), ("f16", "f16"), ("f32", "f16")):
+    for dim in (64, 128):
+        for q, kv in (([200], [2000]), ([5, 1, 2], [700, 65, 900]), ([1, 70, 64], [700, 1000, 230])):
+            s = t.Tree(q, kv, 8, 2, dim, act, cache, 64, seed=70)
+            torch.cuda.synchronize()
+            begin = time.time()
+            s.attend()
+            torch.cuda.synchronize()
+            assert time.time() - begin < 2, time.time() - begin
+            assert int(s.status.item()) & wcb.PAGED_ABORTED, (act, cache, dim, q)
+# what brings nothing by bulk copy works as ever: an f32 cache on the tensor cores
+s = t.Tree([200], [900], 8, 2, 64, "f32", "f32", 16, seed=71)
+s.attend()
+s.check()
+print("every wait ended")
+"""
+
+
+def test_waits_end(gpu):
+    """Copies that do not come (test_gpu_paged_waits.py): each wait runs out, the call says so, the device stays usable."""
+    r = _run(WAITS, {"WCB_TEST_WITHHOLD_COPY": "1"})
+    assert r.returncode == 0 and "every wait ended" in r.stdout, r.stdout[-500:] + r.stderr[-2000:]
