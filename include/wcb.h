@@ -572,7 +572,8 @@ typedef struct wcb_sampling {
  * k tokens, top_p of those the ones before which less than top_p of their sum
  * lies, min_p those that weigh at least min_p (the largest weighs 1). The token
  * is the lowest index at which the sum of the kept weights, in the order of
- * indices, exceeds u times the sum of all. Weights and sums are kept in 64 bits.
+ * indices, exceeds u times the sum of all. Weights are computed in 64 bits; for the
+ * sums they are rounded to steps of 2^-43, and below 2^-59 they count as none.
  * sampling NULL: all of the row at temperature 1. probs
  * (or NULL): [n_rows][vocab] f32 (probs_stride apart, 0: vocab), the
  * probabilities that the draw went by, zero for what was not kept: the input of

@@ -10,7 +10,7 @@
 // of squares is a shuffle over head_dim / 16 lanes, pairs of either kind lie in one thread and
 // neighbouring threads in neighbouring 16 bytes. The token's cosines and
 // sines are computed once by the first rot / 2 threads into shared memory:
-// position * inv_freq / 2 pi is reduced to a fraction of a turn in 64 bits (in
+// position * inv_freq / 2 pi (a tree's token: context + depth) is reduced to a fraction of a turn in 64 bits (in
 // 32 bits a position of 10^6 is off by up to 0.06 rad), its sine and cosine taken
 // in 32.
 //

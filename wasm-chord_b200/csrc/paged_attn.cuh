@@ -45,6 +45,10 @@
 // (1.1 GB), 182 us run after run, 93 % of the copy rate; one of 131071 keys (537 MB) 96 us, 86 %, the rest is the
 // launch, the first loads and the join; 16 sequences of 1 to 6 tokens over 500 to 2304
 // keys, 32/32 heads (349 MB), 66 us, 81 %; one sequence of 320 keys 8 us, all of it latency.
+//
+// TREE: the new tokens see their context and those new tokens that their rows of a bit mask name; only tiles that hold new
+// tokens look at the mask, a key at a time. One tree of 26 tokens over 333 keys, 32/4 heads of 64, f32 over f16: 14.5 us,
+// latency (place, loads, join of the pieces).
 #pragma once
 #include <cuda.h>
 #include <cudaTypedefs.h>

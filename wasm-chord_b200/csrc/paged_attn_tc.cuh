@@ -28,8 +28,15 @@
 // chain within a half, S to registers, exponentials, P back, products, none of which is near its limit by itself (tensor
 // pipe 47 %, exponentials 49 %, issue 36 % busy): 1250 clocks a half with both row tiles; without the
 // exponentials 600, and the products' 2560 clocks become the bound. Part of the exponentials by a polynomial on the
-// multiply-add units (a quarter, an eighth) gained nothing. About 120 bytes of registers spill. Short units: 11
-// sequences of 204 tokens 72 us (82 with units that are cut in two for one tile).
+// multiply-add units (a quarter, an eighth) gained nothing. About 240 bytes of registers spill. Short units: 11
+// sequences of 204 tokens, 32/4 heads of 64, f16, 31 us, 6 of 919 99 us: the queries' loads, one after another, were 6 us of each
+// unit before they went by cp.async (72 and 158 us).
+//
+// TREE: the new tokens of a sequence see its context and, among themselves, what their rows of a bit mask name
+// (Sight in paged_tc.cuh: 32 keys at a time, in tiles that hold new tokens alone). All rows of a
+// sequence then read all of its keys. 32 trees of 1 to 64 tokens over 65 to 4096 keys, 64/8 heads of 128, bf16 (332 MB): 160 us. The products
+// take 2.7 us for two row tiles and 128 keys, 2.1 us for one (it is the same chain of waits); the blocks' row tiles
+// are used to 75 %, a unit's start and end cost 4 us, and the last join 10 us.
 // P is rounded once to the 16-bit type: kept in two parts, as for few rows, P V would be two products, and a bf16 output would
 // still be off by its own rounding (relative error 1.7e-3 in place of 2.3e-3 at the size above).
 #pragma once

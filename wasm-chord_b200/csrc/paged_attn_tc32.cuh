@@ -1,6 +1,6 @@
 // Attention of many new rows over a paged cache on the 5th-generation tensor
 // cores, f32 activations over a cache of any type (the formulas and the line of tiles:
-// paged_attn.cuh; the 16-bit kernel this one is built like: paged_attn_tc.cu).
+// paged_attn.cuh; the 16-bit kernel this one is built like: paged_attn_tc.cuh).
 //
 // f32 numbers go to the tensor cores as sums of two f16 numbers, x = 2^e (hi + lo), 22 bits: the
 // exponents are a row's (q) or 8 keys' (k and v), so that the largest of them lies below 2^14 and
@@ -147,7 +147,7 @@ attend_tc32_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__
 
   if (warp >= MMA_WARP) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::R_MMA));
-    // ---- issuing warps (paged_attn_tc.cu says how) ------------------------------
+    // ---- issuing warps (paged_attn_tc.cuh says how) ------------------------------
     const int w = __shfl_sync(0xffffffffu, warp - MMA_WARP, 0);
     if (w < RT) {
       uint32_t elected;

@@ -6,7 +6,9 @@
 // all loads before the first store; no thread reads what another writes. A CTA finds the moves of its sequence (those
 // with path[i] > i) once, then each of its threads goes through them.
 //
-// Bound by latency: lengths, path, page table and the tokens are four loads that wait for one another.
+// Bound by latency: lengths, path, page table and the tokens are four loads that wait for one another. One sequence in 22 layers
+// 4 us; 32 sequences in 80 layers of 8 heads of 128, bf16, 54 tokens moved (35 MB) 12 to 15 us, 40 % of the copy rate: a CTA
+// for each layer's keys or values (16.4 us) made the lookups as often. Paths of up to 32 tokens (214 moved, 140 MB) 35 us, 61 %.
 #include "paged_common.cuh"
 
 namespace wcb {

@@ -1,5 +1,5 @@
-// What the two tensor-core attention kernels share (paged_attn_tc.cu: 16-bit
-// activations, paged_attn_tc32.cu: f32 activations): tcgen05 descriptors and instructions, bounded
+// What the two tensor-core attention kernels share (paged_attn_tc.cuh: 16-bit
+// activations, paged_attn_tc32.cuh: f32 activations): tcgen05 descriptors and instructions, bounded
 // waits, the walk over a CTA's units.
 #pragma once
 #include "paged_attn.cuh"

@@ -4,7 +4,8 @@
 // next[p] = the lowest i with parent[i] = p and token[i] = sampled[p]; the way is 0, next[0], next[next[0]] ..
 // Bound by latency: 12 bytes a node. One CTA a sequence finds next[] of all nodes at once in shared
 // memory, one thread walks it; so the loads of a tree are three dependent ones, not three for each level. A
-// sequence of more than NODES tokens is searched level by level instead.
+// sequence of more than NODES tokens is searched level by level instead. One tree of 26 tokens 2.9 us, 256 of 32 to 128 tokens 3.3 us
+// (GPU time in a graph), of which a launch is two.
 #include "paged_common.cuh"
 
 namespace wcb {
