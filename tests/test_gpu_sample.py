@@ -286,3 +286,15 @@ def test_rows_far_apart(gpu):
     out = torch.empty(2, dtype=torch.int32, device="cuda")
     wcb.sample_dev(rows.data_ptr(), wcb.KV_F32, 2, v, None, u.data_ptr(), out.data_ptr(), row_stride=stride)
     assert out.tolist() == sample_plain(l.astype(np.float64), [1.0] * 2, [0] * 2, [1.0] * 2, [0.0] * 2, u.double().cpu().numpy())[0]
+
+
+# more rows than run at once are taken in an order of their own: each is done once, whatever its settings
+@pytest.mark.parametrize("n", [297, 700, 2048, 2049])
+@pytest.mark.parametrize("given", ["all", "top_p", "top_k", "temperature"])
+def test_many_rows_of_many_kinds(gpu, n, given):
+    r = np.random.RandomState(n)
+    rows = [SETTINGS[i] for i in r.randint(0, len(SETTINGS), n)]
+    t, k, p, m = (list(x) for x in zip(*rows))
+    if given != "all":
+        t, k, p, m = (x if given == name else None for x, name in ((t, "temperature"), (k, "top_k"), (p, "top_p"), (m, "min_p")))
+    check(r.randn(n, 211) * 3, "f32", t, k, p, m, r.rand(n).tolist())

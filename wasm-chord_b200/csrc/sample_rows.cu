@@ -21,7 +21,7 @@
 //
 // Measured: one row of 32000, f32, top-k 40 and top-p 0.9: 15 us, latency (8 CTAs; of 26000 clocks the loads and the largest logit take 3000, bins
 // 9000, the pass 1000, the lists 9000, the draw 3000: a barrier of the cluster costs 1200). 416 rows of 32000, bf16, eight kinds of
-// settings: 65 us (rows without filters alone 35, with top-p 0.95 73, greedy 12; 27 MB, floor 4 us). 192 rows of 100003, f32, with probabilities: 132 us
+// settings: 49 us (rows without filters alone 35, with top-p 0.95 73, greedy 12; 27 MB, floor 4 us). 192 rows of 100003, f32, with probabilities: 115 us
 // (154 MB, floor 23 us). What bounds many rows: the 64-bit units, 15 operations a weight at 3.3 clocks a warp (half of the time
 // without filters), integer operations beside them, and shared-memory atomics (9 clocks for 32 logits) for the bins. Tried: a table of 64
 // powers instead of the longer polynomial (bank conflicts took what it saved), conversions to 64 bits by integer operations (no
@@ -51,6 +51,7 @@ constexpr int DIGITS = 1024;
 constexpr int CONTROL = 256;  // threads that go through bins, digits and lists: what they do is no less for being shared by more
 constexpr int LIST = 4096;  // tokens that a row's list holds, an equal part for each CTA
 constexpr int CHUNK = 256;  // logits of one warp's round, 8 a lane
+constexpr int COSTED = 2048;  // rows of a call that are put in order
 
 // order-preserving bits of a number (-0 is 0)
 __device__ __forceinline__ uint32_t key_of(float l) {
@@ -119,8 +120,9 @@ struct SampleShared {
   uint32_t found;
   int k_bin, above_k, whole;  // top-k's bin (BINS: there are fewer tokens), tokens above it, whether all of it is kept
   int first, last;            // bins between which top-p ends
-  int listed, fits;
+  int listed, fits, row;
   Cut end;
+  unsigned long long kinds[COSTED / 32];
 };
 
 // Places of a slice in shared memory: as far behind a multiple of 16 bytes as in memory, filled up with -infinity to whole chunks.
@@ -131,13 +133,70 @@ __host__ __device__ constexpr int places(int per) {
 
 // CACHED: the slice fits into shared memory; else it is read again and again
 template <typename T, bool CACHED>
-__global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_constant__ SampleArgs a, int per) {
+__global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_constant__ SampleArgs a, int per, bool by_cost) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = int(cluster.num_blocks()), rank = int(cluster.block_rank());
-  const int row = blockIdx.x / C, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   extern __shared__ __align__(16) unsigned long long chunk_sum[];  // of each chunk of the slice; then the slice
   __shared__ SampleShared sh;
+  // every CTA of the cluster runs before any writes into another's shared memory
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  int row = blockIdx.x / C;
+  if (by_cost) {
+    // Of more rows than run at once the dear ones come first, so that none of them begins last: the row that has this place
+    // in the order of (kind, row). Counts of the four kinds in 16 bits each, by 32 rows.
+    constexpr int STRIPS = COSTED / SR_THREADS;
+    int kind[STRIPS];
+    unsigned same[STRIPS];
+#pragma unroll
+    for (int j = 0; j < STRIPS; ++j) {
+      const int r = j * SR_THREADS + tid;
+      kind[j] = 4;
+      if (r < a.n_rows) {
+        const int k = a.top_k ? __ldg(a.top_k + r) : 0;
+        const bool warm = !a.temperature || __ldg(a.temperature + r) > 0.0f, p = a.top_p && __ldg(a.top_p + r) < 1.0f;
+        kind[j] = !warm ? 3 : p && (k <= 0 || k > 256) ? 0 : k > 0 ? 1 : 2;
+      }
+      unsigned long long counts = 0;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const unsigned mask = __ballot_sync(0xffffffffu, kind[j] == q);
+        if (kind[j] == q) same[j] = mask;
+        counts |= static_cast<unsigned long long>(__popc(mask)) << (16 * q);
+      }
+      if (lane == 0) sh.kinds[j * SR_WARPS + warp] = counts;
+    }
+    __syncthreads();
+    if (warp == 0) {  // what comes before each 32 rows, kind by kind
+      constexpr int PER = STRIPS * SR_WARPS / 32;
+      unsigned long long mine[PER], sum = 0;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        mine[j] = sh.kinds[PER * lane + j];
+        sum += mine[j];
+      }
+      unsigned long long inc = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long t = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += t;
+      }
+      const unsigned long long all = __shfl_sync(0xffffffffu, inc, 31);
+      unsigned long long before = inc - sum + (all << 16) + (all << 32) + (all << 48);  // (kinds before this one)
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        sh.kinds[PER * lane + j] = before;
+        before += mine[j];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < STRIPS; ++j)
+      if (kind[j] < 4 && int((sh.kinds[j * SR_WARPS + warp] >> (16 * kind[j])) & 0xffffu) + __popc(same[j] & ((1u << lane) - 1u)) == row) sh.row = j * SR_THREADS + tid;
+    __syncthreads();
+    row = sh.row;
+  }
   constexpr int V = 16 / int(sizeof(T));
   const int begin = rank * per, mine = max(0, min(per, a.vocab - begin));
   const T* slice = static_cast<const T*>(a.logits) + row * a.stride + begin;
@@ -145,8 +204,6 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
   const int chunks = mine > 0 ? (shift + mine + CHUNK - 1) / CHUNK : 0;
   const int start = begin - shift;  // index of place 0
   T* cache = reinterpret_cast<T*>(chunk_sum + (places<T>(per) / CHUNK + 1) / 2 * 2);
-  // every CTA of the cluster runs before any writes into another's shared memory
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   auto logit = [&](int at) {
     if constexpr (CACHED) return to_f32(cache[at]);
     else return at >= shift && at < shift + mine ? to_f32(slice[at - shift]) : -INFINITY;
@@ -1017,7 +1074,9 @@ cudaError_t run_sample(const SampleArgs& a, int c, int per, size_t shared, cudaS
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, sample_kernel<T, CACHED>, a, per);
+  // (eight kinds of settings: 416 rows of 32000, bf16, 49 us, in their own order 65; 192 of 100003, two CTAs a row, 115 and 132)
+  const bool by_cost = a.n_rows * c > 2 * SMS && a.n_rows <= COSTED && (a.temperature || a.top_k || a.top_p);
+  return cudaLaunchKernelEx(&cfg, sample_kernel<T, CACHED>, a, per, by_cost);
 }
 
 template <typename T>
