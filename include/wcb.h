@@ -577,7 +577,7 @@ typedef struct wcb_sampling {
  * sampling NULL: all of the row at temperature 1. probs
  * (or NULL): [n_rows][vocab] f32 (probs_stride apart, 0: vocab), the
  * probabilities that the draw went by, zero for what was not kept: the input of
- * wcb_spec_verify_dev, for instance. NaN and -infinity are no candidates; if
+ * wcb_spec_verify_dev, for instance; they may not overlap the logits. NaN and -infinity are no candidates; if
  * there are infinities, only they are weighed (all the same). A row without
  * candidates gives -1, zeros, and WCB_PAGED_BAD_PROBS in status (or NULL). */
 uint32_t wcb_sample_dev(const void* logits, uint32_t dtype, uint32_t n_rows, uint32_t vocab, uint64_t row_stride,
