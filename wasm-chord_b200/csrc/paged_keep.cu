@@ -6,8 +6,8 @@
 // all loads before the first store; no thread reads what another writes. A CTA finds the moves of its sequence (those
 // with path[i] > i) once, then each of its threads goes through them.
 //
-// Bound by latency: lengths, path, page table and the tokens are four loads that wait for one another. One sequence in 22 layers
-// 4 us; 32 sequences in 80 layers of 8 heads of 128, bf16, 54 tokens moved (35 MB) 12 to 15 us, 40 % of the copy rate: a CTA
+// Bound by latency: lengths (and path), page table and the tokens are three loads that wait for one another. One sequence in 22 layers
+// 3.5 us; 32 sequences in 80 layers of 8 heads of 128, bf16, 54 tokens moved (35 MB) 11 to 14 us, 40 to 50 % of the copy rate: a CTA
 // for each layer's keys or values (16.4 us) made the lookups as often. Paths of up to 32 tokens (214 moved, 140 MB) 35 us, 61 %.
 #include "paged_common.cuh"
 
@@ -52,14 +52,17 @@ __global__ void __launch_bounds__(KP_THREADS) keep_kernel(const __grid_constant_
   __shared__ int s_moves[KP_THREADS / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, s = blockIdx.x;
   const bool says = blockIdx.y == 0;  // one CTA of a sequence reports
+  // (a thread's first entry of the path, and the one before it, with the lengths: not after them)
+  const int32_t* path = a.path + int64_t(s) * a.max_path;
+  const int first = tid < a.max_path ? __ldg(path + tid) : 0, first_before = tid > 0 && tid < a.max_path ? __ldg(path + tid - 1) : -1;
+  const int given = __ldg(a.count + s);
   const Seq q = read_seq(a.batch, s);
   if (!q.sound && says && tid == 0) report(a.batch, ST_BAD_ROWS);
-  const int count = q.n > 0 ? min(max(__ldg(a.count + s), 0), a.max_path) : 0;
-  const int32_t* path = a.path + int64_t(s) * a.max_path;
+  const int count = q.n > 0 ? min(max(given, 0), a.max_path) : 0;
   // a path that does not ascend, or leaves the new tokens, is not followed
   bool bad = false;
   for (int i = tid; i < count; i += KP_THREADS) {
-    const int p = __ldg(path + i), before = i ? __ldg(path + i - 1) : -1;
+    const int p = i == tid ? first : __ldg(path + i), before = i == tid ? first_before : __ldg(path + i - 1);
     bad |= p <= before || p >= q.n;
   }
   if (__syncthreads_or(bad)) {
@@ -88,7 +91,7 @@ __global__ void __launch_bounds__(KP_THREADS) keep_kernel(const __grid_constant_
     const int i = i0 + tid;
     int64_t of = -1, to = -1;
     if (i < count) {
-      const int p = __ldg(path + i);
+      const int p = i == tid ? first : __ldg(path + i);
       if (p > i) {
         of = slot(context + p);
         to = slot(context + i);
@@ -125,7 +128,7 @@ cudaError_t launch_keep(const KeepArgs& a, cudaStream_t s) {
   const long long items = static_cast<long long>(words) * 2 * a.n_layers;
   // one word of each thread, as far as all CTAs run at once; then more of a thread, so that the lookups are made once for them
   long long y = (items + KP_THREADS - 1) / KP_THREADS;
-  // (32 sequences, 80 layers: short paths 11.7 us with 4 CTAs an SM, 12.6 with 8; paths of up to 32 tokens 38 and 35)
+  // (32 sequences, 80 layers: short paths 11.1 us with 4 CTAs an SM, 12 with 8; paths of up to 32 tokens 38 and 35)
   const long long most = (a.max_path <= 16 ? 4 : 8) * SMS / a.batch.n_seqs;
   if (y > most) y = most < 1 ? 1 : most;
   keep_kernel<<<dim3(a.batch.n_seqs, unsigned(y)), KP_THREADS, 0, s>>>(a);
