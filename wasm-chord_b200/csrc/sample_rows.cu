@@ -687,8 +687,10 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
         if (lane == 0) chunk_sum[c] = v;
       }
     } else {
-      // (past the last bin of interest nothing is done: nearly everywhere, with top-k)
-      const float reach = fmaxf(wanted, fmaxf(list_to, k_list)) - BIN0 + 1.0f;
+      // (past the last bin of interest nothing is done: nearly everywhere, with top-k. Without bins, below the least weight that counts:
+      // there of_top may be rounded by any number of bins)
+      const float slope = binned ? per_bin : 1.0f, base = binned ? of_top : 0.0f;
+      const float reach = binned ? fmaxf(wanted, fmaxf(list_to, k_list)) - BIN0 + 1.0f : -faint;
       for (int c = warp; c < chunks; c += SR_WARPS) {
         unsigned long long v = 0;
         float l[8];
@@ -697,7 +699,7 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
         for (int half = 0; half < 8; half += 4) {
           bool near = false;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) near |= !(fmaf(-l[half + j], per_bin, of_top) > reach);
+          for (int j = 0; j < 4; ++j) near |= !(fmaf(-l[half + j], slope, base) > reach);
           if (!__any_sync(0xffffffffu, near)) continue;
           bool on[4], sures[4], listed[4];
 #pragma unroll
