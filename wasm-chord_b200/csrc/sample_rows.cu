@@ -687,10 +687,13 @@ __global__ void __launch_bounds__(SR_THREADS, 2) sample_kernel(const __grid_cons
         if (lane == 0) chunk_sum[c] = v;
       }
     } else {
-      // (past the last bin of interest nothing is done: nearly everywhere, with top-k. Without bins, below the least weight that counts:
-      // there of_top may be rounded by any number of bins)
-      const float slope = binned ? per_bin : 1.0f, base = binned ? of_top : 0.0f;
-      const float reach = binned ? fmaxf(wanted, fmaxf(list_to, k_list)) - BIN0 + 1.0f : -faint;
+      // (past the last bin of interest nothing is done: nearly everywhere, with top-k. The last bin of all has no end: if it is of interest, what
+      // is passed over is no candidate, or, where nothing is listed, weighs nothing. So too without bins: there of_top may be rounded by any
+      // number of them)
+      const float furthest = fmaxf(wanted, fmaxf(list_to, k_list));
+      const bool ends = binned && furthest < BIN0 + float(BINS - 1);
+      const float slope = ends ? per_bin : 1.0f, base = ends ? of_top : 0.0f;
+      const float reach = ends ? furthest - BIN0 + 1.0f : lists ? -lowest : -faint;
       for (int c = warp; c < chunks; c += SR_WARPS) {
         unsigned long long v = 0;
         float l[8];
