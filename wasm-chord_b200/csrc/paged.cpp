@@ -119,23 +119,31 @@ uint32_t check_rows(const void* p, uint64_t stride, uint64_t width, uint32_t dty
 // 256 (32) 45 / 29, of 512 (64) 33 / 40, of 1024 28 / 64; 32 sequences of 40 rows (256) 70 / 114, of 256 87 / 423;
 // f32 over f32: 1 of 128 rows 41 / 34, of 256 47 / 52, 32 of 40 185 / 290; f32 over bf16: 16 of 612 rows 56 / 92;
 // 64/8 heads of 128, bf16: 1 of 64 rows (16) 46 / 32, of 128 (32) 47 / 45, of 256 (64) 53 / 61.
-constexpr uint64_t TC_MIN = 32, TC_UNITS = 32, TREE_UNITS = 104;
+// Trees leave no sequences to the mma.sync kernel where there is a tensor-core one: the second launch costs more than the small blocks save (with
+// the many / by themselves; 64/8 heads of 128, bf16: 63 single tokens and a tree of 64 over up to 4000 keys 236 / 290, 16 and 16 over up
+// to 2000 106 / 134; 32/4 heads of 64, f32 over f16: the same 182 / 197 and 78 / 95; f32 over f32: 284 / 273 and 115 / 134).
+constexpr uint64_t TC_MIN = 32, TC_UNITS = 32;
+// blocks up to which a tree's call takes smaller ones
+uint64_t tree_units(int head_dim) { return head_dim == 64 ? 128 : 96; }
 struct Plan {
   int rows;     // row block of the mma.sync kernel, 0: not run
   bool tc;
   int split;    // sequences of more rows are the tensor-core kernel's
 };
-Plan plan(uint64_t n_seqs, uint64_t n_kv, uint64_t max_rows, bool tree) {
+Plan plan(uint64_t n_seqs, uint64_t n_kv, uint64_t max_rows, int head_dim, bool tree) {
   Plan p{};
   p.tc = max_rows > TC_MIN && n_seqs * n_kv * ((max_rows + 31) / 32) > TC_UNITS;
   const int few = n_seqs == 1 || tree ? 0 : int(TC_MIN);
   p.split = p.tc ? few : INT_MAX;
   const uint64_t r = p.tc ? uint64_t(few) : max_rows;
   p.rows = r == 0 ? 0 : r <= 8 ? 8 : r <= 16 ? 16 : 32;
-  // A tree's call that leaves SMs without a block of its own takes smaller blocks, whose tiles take less time each: 208 rows
-  // of 4 key heads over 333 keys in blocks of 32 17.3 us, of 16 17.0, of 8 14.7, over 2000 keys 33, 25 and 25; 26 rows of 32 key heads
-  // over 1000 keys (32 blocks, 64, 128) 24.1, 18.8, 21.4.
-  while (tree && p.rows > 8 && n_seqs * n_kv * ((r + p.rows / 2 - 1) / (p.rows / 2)) <= TREE_UNITS) p.rows /= 2;
+  // A tree's call that leaves SMs without a block of its own takes smaller blocks, as long as there are no more than tree_units of them: their
+  // tiles take less time each, but every block reads all of the keys, so that the gain is lost with more blocks, longer contexts and larger heads.
+  // In blocks of 32 / 16 / 8 rows (us; over 300 keys, 1000, 4000), heads of 64, f32 over f16: 104 blocks of 8 (26 tokens of 4 key
+  // heads) 16.7 / 15.7 / 13.3, 29.1 / 20.0 / 18.1, 43.8 / 36.3 / 37.9; 128 (32 tokens) 17.1 / 16.3 / 14.9, 25.0 / 21.9 / 20.4, 47.7 / 42.7 / 43.3;
+  // 160 (10 sequences of 4) 16.6 / 14.8 / 14.3, 23.3 / 21.4 / 21.8, 43.6 / 50.8 / 54.3. Heads of 128, bf16: 96 (12 tokens of 8 key heads) 22.7 /
+  // 15.0 / 13.1, 24.5 / 17.4 / 16.4, 49 / 32.1 / 35.6; 128 (16 tokens) 22.8 / 15.3 / 14.6, 24.6 / 18.8 / 19.9, 54 / 39.3 / 42.4.
+  while (tree && p.rows > 8 && n_seqs * n_kv * ((r + p.rows / 2 - 1) / (p.rows / 2)) <= tree_units(head_dim)) p.rows /= 2;
   return p;
 }
 
@@ -243,7 +251,7 @@ uint32_t attend(const wcb_paged_kv* kv, const wcb_paged_batch* batch, const wcb_
   static const bool withhold = std::getenv("WCB_TEST_WITHHOLD_COPY") != nullptr;
   a.withheld = withhold ? 16 : 0;
   a.wait_ns = withhold ? 20000000ull : 2000000000ull;
-  const Plan p = plan(batch->n_seqs, kv->n_kv_heads, uint64_t(batch->max_q_len) * uint64_t(a.rep), tree != nullptr);
+  const Plan p = plan(batch->n_seqs, kv->n_kv_heads, uint64_t(batch->max_q_len) * uint64_t(a.rep), a.pool.head_dim, tree != nullptr);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
   if (p.tc) {
@@ -310,7 +318,7 @@ uint32_t wcb_paged_attention_workspace(const wcb_paged_kv* kv, const wcb_paged_b
     return bad("Invalid tensor shape: need n_heads % n_kv_heads == 0 (<= 64 per kv head)");
   const uint64_t rows = uint64_t(batch->max_q_len) * (n_heads / kv->n_kv_heads);
   // (a tree's call needs no more than a chain's)
-  *bytes = workspace_bytes(plan(batch->n_seqs, kv->n_kv_heads, rows, false), pool.head_dim);
+  *bytes = workspace_bytes(plan(batch->n_seqs, kv->n_kv_heads, rows, pool.head_dim, false), pool.head_dim);
   return WCB_OK;
 }
 
