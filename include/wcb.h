@@ -499,8 +499,11 @@ uint32_t wcb_spec_verify_dev(const int32_t* draft, const int32_t* draft_len, con
  * its slot is that of wcb_paged_append_dev, one after another. mask: bit i % 32 of
  * word mask[row * mask_words + i / 32] is set if row's token sees the i-th new
  * token of its sequence; of a tree, its ancestors and itself. The mask need not
- * be a tree's; tokens that 32 * mask_words bits do not reach are not seen.
- * Rows of no sequence may hold anything. */
+ * be a tree's; tokens that 32 * mask_words bits do not reach are not seen, bits
+ * past the new tokens are not looked at. (A row whose slot would be negative
+ * sees, of a tree, nothing but tokens without a place, and gives zeros; with a
+ * mask of another kind it sees those it names that have one.) Rows of no sequence
+ * may hold anything. */
 typedef struct wcb_paged_tree {
   uint32_t struct_size; /* sizeof(wcb_paged_tree) */
   uint32_t mask_words;  /* 32-bit words of a row's mask */
@@ -509,7 +512,9 @@ typedef struct wcb_paged_tree {
 } wcb_paged_tree;
 
 /* depth [n] and mask [n][mask_words] of one tree from parent [n], all on the
- * host: parent[i] < i is the i-th token's parent (parent[0] is not read). */
+ * host: parent[i] < i is the i-th token's parent (parent[0] is not read). The
+ * mask knows no window: where trees may be deeper than the window of their
+ * attention, the caller clears the bits of ancestors that lie outside of it. */
 uint32_t wcb_paged_tree_fill(const int32_t* parent, uint32_t n, uint32_t mask_words, int32_t* depth, uint32_t* mask);
 
 /* wcb_paged_append_dev with positions by depth: queries and keys turn by
@@ -555,7 +560,8 @@ uint32_t wcb_paged_keep_dev(const wcb_paged_kv* const* layers, uint32_t n_layers
 /* Settings of each row of a wcb_sample_dev call, device arrays of n_rows values;
  * NULL switches one off for all rows. temperature (NULL: 1): not above zero means
  * the largest logit's token. top_k: 0 or less is off. top_p: 1 or more is off.
- * min_p: 0 or less is off, above 1 counts as 1. (NaN: off.) */
+ * min_p: 0 or less is off, above 1 counts as 1. NaN is not above zero as a
+ * temperature (the largest logit's token), off as top_p and min_p. */
 typedef struct wcb_sampling {
   uint32_t struct_size; /* sizeof(wcb_sampling) */
   uint32_t reserved;    /* 0 */
@@ -570,7 +576,7 @@ typedef struct wcb_sampling {
  * (held to that). Token j weighs exp((l_j - max l) / temperature). In the order of
  * falling logits, the lowest index first among equal ones, top_k keeps the first
  * k tokens, top_p of those the ones before which less than top_p of their sum
- * lies, min_p those that weigh at least min_p (the largest weighs 1). The token
+ * lies (and always the first), min_p those that weigh at least min_p (the largest weighs 1). The token
  * is the lowest index at which the sum of the kept weights, in the order of
  * indices, exceeds u times the sum of all. Weights are computed in 64 bits; for the
  * sums they are rounded to steps of 2^-43, and below 2^-59 they count as none.

@@ -28,7 +28,8 @@
 // chain within a half, S to registers, exponentials, P back, products, none of which is near its limit by itself (tensor
 // pipe 47 %, exponentials 49 %, issue 36 % busy): 1250 clocks a half with both row tiles; without the
 // exponentials 600, and the products' 2560 clocks become the bound. Part of the exponentials by a polynomial on the
-// multiply-add units (a quarter, an eighth) gained nothing. About 240 bytes of registers spill. Short units: 11
+// multiply-add units (a quarter, an eighth) gained nothing. Registers spill: 348 to 360 bytes of stores (236 to 252 in
+// the form for trees). Short units: 11
 // sequences of 204 tokens, 32/4 heads of 64, f16, 31 us, 6 of 919 99 us: the queries' loads, one after another, were 6 us of each
 // unit before they went by cp.async (72 and 158 us).
 //

@@ -126,9 +126,11 @@ __global__ void __launch_bounds__(KP_THREADS) keep_kernel(const __grid_constant_
 cudaError_t launch_keep(const KeepArgs& a, cudaStream_t s) {
   const int words = a.pool.n_kv * a.pool.head_dim * a.size / 16;
   const long long items = static_cast<long long>(words) * 2 * a.n_layers;
-  // one word of each thread, as far as all CTAs run at once; then more of a thread, so that the lookups are made once for them
+  // one word of each thread, up to some CTAs an SM; then more of a thread, so that the lookups are made once for them. (Three CTAs run on an
+  // SM, by 154 registers a thread; a fourth that begins as the first end is worth its lookups.)
   long long y = (items + KP_THREADS - 1) / KP_THREADS;
-  // (32 sequences, 80 layers: short paths 11.1 us with 4 CTAs an SM, 12 with 8; paths of up to 32 tokens 38 and 35)
+  // (CTAs an SM 3 / 4 / 8. 32 sequences, 80 layers, 8 heads of 128, bf16, paths of up to 8 tokens 16.7 / 13.8 / 14.5 us; 64 in 32 layers 13.3 / 11.1 /
+  // 11.6; 9 in 80 5.5 / 6.5 / 8.7; 24 in 80, up to 32 tokens 32 / 28 / 25.5)
   const long long most = (a.max_path <= 16 ? 4 : 8) * SMS / a.batch.n_seqs;
   if (y > most) y = most < 1 ? 1 : most;
   keep_kernel<<<dim3(a.batch.n_seqs, unsigned(y)), KP_THREADS, 0, s>>>(a);

@@ -21,9 +21,10 @@
 //
 // Measured: one row of 32000, f32, top-k 40 and top-p 0.9: 15 us, latency (8 CTAs; of 26000 clocks the loads and the largest logit take 3000, bins
 // 9000, the pass 1000, the lists 9000, the draw 3000: a barrier of the cluster costs 1200). 416 rows of 32000, bf16, eight kinds of
-// settings: 49 us (rows without filters alone 35, with top-p 0.95 73, greedy 12; 27 MB, floor 4 us). 192 rows of 100003, f32, with probabilities: 115 us
-// (154 MB, floor 23 us). What bounds many rows: the 64-bit units, 15 operations a weight at 3.3 clocks a warp (half of the time
-// without filters), integer operations beside them, and shared-memory atomics (9 clocks for 32 logits) for the bins. Tried: a table of 64
+// settings: 49 us (rows without filters alone 35, with top-p 0.95 73, greedy 12; 27 MB, floor 4 us). 192 rows of 100003, f32, with probabilities: 116 us
+// (154 MB, floor 23 us). What bounds many rows: instructions (issue 57 %), integer ones first (bins, masks, 64-bit sums: that pipe 40 %), with
+// shared-memory atomics (9 clocks for 32 logits) for the bins, then barriers between short steps; the 64-bit units, 15 operations a
+// weight at 3.3 clocks a warp, are busy for 11 to 17 %, and bound only rows without filters. Tried: a table of 64
 // powers instead of the longer polynomial (bank conflicts took what it saved), conversions to 64 bits by integer operations (no
 // difference), 256 threads a CTA (66 to 76 us), lists of up to 512 tokens sorted (14000 clocks; digits 8000).
 #include <cooperative_groups.h>

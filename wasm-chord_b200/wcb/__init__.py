@@ -680,7 +680,8 @@ class PagedTree:
 
 def paged_tree_fill(parent: Sequence[int], mask_words: int = 0) -> Tuple[np.ndarray, np.ndarray]:
     """depth (int32 [n]) and mask (uint32 [n][mask_words]) of one tree, on the host. parent[i] < i:
-    the i-th token's parent; the first is the root. mask_words 0: as many as the tree needs."""
+    the i-th token's parent; the first is the root. mask_words 0: as many as the tree needs. (For
+    attention under a window that is shorter than a tree is deep, clear the bits of the ancestors outside of it.)"""
     p = np.ascontiguousarray(parent, dtype=np.int32)
     words = mask_words or max(1, -(-p.size // 32))
     depth, mask = np.empty(p.size, dtype=np.int32), np.empty((p.size, words), dtype=np.uint32)
@@ -735,7 +736,7 @@ def paged_keep_dev(layers: PagedLayers, batch: PagedBatch, path_ptr: int, max_pa
 
 class Sampling:
     """Each row's settings (wcb_sampling): device arrays temperature, top_p, min_p (float32)
-    and top_k (int32); 0 switches one off."""
+    and top_k (int32); 0 switches one off. (A temperature that is NaN or not above zero: the largest logit's token.)"""
 
     def __init__(self, temperature_ptr: int = 0, top_k_ptr: int = 0, top_p_ptr: int = 0, min_p_ptr: int = 0):
         self._c = _Sampling(C.sizeof(_Sampling), 0, temperature_ptr or None, top_k_ptr or None, top_p_ptr or None,
